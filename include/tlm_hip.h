@@ -576,6 +576,55 @@ void tlm_hip_model_reset_stats(tlm_hip_model *M);   /* tlm_model_reset_stats (sr
  * 441-460); NULL when every expert is resident */
 tlm_hip_store *tlm_hip_model_expert_store(const tlm_hip_model *M);
 
+/* ---- 8-bit floating point ----------------------------------------------------
+ * Weights as E4M3 codes (OCP: bias 7, largest 448, no infinities, NaN 0x7F /
+ * 0xFF) with one f32 scale per block of 128 rows x 128 values, the form in
+ * which the reference reads FP8 checkpoints (src/lib/tlm_quant.c:761-776;
+ * a last block of either axis may be part empty).  Matrices are packed once; the
+ * calls keep nothing from one to the next and may be captured into a graph.
+ *
+ * tlm_hip_fp8_pack: codes W (row r at W + r row_bytes) and scales (block
+ * (i, j) at scale[i scale_stride + j]) -> the packed layout, codes and scales
+ * in one piece of tlm_hip_fp8_packed_bytes(rows, n) bytes (0 for bad sizes), dst
+ * 16-byte aligned.  Any rows and n >= 1, any row_bytes >= n, any alignment of W. */
+#define TLM_HIP_DT_FP8 100   /* this library's dtype code of such a packed matrix */
+size_t tlm_hip_fp8_packed_bytes(int64_t rows, int64_t n);
+int    tlm_hip_fp8_pack(const void *W, size_t row_bytes, const float *scale, int64_t scale_stride, int64_t rows,
+                        int64_t n, void *dst, void *stream);
+/* ntok vectors of n values (dt: F32 0, F16 1 or BF16 2; token t at x + t xstride
+ * elements) -> E4M3 codes [ntok][np], np = n rounded up to 128 (codes past n
+ * are 0), and scales [ntok][np / 128].  A block's scale is the least power of
+ * two 2^e, e >= -126, with max |x| <= 448 * 2^e (0 for a block of zeros); each
+ * code is x / scale rounded to nearest, ties to even.  An infinity or NaN in a
+ * block makes its scale NaN and its codes 0.  codes 16-byte aligned. */
+int    tlm_hip_fp8_quantize(int dt, const void *x, int64_t xstride, int64_t n, int64_t ntok, void *codes,
+                            float *scale, void *stream);
+/* Y[t * ystride + r] = sum over the blocks b of scale[t][b] * sw[r / 128][b] *
+ * (codes of token t . codes of row r), r < rows, t < ntok, stored as dt (F32,
+ * F16 or BF16).  codes / scale as tlm_hip_fp8_quantize writes them (any f32
+ * scales; codes past n must be 0).  Products are exact, sums f32 in a fixed order:
+ * a call repeats its bits; the number of tokens may change them.  Elements of Y
+ * past rows and rows of Y past ntok are left as they are. */
+int    tlm_hip_fp8_matmul(const void *Wp, int64_t rows, int64_t n, const void *codes, const float *scale,
+                          int64_t ntok, int dt, void *Y, int64_t ystride, void *stream);
+/* A routed MoE block for T tokens of as many sequences (T <=
+ * TLM_HIP_FP8_MOE_MAX_TOKENS): out[t] = h[t] + MoE(h[t]) as tlm_hip_moe_layer's block
+ * computes it (rmsnorm, router, softmax or sigmoid routing, SwiGLU experts,
+ * rank-order combine, shared expert), with expert_dt / shared_dt
+ * TLM_HIP_DT_FP8 and matrices of tlm_hip_fp8_pack.  Activations stay f32
+ * from end to end (no activation quantisation).  Any D <= 16384, widths up
+ * to 65536; h and out [T x D] f32, out == h or not overlapping.  ids / w
+ * [T x k] (device, may be NULL) receive the routing.  Softmax routing selects by
+ * the router's scores, sigmoid routing by score + bias, ties to the lower
+ * index; where the mask leaves fewer than k experts the ranks behind them get id
+ * -1 and weight 0.  workspace: tlm_hip_fp8_moe_workspace_bytes(d, T) bytes,
+ * 256-byte aligned, nothing in it needs to be kept or zeroed; calls that may
+ * overlap (other streams) need different workspaces. */
+#define TLM_HIP_FP8_MOE_MAX_TOKENS 64
+size_t tlm_hip_fp8_moe_workspace_bytes(const tlm_hip_moe_desc *d, int64_t T);
+int    tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64_t T, int32_t *ids, float *w,
+                       void *workspace, void *stream);
+
 /* ---- reference tier ABI --------------------------------------------------
  * Layout-compatible with tlm_quant_kernels (src/lib/tlm_quant.h:152-166, a
  * name and two tables of TLM_QK_COUNT = 10 function pointers indexed F32,

@@ -5,5 +5,5 @@ include/tlm_hip.h); this package only binds it.  There is no CPU fallback:
 importing fails if the library is not built.
 """
 from ._lib import EXPORTS, LIB_PATH, HipError, lib  # noqa: F401
-from . import quant  # noqa: F401
+from . import fp8, quant  # noqa: F401
 from .moe import MoeBlock, MoeStack  # noqa: F401
