@@ -4,8 +4,10 @@ the activation quantiser (bit for bit) and the product.
 Tolerance of a product, counted from its roundings: a block's 128 products are
 exact, their sum takes 127 additions, the chain one fma per block and one
 product of the two scales, so an f32 result is off by at most
-(127 + nb + 2) 2^-24 S with S the sum of the magnitudes; a 16-bit output adds half a
-step of its type."""
+(127 + nb + 2) 2^-24 S with S the sum of the magnitudes.  A 16-bit output adds half a
+step of its type, and its sums may come from the 8-bit matrix instructions, which align
+every 8 products to the largest of them and cut what lies below 2^-13 of that one's
+power of two: at most 7 products lose less than 2^-13 max each, 7 * 2^-13 S in all."""
 import numpy as np
 import pytest
 import torch
@@ -63,6 +65,7 @@ def check_product(Y, w, s, codes, scale, n):
     want, size = X @ W.T, X.abs() @ W.abs().T
     nb = -(-n // 128)
     tol = (127 + nb + 2) * 2.0 ** -24 * size + HALF_STEP[Y.dtype] * want.abs() * (Y.dtype != torch.float32)
+    tol += 7 * 2.0 ** -13 * size * (Y.dtype != torch.float32)
     tol += 2.0 ** -25 * (Y.dtype == torch.float16)       # half a step of a subnormal binary16
     off = ((Y.double() - want).abs() - tol).max().item()
     assert off <= 0, (off, ((Y.double() - want).abs() / tol).max().item())

@@ -100,7 +100,7 @@ struct MmArgs {
     const float *sa;
     void *y;
     int64_t rows, ystride, T;
-    int nb;
+    int nb, wide;   /* wide: every run of four rows of Y may be stored at once */
 };
 
 template <class T>
@@ -132,6 +132,160 @@ __global__ __launch_bounds__(256) void k_fp8_mm(MmArgs a) {
     for (int v = 0; v < 4; v++) {
         const int64_t r = tile * 16 + 4 * g + v;
         if (r < a.rows) ((T *)a.y)[t * a.ystride + r] = to_out<T>(acc[v]);
+    }
+}
+
+/* ---- product, tiles through LDS ------------------------------------------------ */
+template <class T, int WM, int WN, int TM, int TN>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN / 4, WM * WN / 4)))
+void k_fp8_tile(MmArgs a, int mtiles, int ntiles) {
+    constexpr int NWV = WM * WN, MT = WM * TM, NT = WN * TN, UNITS = MT + NT, PER = UNITS / NWV;
+    static_assert(MT % NWV == 0 && NT % NWV == 0 && 8 % TM == 0 && MT % 8 == 0, "units are dealt evenly; a wave's rows share a scale");
+    __shared__ __align__(16) uint8_t s0[UNITS * FP8_UNIT], s1[UNITS * FP8_UNIT];
+    /* scales: a wave brings those of its share of the tokens, then the row blocks' */
+    constexpr int TPW = NT * 16 / NWV;
+    __shared__ float f0[NWV * 64], f1[NWV * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN, g = lane >> 4, c = lane & 15;
+    int bm, bn;
+    {   /* groups go to the eight XCDs in turn: give each XCD a run of tiles that share rows and tokens */
+        const int total = mtiles * ntiles, id = blockIdx.x, xcd = id & 7, at = id >> 3;
+        const int q = total >> 3, r = total & 7;
+        const int t = xcd * q + (xcd < r ? xcd : r) + at;
+        constexpr int BAND = 8;   /* row tiles of a band */
+        const int band = t / (BAND * ntiles), in = t % (BAND * ntiles);
+        const int width = mtiles - band * BAND < BAND ? mtiles - band * BAND : BAND;
+        bm = band * BAND + in % width;
+        bn = in / width;
+    }
+    const int tile0 = bm * MT, last = (int)fp8_tiles(a.rows) - 1;
+    const int64_t t0 = (int64_t)bn * NT * 16;
+    /* units wave, wave + NWV, ...: a uniform base that moves from block to block, and this lane's offset */
+    const GAS uint8_t *base[PER];
+    uint32_t off[PER][2];
+    const int left = (int)(a.T - 1 - t0 < NT * 16 ? a.T - 1 - t0 : NT * 16);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int u = wave + i * NWV;
+        if (i * NWV < MT) {
+            const int tile = tile0 + u < last ? tile0 + u : last;
+            base[i] = (const GAS uint8_t *)a.W + (size_t)tile * a.nb * FP8_UNIT;
+            off[i][0] = lane * 16;
+            off[i][1] = lane * 16 + 1024;
+        } else {
+            base[i] = (const GAS uint8_t *)a.x + (size_t)t0 * a.nb * FP8_BLOCK;
+            for (int h = 0; h < 2; h++) {
+                const int t = (u - MT) * 16 + 8 * h + (lane >> 3);
+                off[i][h] = (uint32_t)(t < left ? t : left) * (uint32_t)a.nb * FP8_BLOCK +
+                            16 * ((lane & 7) ^ (lane >> 3));
+            }
+        }
+    }
+    const int st = wave * TPW + lane, sr = lane - TPW, rlast = last / 8 - tile0 / 8;
+    const GAS float *ssrc = lane < TPW ? (const GAS float *)a.sa + (t0 + (st < left ? st : left)) * a.nb
+                                       : (const GAS float *)a.sw + (size_t)(tile0 / 8 + (sr < rlast ? sr : rlast)) * a.nb;
+    int pos = 0;   /* the block that the next load brings; past the last one it is brought again, unread */
+    auto load = [&](uint8_t *s, float *f) {
+        const bool more = ++pos < a.nb;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int u = wave + i * NWV;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                __builtin_amdgcn_global_load_lds((const GAS void *)(base[i] + off[i][h]),
+                                                 (LAS void *)(s + u * FP8_UNIT + h * 1024), 16, 0, 0);
+            base[i] += !more ? 0 : i * NWV < MT ? FP8_UNIT : FP8_BLOCK;
+        }
+        __builtin_amdgcn_global_load_lds((const GAS void *)ssrc, (LAS void *)(f + wave * 64), 4, 0, 0);
+        ssrc += more ? 1 : 0;
+    };
+    f32x4 acc[TM][TN] = {};
+    auto frag = [&](const uint8_t *s, int u) {
+        const LAS i32x4 *p = (const LAS i32x4 *)(s + u * FP8_UNIT + lane * 16);
+        return fp8_join(p[0], p[64]);
+    };
+    struct Cols {
+        i32x8 b[TN];
+        float sc[TN], w;
+    };
+    auto columns = [&](Cols &k, const uint8_t *s, const float *f, int j) {
+        const LAS uint8_t *p = (const LAS uint8_t *)s + (MT + wn * TN + j) * FP8_UNIT + c * FP8_BLOCK;
+        k.b[j] = fp8_join(*(const LAS i32x4 *)(p + 16 * (g ^ (c & 7))), *(const LAS i32x4 *)(p + 16 * ((4 + g) ^ (c & 7))));
+        const int t = (wn * TN + j) * 16;
+        k.sc[j] = ((const LAS float *)f)[t / TPW * 64 + t % TPW + c];
+        if (j == 0) k.w = ((const LAS float *)f)[TPW + wm * TM / 8];
+    };
+    /* One block: the matrix instructions of row tile i run beside the fmas of the ones before
+     * (a ring of RING results) and the reads of row tile i + 1.  Once row tile TM - 1 is in
+     * registers the stage is free: the waves meet, the next block's loads go out into it, and the
+     * next block's columns are read from the other stage under the last instructions. */
+    constexpr int RING = 4;
+    i32x8 av[2];
+    auto compute = [&](Cols &k, Cols &kn, uint8_t *s, float *f, const uint8_t *sn, const float *fn, bool on) {
+        f32x4 p[RING];
+        float sc[TN];
+#pragma unroll
+        for (int j = 0; j < TN; j++) sc[j] = k.w * k.sc[j];
+        auto fold = [&](int m) {
+            const int i = m / TN, j = m % TN;
+#pragma unroll
+            for (int v = 0; v < 4; v++) acc[i][j][v] = fmaf(p[m % RING][v], sc[j], acc[i][j][v]);
+        };
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            if (i + 1 < TM) av[(i + 1) & 1] = frag(s, wm * TM + i + 1);
+            if (i + 1 == TM && on) {
+                __syncthreads();
+                load(s, f);
+            }
+#pragma unroll
+            for (int j = 0; j < TN; j++) {
+                const int m = i * TN + j;
+                p[m % RING] = fp8_mfma(av[i & 1], k.b[j], (f32x4){0, 0, 0, 0});
+                if (m >= RING - 1) fold(m - RING + 1);
+                if (i + 1 == TM && on) columns(kn, sn, fn, j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (on) av[TM & 1] = frag(sn, wm * TM);
+#pragma unroll
+        for (int m = TM * TN - RING + 1; m < TM * TN; m++) fold(m);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    static_assert(TM % 2 == 0, "av[0] holds every block's first row tile");
+    Cols k0, k1;
+    load(s0, f0);
+    __syncthreads();
+    load(s1, f1);
+#pragma unroll
+    for (int j = 0; j < TN; j++) columns(k0, s0, f0, j);
+    av[0] = frag(s0, wm * TM);
+    for (int n2 = a.nb >> 1; n2 > 0; n2--) {
+        compute(k0, k1, s0, f0, s1, f1, true);
+        compute(k1, k0, s1, f1, s0, f0, true);
+    }
+    if (a.nb & 1) compute(k0, k1, s0, f0, s1, f1, false);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < TN; j++) {
+        const int64_t t = t0 + (wn * TN + j) * 16 + c;
+        if (t >= a.T) continue;
+        T *y = (T *)a.y + t * a.ystride;
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            const int64_t r = (int64_t)(tile0 + wm * TM + i) * 16 + 4 * g;
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 o;
+#pragma unroll
+            for (int v = 0; v < 4; v++) o[v] = to_out<T>(acc[i][j][v]);
+            if (a.wide && r + 3 < a.rows) {
+                *(T4 *)(y + r) = o;
+            } else {
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+                    if (r + v < a.rows) y[r + v] = o[v];
+            }
+        }
     }
 }
 
@@ -226,9 +380,15 @@ int tlm_hip_fp8_matmul(const void *Wp, int64_t rows, int64_t n, const void *code
     if (ntok > 1000000)
         return tlmh_seterr(TLM_HIP_ERANGE, "fp8_matmul: %lld tokens are too many for one launch", (long long)ntok);
     const MmArgs a = {(const uint8_t *)Wp, (const float *)((const uint8_t *)Wp + fp8_code_bytes(rows, n)),
-                      (const uint8_t *)codes, scale, Y, rows, ystride, ntok, (int)fp8_blocks(n)};
+                      (const uint8_t *)codes, scale, Y, rows, ystride, ntok, (int)fp8_blocks(n),
+                      aligned(Y, 4 * (size_t)type_bytes(dt)) && (ystride % 4 == 0 || ntok == 1)};
     const dim3 grid((unsigned)((fp8_tiles(rows) + 3) / 4), (unsigned)((ntok + 15) / 16));
     hipStream_t s = (hipStream_t)stream;
+    if (ntok >= 256 && dt == DT_BF16) {
+        const int mt = (int)((rows + 255) / 256), nt = (int)((ntok + 255) / 256);
+        hipLaunchKernelGGL((k_fp8_tile<__bf16, 2, 4, 8, 4>), dim3((unsigned)(mt * nt)), dim3(512), 0, s, a, mt, nt);
+        return tlmh_check(hipGetLastError(), "fp8_matmul launch");
+    }
     if (dt == DT_F32) hipLaunchKernelGGL(k_fp8_mm<float>, grid, dim3(256), 0, s, a);
     else if (dt == DT_F16) hipLaunchKernelGGL(k_fp8_mm<_Float16>, grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL(k_fp8_mm<__bf16>, grid, dim3(256), 0, s, a);
