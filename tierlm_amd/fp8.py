@@ -16,35 +16,46 @@ import ctypes as C
 import torch
 
 from ._lib import MoeDesc, check, lib
-from .quant import _ptr, stream
 
 FP8 = 100                       # TLM_HIP_DT_FP8
 BLOCK = 128
 MOE_MAX_TOKENS = 64             # TLM_HIP_FP8_MOE_MAX_TOKENS
 E4M3 = torch.float8_e4m3fn
+_CODES = (E4M3, torch.uint8)
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+_quantize, _matmul, _moe = lib.tlm_hip_fp8_quantize, lib.tlm_hip_fp8_matmul, lib.tlm_hip_fp8_moe
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _blocks(n):
     return -(-n // BLOCK)
 
 
-def _want(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
-def _on_device(*tensors):
+def _here(*tensors):
+    """The current device's index, on which all the tensors must be."""
+    dev = torch.cuda.current_device() if torch.cuda.is_initialized() or torch.cuda.is_available() else -1
     for t in tensors:
-        _want(t.is_cuda and t.device.index == torch.cuda.current_device(),
-              f"a tensor is on {t.device}, not on the current HIP device")
+        if t.get_device() != dev or dev < 0:
+            raise ValueError(f"a tensor is on {t.device}, not on the current HIP device")
+    return dev
+
+
+def _rows_ok(t):
+    """2-D with contiguous rows that do not overlap (any row stride)."""
+    if t.dim() != 2:
+        return False
+    s0, s1 = t.stride()
+    rows, n = t.shape
+    return (s1 == 1 or n == 1) and (s0 >= n or rows <= 1)
 
 
 def _out(t, shape, dtype, like, what):
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    _want(tuple(t.shape) == tuple(shape) and t.dtype == dtype and t.is_contiguous(),
-          f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+        return like.new_empty(shape, dtype=dtype)
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
     return t
 
 
@@ -55,56 +66,63 @@ def packed_bytes(rows, n):
 def pack(W, scale, out=None):
     """E4M3 rows W [rows, n] (float8_e4m3fn or uint8 codes, any row stride) and
     f32 scales [rows / 128, n / 128] (rounded up) -> the packed matrix (uint8)."""
-    _want(W.dim() == 2 and W.dtype in (E4M3, torch.uint8) and W.numel() > 0 and (W.shape[1] == 1 or W.stride(1) == 1),
-          "W must be a 2-D float8_e4m3fn or uint8 tensor with contiguous rows")
+    if W.dtype not in _CODES or not _rows_ok(W) or W.numel() == 0:
+        raise ValueError("W must be a 2-D float8_e4m3fn or uint8 tensor with contiguous rows")
     rows, n = W.shape
-    _want(tuple(scale.shape) == (_blocks(rows), _blocks(n)) and scale.dtype == torch.float32 and
-          (scale.shape[1] == 1 or scale.stride(1) == 1),
-          f"scale must be float32 [{_blocks(rows)}, {_blocks(n)}] with contiguous rows")
-    rb, ss = (W.stride(0) if rows > 1 else n), (scale.stride(0) if scale.shape[0] > 1 else _blocks(n))
-    _want(rb >= n and ss >= _blocks(n), "rows of W or scale overlap")
+    if scale.shape != (_blocks(rows), _blocks(n)) or scale.dtype != torch.float32 or not _rows_ok(scale):
+        raise ValueError(f"scale must be float32 [{_blocks(rows)}, {_blocks(n)}] with contiguous rows")
+    dev = _here(W, scale)
     out = _out(out, (packed_bytes(rows, n),), torch.uint8, W, "out")
-    _on_device(W, scale, out)
-    check(lib.tlm_hip_fp8_pack(_ptr(W), rb, _ptr(scale), ss, rows, n, _ptr(out), stream()))
+    _here(out)
+    check(lib.tlm_hip_fp8_pack(W.data_ptr(), max(W.stride(0), n), scale.data_ptr(), max(scale.stride(0), _blocks(n)),
+                               rows, n, out.data_ptr(), _raw_stream(dev)))
     return out
 
 
 def quantize(x, codes=None, scale=None):
     """x [T, n] (or [n]) -> E4M3 codes [T, np] and f32 scales [T, np / 128], np
     = n rounded up to 128; rows of x may have any stride."""
-    x = x[None] if x.dim() == 1 else x
-    _want(x.dim() == 2 and x.dtype in _TYPES and x.shape[1] > 0 and (x.shape[1] == 1 or x.stride(1) == 1),
-          "x must be float32, float16 or bfloat16 [T, n] with contiguous rows")
+    if x.dim() == 1:
+        x = x[None]
+    dt = _TYPES.get(x.dtype)
+    if dt is None or not _rows_ok(x) or x.shape[1] == 0:
+        raise ValueError("x must be float32, float16 or bfloat16 [T, n] with contiguous rows")
     T, n = x.shape
-    xs = x.stride(0) if T > 1 else n
-    _want(xs >= n, "rows of x overlap")
-    codes = _out(codes, (T, _blocks(n) * BLOCK), E4M3, x, "codes")
-    scale = _out(scale, (T, _blocks(n)), torch.float32, x, "scale")
-    _on_device(x, codes, scale)
-    check(lib.tlm_hip_fp8_quantize(_TYPES[x.dtype], _ptr(x), xs, n, T, _ptr(codes), _ptr(scale), stream()))
+    nb = -(-n // BLOCK)
+    codes = _out(codes, (T, nb * BLOCK), E4M3, x, "codes")
+    scale = _out(scale, (T, nb), torch.float32, x, "scale")
+    rc = _quantize(dt, x.data_ptr(), x.stride(0), n, T, codes.data_ptr(), scale.data_ptr(),
+                   _raw_stream(_here(x, codes, scale)))
+    if rc:
+        check(rc)
     return codes, scale
 
 
 def matmul(Wp, rows, n, codes, scale, out=None, dtype=torch.float32):
     """Y[t, r] = packed row r . token t: codes [T, np] and scale [T, np / 128] as
     quantize() gives them; Y [T, rows] of `dtype`, or `out` (rows of any stride)."""
-    _want(rows > 0 and n > 0 and Wp.dtype == torch.uint8 and Wp.is_contiguous() and Wp.numel() >= packed_bytes(rows, n),
-          f"Wp is not a packed matrix of {rows} x {n}")
-    _want(codes.dim() == 2 and codes.dtype in (E4M3, torch.uint8) and codes.is_contiguous() and
-          codes.shape[1] == _blocks(n) * BLOCK, f"codes must be contiguous E4M3 [T, {_blocks(n) * BLOCK}]")
+    nb = -(-n // BLOCK)
+    if rows <= 0 or n <= 0 or Wp.dtype != torch.uint8 or not Wp.is_contiguous() or \
+            Wp.numel() < lib.tlm_hip_fp8_packed_bytes(rows, n):
+        raise ValueError(f"Wp is not a packed matrix of {rows} x {n}")
+    if codes.dtype not in _CODES or codes.dim() != 2 or codes.shape[1] != nb * BLOCK or not codes.is_contiguous():
+        raise ValueError(f"codes must be contiguous E4M3 [T, {nb * BLOCK}]")
     T = codes.shape[0]
-    _want(tuple(scale.shape) == (T, _blocks(n)) and scale.dtype == torch.float32 and scale.is_contiguous(),
-          f"scale must be contiguous float32 [{T}, {_blocks(n)}]")
+    if scale.shape != (T, nb) or scale.dtype != torch.float32 or not scale.is_contiguous():
+        raise ValueError(f"scale must be contiguous float32 [{T}, {nb}]")
     if out is None:
-        _want(dtype in _TYPES, "dtype must be float32, float16 or bfloat16")
-        out = torch.empty((T, rows), dtype=dtype, device=Wp.device)
-    _want(tuple(out.shape) == (T, rows) and out.dtype in _TYPES and (rows == 1 or out.stride(1) == 1),
-          f"out must be float32, float16 or bfloat16 [{T}, {rows}] with contiguous rows")
-    ys = out.stride(0) if T > 1 else rows
-    _want(ys >= rows, "rows of out overlap")
-    _on_device(Wp, codes, scale, out)
-    check(lib.tlm_hip_fp8_matmul(_ptr(Wp), rows, n, _ptr(codes), _ptr(scale), T, _TYPES[out.dtype], _ptr(out), ys,
-                                 stream()))
+        if dtype not in _TYPES:
+            raise ValueError("dtype must be float32, float16 or bfloat16")
+        out = Wp.new_empty((T, rows), dtype=dtype)
+        dt = _TYPES[dtype]
+    else:
+        dt = _TYPES.get(out.dtype)
+        if out.shape != (T, rows) or dt is None or not _rows_ok(out):
+            raise ValueError(f"out must be float32, float16 or bfloat16 [{T}, {rows}] with contiguous rows")
+    rc = _matmul(Wp.data_ptr(), rows, n, codes.data_ptr(), scale.data_ptr(), T, dt, out.data_ptr(),
+                 out.stride(0), _raw_stream(_here(Wp, codes, scale, out)))
+    if rc:
+        check(rc)
     return out
 
 
@@ -118,20 +136,22 @@ class MoeBlock:
 
     def __init__(self, *, D, de, E, k, ffn_norm, router_w, expert_ptrs, router=0, routed_scale=1.0, eps=1e-6,
                  router_bias=None, mask=None, ds=0, shared=None, shared_gate_inp=None):
-        _want(len(expert_ptrs) == 3 * E and all(expert_ptrs), "expert_ptrs must hold 3 E packed matrices")
-        _want((ds > 0) == (shared is not None), "ds and shared go together")
+        if len(expert_ptrs) != 3 * E or not all(expert_ptrs):
+            raise ValueError("expert_ptrs must hold 3 E packed matrices")
+        if (ds > 0) != (shared is not None):
+            raise ValueError("ds and shared go together")
         for t, shape, dt, what in ((ffn_norm, (D,), torch.float32, "ffn_norm"),
                                    (router_w, (E, D), torch.float32, "router_w"),
                                    (router_bias, (E,), torch.float32, "router_bias"), (mask, (E,), torch.uint8, "mask"),
                                    (shared_gate_inp, (D,), torch.float32, "shared_gate_inp")):
-            _want(t is None or (tuple(t.shape) == shape and t.dtype == dt and t.is_contiguous()),
-                  f"{what} must be a contiguous {dt} tensor of shape {shape}")
             if t is not None:
-                _on_device(t)
+                _out(t, shape, dt, t, what)
+                _here(t)
         if shared is not None:
-            _want(len(shared) == 3 and all(m.numel() >= packed_bytes(*rn) for m, rn in
-                                           zip(shared, ((ds, D), (ds, D), (D, ds)))), "shared must be 3 packed matrices")
-            _on_device(*shared)
+            if len(shared) != 3 or any(m.numel() < packed_bytes(*rn)
+                                       for m, rn in zip(shared, ((ds, D), (ds, D), (D, ds)))):
+                raise ValueError("shared must be 3 packed matrices")
+            _here(*shared)
         self.keep = [ffn_norm, router_w, router_bias, mask, shared, shared_gate_inp]
         self.device = ffn_norm.device
         self.table = torch.tensor(list(expert_ptrs), dtype=torch.int64, device=self.device)
@@ -142,15 +162,17 @@ class MoeBlock:
         sg, su, sd = shared if shared is not None else (None, None, None)
         self.desc = MoeDesc(D, de, ds, E, k, router, routed_scale, eps, FP8, FP8, p(ffn_norm), p(router_w),
                             p(router_bias), p(mask), self.table.data_ptr(), p(sg), p(su), p(sd), p(shared_gate_inp))
-        check(lib.tlm_hip_fp8_moe(C.byref(self.desc), None, None, 0, None, None, None, None))   # the sizes fit
+        self._desc = C.byref(self.desc)
+        self.D, self.k = D, k
+        check(_moe(self._desc, None, None, 0, None, None, None, None))   # the sizes fit
         self.workspace, self._room = None, 0
 
     def reserve(self, T):
         """Make the workspace large enough for T tokens."""
         if T > self._room:
-            nbytes = int(lib.tlm_hip_fp8_moe_workspace_bytes(C.byref(self.desc), T))
+            nbytes = int(lib.tlm_hip_fp8_moe_workspace_bytes(self._desc, T))
             if not nbytes:
-                check(lib.tlm_hip_fp8_moe(C.byref(self.desc), None, None, T, None, None, None, None))
+                check(_moe(self._desc, None, None, T, None, None, None, None))
             self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             self._room = T
 
@@ -158,17 +180,22 @@ class MoeBlock:
         """out = h + MoE(h) for h (f32 [T, D] or [D]), T <= 64; without `out` h itself
         is updated.  ids (int32) / w (f32), [T, k], receive the routing.  Returns
         out."""
-        D, k = self.desc.D, self.desc.k
-        T = h.numel() // D
-        _want(h.dtype == torch.float32 and h.is_contiguous() and h.dim() in (1, 2) and h.shape[-1] == D,
-              f"h must be contiguous float32 [T, {D}]")
+        if h.dtype != torch.float32 or not h.is_contiguous() or h.dim() not in (1, 2) or h.shape[-1] != self.D:
+            raise ValueError(f"h must be contiguous float32 [T, {self.D}]")
+        T = h.shape[0] if h.dim() == 2 else 1
         out = h if out is None else _out(out, h.shape, torch.float32, h, "out")
-        _on_device(h, out)
-        for t, dt, what in ((ids, torch.int32, "ids"), (w, torch.float32, "w")):
-            if t is not None:
-                _out(t, (T, k), dt, h, what)
-                _on_device(t)
-        self.reserve(T)
-        check(lib.tlm_hip_fp8_moe(C.byref(self.desc), _ptr(h), _ptr(out), T, _ptr(ids), _ptr(w),
-                                  _ptr(self.workspace), stream()))
+        dev = _here(h, out)
+        pi = pw = None
+        if ids is not None:
+            _here(_out(ids, (T, self.k), torch.int32, h, "ids"))
+            pi = ids.data_ptr()
+        if w is not None:
+            _here(_out(w, (T, self.k), torch.float32, h, "w"))
+            pw = w.data_ptr()
+        if T > self._room:
+            self.reserve(T)
+        if T:
+            rc = _moe(self._desc, h.data_ptr(), out.data_ptr(), T, pi, pw, self.workspace.data_ptr(), _raw_stream(dev))
+            if rc:
+                check(rc)
         return out
