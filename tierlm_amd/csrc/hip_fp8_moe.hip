@@ -31,7 +31,7 @@ constexpr int NT = 4;              /* column tiles at a time */
 __host__ __device__ inline size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct Layout {
-    size_t xp, key, score, sgate, hid, shid, eo, seo, total;
+    size_t xp, key, score, sgate, ids, w, dptr, hid, shid, eo, seo, total;
     int nbd, nbe, nbs;             /* blocks of D, of the expert width, of the shared width */
 };
 
@@ -45,6 +45,9 @@ Layout layout(const tlm_hip_moe_desc &d, int64_t T) {
     L.key = o;   o += al256((size_t)T * d.E * 4);
     L.score = o; o += al256((size_t)T * d.E * 4);
     L.sgate = o; o += al256((size_t)T * 4);
+    L.ids = o;   o += al256((size_t)T * d.k * 4);
+    L.w = o;     o += al256((size_t)T * d.k * 4);
+    L.dptr = o;  o += al256((size_t)T * d.k * 8);
     L.hid = o;   o += al256((size_t)T * d.k * 3 * L.nbe * FP8_BLOCK * 2);
     L.shid = o;  o += al256((size_t)T * 3 * L.nbs * FP8_BLOCK * 2);
     L.eo = o;    o += al256((size_t)T * d.k * d.D * 4);
@@ -76,111 +79,216 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 }
 __device__ __forceinline__ float silu(float x) { return x / (1.0f + expf_ref(-x)); }
 
-/* ---- K1 --------------------------------------------------------------------- */
-constexpr int ROUTER_EXPERTS = 8;   /* experts per group */
+/* ---- K1 ---------------------------------------------------------------------
+ * A wave per router row (the shared expert's gate is one more), `tg` tokens of x in LDS: the
+ * row's first 2048 values are on their way while the tokens are normalised.  Sums of four
+ * products in float, those in double: two experts' scores keep their order down to the
+ * last bits of a float. */
+constexpr int ROUTER_TOKENS = 4;
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-__global__ __launch_bounds__(256) void k_fm_router(Args a) {
+/* four values of a row of D at i, zeros behind its end */
+__device__ __forceinline__ f32x4 row4(const GAS float *p, int i, int D) {
+    f32x4 v = {0, 0, 0, 0};
+    if (i + 3 < D) {
+        v = *(const GAS f32x4u *)(p + i);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            if (i + q < D) v[q] = p[i + q];
+    }
+    return v;
+}
+
+__global__ __launch_bounds__(256) void k_fm_router(Args a, int tg) {
     extern __shared__ __align__(16) float s_x[];
-    __shared__ double s_red[4];
+    __shared__ double s_red[4][ROUTER_TOKENS];
     const tlm_hip_moe_desc &d = a.d;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t = blockIdx.y;
-    const int D = (int)d.D;
-    const float *h = a.h + (size_t)t * D;
-    double ss = 0.0;
-    for (int i = tid; i < D; i += 256) {
-        const float v = h[i];
-        s_x[i] = v;
-        ss += (double)v * (double)v;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), t0 = blockIdx.y * tg;
+    const int D = (int)d.D, Dq = (D + 3) & ~3, nt = a.T - t0 < tg ? a.T - t0 : tg;
+    const int e = blockIdx.x * 4 + wave;
+    const bool live = e < d.E || (e == d.E && d.ds > 0 && d.shared_gate_inp);
+    const GAS float *w = (const GAS float *)(live && e == d.E ? d.shared_gate_inp : d.router_w + (size_t)(live ? e : 0) * D);
+    constexpr int NV = 8;
+    f32x4 wv[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) wv[j] = row4(w, 4 * lane + 256 * j, D);
+    const GAS float *h = (const GAS float *)a.h + (size_t)t0 * D, *nw = (const GAS float *)d.ffn_norm;
+    for (int t = 0; t < nt; t++) {
+        double ss = 0.0;
+        for (int i = 4 * tid; i < Dq; i += 1024) {
+            const f32x4 v = row4(h + (size_t)t * D, i, D);
+            *(f32x4 *)(s_x + t * Dq + i) = v;
+#pragma unroll
+            for (int q = 0; q < 4; q++) ss += (double)v[q] * (double)v[q];
+        }
+        ss = wave_sum_f64(ss);
+        if (lane == 0) s_red[wave][t] = ss;
     }
-    ss = wave_sum_f64(ss);
-    if (lane == 0) s_red[wave] = ss;
     __syncthreads();
-    ss = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
-    const float rn = 1.0f / sqrtf((float)(ss / (double)D) + d.eps);
     const int Dp = a.L.nbd * FP8_BLOCK;
-    uint16_t *xp = (uint16_t *)(a.ws + a.L.xp) + (size_t)t * 3 * Dp;
-    for (int i = tid; i < Dp; i += 256) {
-        const float v = i < D ? s_x[i] * rn * d.ffn_norm[i] : 0.0f;
-        if (i < D) s_x[i] = v;
-        if ((i >> 8) % gridDim.x == blockIdx.x) {   /* the groups share the planes' writing */
-            uint16_t p[3];
-            split3(v, p);
-            xp[i] = p[0];
-            xp[Dp + i] = p[1];
-            xp[2 * Dp + i] = p[2];
+    for (int t = 0; t < nt; t++) {
+        const double ss = (s_red[0][t] + s_red[1][t]) + (s_red[2][t] + s_red[3][t]);
+        const float rn = 1.0f / sqrtf((float)(ss / (double)D) + d.eps);
+        uint16_t *xp = (uint16_t *)(a.ws + a.L.xp) + (size_t)(t0 + t) * 3 * Dp;
+        for (int i = 4 * tid; i < Dp; i += 1024) {
+            f32x4 v = {0, 0, 0, 0};
+            if (i < Dq) {
+                const f32x4 g = row4(nw, i, D);
+                v = *(const f32x4 *)(s_x + t * Dq + i) * rn * g;
+                *(f32x4 *)(s_x + t * Dq + i) = v;
+            }
+            if ((i >> 8) % gridDim.x == blockIdx.x) {   /* the groups share the planes' writing */
+                u16x4 o[3];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint16_t p[3];
+                    split3(v[q], p);
+#pragma unroll
+                    for (int j = 0; j < 3; j++) o[j][q] = p[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 3; j++) *(u16x4 *)(xp + j * Dp + i) = o[j];
+            }
         }
     }
     __syncthreads();
-    const int rows = (int)min((int64_t)ROUTER_EXPERTS, (int64_t)d.E - (int64_t)blockIdx.x * ROUTER_EXPERTS);
-    const bool gate = d.ds > 0 && d.shared_gate_inp && blockIdx.x == 0;
-    for (int r = wave; r < rows + (gate ? 1 : 0); r += 4) {
-        const int e = blockIdx.x * ROUTER_EXPERTS + r;
-        const float *w = r < rows ? d.router_w + (size_t)e * D : d.shared_gate_inp;
-        /* double: two experts' scores keep their order down to the last bit of a float */
-        double acc = 0.0;
-        for (int i = lane; i < D; i += 64) acc = __builtin_fma((double)w[i], (double)s_x[i], acc);
-        acc = wave_sum_f64(acc);
-        if (lane != 0) continue;
-        const float l = (float)acc;
-        if (r == rows) {
-            ((float *)(a.ws + a.L.sgate))[t] = 1.0f / (1.0f + expf_ref(-l));
-            continue;
+    if (!live) return;
+    double acc[ROUTER_TOKENS] = {};
+    for (int i0 = 0; i0 < Dq; i0 += 256 * NV) {
+        if (i0 > 0)
+#pragma unroll
+            for (int j = 0; j < NV; j++) wv[j] = row4(w, i0 + 4 * lane + 256 * j, D);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int i = i0 + 4 * lane + 256 * j;
+            if (i >= Dq) continue;
+#pragma unroll
+            for (int t = 0; t < ROUTER_TOKENS; t++)
+                if (t < nt) {
+                    const f32x4 x = *(const f32x4 *)(s_x + t * Dq + i);
+                    float p = wv[j][0] * x[0];
+#pragma unroll
+                    for (int q = 1; q < 4; q++) p = fmaf(wv[j][q], x[q], p);
+                    acc[t] += (double)p;
+                }
         }
-        float score = l, sel = l;
-        if (d.router == 2) {
-            score = 1.0f / (1.0f + expf_ref(-l));
-            sel = d.router_bias ? score + d.router_bias[e] : score;
-        }
-        ((float *)(a.ws + a.L.score))[t * d.E + e] = score;
-        ((uint32_t *)(a.ws + a.L.key))[t * d.E + e] = d.mask && d.mask[e] ? 0u : order_key(sel);
     }
+#pragma unroll
+    for (int t = 0; t < ROUTER_TOKENS; t++) {
+        if (t >= nt) break;
+        const float l = (float)wave_sum_f64(acc[t]);
+        if (lane != 0) continue;
+        if (e == d.E) {
+            ((float *)(a.ws + a.L.sgate))[t0 + t] = 1.0f / (1.0f + expf_ref(-l));
+        } else {
+            float score = l, sel = l;
+            if (d.router == 2) {
+                score = 1.0f / (1.0f + expf_ref(-l));
+                sel = d.router_bias ? score + d.router_bias[e] : score;
+            }
+            ((float *)(a.ws + a.L.score))[(t0 + t) * d.E + e] = score;
+            ((uint32_t *)(a.ws + a.L.key))[(t0 + t) * d.E + e] = d.mask && d.mask[e] ? 0u : order_key(sel);
+        }
+    }
+}
+
+/* ---- routing ------------------------------------------------------------------
+ * Expert e is among token t's k if fewer than k of t's keys are ahead of its own; the count is
+ * its rank.  256 threads, thread e counts for expert e. */
+__device__ __forceinline__ bool ahead(uint32_t kf, int f, uint32_t ke, int e) {
+    return kf > ke || (kf == ke && f < e);
+}
+struct Route {
+    uint32_t key[MAXE];
+    int ids[MAXK];
+    float w[MAXK];
+    float redf[4];
+    double red[4];
+};
+/* Token t's rank of expert `tid` (MAXE where it cannot be chosen), from keys brought to LDS.  Ends in
+ * a barrier. */
+__device__ __forceinline__ int rank_of(const Args &a, int t, Route *R, int tid) {
+    const int E = a.d.E;
+    if (tid < MAXE) R->key[tid] = tid < E ? ((const GAS uint32_t *)(a.ws + a.L.key))[(size_t)t * E + tid] : 0u;
+    if (tid < MAXK) {
+        R->ids[tid] = -1;
+        R->w[tid] = 0.0f;
+    }
+    __syncthreads();
+    if (tid >= E || R->key[tid] == 0u) return MAXE;
+    const uint32_t ke = R->key[tid];
+    int c[4] = {0, 0, 0, 0};
+    for (int f = 0; f < E; f += 4) {   /* keys past E are 0, never ahead */
+        const u32x4 k = *(const LAS u32x4 *)&R->key[f];
+#pragma unroll
+        for (int q = 0; q < 4; q++) c[q] += ahead(k[q], f + q, ke, tid) ? 1 : 0;
+    }
+    return (c[0] + c[1]) + (c[2] + c[3]);
+}
+/* A token's experts and weights in rank order into the workspace and the caller's arrays: ranks past the
+ * number of experts that can be chosen get id -1 and weight 0.  All threads of a group of 256. */
+__device__ void route_token(const Args &a, int t, Route *R, int rank) {
+    const tlm_hip_moe_desc &d = a.d;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = d.E, k = d.k;
+    const bool can = rank < MAXE;
+    const float l = tid < E ? ((const GAS float *)(a.ws + a.L.score))[(size_t)t * E + tid] : 0.0f;
+    float p = l;
+    if (d.router != 2) {   /* softmax over the experts that can be chosen */
+        const bool on = can && l == l;
+        const float m = wave_max_f32(on ? l : -INFINITY);
+        if (lane == 0) R->redf[wave] = m;
+        __syncthreads();
+        float mx = R->redf[0];
+        for (int q = 1; q < 4; q++) mx = R->redf[q] > mx ? R->redf[q] : mx;
+        const float x = on && mx > -INFINITY ? expf_ref(l - mx) : 0.0f;
+        const double sum = wave_sum_f64((double)x);
+        if (lane == 0) R->red[wave] = sum;
+        __syncthreads();
+        const double st = (R->red[0] + R->red[1]) + (R->red[2] + R->red[3]);
+        p = st > 0.0 ? (float)((double)x / st) : 0.0f;
+    }
+    if (rank < k) {
+        R->ids[rank] = tid;
+        R->w[rank] = p;
+    }
+    __syncthreads();
+    if (wave == 0) {   /* renormalise over the chosen, then scale */
+        float wr = lane < k ? R->w[lane] : 0.0f;
+        if (d.router != 1) {
+            double s = 0.0;
+            for (int r = 0; r < k; r++) s += (double)rdlane_f32(wr, r);
+            if (d.router == 2) s += 1e-20;
+            if (s > 0.0) wr = (float)((double)wr / s);
+        }
+        wr *= d.routed_scale;
+        if (lane < k) {
+            const int id = R->ids[lane], at = t * k + lane;
+            ((int32_t *)(a.ws + a.L.ids))[at] = id;
+            ((float *)(a.ws + a.L.w))[at] = wr;
+            ((const void **)(a.ws + a.L.dptr))[at] = id >= 0 ? d.experts[3 * (size_t)id + 2] : nullptr;
+            if (a.ids) a.ids[at] = id;
+            if (a.w) a.w[at] = wr;
+        }
+    }
+}
+__global__ __launch_bounds__(256) void k_fm_route(Args a) {
+    __shared__ __align__(16) Route R;
+    const int rank = rank_of(a, blockIdx.x, &R, threadIdx.x);
+    route_token(a, blockIdx.x, &R, rank);
 }
 
 /* ---- an expert's tokens ------------------------------------------------------ */
 struct List {
-    int n;
+    int n, e;
     uint8_t tok[MAXT], rank[MAXT];
 };
-
-__device__ __forceinline__ bool ahead(uint32_t kf, int f, uint32_t ke, int e) {
-    return kf > ke || (kf == ke && f < e);
-}
-
-/* The tokens that chose expert e, ascending, with its rank among their k.  All
- * threads; ends in a barrier. */
-__device__ void find_tokens(const Args &a, int e, List *s, uint8_t *s_sel) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = a.d.E;
-    const uint32_t *key = (const uint32_t *)(a.ws + a.L.key);
-    for (int t = wave; t < a.T; t += NW) {
-        const uint32_t ke = key[t * E + e];
-        int rank = 0;
-        for (int f0 = 0; f0 < E; f0 += 64) {
-            const int f = f0 + lane;
-            const uint32_t kf = f < E ? key[t * E + f] : 0u;
-            rank += __builtin_popcountll(__ballot(f < E && kf && ahead(kf, f, ke, e)));
-        }
-        if (lane == 0) s_sel[t] = ke && rank < a.d.k ? (uint8_t)(rank + 1) : 0;
-    }
-    __syncthreads();
-    if (wave == 0) {
-        const int sel = lane < a.T ? s_sel[lane] : 0;
-        const unsigned long long m = __ballot(sel != 0);
-        if (sel) {
-            const int at = __builtin_popcountll(m & ((1ull << lane) - 1));
-            s->tok[at] = (uint8_t)lane;
-            s->rank[at] = (uint8_t)(sel - 1);
-        }
-        if (lane == 0) s->n = __builtin_popcountll(m);
-    }
-    __syncthreads();
-}
-
-/* The list of slot `slot`: the shared expert (every token), expert `slot`, or, with
- * fewer choices than experts, the expert of token slot / k at rank slot % k unless an
- * earlier token chose it too.  Returns the expert, or -1 for nothing to do;
- * E for the shared one. */
-__device__ int slot_list(const Args &a, int slot, List *s, uint8_t *s_sel, int *s_e) {
-    const int tid = threadIdx.x, E = a.d.E;
+/* The pairs (token, rank) of slot `slot` and its expert: every token for the shared expert (E); expert
+ * `slot`'s; or, with fewer choices than experts, those of the expert that pair `slot` chose, unless an
+ * earlier pair chose it too (-1: nothing to do).  All threads; ends in a barrier. */
+__device__ int slot_list(const Args &a, int slot, List *s) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.d.k, pairs = a.T * k;
+    const GAS int32_t *ids = (const GAS int32_t *)(a.ws + a.L.ids);
     if (slot == a.slots) {
         if (tid < a.T) {
             s->tok[tid] = (uint8_t)tid;
@@ -188,26 +296,27 @@ __device__ int slot_list(const Args &a, int slot, List *s, uint8_t *s_sel, int *
         }
         if (tid == 0) s->n = a.T;
         __syncthreads();
-        return E;
+        return a.d.E;
     }
-    int e = slot;
-    if (!a.by_expert) {
-        const uint32_t *key = (const uint32_t *)(a.ws + a.L.key) + (size_t)(slot / a.d.k) * E;
-        if (tid == 0) *s_e = -1;
-        __syncthreads();
-        const uint32_t ke = tid < E ? key[tid] : 0u;
-        int rank = 0;
-        for (int f = 0; f < E; f++) {
-            const uint32_t kf = key[f];
-            rank += kf && ahead(kf, f, ke, tid) ? 1 : 0;
+    const int e = a.by_expert ? slot : uniform(ids[slot]);
+    if (e < 0) return -1;
+    if (wave == 0) {
+        int n = 0;
+        for (int p0 = 0; p0 < pairs; p0 += 64) {
+            const int p = p0 + lane, id = p < pairs ? ids[p] : -1;
+            const unsigned long long m = __ballot(id == e);
+            if (id == e) {
+                const int at = n + __builtin_popcountll(m & ((1ull << lane) - 1));
+                s->tok[at] = (uint8_t)(p / k);
+                s->rank[at] = (uint8_t)(p % k);
+                if (at == 0) s->e = p;
+            }
+            n += __builtin_popcountll(m);
         }
-        if (tid < E && ke && rank == slot % a.d.k) *s_e = tid;
-        __syncthreads();
-        e = *s_e;
-        if (e < 0) return -1;
+        if (lane == 0) s->n = n;
     }
-    find_tokens(a, e, s, s_sel);
-    if (s->n == 0 || (!a.by_expert && s->tok[0] != slot / a.d.k)) return -1;
+    __syncthreads();
+    if (s->n == 0 || (!a.by_expert && s->e != slot)) return -1;
     return e;
 }
 
@@ -222,56 +331,67 @@ __device__ __forceinline__ Mat mat_of(const void *packed, int tile, int64_t rows
             (const GAS float *)(p + fp8_code_bytes(rows, (int64_t)nb * FP8_BLOCK)) + tile / 8 * nb};
 }
 
-/* This wave's share of the blocks, for NQ column tiles; x[q]: this lane's column of
- * planes.  No branch stands between a matrix instruction and the reads of its result: the
+/* This wave's share of the blocks, for NQ column tiles, U blocks in flight; x[q]: this lane's
+ * column of planes.  No branch stands between a matrix instruction and the reads of its result: the
  * compiler here has left out the wait on such a path. */
-template <int M, int NQ>
-__device__ __forceinline__ void run_tiles(const Mat (&m)[M], int nb, int wave, const uint16_t *const (&x)[NT],
+template <int M, int NQ, int U>
+__device__ __forceinline__ void run_tiles(const Mat (&m)[M], int nb, int wave, const GAS uint16_t *const (&x)[NT],
                                           f32x4 (&acc)[M][NT]) {
     const int lane = threadIdx.x & 63;
-    for (int b = wave; b < nb; b += NW) {
-        i32x4 w[M][2];
-        float sw[M];
+    for (int b0 = wave; b0 < nb; b0 += NW * U) {
+        i32x4 w[U][M][2];
+        float sw[U][M];
+        bf16x8 xv[U][NQ][4];
 #pragma unroll
-        for (int i = 0; i < M; i++) {
-            sw[i] = m[i].sw[b];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-                w[i][h] = *(const GAS i32x4 *)(m[i].w + (size_t)b * FP8_UNIT + h * 1024 + lane * 16);
-        }
-        f32x4 p[M][NQ] = {};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            bf16x8 wv[M];
+        for (int u = 0; u < U; u++) {
+            const int b = b0 + u * NW < nb ? b0 + u * NW : nb - 1;   /* past the end: read again, not added */
 #pragma unroll
             for (int i = 0; i < M; i++) {
-                const i32x4 c = w[i][j >> 1];
-                wv[i] = (j & 1) ? fp8_to_bf16(c[2], c[3]) : fp8_to_bf16(c[0], c[1]);
+                sw[u][i] = m[i].sw[b];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    w[u][i][h] = *(const GAS i32x4 *)(m[i].w + (size_t)b * FP8_UNIT + h * 1024 + lane * 16);
             }
 #pragma unroll
-            for (int q = 0; q < NQ; q++) {
-                const bf16x8 xv = *(const GAS bf16x8 *)(x[q] + b * FP8_BLOCK + 64 * (j >> 1) + 8 * (j & 1));
+            for (int q = 0; q < NQ; q++)
 #pragma unroll
-                for (int i = 0; i < M; i++)
-                    p[i][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[i], xv, p[i][q], 0, 0, 0);
-            }
+                for (int j = 0; j < 4; j++)
+                    xv[u][q][j] = *(const GAS bf16x8 *)(x[q] + b * FP8_BLOCK + 64 * (j >> 1) + 8 * (j & 1));
         }
 #pragma unroll
-        for (int q = 0; q < NQ; q++)
+        for (int u = 0; u < U; u++) {
+            const bool on = u == 0 || b0 + u * NW < nb;
+            f32x4 p[M][NQ] = {};
 #pragma unroll
-            for (int i = 0; i < M; i++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-                for (int v = 0; v < 4; v++) acc[i][q][v] = fmaf(p[i][q][v], sw[i], acc[i][q][v]);
+                for (int i = 0; i < M; i++) {
+                    const i32x4 c = w[u][i][j >> 1];
+                    const bf16x8 wv = (j & 1) ? fp8_to_bf16(c[2], c[3]) : fp8_to_bf16(c[0], c[1]);
+#pragma unroll
+                    for (int q = 0; q < NQ; q++)
+                        p[i][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[u][q][j], p[i][q], 0, 0, 0);
+                }
+#pragma unroll
+            for (int q = 0; q < NQ; q++)
+#pragma unroll
+                for (int i = 0; i < M; i++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const float t = fmaf(p[i][q][v], sw[u][i], acc[i][q][v]);
+                        acc[i][q][v] = on ? t : acc[i][q][v];
+                    }
+        }
     }
 }
 template <int M>
-__device__ __forceinline__ void run_blocks(const Mat (&m)[M], int nb, int wave, const uint16_t *const (&x)[NT], int nt,
-                                           f32x4 (&acc)[M][NT]) {
+__device__ __forceinline__ void run_blocks(const Mat (&m)[M], int nb, int wave, const GAS uint16_t *const (&x)[NT],
+                                           int nt, f32x4 (&acc)[M][NT]) {
     switch (nt) {
-    case 1: run_tiles<M, 1>(m, nb, wave, x, acc); break;
-    case 2: run_tiles<M, 2>(m, nb, wave, x, acc); break;
-    case 3: run_tiles<M, 3>(m, nb, wave, x, acc); break;
-    default: run_tiles<M, 4>(m, nb, wave, x, acc); break;
+    case 1: run_tiles<M, 1, 4 / M>(m, nb, wave, x, acc); break;
+    case 2: run_tiles<M, 2, 2 / M>(m, nb, wave, x, acc); break;
+    case 3: run_tiles<M, 3, 1>(m, nb, wave, x, acc); break;
+    default: run_tiles<M, 4, 1>(m, nb, wave, x, acc); break;
     }
 }
 
@@ -295,10 +415,9 @@ __device__ __forceinline__ int column_index(int i0, int q, int n) {
 __device__ __forceinline__ int column_plane() { return (threadIdx.x & 15) % 3; }
 
 /* ---- K2 ----------------------------------------------------------------------- */
+template <bool ONE>
 __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
     __shared__ List s;
-    __shared__ uint8_t s_sel[MAXT];
-    __shared__ int s_e;
     __shared__ Sums s_g, s_u;
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -307,7 +426,27 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
     const int64_t rows = shared ? d.ds : d.de;
     const int nbo = shared ? a.L.nbs : a.L.nbe;      /* blocks of the width that this launch makes */
     if (tile >= nbo * 8) return;
-    const int e = uniform(slot_list(a, slot, &s, s_sel, &s_e));
+    int e;
+    if constexpr (ONE) {   /* one token: every group routes it, the first one for all to read */
+        Route *R = (Route *)&s_g;
+        const int rank = rank_of(a, 0, R, tid);
+        if (tile == 0 && slot == 0) {
+            route_token(a, 0, R, rank);
+            __syncthreads();
+        }
+        if (tid == 0) {
+            s.n = 1;
+            s.e = shared ? d.E : -1;
+            s.tok[0] = 0;
+            s.rank[0] = (uint8_t)(shared ? 0 : slot);
+        }
+        __syncthreads();
+        if (!shared && rank == slot) s.e = tid;
+        __syncthreads();
+        e = uniform(s.e);
+    } else {
+        e = uniform(slot_list(a, slot, &s));
+    }
     if (e < 0) return;
     const int n = uniform(s.n);
     uint16_t *hid = (uint16_t *)(a.ws + (shared ? a.L.shid : a.L.hid));
@@ -319,12 +458,12 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
         m[0] = mat_of(shared ? d.sg : tab[0], tile, rows, a.L.nbd);
         m[1] = mat_of(shared ? d.su : tab[1], tile, rows, a.L.nbd);
     }
-    const uint16_t *xp = (const uint16_t *)(a.ws + a.L.xp);
+    const GAS uint16_t *xp = (const GAS uint16_t *)(a.ws + a.L.xp);
     const int Dp = a.L.nbd * FP8_BLOCK;
     for (int i0 = 0; i0 < n; i0 += NT * TPT) {
         const int left = n - i0 < NT * TPT ? n - i0 : NT * TPT;
         if (!pad) {
-            const uint16_t *x[NT];
+            const GAS uint16_t *x[NT];
 #pragma unroll
             for (int q = 0; q < NT; q++)
                 x[q] = xp + ((size_t)s.tok[column_index(i0, q, n)] * 3 + column_plane()) * Dp + 16 * (lane >> 4);
@@ -356,22 +495,20 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
 /* ---- K3 ----------------------------------------------------------------------- */
 __global__ __launch_bounds__(256) void k_fm_down(Args a) {
     __shared__ List s;
-    __shared__ uint8_t s_sel[MAXT];
-    __shared__ int s_e;
     __shared__ Sums s_y;
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int tile = blockIdx.x, slot = blockIdx.y;
     const bool shared = slot == a.slots;
-    const int e = uniform(slot_list(a, slot, &s, s_sel, &s_e));
+    const int e = uniform(slot_list(a, slot, &s));
     if (e < 0) return;
     const int n = uniform(s.n), nb = shared ? a.L.nbs : a.L.nbe, wi = nb * FP8_BLOCK;
-    const uint16_t *hid = (const uint16_t *)(a.ws + (shared ? a.L.shid : a.L.hid));
+    const GAS uint16_t *hid = (const GAS uint16_t *)(a.ws + (shared ? a.L.shid : a.L.hid));
     float *eo = (float *)(a.ws + (shared ? a.L.seo : a.L.eo));
     const Mat m[1] = {mat_of(shared ? d.sd : d.experts[3 * (size_t)e + 2], tile, d.D, nb)};
     for (int i0 = 0; i0 < n; i0 += NT * TPT) {
         const int left = n - i0 < NT * TPT ? n - i0 : NT * TPT;
-        const uint16_t *x[NT];
+        const GAS uint16_t *x[NT];
 #pragma unroll
         for (int q = 0; q < NT; q++) {
             const int i = column_index(i0, q, n), t = s.tok[i];
@@ -391,84 +528,106 @@ __global__ __launch_bounds__(256) void k_fm_down(Args a) {
     }
 }
 
-/* ---- K4 ----------------------------------------------------------------------- */
-/* A token's experts and weights in rank order: ranks past the number of experts that
- * can be chosen get id -1 and weight 0.  All threads; ends in a barrier. */
-struct Route {
-    int ids[MAXK];
-    float w[MAXK];
-    float redf[NW];
-    double red[NW];
-};
-__device__ void route_token(const Args &a, int t, Route *R) {
+/* ---- K3 for few tokens: down and the sum ------------------------------------------
+ * A group takes 16 rows of one token's result: the blocks of all its experts' down rows, and of
+ * the shared expert's, are dealt to 8 waves, each scaled by its expert's weight as it is added.  A
+ * matrix that two tokens share is read by both. */
+constexpr int DW = 8;
+constexpr int FEW = 8;
+template <int U>
+__global__ __launch_bounds__(64 * DW) void k_fm_down_few(Args a) {
+    __shared__ f32x4 s_sum[DW][64];
+    __shared__ const uint8_t *s_ptr[MAXK + 1];
+    __shared__ float s_w[MAXK + 1];
     const tlm_hip_moe_desc &d = a.d;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = d.E, k = d.k;
-    const uint32_t *key = (const uint32_t *)(a.ws + a.L.key) + (size_t)t * E;
-    const bool in = tid < E;
-    const uint32_t ke = in ? key[tid] : 0u;
-    const float l = in ? ((const float *)(a.ws + a.L.score))[t * E + tid] : 0.0f;
-    if (tid < MAXK) {
-        R->ids[tid] = -1;
-        R->w[tid] = 0.0f;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4;
+    const int tile = blockIdx.x, t = blockIdx.y, k = d.k, nbe = a.L.nbe, nbs = a.L.nbs;
+    if (tid < k) {
+        s_ptr[tid] = ((const uint8_t *const GAS *)(a.ws + a.L.dptr))[t * k + tid];
+        s_w[tid] = ((const GAS float *)(a.ws + a.L.w))[t * k + tid];
     }
-    float p = l;
-    if (d.router != 2) {   /* softmax over the experts that can be chosen */
-        const bool on = ke && l == l;
-        const float m = wave_max_f32(on ? l : -INFINITY);
-        if (lane == 0) R->redf[wave] = m;
-        __syncthreads();
-        float mx = R->redf[0];
-        for (int q = 1; q < NW; q++) mx = R->redf[q] > mx ? R->redf[q] : mx;
-        const float x = on && mx > -INFINITY ? expf_ref(l - mx) : 0.0f;
-        const double sum = wave_sum_f64((double)x);
-        if (lane == 0) R->red[wave] = sum;
-        __syncthreads();
-        const double st = (R->red[0] + R->red[1]) + (R->red[2] + R->red[3]);
-        p = st > 0.0 ? (float)((double)x / st) : 0.0f;
-    }
-    int rank = 0;
-    for (int f = 0; f < E; f++) {
-        const uint32_t kf = key[f];
-        rank += kf && ahead(kf, f, ke, tid) ? 1 : 0;
+    if (tid == k && nbs) {
+        s_ptr[k] = (const uint8_t *)d.sd;
+        s_w[k] = d.shared_gate_inp ? ((const GAS float *)(a.ws + a.L.sgate))[t] : 1.0f;
     }
     __syncthreads();
-    if (ke && rank < k) {
-        R->ids[rank] = tid;
-        R->w[rank] = p;
-    }
-    __syncthreads();
-    if (wave == 0) {   /* renormalise over the chosen, then scale */
-        float wr = lane < k ? R->w[lane] : 0.0f;
-        if (d.router != 1) {
-            double s = 0.0;
-            for (int r = 0; r < k; r++) s += (double)rdlane_f32(wr, r);
-            if (d.router == 2) s += 1e-20;
-            if (s > 0.0) wr = (float)((double)wr / s);
+    const int units = k * nbe + nbs, plane = (lane & 15) % 3;
+    const size_t code_e = (size_t)fp8_tiles(d.D) * nbe * FP8_UNIT, code_s = (size_t)fp8_tiles(d.D) * nbs * FP8_UNIT;
+    const GAS uint16_t *hid = (const GAS uint16_t *)(a.ws + a.L.hid) + ((size_t)t * k * 3 + plane) * nbe * FP8_BLOCK + 16 * g;
+    const GAS uint16_t *shid = (const GAS uint16_t *)(a.ws + a.L.shid) + ((size_t)t * 3 + plane) * nbs * FP8_BLOCK + 16 * g;
+    f32x4 acc = {0, 0, 0, 0};
+    for (int u0 = wave; u0 < units; u0 += DW * U) {
+        i32x4 w[U][2];
+        bf16x8 x[U][4];
+        float sc[U];
+        bool on[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int v = u0 + u * DW < units ? u0 + u * DW : u0;   /* past the end: read again, not added */
+            const int r = v < k * nbe ? v / nbe : k, nb = r < k ? nbe : nbs, b = v - r * nbe;
+            const GAS uint8_t *p = (const GAS uint8_t *)s_ptr[r];
+            on[u] = u0 + u * DW < units && p != nullptr;   /* a rank without an expert adds nothing: */
+            const GAS uint8_t *q = (const GAS uint8_t *)a.ws, *z = q;   /* the workspace (over 2 KB) is read for it */
+            if (p) {
+                q = p + ((size_t)tile * nb + b) * FP8_UNIT;
+                z = p + (r < k ? code_e : code_s) + 4 * (tile / 8 * nb + b);
+            }
+            w[u][0] = *(const GAS i32x4 *)(q + lane * 16);
+            w[u][1] = *(const GAS i32x4 *)(q + lane * 16 + 1024);
+            sc[u] = s_w[r] * *(const GAS float *)z;
+            const GAS uint16_t *xx = (r < k ? hid + (size_t)r * 3 * nbe * FP8_BLOCK : shid) + b * FP8_BLOCK;
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[u][j] = *(const GAS bf16x8 *)(xx + 64 * (j >> 1) + 8 * (j & 1));
         }
-        wr *= d.routed_scale;
-        if (lane < k) R->w[lane] = wr;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            f32x4 p = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const i32x4 c = w[u][j >> 1];
+                const bf16x8 wv = (j & 1) ? fp8_to_bf16(c[2], c[3]) : fp8_to_bf16(c[0], c[1]);
+                p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, x[u][j], p, 0, 0, 0);
+            }
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const float f = fmaf(p[v], sc[u], acc[v]);
+                acc[v] = on[u] ? f : acc[v];
+            }
+        }
     }
+    s_sum[wave][lane] = acc;
     __syncthreads();
+    const int64_t i = (int64_t)tile * 16 + tid;
+    if (tid >= 16 || i >= d.D) return;
+    float p[3];
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < DW; q++) v += s_sum[q][(tid >> 2) * 16 + j][tid & 3];
+        p[j] = v;
+    }
+    const size_t at = (size_t)t * d.D + i;
+    a.out[at] = a.h[at] + (p[0] + (p[1] + p[2]));
 }
 
+/* ---- K4 ----------------------------------------------------------------------- */
 __global__ __launch_bounds__(256) void k_fm_combine(Args a) {
-    __shared__ Route R;
     const tlm_hip_moe_desc &d = a.d;
     const int t = blockIdx.y;
-    route_token(a, t, &R);
-    if (blockIdx.x == 0 && (int)threadIdx.x < d.k) {
-        if (a.ids) a.ids[t * d.k + threadIdx.x] = R.ids[threadIdx.x];
-        if (a.w) a.w[t * d.k + threadIdx.x] = R.w[threadIdx.x];
-    }
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= d.D) return;
-    const float *eo = (const float *)(a.ws + a.L.eo) + (size_t)t * d.k * d.D + i;
+    const GAS float *eo = (const GAS float *)(a.ws + a.L.eo) + (size_t)t * d.k * d.D + i;
+    const GAS int32_t *ids = (const GAS int32_t *)(a.ws + a.L.ids) + t * d.k;
+    const GAS float *w = (const GAS float *)(a.ws + a.L.w) + t * d.k;
     float acc = 0.0f;
-    for (int r = 0; r < d.k; r++)
-        if (R.ids[r] >= 0) acc += R.w[r] * eo[(size_t)r * d.D];
+    for (int r = 0; r < d.k; r++) {
+        const float v = eo[(size_t)r * d.D];
+        acc = ids[r] >= 0 ? acc + w[r] * v : acc;   /* a rank without an expert has no result */
+    }
     if (d.ds > 0) {
-        const float g = d.shared_gate_inp ? ((const float *)(a.ws + a.L.sgate))[t] : 1.0f;
-        acc += g * ((const float *)(a.ws + a.L.seo))[(size_t)t * d.D + i];
+        const float g = d.shared_gate_inp ? ((const GAS float *)(a.ws + a.L.sgate))[t] : 1.0f;
+        acc += g * ((const GAS float *)(a.ws + a.L.seo))[(size_t)t * d.D + i];
     }
     a.out[(size_t)t * d.D + i] = a.h[(size_t)t * d.D + i] + acc;
 }
@@ -519,16 +678,28 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     a.w = w;
     a.ws = (uint8_t *)workspace;
     a.T = (int)T;
-    a.by_expert = T * d->k >= d->E;
+    a.by_expert = T > 1 && T * d->k >= d->E;
     a.slots = a.by_expert ? d->E : (int)(T * d->k);
     const unsigned ny = (unsigned)(a.slots + (d->ds > 0 ? 1 : 0));
     const int wide = a.L.nbe > a.L.nbs ? a.L.nbe : a.L.nbs;
     hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(k_fm_router, dim3((unsigned)((d->E + ROUTER_EXPERTS - 1) / ROUTER_EXPERTS), (unsigned)T),
-                       dim3(256), (size_t)d->D * 4, s, a);
-    hipLaunchKernelGGL(k_fm_gateup, dim3((unsigned)wide * 8, ny), dim3(64 * NW), 0, s, a);
-    hipLaunchKernelGGL(k_fm_down, dim3((unsigned)fp8_tiles(d->D), ny), dim3(64 * NW), 0, s, a);
-    hipLaunchKernelGGL(k_fm_combine, dim3((unsigned)((d->D + 255) / 256), (unsigned)T), dim3(256), 0, s, a);
+    const int tg = d->D > 8192 ? 1 : d->D > 4096 ? 2 : ROUTER_TOKENS;   /* at most 64 KB of x in LDS */
+    const unsigned rows = (unsigned)(d->E + (d->ds > 0 && d->shared_gate_inp ? 1 : 0));
+    hipLaunchKernelGGL(k_fm_router, dim3((rows + 3) / 4, (unsigned)((T + tg - 1) / tg)), dim3(256),
+                       (size_t)(T < tg ? T : tg) * ((d->D + 3) & ~(int64_t)3) * 4, s, a, tg);
+    if (T == 1) {
+        hipLaunchKernelGGL(k_fm_gateup<true>, dim3((unsigned)wide * 8, ny), dim3(64 * NW), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(k_fm_route, dim3((unsigned)T), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(k_fm_gateup<false>, dim3((unsigned)wide * 8, ny), dim3(64 * NW), 0, s, a);
+    }
+    if (T <= FEW) {
+        const dim3 grid((unsigned)fp8_tiles(d->D), (unsigned)T);
+        hipLaunchKernelGGL(k_fm_down_few<3>, grid, dim3(64 * DW), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(k_fm_down, dim3((unsigned)fp8_tiles(d->D), ny), dim3(64 * NW), 0, s, a);
+        hipLaunchKernelGGL(k_fm_combine, dim3((unsigned)((d->D + 255) / 256), (unsigned)T), dim3(256), 0, s, a);
+    }
     return tlmh_check(hipGetLastError(), "fp8_moe launch");
 }
 
