@@ -26,7 +26,7 @@ constexpr int MAXT = TLM_HIP_FP8_MOE_MAX_TOKENS;   /* 64: a token per lane in th
 constexpr int MAXE = 256, MAXK = 32;
 constexpr int NW = 4;              /* waves per group of K2 and K3: the blocks of a row are dealt to them */
 constexpr int TPT = 5;             /* tokens per 16 columns */
-constexpr int NT = 4;              /* column tiles at a time */
+constexpr int GT = 4, DT = 2;      /* column tiles at a time: gate/up, down */
 
 __host__ __device__ inline size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -109,48 +109,74 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a, int tg) {
     const int e = blockIdx.x * 4 + wave;
     const bool live = e < d.E || (e == d.E && d.ds > 0 && d.shared_gate_inp);
     const GAS float *w = (const GAS float *)(live && e == d.E ? d.shared_gate_inp : d.router_w + (size_t)(live ? e : 0) * D);
+    const GAS float *h = (const GAS float *)a.h + (size_t)t0 * D, *nw = (const GAS float *)d.ffn_norm;
+    /* the tokens and the norm weights first: they are waited for first */
+    constexpr int NC = 4;   /* runs of 1024 values held in registers; a longer row's others are read again */
+    f32x4 hv[NC][ROUTER_TOKENS], gv[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int i = 4 * tid + 1024 * c;
+        if (1024 * c < D) {
+#pragma unroll
+            for (int t = 0; t < ROUTER_TOKENS; t++)
+                if (t < nt) hv[c][t] = row4(h + (size_t)t * D, i, D);
+            gv[c] = row4(nw, i, D);
+        }
+    }
     constexpr int NV = 8;
     f32x4 wv[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) wv[j] = row4(w, 4 * lane + 256 * j, D);
-    const GAS float *h = (const GAS float *)a.h + (size_t)t0 * D, *nw = (const GAS float *)d.ffn_norm;
-    for (int t = 0; t < nt; t++) {
-        double ss = 0.0;
-        for (int i = 4 * tid; i < Dq; i += 1024) {
-            const f32x4 v = row4(h + (size_t)t * D, i, D);
-            *(f32x4 *)(s_x + t * Dq + i) = v;
+    double ss[ROUTER_TOKENS] = {};
 #pragma unroll
-            for (int q = 0; q < 4; q++) ss += (double)v[q] * (double)v[q];
+    for (int c = 0; c < NC; c++)
+        if (1024 * c < D)
+#pragma unroll
+            for (int t = 0; t < ROUTER_TOKENS; t++)
+                if (t < nt)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) ss[t] += (double)hv[c][t][q] * (double)hv[c][t][q];
+    for (int i = 4 * tid + 1024 * NC; i < Dq; i += 1024)
+        for (int t = 0; t < nt; t++) {
+            const f32x4 v = row4(h + (size_t)t * D, i, D);
+#pragma unroll
+            for (int q = 0; q < 4; q++) ss[t] += (double)v[q] * (double)v[q];
         }
-        ss = wave_sum_f64(ss);
-        if (lane == 0) s_red[wave][t] = ss;
-    }
+#pragma unroll
+    for (int t = 0; t < ROUTER_TOKENS; t++)
+        if (t < nt) {
+            const double v = wave_sum_f64(ss[t]);
+            if (lane == 0) s_red[wave][t] = v;
+        }
     __syncthreads();
     const int Dp = a.L.nbd * FP8_BLOCK;
-    for (int t = 0; t < nt; t++) {
-        const double ss = (s_red[0][t] + s_red[1][t]) + (s_red[2][t] + s_red[3][t]);
-        const float rn = 1.0f / sqrtf((float)(ss / (double)D) + d.eps);
+    auto put = [&](int i, int t, f32x4 v) {
+        if (i < Dq) *(f32x4 *)(s_x + t * Dq + i) = v;
+        if ((i >> 8) % gridDim.x != blockIdx.x) return;   /* the groups share the planes' writing */
         uint16_t *xp = (uint16_t *)(a.ws + a.L.xp) + (size_t)(t0 + t) * 3 * Dp;
-        for (int i = 4 * tid; i < Dp; i += 1024) {
-            f32x4 v = {0, 0, 0, 0};
-            if (i < Dq) {
-                const f32x4 g = row4(nw, i, D);
-                v = *(const f32x4 *)(s_x + t * Dq + i) * rn * g;
-                *(f32x4 *)(s_x + t * Dq + i) = v;
-            }
-            if ((i >> 8) % gridDim.x == blockIdx.x) {   /* the groups share the planes' writing */
-                u16x4 o[3];
+        u16x4 o[3];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint16_t p[3];
-                    split3(v[q], p);
+        for (int q = 0; q < 4; q++) {
+            uint16_t p[3];
+            split3(v[q], p);
 #pragma unroll
-                    for (int j = 0; j < 3; j++) o[j][q] = p[j];
-                }
-#pragma unroll
-                for (int j = 0; j < 3; j++) *(u16x4 *)(xp + j * Dp + i) = o[j];
-            }
+            for (int j = 0; j < 3; j++) o[j][q] = p[j];
         }
+#pragma unroll
+        for (int j = 0; j < 3; j++) *(u16x4 *)(xp + j * Dp + i) = o[j];
+    };
+#pragma unroll
+    for (int t = 0; t < ROUTER_TOKENS; t++) {
+        if (t >= nt) break;
+        const double sum = (s_red[0][t] + s_red[1][t]) + (s_red[2][t] + s_red[3][t]);
+        const float rn = 1.0f / sqrtf((float)(sum / (double)D) + d.eps);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const int i = 4 * tid + 1024 * c;
+            if (1024 * c < D && i < Dp) put(i, t, hv[c][t] * rn * gv[c]);   /* zeros behind D */
+        }
+        for (int i = 4 * tid + 1024 * NC; i < Dp; i += 1024)
+            put(i, t, row4(h + (size_t)t * D, i, D) * rn * row4(nw, i, D));
     }
     __syncthreads();
     if (!live) return;
@@ -203,54 +229,72 @@ struct Route {
     uint32_t key[MAXE];
     int ids[MAXK];
     float w[MAXK];
-    float redf[4];
-    double red[4];
+    const void *down[MAXK];
+    float redf[8];
+    double red[8];
 };
-/* Token t's rank of expert `tid` (MAXE where it cannot be chosen), from keys brought to LDS.  Ends in
- * a barrier. */
-__device__ __forceinline__ int rank_of(const Args &a, int t, Route *R, int tid) {
-    const int E = a.d.E;
-    if (tid < MAXE) R->key[tid] = tid < E ? ((const GAS uint32_t *)(a.ws + a.L.key))[(size_t)t * E + tid] : 0u;
+/* What thread e holds of its expert for one token: everything that routing reads, asked for at once. */
+struct Choice {
+    uint32_t key;
+    float score;
+    const void *gate, *up, *down;
+};
+__device__ __forceinline__ Choice choice_of(const Args &a, int t, int tid) {
+    const bool in = tid < a.d.E;
+    const int e = in ? tid : 0;
+    const size_t at = (size_t)t * a.d.E + e;
+    Choice c;
+    c.key = ((const GAS uint32_t *)(a.ws + a.L.key))[at];
+    c.score = ((const GAS float *)(a.ws + a.L.score))[at];
+    const void *const GAS *tab = (const void *const GAS *)a.d.experts + 3 * (size_t)e;
+    c.gate = tab[0];
+    c.up = tab[1];
+    c.down = tab[2];
+    if (!in) c.key = 0u;
+    return c;
+}
+/* The rank of thread tid's expert (MAXE where it cannot be chosen).  All threads of the group, 256 or more. */
+__device__ __forceinline__ int rank_of(const Args &a, const Choice &c, Route *R, int tid) {
+    if (tid < MAXE) R->key[tid] = c.key;
     if (tid < MAXK) {
         R->ids[tid] = -1;
         R->w[tid] = 0.0f;
+        R->down[tid] = nullptr;
     }
     __syncthreads();
-    if (tid >= E || R->key[tid] == 0u) return MAXE;
-    const uint32_t ke = R->key[tid];
-    int c[4] = {0, 0, 0, 0};
-    for (int f = 0; f < E; f += 4) {   /* keys past E are 0, never ahead */
+    int n[4] = {0, 0, 0, 0};
+    for (int f = 0; f < a.d.E; f += 4) {   /* keys past E are 0, never ahead of one that can be chosen */
         const u32x4 k = *(const LAS u32x4 *)&R->key[f];
 #pragma unroll
-        for (int q = 0; q < 4; q++) c[q] += ahead(k[q], f + q, ke, tid) ? 1 : 0;
+        for (int q = 0; q < 4; q++) n[q] += ahead(k[q], f + q, c.key, tid) ? 1 : 0;
     }
-    return (c[0] + c[1]) + (c[2] + c[3]);
+    return c.key ? (n[0] + n[1]) + (n[2] + n[3]) : MAXE;
 }
 /* A token's experts and weights in rank order into the workspace and the caller's arrays: ranks past the
- * number of experts that can be chosen get id -1 and weight 0.  All threads of a group of 256. */
-__device__ void route_token(const Args &a, int t, Route *R, int rank) {
+ * number of experts that can be chosen get id -1 and weight 0.  All threads of a group of WV waves. */
+template <int WV> __device__ void route_token(const Args &a, int t, const Choice &c, Route *R, int rank) {
     const tlm_hip_moe_desc &d = a.d;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = d.E, k = d.k;
-    const bool can = rank < MAXE;
-    const float l = tid < E ? ((const GAS float *)(a.ws + a.L.score))[(size_t)t * E + tid] : 0.0f;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = d.k;
+    const float l = c.score;
     float p = l;
     if (d.router != 2) {   /* softmax over the experts that can be chosen */
-        const bool on = can && l == l;
+        const bool on = c.key && l == l;
         const float m = wave_max_f32(on ? l : -INFINITY);
         if (lane == 0) R->redf[wave] = m;
         __syncthreads();
         float mx = R->redf[0];
-        for (int q = 1; q < 4; q++) mx = R->redf[q] > mx ? R->redf[q] : mx;
+        for (int q = 1; q < WV; q++) mx = R->redf[q] > mx ? R->redf[q] : mx;
         const float x = on && mx > -INFINITY ? expf_ref(l - mx) : 0.0f;
         const double sum = wave_sum_f64((double)x);
         if (lane == 0) R->red[wave] = sum;
         __syncthreads();
-        const double st = (R->red[0] + R->red[1]) + (R->red[2] + R->red[3]);
+        const double st = (R->red[0] + R->red[1]) + (R->red[2] + R->red[3]);   /* no expert is past 256 */
         p = st > 0.0 ? (float)((double)x / st) : 0.0f;
     }
     if (rank < k) {
         R->ids[rank] = tid;
         R->w[rank] = p;
+        R->down[rank] = c.down;
     }
     __syncthreads();
     if (wave == 0) {   /* renormalise over the chosen, then scale */
@@ -266,7 +310,7 @@ __device__ void route_token(const Args &a, int t, Route *R, int rank) {
             const int id = R->ids[lane], at = t * k + lane;
             ((int32_t *)(a.ws + a.L.ids))[at] = id;
             ((float *)(a.ws + a.L.w))[at] = wr;
-            ((const void **)(a.ws + a.L.dptr))[at] = id >= 0 ? d.experts[3 * (size_t)id + 2] : nullptr;
+            ((const void **)(a.ws + a.L.dptr))[at] = R->down[lane];
             if (a.ids) a.ids[at] = id;
             if (a.w) a.w[at] = wr;
         }
@@ -274,13 +318,14 @@ __device__ void route_token(const Args &a, int t, Route *R, int rank) {
 }
 __global__ __launch_bounds__(256) void k_fm_route(Args a) {
     __shared__ __align__(16) Route R;
-    const int rank = rank_of(a, blockIdx.x, &R, threadIdx.x);
-    route_token(a, blockIdx.x, &R, rank);
+    const Choice c = choice_of(a, blockIdx.x, threadIdx.x);
+    const int rank = rank_of(a, c, &R, threadIdx.x);
+    route_token<4>(a, blockIdx.x, c, &R, rank);
 }
 
 /* ---- an expert's tokens ------------------------------------------------------ */
 struct List {
-    int n, e;
+    int n, e, cnt[2][4];
     uint8_t tok[MAXT], rank[MAXT];
 };
 /* The pairs (token, rank) of slot `slot` and its expert: every token for the shared expert (E); expert
@@ -298,23 +343,40 @@ __device__ int slot_list(const Args &a, int slot, List *s) {
         __syncthreads();
         return a.d.E;
     }
+    /* thread tid looks at pairs tid, tid + 256, ...: the first 512 at once */
+    int id[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) id[j] = tid + 256 * j < pairs ? ids[tid + 256 * j] : -1;
     const int e = a.by_expert ? slot : uniform(ids[slot]);
     if (e < 0) return -1;
-    if (wave == 0) {
-        int n = 0;
-        for (int p0 = 0; p0 < pairs; p0 += 64) {
-            const int p = p0 + lane, id = p < pairs ? ids[p] : -1;
-            const unsigned long long m = __ballot(id == e);
-            if (id == e) {
-                const int at = n + __builtin_popcountll(m & ((1ull << lane) - 1));
+    int n = 0;
+    for (int p0 = 0; p0 < pairs; p0 += 512) {
+        if (p0 > 0)
+#pragma unroll
+            for (int j = 0; j < 2; j++) id[j] = p0 + tid + 256 * j < pairs ? ids[p0 + tid + 256 * j] : -1;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const unsigned long long m = __ballot(id[j] == e);
+            if (lane == 0) s->cnt[j][wave] = __builtin_popcountll(m);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            int at = n;
+            for (int q = 0; q < 4 * j + wave; q++) at += s->cnt[q >> 2][q & 3];
+            const unsigned long long m = __ballot(id[j] == e);
+            if (id[j] == e) {
+                const int p = p0 + tid + 256 * j;
+                at += __builtin_popcountll(m & ((1ull << lane) - 1));
                 s->tok[at] = (uint8_t)(p / k);
                 s->rank[at] = (uint8_t)(p % k);
                 if (at == 0) s->e = p;
             }
-            n += __builtin_popcountll(m);
         }
-        if (lane == 0) s->n = n;
+        for (int q = 0; q < 8; q++) n += s->cnt[q >> 2][q & 3];
+        __syncthreads();
     }
+    if (tid == 0) s->n = n;
     __syncthreads();
     if (s->n == 0 || (!a.by_expert && s->e != slot)) return -1;
     return e;
@@ -334,7 +396,7 @@ __device__ __forceinline__ Mat mat_of(const void *packed, int tile, int64_t rows
 /* This wave's share of the blocks, for NQ column tiles, U blocks in flight; x[q]: this lane's
  * column of planes.  No branch stands between a matrix instruction and the reads of its result: the
  * compiler here has left out the wait on such a path. */
-template <int M, int NQ, int U>
+template <int M, int NQ, int U, int NT>
 __device__ __forceinline__ void run_tiles(const Mat (&m)[M], int nb, int wave, const GAS uint16_t *const (&x)[NT],
                                           f32x4 (&acc)[M][NT]) {
     const int lane = threadIdx.x & 63;
@@ -384,20 +446,20 @@ __device__ __forceinline__ void run_tiles(const Mat (&m)[M], int nb, int wave, c
         }
     }
 }
-template <int M>
+template <int M, int NT>
 __device__ __forceinline__ void run_blocks(const Mat (&m)[M], int nb, int wave, const GAS uint16_t *const (&x)[NT],
                                            int nt, f32x4 (&acc)[M][NT]) {
-    switch (nt) {
-    case 1: run_tiles<M, 1, 4 / M>(m, nb, wave, x, acc); break;
-    case 2: run_tiles<M, 2, 2 / M>(m, nb, wave, x, acc); break;
-    case 3: run_tiles<M, 3, 1>(m, nb, wave, x, acc); break;
-    default: run_tiles<M, 4, 1>(m, nb, wave, x, acc); break;
+    if (nt == 1) run_tiles<M, 1, M == 2 ? 2 : 1, NT>(m, nb, wave, x, acc);
+    else if (nt == 2) run_tiles<M, 2, 1, NT>(m, nb, wave, x, acc);
+    else if constexpr (NT > 2) {
+        if (nt == 3) run_tiles<M, 3, 1, NT>(m, nb, wave, x, acc);
+        else run_tiles<M, 4, 1, NT>(m, nb, wave, x, acc);
     }
 }
 
-typedef f32x4 Sums[NW][NT][64];
+template <int NT> using Sums = f32x4[NW][NT][64];
 /* the waves' and planes' sums for row r of the tile and token i of the pass */
-__device__ __forceinline__ float total(const Sums &s, int r, int i) {
+template <int NT> __device__ __forceinline__ float total(const Sums<NT> &s, int r, int i) {
     const int q = i / TPT, l0 = (r >> 2) * 16 + 3 * (i % TPT), v = r & 3;
     float p[3];
 #pragma unroll
@@ -415,10 +477,112 @@ __device__ __forceinline__ int column_index(int i0, int q, int n) {
 __device__ __forceinline__ int column_plane() { return (threadIdx.x & 15) % 3; }
 
 /* ---- K2 ----------------------------------------------------------------------- */
-template <bool ONE>
+/* One token: every group routes it (all of its loads at once, then a count), so that nothing waits for
+ * a launch of its own; the last row of groups does it for the later launch and for the caller.
+ * 8 waves share the blocks of 16 rows of gate and up, two in flight each. */
+__global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
+    constexpr int W = 8, U = 2;
+    __shared__ __align__(16) Route R;
+    __shared__ const void *s_m[2];
+    __shared__ f32x4 s_g[W][64], s_u[W][64];
+    const tlm_hip_moe_desc &d = a.d;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int tile = blockIdx.x, slot = blockIdx.y;
+    const bool shared = slot == a.slots && d.ds > 0;
+    const int64_t rows = shared ? d.ds : d.de;
+    const int nbo = shared ? a.L.nbs : a.L.nbe;
+    if (tile >= nbo * 8) return;
+    if (!shared) {
+        const bool all = slot >= a.slots;   /* the row of groups that routes for the others; one is enough */
+        if (all && tile != 0) return;
+        const Choice c = choice_of(a, 0, tid);
+        const int rank = rank_of(a, c, &R, tid);
+        if (all) {
+            route_token<8>(a, 0, c, &R, rank);
+            return;
+        }
+        if (tid == 0) s_m[0] = nullptr;
+        __syncthreads();
+        if (rank == slot) {
+            s_m[0] = c.gate;
+            s_m[1] = c.up;
+        }
+        __syncthreads();
+        if (!s_m[0]) return;   /* fewer experts than ranks */
+    }
+    uint16_t *hid = (uint16_t *)(a.ws + (shared ? a.L.shid : a.L.hid));
+    const int wo = nbo * FP8_BLOCK, nb = a.L.nbd;
+    const bool pad = tile >= fp8_tiles(rows);
+    f32x4 acc[2] = {};
+    if (!pad) {
+        const Mat m[2] = {mat_of(shared ? d.sg : s_m[0], tile, rows, nb), mat_of(shared ? d.su : s_m[1], tile, rows, nb)};
+        const GAS uint16_t *x = (const GAS uint16_t *)(a.ws + a.L.xp) + (size_t)column_plane() * nb * FP8_BLOCK + 16 * (lane >> 4);
+        for (int b0 = wave; b0 < nb; b0 += W * U) {
+            i32x4 w[U][2][2];
+            float sw[U][2];
+            bf16x8 xv[U][4];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int b = b0 + u * W < nb ? b0 + u * W : nb - 1;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    sw[u][i] = m[i].sw[b];
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        w[u][i][h] = *(const GAS i32x4 *)(m[i].w + (size_t)b * FP8_UNIT + h * 1024 + lane * 16);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) xv[u][j] = *(const GAS bf16x8 *)(x + b * FP8_BLOCK + 64 * (j >> 1) + 8 * (j & 1));
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const bool on = u == 0 || b0 + u * W < nb;
+                f32x4 p[2] = {};
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const i32x4 c = w[u][i][j >> 1];
+                        p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16((j & 1) ? fp8_to_bf16(c[2], c[3]) : fp8_to_bf16(c[0], c[1]),
+                                                                       xv[u][j], p[i], 0, 0, 0);
+                    }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const float t = fmaf(p[i][v], sw[u][i], acc[i][v]);
+                        acc[i][v] = on ? t : acc[i][v];
+                    }
+            }
+        }
+    }
+    s_g[wave][lane] = acc[0];
+    s_u[wave][lane] = acc[1];
+    __syncthreads();
+    if (tid >= 16) return;
+    float g[3], u[3];
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+        const int l = (tid >> 2) * 16 + j;
+        g[j] = u[j] = 0.0f;
+#pragma unroll
+        for (int q = 0; q < W; q++) {
+            g[j] += s_g[q][l][tid & 3];
+            u[j] += s_u[q][l][tid & 3];
+        }
+    }
+    uint16_t p[3];
+    split3(silu(g[0] + (g[1] + g[2])) * (u[0] + (u[1] + u[2])), p);   /* 0 in the padding */
+    const size_t at = (size_t)(shared ? 0 : slot) * 3 * wo + tile * 16 + tid;
+#pragma unroll
+    for (int j = 0; j < 3; j++) hid[at + (size_t)j * wo] = p[j];
+}
+
+/* More tokens: 16 rows of one expert's gate and up for all of its tokens. */
 __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
     __shared__ List s;
-    __shared__ Sums s_g, s_u;
+    constexpr int NT = GT;
+    __shared__ Sums<NT> s_g, s_u;
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int tile = blockIdx.x, slot = blockIdx.y;
@@ -426,27 +590,7 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
     const int64_t rows = shared ? d.ds : d.de;
     const int nbo = shared ? a.L.nbs : a.L.nbe;      /* blocks of the width that this launch makes */
     if (tile >= nbo * 8) return;
-    int e;
-    if constexpr (ONE) {   /* one token: every group routes it, the first one for all to read */
-        Route *R = (Route *)&s_g;
-        const int rank = rank_of(a, 0, R, tid);
-        if (tile == 0 && slot == 0) {
-            route_token(a, 0, R, rank);
-            __syncthreads();
-        }
-        if (tid == 0) {
-            s.n = 1;
-            s.e = shared ? d.E : -1;
-            s.tok[0] = 0;
-            s.rank[0] = (uint8_t)(shared ? 0 : slot);
-        }
-        __syncthreads();
-        if (!shared && rank == slot) s.e = tid;
-        __syncthreads();
-        e = uniform(s.e);
-    } else {
-        e = uniform(slot_list(a, slot, &s));
-    }
+    const int e = uniform(slot_list(a, slot, &s));
     if (e < 0) return;
     const int n = uniform(s.n);
     uint16_t *hid = (uint16_t *)(a.ws + (shared ? a.L.shid : a.L.hid));
@@ -468,7 +612,7 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
             for (int q = 0; q < NT; q++)
                 x[q] = xp + ((size_t)s.tok[column_index(i0, q, n)] * 3 + column_plane()) * Dp + 16 * (lane >> 4);
             f32x4 acc[2][NT] = {};
-            run_blocks<2>(m, a.L.nbd, wave, x, (left + TPT - 1) / TPT, acc);
+            run_blocks<2, NT>(m, a.L.nbd, wave, x, (left + TPT - 1) / TPT, acc);
 #pragma unroll
             for (int q = 0; q < NT; q++) {
                 s_g[wave][q][lane] = acc[0][q];
@@ -479,7 +623,7 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
         for (int o = tid; o < left * 16; o += 256) {
             const int r = o & 15, i = o >> 4;
             float v = 0.0f;
-            if (!pad) v = silu(total(s_g, r, i)) * total(s_u, r, i);
+            if (!pad) v = silu(total<NT>(s_g, r, i)) * total<NT>(s_u, r, i);
             uint16_t p[3];
             split3(v, p);
             const int t = s.tok[i0 + i];
@@ -493,19 +637,25 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
 }
 
 /* ---- K3 ----------------------------------------------------------------------- */
+/* DM row tiles a group: the planes are read once for all of them. */
+constexpr int DM = 4;
 __global__ __launch_bounds__(256) void k_fm_down(Args a) {
     __shared__ List s;
-    __shared__ Sums s_y;
+    constexpr int NT = DT;
+    __shared__ Sums<NT> s_y;
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int tile = blockIdx.x, slot = blockIdx.y;
+    const int tile0 = blockIdx.x * DM, slot = blockIdx.y, tiles = (int)fp8_tiles(d.D);
     const bool shared = slot == a.slots;
     const int e = uniform(slot_list(a, slot, &s));
     if (e < 0) return;
     const int n = uniform(s.n), nb = shared ? a.L.nbs : a.L.nbe, wi = nb * FP8_BLOCK;
     const GAS uint16_t *hid = (const GAS uint16_t *)(a.ws + (shared ? a.L.shid : a.L.hid));
     float *eo = (float *)(a.ws + (shared ? a.L.seo : a.L.eo));
-    const Mat m[1] = {mat_of(shared ? d.sd : d.experts[3 * (size_t)e + 2], tile, d.D, nb)};
+    const void *packed = shared ? d.sd : d.experts[3 * (size_t)e + 2];
+    Mat m[DM];
+#pragma unroll
+    for (int i = 0; i < DM; i++) m[i] = mat_of(packed, tile0 + i < tiles ? tile0 + i : tiles - 1, d.D, nb);
     for (int i0 = 0; i0 < n; i0 += NT * TPT) {
         const int left = n - i0 < NT * TPT ? n - i0 : NT * TPT;
         const GAS uint16_t *x[NT];
@@ -514,17 +664,20 @@ __global__ __launch_bounds__(256) void k_fm_down(Args a) {
             const int i = column_index(i0, q, n), t = s.tok[i];
             x[q] = hid + ((size_t)(shared ? t : t * d.k + s.rank[i]) * 3 + column_plane()) * wi + 16 * (lane >> 4);
         }
-        f32x4 acc[1][NT] = {};
-        run_blocks<1>(m, nb, wave, x, (left + TPT - 1) / TPT, acc);
+        f32x4 acc[DM][NT] = {};
+        run_blocks<DM, NT>(m, nb, wave, x, (left + TPT - 1) / TPT, acc);
 #pragma unroll
-        for (int q = 0; q < NT; q++) s_y[wave][q][lane] = acc[0][q];
-        __syncthreads();
-        for (int o = tid; o < left * 16; o += 256) {
-            const int r = o & 15, i = o >> 4, t = s.tok[i0 + i];
-            if (tile * 16 + r < d.D)
-                eo[(size_t)(shared ? t : t * d.k + s.rank[i0 + i]) * d.D + tile * 16 + r] = total(s_y, r, i);
+        for (int j = 0; j < DM; j++) {
+#pragma unroll
+            for (int q = 0; q < NT; q++) s_y[wave][q][lane] = acc[j][q];
+            __syncthreads();
+            for (int o = tid; o < left * 16; o += 256) {
+                const int r = o & 15, i = o >> 4, t = s.tok[i0 + i];
+                const int64_t row = (int64_t)(tile0 + j) * 16 + r;
+                if (row < d.D) eo[(size_t)(shared ? t : t * d.k + s.rank[i0 + i]) * d.D + row] = total<NT>(s_y, r, i);
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -688,16 +841,16 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     hipLaunchKernelGGL(k_fm_router, dim3((rows + 3) / 4, (unsigned)((T + tg - 1) / tg)), dim3(256),
                        (size_t)(T < tg ? T : tg) * ((d->D + 3) & ~(int64_t)3) * 4, s, a, tg);
     if (T == 1) {
-        hipLaunchKernelGGL(k_fm_gateup<true>, dim3((unsigned)wide * 8, ny), dim3(64 * NW), 0, s, a);
+        hipLaunchKernelGGL(k_fm_gateup_one, dim3((unsigned)wide * 8, ny + 1), dim3(512), 0, s, a);
     } else {
         hipLaunchKernelGGL(k_fm_route, dim3((unsigned)T), dim3(256), 0, s, a);
-        hipLaunchKernelGGL(k_fm_gateup<false>, dim3((unsigned)wide * 8, ny), dim3(64 * NW), 0, s, a);
+        hipLaunchKernelGGL(k_fm_gateup, dim3((unsigned)wide * 8, ny), dim3(64 * NW), 0, s, a);
     }
     if (T <= FEW) {
         const dim3 grid((unsigned)fp8_tiles(d->D), (unsigned)T);
         hipLaunchKernelGGL(k_fm_down_few<3>, grid, dim3(64 * DW), 0, s, a);
     } else {
-        hipLaunchKernelGGL(k_fm_down, dim3((unsigned)fp8_tiles(d->D), ny), dim3(64 * NW), 0, s, a);
+        hipLaunchKernelGGL(k_fm_down, dim3((unsigned)((fp8_tiles(d->D) + DM - 1) / DM), ny), dim3(64 * NW), 0, s, a);
         hipLaunchKernelGGL(k_fm_combine, dim3((unsigned)((d->D + 255) / 256), (unsigned)T), dim3(256), 0, s, a);
     }
     return tlmh_check(hipGetLastError(), "fp8_moe launch");
