@@ -65,6 +65,7 @@ struct Args {
     float *w;
     uint8_t *ws;
     int T, slots, by_expert;
+    int ce, cs;   /* groups among which an expert's, and the shared expert's, tokens are dealt */
 };
 
 /* a value that all lanes of a wave share, in a scalar register: branches on it are the
@@ -80,11 +81,10 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 __device__ __forceinline__ float silu(float x) { return x / (1.0f + expf_ref(-x)); }
 
 /* ---- K1 ---------------------------------------------------------------------
- * A wave per router row (the shared expert's gate is one more), `tg` tokens of x in LDS: the
+ * A wave per router row (the shared expert's gate is one more), TG tokens of x in LDS: the
  * row's first 2048 values are on their way while the tokens are normalised.  Sums of four
  * products in float, those in double: two experts' scores keep their order down to the
  * last bits of a float. */
-constexpr int ROUTER_TOKENS = 4;
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 /* four values of a row of D at i, zeros behind its end */
@@ -100,25 +100,26 @@ __device__ __forceinline__ f32x4 row4(const GAS float *p, int i, int D) {
     return v;
 }
 
-__global__ __launch_bounds__(256) void k_fm_router(Args a, int tg) {
+template <int TG>
+__global__ __launch_bounds__(256) void k_fm_router(Args a) {
     extern __shared__ __align__(16) float s_x[];
-    __shared__ double s_red[4][ROUTER_TOKENS];
+    __shared__ double s_red[4][TG];
     const tlm_hip_moe_desc &d = a.d;
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), t0 = blockIdx.y * tg;
-    const int D = (int)d.D, Dq = (D + 3) & ~3, nt = a.T - t0 < tg ? a.T - t0 : tg;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), t0 = blockIdx.y * TG;
+    const int D = (int)d.D, Dq = (D + 3) & ~3, nt = TG == 1 || a.T - t0 >= TG ? TG : a.T - t0;
     const int e = blockIdx.x * 4 + wave;
     const bool live = e < d.E || (e == d.E && d.ds > 0 && d.shared_gate_inp);
     const GAS float *w = (const GAS float *)(live && e == d.E ? d.shared_gate_inp : d.router_w + (size_t)(live ? e : 0) * D);
     const GAS float *h = (const GAS float *)a.h + (size_t)t0 * D, *nw = (const GAS float *)d.ffn_norm;
     /* the tokens and the norm weights first: they are waited for first */
     constexpr int NC = 4;   /* runs of 1024 values held in registers; a longer row's others are read again */
-    f32x4 hv[NC][ROUTER_TOKENS], gv[NC];
+    f32x4 hv[NC][TG], gv[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
         const int i = 4 * tid + 1024 * c;
         if (1024 * c < D) {
 #pragma unroll
-            for (int t = 0; t < ROUTER_TOKENS; t++)
+            for (int t = 0; t < TG; t++)
                 if (t < nt) hv[c][t] = row4(h + (size_t)t * D, i, D);
             gv[c] = row4(nw, i, D);
         }
@@ -127,12 +128,12 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a, int tg) {
     f32x4 wv[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) wv[j] = row4(w, 4 * lane + 256 * j, D);
-    double ss[ROUTER_TOKENS] = {};
+    double ss[TG] = {};
 #pragma unroll
     for (int c = 0; c < NC; c++)
         if (1024 * c < D)
 #pragma unroll
-            for (int t = 0; t < ROUTER_TOKENS; t++)
+            for (int t = 0; t < TG; t++)
                 if (t < nt)
 #pragma unroll
                     for (int q = 0; q < 4; q++) ss[t] += (double)hv[c][t][q] * (double)hv[c][t][q];
@@ -143,16 +144,16 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a, int tg) {
             for (int q = 0; q < 4; q++) ss[t] += (double)v[q] * (double)v[q];
         }
 #pragma unroll
-    for (int t = 0; t < ROUTER_TOKENS; t++)
+    for (int t = 0; t < TG; t++)
         if (t < nt) {
             const double v = wave_sum_f64(ss[t]);
             if (lane == 0) s_red[wave][t] = v;
         }
     __syncthreads();
     const int Dp = a.L.nbd * FP8_BLOCK;
-    auto put = [&](int i, int t, f32x4 v) {
+    auto put = [&](int i, int t, f32x4 v, bool mine) {
         if (i < Dq) *(f32x4 *)(s_x + t * Dq + i) = v;
-        if ((i >> 8) % gridDim.x != blockIdx.x) return;   /* the groups share the planes' writing */
+        if (!mine) return;   /* the groups share the planes' writing */
         uint16_t *xp = (uint16_t *)(a.ws + a.L.xp) + (size_t)(t0 + t) * 3 * Dp;
         u16x4 o[3];
 #pragma unroll
@@ -165,22 +166,25 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a, int tg) {
 #pragma unroll
         for (int j = 0; j < 3; j++) *(u16x4 *)(xp + j * Dp + i) = o[j];
     };
+    bool mine[NC];
 #pragma unroll
-    for (int t = 0; t < ROUTER_TOKENS; t++) {
+    for (int c = 0; c < NC; c++) mine[c] = ((4 * tid + 1024 * c) >> 8) % gridDim.x == blockIdx.x;
+#pragma unroll
+    for (int t = 0; t < TG; t++) {
         if (t >= nt) break;
         const double sum = (s_red[0][t] + s_red[1][t]) + (s_red[2][t] + s_red[3][t]);
         const float rn = 1.0f / sqrtf((float)(sum / (double)D) + d.eps);
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             const int i = 4 * tid + 1024 * c;
-            if (1024 * c < D && i < Dp) put(i, t, hv[c][t] * rn * gv[c]);   /* zeros behind D */
+            if (1024 * c < D && i < Dp) put(i, t, hv[c][t] * rn * gv[c], mine[c]);   /* zeros behind D */
         }
         for (int i = 4 * tid + 1024 * NC; i < Dp; i += 1024)
-            put(i, t, row4(h + (size_t)t * D, i, D) * rn * row4(nw, i, D));
+            put(i, t, row4(h + (size_t)t * D, i, D) * rn * row4(nw, i, D), (i >> 8) % gridDim.x == blockIdx.x);
     }
     __syncthreads();
     if (!live) return;
-    double acc[ROUTER_TOKENS] = {};
+    double acc[TG] = {};
     for (int i0 = 0; i0 < Dq; i0 += 256 * NV) {
         if (i0 > 0)
 #pragma unroll
@@ -190,7 +194,7 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a, int tg) {
             const int i = i0 + 4 * lane + 256 * j;
             if (i >= Dq) continue;
 #pragma unroll
-            for (int t = 0; t < ROUTER_TOKENS; t++)
+            for (int t = 0; t < TG; t++)
                 if (t < nt) {
                     const f32x4 x = *(const f32x4 *)(s_x + t * Dq + i);
                     float p = wv[j][0] * x[0];
@@ -201,7 +205,7 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a, int tg) {
         }
     }
 #pragma unroll
-    for (int t = 0; t < ROUTER_TOKENS; t++) {
+    for (int t = 0; t < TG; t++) {
         if (t >= nt) break;
         const float l = (float)wave_sum_f64(acc[t]);
         if (lane != 0) continue;
@@ -263,6 +267,7 @@ __device__ __forceinline__ int rank_of(const Args &a, const Choice &c, Route *R,
     }
     __syncthreads();
     int n[4] = {0, 0, 0, 0};
+#pragma unroll 4
     for (int f = 0; f < a.d.E; f += 4) {   /* keys past E are 0, never ahead of one that can be chosen */
         const u32x4 k = *(const LAS u32x4 *)&R->key[f];
 #pragma unroll
@@ -328,6 +333,14 @@ struct List {
     int n, e, cnt[2][4];
     uint8_t tok[MAXT], rank[MAXT];
 };
+/* Which tokens of which slot a group takes: every `parts`th run from `part` on. */
+struct Part {
+    int slot, part, parts;
+};
+__device__ __forceinline__ Part part_of(const Args &a, int y) {
+    if (y >= a.slots * a.ce) return {a.slots, y - a.slots * a.ce, a.cs};
+    return {y / a.ce, y % a.ce, a.ce};
+}
 /* The pairs (token, rank) of slot `slot` and its expert: every token for the shared expert (E); expert
  * `slot`'s; or, with fewer choices than experts, those of the expert that pair `slot` chose, unless an
  * earlier pair chose it too (-1: nothing to do).  All threads; ends in a barrier. */
@@ -585,7 +598,8 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
     __shared__ Sums<NT> s_g, s_u;
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int tile = blockIdx.x, slot = blockIdx.y;
+    const Part pt = part_of(a, blockIdx.y);
+    const int tile = blockIdx.x, slot = pt.slot;
     const bool shared = slot == a.slots;
     const int64_t rows = shared ? d.ds : d.de;
     const int nbo = shared ? a.L.nbs : a.L.nbe;      /* blocks of the width that this launch makes */
@@ -604,7 +618,7 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
     }
     const GAS uint16_t *xp = (const GAS uint16_t *)(a.ws + a.L.xp);
     const int Dp = a.L.nbd * FP8_BLOCK;
-    for (int i0 = 0; i0 < n; i0 += NT * TPT) {
+    for (int i0 = pt.part * NT * TPT; i0 < n; i0 += pt.parts * NT * TPT) {
         const int left = n - i0 < NT * TPT ? n - i0 : NT * TPT;
         if (!pad) {
             const GAS uint16_t *x[NT];
@@ -645,7 +659,8 @@ __global__ __launch_bounds__(256) void k_fm_down(Args a) {
     __shared__ Sums<NT> s_y;
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int tile0 = blockIdx.x * DM, slot = blockIdx.y, tiles = (int)fp8_tiles(d.D);
+    const Part pt = part_of(a, blockIdx.y);
+    const int tile0 = blockIdx.x * DM, slot = pt.slot, tiles = (int)fp8_tiles(d.D);
     const bool shared = slot == a.slots;
     const int e = uniform(slot_list(a, slot, &s));
     if (e < 0) return;
@@ -656,7 +671,7 @@ __global__ __launch_bounds__(256) void k_fm_down(Args a) {
     Mat m[DM];
 #pragma unroll
     for (int i = 0; i < DM; i++) m[i] = mat_of(packed, tile0 + i < tiles ? tile0 + i : tiles - 1, d.D, nb);
-    for (int i0 = 0; i0 < n; i0 += NT * TPT) {
+    for (int i0 = pt.part * NT * TPT; i0 < n; i0 += pt.parts * NT * TPT) {
         const int left = n - i0 < NT * TPT ? n - i0 : NT * TPT;
         const GAS uint16_t *x[NT];
 #pragma unroll
@@ -785,6 +800,14 @@ __global__ __launch_bounds__(256) void k_fm_combine(Args a) {
     a.out[(size_t)t * d.D + i] = a.h[(size_t)t * d.D + i] + acc;
 }
 
+/* The shared expert's tokens go to as many groups as its runs of `run`; an expert's as well where the mean
+ * list is over half a run (else most of those groups would find nothing to do). */
+void spread(Args &a, int run) {
+    const int runs = (a.T + run - 1) / run;
+    a.cs = a.d.ds > 0 ? runs : 0;
+    a.ce = a.by_expert && 2 * a.T * a.d.k > run * a.d.E ? runs : 1;
+}
+
 int check(const tlm_hip_moe_desc *d, int64_t T) {
     if (!d) return tlmh_seterr(TLM_HIP_EINVAL, "fp8_moe: NULL descriptor");
     if (d->E <= 0 || d->E > MAXE || d->k <= 0 || d->k > MAXK || d->k > d->E)
@@ -836,21 +859,28 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     const unsigned ny = (unsigned)(a.slots + (d->ds > 0 ? 1 : 0));
     const int wide = a.L.nbe > a.L.nbs ? a.L.nbe : a.L.nbs;
     hipStream_t s = (hipStream_t)stream;
-    const int tg = d->D > 8192 ? 1 : d->D > 4096 ? 2 : ROUTER_TOKENS;   /* at most 64 KB of x in LDS */
     const unsigned rows = (unsigned)(d->E + (d->ds > 0 && d->shared_gate_inp ? 1 : 0));
-    hipLaunchKernelGGL(k_fm_router, dim3((rows + 3) / 4, (unsigned)((T + tg - 1) / tg)), dim3(256),
-                       (size_t)(T < tg ? T : tg) * ((d->D + 3) & ~(int64_t)3) * 4, s, a, tg);
+    const size_t xrow = (size_t)((d->D + 3) & ~(int64_t)3) * 4;
+    /* one token a group while that does not fill the chip; four share each router row's read beyond, if
+     * their x fits 64 KB of LDS */
+    if (T > 16 && d->D <= 4096)
+        hipLaunchKernelGGL(k_fm_router<4>, dim3((rows + 3) / 4, (unsigned)((T + 3) / 4)), dim3(256), 4 * xrow, s, a);
+    else
+        hipLaunchKernelGGL(k_fm_router<1>, dim3((rows + 3) / 4, (unsigned)T), dim3(256), xrow, s, a);
     if (T == 1) {
         hipLaunchKernelGGL(k_fm_gateup_one, dim3((unsigned)wide * 8, ny + 1), dim3(512), 0, s, a);
     } else {
         hipLaunchKernelGGL(k_fm_route, dim3((unsigned)T), dim3(256), 0, s, a);
-        hipLaunchKernelGGL(k_fm_gateup, dim3((unsigned)wide * 8, ny), dim3(64 * NW), 0, s, a);
+        spread(a, GT * TPT);
+        hipLaunchKernelGGL(k_fm_gateup, dim3((unsigned)wide * 8, (unsigned)(a.slots * a.ce + a.cs)), dim3(64 * NW), 0, s, a);
     }
     if (T <= FEW) {
         const dim3 grid((unsigned)fp8_tiles(d->D), (unsigned)T);
         hipLaunchKernelGGL(k_fm_down_few<3>, grid, dim3(64 * DW), 0, s, a);
     } else {
-        hipLaunchKernelGGL(k_fm_down, dim3((unsigned)((fp8_tiles(d->D) + DM - 1) / DM), ny), dim3(64 * NW), 0, s, a);
+        spread(a, DT * TPT);
+        hipLaunchKernelGGL(k_fm_down, dim3((unsigned)((fp8_tiles(d->D) + DM - 1) / DM), (unsigned)(a.slots * a.ce + a.cs)),
+                           dim3(64 * NW), 0, s, a);
         hipLaunchKernelGGL(k_fm_combine, dim3((unsigned)((d->D + 255) / 256), (unsigned)T), dim3(256), 0, s, a);
     }
     return tlmh_check(hipGetLastError(), "fp8_moe launch");
