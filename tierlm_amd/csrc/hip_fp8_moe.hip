@@ -78,11 +78,17 @@ __device__ __forceinline__ uint32_t order_key(float f) {
     const uint32_t b = __float_as_uint(f != f ? -INFINITY : f + 0.0f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float silu(float x) { return x / (1.0f + expf_ref(-x)); }
+/* with the exponential's table in the wave's lanes: every lane takes part */
+__device__ __forceinline__ float silu(float x, const ExpTabLanes &tab) { return x / (1.0f + expf_ref_with(-x, tab)); }
+
+/* Kernel arguments named here are fetched at once, not in turn where each is first used. */
+template <class T> __device__ __forceinline__ void arg_now(T v) { asm volatile("" ::"s"(v)); }
+template <class... T> __device__ __forceinline__ void args_now(T... v) { (arg_now(v), ...); }
 
 /* ---- K1 ---------------------------------------------------------------------
- * A wave per router row (the shared expert's gate is one more), TG tokens of x in LDS: the
- * row's first 2048 values are on their way while the tokens are normalised.  Sums of four
+ * A group per token and four router rows (the shared expert's gate is one more), x in LDS: the
+ * rows' first 2048 values are on their way while the token is normalised.  (Four tokens a group, the
+ * rows read once for them: 17.9 us for 64 tokens of 4096, longer than the rows' reads from L2.)  Sums of four
  * products in float, those in double: two experts' scores keep their order down to the
  * last bits of a float. */
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -100,61 +106,53 @@ __device__ __forceinline__ f32x4 row4(const GAS float *p, int i, int D) {
     return v;
 }
 
-template <int TG>
 __global__ __launch_bounds__(256) void k_fm_router(Args a) {
     extern __shared__ __align__(16) float s_x[];
-    __shared__ double s_red[4][TG];
+    __shared__ double s_red[4];
     const tlm_hip_moe_desc &d = a.d;
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), t0 = blockIdx.y * TG;
-    const int D = (int)d.D, Dq = (D + 3) & ~3, nt = TG == 1 || a.T - t0 >= TG ? TG : a.T - t0;
-    const int e = blockIdx.x * 4 + wave;
+    args_now(d.D, d.E, d.ds, d.router, d.eps, d.ffn_norm, d.router_w, d.router_bias, d.mask, d.shared_gate_inp, a.h, a.ws,
+             a.L.xp, a.L.key, a.L.score, a.L.sgate, a.L.nbd);
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), t = blockIdx.y;
+    const int D = (int)d.D, Dq = (D + 3) & ~3, e = blockIdx.x * 4 + wave;
     const bool live = e < d.E || (e == d.E && d.ds > 0 && d.shared_gate_inp);
     const GAS float *w = (const GAS float *)(live && e == d.E ? d.shared_gate_inp : d.router_w + (size_t)(live ? e : 0) * D);
-    const GAS float *h = (const GAS float *)a.h + (size_t)t0 * D, *nw = (const GAS float *)d.ffn_norm;
-    /* the tokens and the norm weights first: they are waited for first */
+    const GAS float *h = (const GAS float *)a.h + (size_t)t * D, *nw = (const GAS float *)d.ffn_norm;
+    /* the token and the norm weights first: they are waited for first */
     constexpr int NC = 4;   /* runs of 1024 values held in registers; a longer row's others are read again */
-    f32x4 hv[NC][TG], gv[NC];
+    f32x4 hv[NC], gv[NC];
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        const int i = 4 * tid + 1024 * c;
+    for (int c = 0; c < NC; c++)
         if (1024 * c < D) {
-#pragma unroll
-            for (int t = 0; t < TG; t++)
-                if (t < nt) hv[c][t] = row4(h + (size_t)t * D, i, D);
-            gv[c] = row4(nw, i, D);
+            hv[c] = row4(h, 4 * tid + 1024 * c, D);
+            gv[c] = row4(nw, 4 * tid + 1024 * c, D);
         }
-    }
     constexpr int NV = 8;
     f32x4 wv[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) wv[j] = row4(w, 4 * lane + 256 * j, D);
-    double ss[TG] = {};
+    ExpTabLanes tab;
+    tab.load();
+    double ss = 0.0;
 #pragma unroll
     for (int c = 0; c < NC; c++)
         if (1024 * c < D)
 #pragma unroll
-            for (int t = 0; t < TG; t++)
-                if (t < nt)
+            for (int q = 0; q < 4; q++) ss += (double)hv[c][q] * (double)hv[c][q];
+    for (int i = 4 * tid + 1024 * NC; i < Dq; i += 1024) {
+        const f32x4 v = row4(h, i, D);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) ss[t] += (double)hv[c][t][q] * (double)hv[c][t][q];
-    for (int i = 4 * tid + 1024 * NC; i < Dq; i += 1024)
-        for (int t = 0; t < nt; t++) {
-            const f32x4 v = row4(h + (size_t)t * D, i, D);
-#pragma unroll
-            for (int q = 0; q < 4; q++) ss[t] += (double)v[q] * (double)v[q];
-        }
-#pragma unroll
-    for (int t = 0; t < TG; t++)
-        if (t < nt) {
-            const double v = wave_sum_f64(ss[t]);
-            if (lane == 0) s_red[wave][t] = v;
-        }
+        for (int q = 0; q < 4; q++) ss += (double)v[q] * (double)v[q];
+    }
+    ss = wave_sum_f64(ss);
+    if (lane == 0) s_red[wave] = ss;
     __syncthreads();
+    ss = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
+    const float rn = 1.0f / sqrtf((float)(ss / (double)D) + d.eps);
     const int Dp = a.L.nbd * FP8_BLOCK;
-    auto put = [&](int i, int t, f32x4 v, bool mine) {
-        if (i < Dq) *(f32x4 *)(s_x + t * Dq + i) = v;
-        if (!mine) return;   /* the groups share the planes' writing */
-        uint16_t *xp = (uint16_t *)(a.ws + a.L.xp) + (size_t)(t0 + t) * 3 * Dp;
+    uint16_t *xp = (uint16_t *)(a.ws + a.L.xp) + (size_t)t * 3 * Dp;
+    auto put = [&](int i, f32x4 v) {
+        if (i < Dq) *(f32x4 *)(s_x + i) = v;
+        if ((i >> 8) % gridDim.x != blockIdx.x) return;   /* the groups share the planes' writing */
         u16x4 o[3];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
@@ -166,25 +164,15 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
 #pragma unroll
         for (int j = 0; j < 3; j++) *(u16x4 *)(xp + j * Dp + i) = o[j];
     };
-    bool mine[NC];
 #pragma unroll
-    for (int c = 0; c < NC; c++) mine[c] = ((4 * tid + 1024 * c) >> 8) % gridDim.x == blockIdx.x;
-#pragma unroll
-    for (int t = 0; t < TG; t++) {
-        if (t >= nt) break;
-        const double sum = (s_red[0][t] + s_red[1][t]) + (s_red[2][t] + s_red[3][t]);
-        const float rn = 1.0f / sqrtf((float)(sum / (double)D) + d.eps);
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const int i = 4 * tid + 1024 * c;
-            if (1024 * c < D && i < Dp) put(i, t, hv[c][t] * rn * gv[c], mine[c]);   /* zeros behind D */
-        }
-        for (int i = 4 * tid + 1024 * NC; i < Dp; i += 1024)
-            put(i, t, row4(h + (size_t)t * D, i, D) * rn * row4(nw, i, D), (i >> 8) % gridDim.x == blockIdx.x);
+    for (int c = 0; c < NC; c++) {
+        const int i = 4 * tid + 1024 * c;
+        if (1024 * c < D && i < Dp) put(i, hv[c] * rn * gv[c]);   /* zeros behind D */
     }
+    for (int i = 4 * tid + 1024 * NC; i < Dp; i += 1024) put(i, row4(h, i, D) * rn * row4(nw, i, D));
     __syncthreads();
     if (!live) return;
-    double acc[TG] = {};
+    double acc = 0.0;
     for (int i0 = 0; i0 < Dq; i0 += 256 * NV) {
         if (i0 > 0)
 #pragma unroll
@@ -193,34 +181,24 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
         for (int j = 0; j < NV; j++) {
             const int i = i0 + 4 * lane + 256 * j;
             if (i >= Dq) continue;
+            const f32x4 x = *(const f32x4 *)(s_x + i);
+            float p = wv[j][0] * x[0];
 #pragma unroll
-            for (int t = 0; t < TG; t++)
-                if (t < nt) {
-                    const f32x4 x = *(const f32x4 *)(s_x + t * Dq + i);
-                    float p = wv[j][0] * x[0];
-#pragma unroll
-                    for (int q = 1; q < 4; q++) p = fmaf(wv[j][q], x[q], p);
-                    acc[t] += (double)p;
-                }
+            for (int q = 1; q < 4; q++) p = fmaf(wv[j][q], x[q], p);
+            acc += (double)p;
         }
     }
-#pragma unroll
-    for (int t = 0; t < TG; t++) {
-        if (t >= nt) break;
-        const float l = (float)wave_sum_f64(acc[t]);
-        if (lane != 0) continue;
-        if (e == d.E) {
-            ((float *)(a.ws + a.L.sgate))[t0 + t] = 1.0f / (1.0f + expf_ref(-l));
-        } else {
-            float score = l, sel = l;
-            if (d.router == 2) {
-                score = 1.0f / (1.0f + expf_ref(-l));
-                sel = d.router_bias ? score + d.router_bias[e] : score;
-            }
-            ((float *)(a.ws + a.L.score))[(t0 + t) * d.E + e] = score;
-            ((uint32_t *)(a.ws + a.L.key))[(t0 + t) * d.E + e] = d.mask && d.mask[e] ? 0u : order_key(sel);
-        }
+    const float l = (float)wave_sum_f64(acc);   /* the same in every lane */
+    const float sig = 1.0f / (1.0f + expf_ref_with(-l, tab));
+    if (lane != 0) return;
+    if (e == d.E) {
+        ((float *)(a.ws + a.L.sgate))[t] = sig;
+        return;
     }
+    const float score = d.router == 2 ? sig : l;
+    const float sel = d.router == 2 && d.router_bias ? score + d.router_bias[e] : score;
+    ((float *)(a.ws + a.L.score))[t * d.E + e] = score;
+    ((uint32_t *)(a.ws + a.L.key))[t * d.E + e] = d.mask && d.mask[e] ? 0u : order_key(sel);
 }
 
 /* ---- routing ------------------------------------------------------------------
@@ -277,7 +255,8 @@ __device__ __forceinline__ int rank_of(const Args &a, const Choice &c, Route *R,
 }
 /* A token's experts and weights in rank order into the workspace and the caller's arrays: ranks past the
  * number of experts that can be chosen get id -1 and weight 0.  All threads of a group of WV waves. */
-template <int WV> __device__ void route_token(const Args &a, int t, const Choice &c, Route *R, int rank) {
+template <int WV>
+__device__ void route_token(const Args &a, int t, const Choice &c, Route *R, int rank, const ExpTabLanes &tab) {
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = d.k;
     const float l = c.score;
@@ -289,7 +268,8 @@ template <int WV> __device__ void route_token(const Args &a, int t, const Choice
         __syncthreads();
         float mx = R->redf[0];
         for (int q = 1; q < WV; q++) mx = R->redf[q] > mx ? R->redf[q] : mx;
-        const float x = on && mx > -INFINITY ? expf_ref(l - mx) : 0.0f;
+        const float ex = expf_ref_with(l - mx, tab);   /* every lane takes part */
+        const float x = on && mx > -INFINITY ? ex : 0.0f;
         const double sum = wave_sum_f64((double)x);
         if (lane == 0) R->red[wave] = sum;
         __syncthreads();
@@ -323,9 +303,13 @@ template <int WV> __device__ void route_token(const Args &a, int t, const Choice
 }
 __global__ __launch_bounds__(256) void k_fm_route(Args a) {
     __shared__ __align__(16) Route R;
+    args_now(a.d.E, a.d.k, a.d.router, a.d.routed_scale, a.d.experts, a.ids, a.w, a.ws, a.L.key, a.L.score, a.L.ids, a.L.w,
+             a.L.dptr);
     const Choice c = choice_of(a, blockIdx.x, threadIdx.x);
+    ExpTabLanes tab;
+    tab.load();
     const int rank = rank_of(a, c, &R, threadIdx.x);
-    route_token<4>(a, blockIdx.x, c, &R, rank);
+    route_token<4>(a, blockIdx.x, c, &R, rank, tab);
 }
 
 /* ---- an expert's tokens ------------------------------------------------------ */
@@ -501,17 +485,21 @@ __global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int tile = blockIdx.x, slot = blockIdx.y;
+    args_now(d.E, d.k, d.de, d.ds, d.router, d.routed_scale, d.experts, d.sg, d.su, a.ids, a.w, a.ws, a.slots, a.L.xp, a.L.key,
+             a.L.score, a.L.ids, a.L.w, a.L.dptr, a.L.hid, a.L.shid, a.L.nbd, a.L.nbe, a.L.nbs);
     const bool shared = slot == a.slots && d.ds > 0;
     const int64_t rows = shared ? d.ds : d.de;
     const int nbo = shared ? a.L.nbs : a.L.nbe;
     if (tile >= nbo * 8) return;
+    ExpTabLanes tab;
+    tab.load();
     if (!shared) {
         const bool all = slot >= a.slots;   /* the row of groups that routes for the others; one is enough */
         if (all && tile != 0) return;
         const Choice c = choice_of(a, 0, tid);
         const int rank = rank_of(a, c, &R, tid);
         if (all) {
-            route_token<8>(a, 0, c, &R, rank);
+            route_token<8>(a, 0, c, &R, rank, tab);
             return;
         }
         if (tid == 0) s_m[0] = nullptr;
@@ -572,23 +560,25 @@ __global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
     s_g[wave][lane] = acc[0];
     s_u[wave][lane] = acc[1];
     __syncthreads();
-    if (tid >= 16) return;
+    if (wave != 0) return;
+    const int r = lane & 15;   /* a row; the other lanes repeat it */
     float g[3], u[3];
 #pragma unroll
     for (int j = 0; j < 3; j++) {
-        const int l = (tid >> 2) * 16 + j;
+        const int l = (r >> 2) * 16 + j;
         g[j] = u[j] = 0.0f;
 #pragma unroll
         for (int q = 0; q < W; q++) {
-            g[j] += s_g[q][l][tid & 3];
-            u[j] += s_u[q][l][tid & 3];
+            g[j] += s_g[q][l][r & 3];
+            u[j] += s_u[q][l][r & 3];
         }
     }
     uint16_t p[3];
-    split3(silu(g[0] + (g[1] + g[2])) * (u[0] + (u[1] + u[2])), p);   /* 0 in the padding */
-    const size_t at = (size_t)(shared ? 0 : slot) * 3 * wo + tile * 16 + tid;
+    split3(silu(g[0] + (g[1] + g[2]), tab) * (u[0] + (u[1] + u[2])), p);   /* 0 in the padding */
+    const size_t at = (size_t)(shared ? 0 : slot) * 3 * wo + tile * 16 + r;
+    if (lane < 16)
 #pragma unroll
-    for (int j = 0; j < 3; j++) hid[at + (size_t)j * wo] = p[j];
+        for (int j = 0; j < 3; j++) hid[at + (size_t)j * wo] = p[j];
 }
 
 /* More tokens: 16 rows of one expert's gate and up for all of its tokens. */
@@ -604,17 +594,19 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
     const int64_t rows = shared ? d.ds : d.de;
     const int nbo = shared ? a.L.nbs : a.L.nbe;      /* blocks of the width that this launch makes */
     if (tile >= nbo * 8) return;
+    ExpTabLanes tab;
+    tab.load();
     const int e = uniform(slot_list(a, slot, &s));
     if (e < 0) return;
     const int n = uniform(s.n);
     uint16_t *hid = (uint16_t *)(a.ws + (shared ? a.L.shid : a.L.hid));
     const int wo = nbo * FP8_BLOCK;
     const bool pad = tile >= fp8_tiles(rows);        /* the padding of the next product's length: zeros */
-    const void *const *tab = d.experts + 3 * (size_t)(shared ? 0 : e);
+    const void *const *mats = d.experts + 3 * (size_t)(shared ? 0 : e);
     Mat m[2];
     if (!pad) {
-        m[0] = mat_of(shared ? d.sg : tab[0], tile, rows, a.L.nbd);
-        m[1] = mat_of(shared ? d.su : tab[1], tile, rows, a.L.nbd);
+        m[0] = mat_of(shared ? d.sg : mats[0], tile, rows, a.L.nbd);
+        m[1] = mat_of(shared ? d.su : mats[1], tile, rows, a.L.nbd);
     }
     const GAS uint16_t *xp = (const GAS uint16_t *)(a.ws + a.L.xp);
     const int Dp = a.L.nbd * FP8_BLOCK;
@@ -634,17 +626,18 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
             }
         }
         __syncthreads();
-        for (int o = tid; o < left * 16; o += 256) {
-            const int r = o & 15, i = o >> 4;
-            float v = 0.0f;
-            if (!pad) v = silu(total<NT>(s_g, r, i)) * total<NT>(s_u, r, i);
+        for (int o0 = 0; o0 < left * 16; o0 += 256) {   /* whole waves: the exponential's table is in their lanes */
+            const int o = o0 + tid, r = o & 15, i = (o >> 4) < left ? o >> 4 : left - 1;
+            const float v = pad ? 0.0f : silu(total<NT>(s_g, r, i), tab) * total<NT>(s_u, r, i);
             uint16_t p[3];
             split3(v, p);
             const int t = s.tok[i0 + i];
             const size_t at = (size_t)(shared ? t : t * d.k + s.rank[i0 + i]) * 3 * wo + tile * 16 + r;
-            hid[at] = p[0];
-            hid[at + wo] = p[1];
-            hid[at + 2 * wo] = p[2];
+            if (o < left * 16) {
+                hid[at] = p[0];
+                hid[at + wo] = p[1];
+                hid[at + 2 * wo] = p[2];
+            }
         }
         __syncthreads();
     }
@@ -709,6 +702,8 @@ __global__ __launch_bounds__(64 * DW) void k_fm_down_few(Args a) {
     __shared__ float s_w[MAXK + 1];
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4;
+    args_now(d.D, d.k, d.sd, d.shared_gate_inp, a.h, a.out, a.ws, a.L.ids, a.L.w, a.L.dptr, a.L.sgate, a.L.hid, a.L.shid,
+             a.L.nbe, a.L.nbs);
     const int tile = blockIdx.x, t = blockIdx.y, k = d.k, nbe = a.L.nbe, nbs = a.L.nbs;
     if (tid < k) {
         s_ptr[tid] = ((const uint8_t *const GAS *)(a.ws + a.L.dptr))[t * k + tid];
@@ -860,13 +855,7 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     const int wide = a.L.nbe > a.L.nbs ? a.L.nbe : a.L.nbs;
     hipStream_t s = (hipStream_t)stream;
     const unsigned rows = (unsigned)(d->E + (d->ds > 0 && d->shared_gate_inp ? 1 : 0));
-    const size_t xrow = (size_t)((d->D + 3) & ~(int64_t)3) * 4;
-    /* one token a group while that does not fill the chip; four share each router row's read beyond, if
-     * their x fits 64 KB of LDS */
-    if (T > 16 && d->D <= 4096)
-        hipLaunchKernelGGL(k_fm_router<4>, dim3((rows + 3) / 4, (unsigned)((T + 3) / 4)), dim3(256), 4 * xrow, s, a);
-    else
-        hipLaunchKernelGGL(k_fm_router<1>, dim3((rows + 3) / 4, (unsigned)T), dim3(256), xrow, s, a);
+    hipLaunchKernelGGL(k_fm_router, dim3((rows + 3) / 4, (unsigned)T), dim3(256), (size_t)((d->D + 3) & ~(int64_t)3) * 4, s, a);
     if (T == 1) {
         hipLaunchKernelGGL(k_fm_gateup_one, dim3((unsigned)wide * 8, ny + 1), dim3(512), 0, s, a);
     } else {
