@@ -6,12 +6,17 @@
 
 namespace {
 
-/* ---- packing: a thread per 16-byte piece ---------------------------------- */
+/* ---- packing: a thread per 16-byte piece, then one per scale ---------------- */
 __global__ __launch_bounds__(256) void k_fp8_pack(const uint8_t *__restrict__ W, size_t row_bytes, int64_t rows,
                                                   int64_t n, int nb, int64_t pieces, int vec,
+                                                  const float *__restrict__ scale, int64_t stride, int64_t scales,
                                                   uint8_t *__restrict__ dst) {
     const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (p >= pieces) return;
+    if (p >= pieces) {
+        const int64_t i = p - pieces;
+        if (i < scales) ((float *)(dst + pieces * 16))[i] = scale[i / nb * stride + i % nb];
+        return;
+    }
     const int64_t unit = p >> 7;
     const int h = (int)(p >> 6) & 1, l = (int)p & 63;
     const int64_t row = unit / nb * TILE_ROWS + (l & 15);
@@ -28,12 +33,6 @@ __global__ __launch_bounds__(256) void k_fp8_pack(const uint8_t *__restrict__ W,
         }
     }
     *(u32x4 *)(dst + p * 16) = v;
-}
-
-__global__ __launch_bounds__(256) void k_fp8_pack_scale(const float *__restrict__ s, int64_t stride, int nb,
-                                                        int64_t count, float *__restrict__ dst) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) dst[i] = s[i / nb * stride + i % nb];
 }
 
 /* ---- activation quantiser --------------------------------------------------
@@ -549,14 +548,13 @@ int tlm_hip_fp8_pack(const void *W, size_t row_bytes, const float *scale, int64_
         return tlmh_seterr(TLM_HIP_EINVAL, "fp8_pack: dst must be 16-byte and scale 4-byte aligned");
     const int nb = (int)fp8_blocks(n);
     const int64_t pieces = (int64_t)(fp8_code_bytes(rows, n) / 16), ns = fp8_blocks(rows) * nb;
-    if ((pieces + 255) / 256 > 0x7FFFFFFF / 256)
+    const int64_t groups = (pieces + ns + 255) / 256;
+    if (groups > 0x7FFFFFFF / 256)
         return tlmh_seterr(TLM_HIP_ERANGE, "fp8_pack: %lld x %lld is too large for one launch", (long long)rows,
                            (long long)n);
     const int vec = aligned(W, 16) && row_bytes % 16 == 0;
-    hipLaunchKernelGGL(k_fp8_pack, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
-                       (const uint8_t *)W, row_bytes, rows, n, nb, pieces, vec, (uint8_t *)dst);
-    hipLaunchKernelGGL(k_fp8_pack_scale, dim3((unsigned)((ns + 255) / 256)), dim3(256), 0, (hipStream_t)stream, scale,
-                       scale_stride, nb, ns, (float *)((uint8_t *)dst + fp8_code_bytes(rows, n)));
+    hipLaunchKernelGGL(k_fp8_pack, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, (const uint8_t *)W,
+                       row_bytes, rows, n, nb, pieces, vec, scale, scale_stride, ns, (uint8_t *)dst);
     return tlmh_check(hipGetLastError(), "fp8_pack launch");
 }
 

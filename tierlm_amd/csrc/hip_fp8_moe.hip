@@ -10,14 +10,21 @@
  * The planes are columns of the matrix product: 16 columns hold five tokens' three
  * planes, whose sums are added at the end, smallest first.
  *
- *   K1 router   x, its planes, the router's scores and the selection keys
- *   K2 gate/up  a group per 16 rows of one expert's gate and up, for all of its
- *               tokens: silu(g) * u as planes
- *   K3 down     a group per 16 rows of one expert's down: the unweighted results
- *   K4 combine  per token: routing weights, the sum in rank order, the residual
- * K2 and K3 find an expert's tokens themselves from the keys: expert e is among
- * token t's k if fewer than k of t's keys are larger than e's, a count that takes
- * a wave a few ballots. */
+ *   K1 router    x, its planes, the router's scores and the selection keys
+ *   K1b route    (not for one token) each token's experts and weights
+ *   K2 gate/up   16 rows of one expert's gate and up, for all of its tokens: silu(g) * u as
+ *                planes; one token routes in this launch
+ *   K3 down      few tokens: 16 rows of one token's result, all its experts, the sum and the
+ *                residual; more: 64 rows of one expert's down for all of its tokens, then
+ *                K4 combine  the sum in rank order and the residual
+ * No launch hands data between its own groups: on this chip a boundary between launches costs
+ * about 1.4 us, a barrier across the groups of one 6 us and more, so three launches for one
+ * token beat two.
+ *
+ * Measured, whole layers: Qwen3-30B-A3B (2048 x 768, 128 experts top-8), one token 22 us (38 MB,
+ * of it router 5, gate/up 10, down 7: launches and dependent reads more than bytes), 8
+ * tokens 71 us (3.4 TB/s of the experts that they reach), 64 tokens 172; Qwen3-235B-A22B (4096 x
+ * 1536), 64 tokens 501 us, 4.75 TB/s, of the 5.1 TB/s that a large copy reaches. */
 #include "tlm_hip_fp8.h"
 
 namespace {
@@ -203,12 +210,12 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
 
 /* ---- routing ------------------------------------------------------------------
  * Expert e is among token t's k if fewer than k of t's keys are ahead of its own; the count is
- * its rank.  256 threads, thread e counts for expert e. */
-__device__ __forceinline__ bool ahead(uint32_t kf, int f, uint32_t ke, int e) {
-    return kf > ke || (kf == ke && f < e);
-}
+ * its rank.  A key is 64 bits, the order of the selection value and then ~e, so that "larger"
+ * is the whole order.  Threads tid, tid + W, ... share the count for expert tid (W = 128 or 256
+ * at the least E): counted by one thread an expert, the compares alone took 2 us. */
 struct Route {
-    uint32_t key[MAXE];
+    unsigned long long key[MAXE];
+    uint16_t cnt[4][MAXE];
     int ids[MAXK];
     float w[MAXK];
     const void *down[MAXK];
@@ -235,23 +242,33 @@ __device__ __forceinline__ Choice choice_of(const Args &a, int t, int tid) {
     if (!in) c.key = 0u;
     return c;
 }
-/* The rank of thread tid's expert (MAXE where it cannot be chosen).  All threads of the group, 256 or more. */
-__device__ __forceinline__ int rank_of(const Args &a, const Choice &c, Route *R, int tid) {
-    if (tid < MAXE) R->key[tid] = c.key;
+/* The rank of thread tid's expert (MAXE where it cannot be chosen, and past E).  All WV waves. */
+template <int WV> __device__ __forceinline__ int rank_of(const Args &a, const Choice &c, Route *R, int tid) {
+    const int W = a.d.E <= 128 ? 128 : 256, parts = WV * 64 / W, e = tid & (W - 1), part = tid / W;
+    if (tid < MAXE) R->key[tid] = c.key ? (unsigned long long)c.key << 32 | (0xFFFFFFFFu - (uint32_t)tid) : 0ull;
     if (tid < MAXK) {
         R->ids[tid] = -1;
         R->w[tid] = 0.0f;
         R->down[tid] = nullptr;
     }
     __syncthreads();
-    int n[4] = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int f = 0; f < a.d.E; f += 4) {   /* keys past E are 0, never ahead of one that can be chosen */
-        const u32x4 k = *(const LAS u32x4 *)&R->key[f];
-#pragma unroll
-        for (int q = 0; q < 4; q++) n[q] += ahead(k[q], f + q, c.key, tid) ? 1 : 0;
+    const unsigned long long ke = R->key[e];
+    if (ke) {
+        int n[4] = {0, 0, 0, 0};
+        const LAS u32x4 *kp = (const LAS u32x4 *)R->key + part * (W / parts / 2);
+#pragma unroll 8
+        for (int f = 0; f < W / parts / 2; f++) {   /* two keys a read; keys past E are 0, never larger */
+            const u32x4 k = kp[f];
+            n[f & 1] += ((unsigned long long)k[1] << 32 | k[0]) > ke ? 1 : 0;
+            n[2 + (f & 1)] += ((unsigned long long)k[3] << 32 | k[2]) > ke ? 1 : 0;
+        }
+        R->cnt[part][e] = (uint16_t)((n[0] + n[1]) + (n[2] + n[3]));
     }
-    return c.key ? (n[0] + n[1]) + (n[2] + n[3]) : MAXE;
+    __syncthreads();
+    if (tid >= W || !ke) return MAXE;
+    int rank = 0;
+    for (int q = 0; q < parts; q++) rank += R->cnt[q][e];
+    return rank;
 }
 /* A token's experts and weights in rank order into the workspace and the caller's arrays: ranks past the
  * number of experts that can be chosen get id -1 and weight 0.  All threads of a group of WV waves. */
@@ -308,7 +325,7 @@ __global__ __launch_bounds__(256) void k_fm_route(Args a) {
     const Choice c = choice_of(a, blockIdx.x, threadIdx.x);
     ExpTabLanes tab;
     tab.load();
-    const int rank = rank_of(a, c, &R, threadIdx.x);
+    const int rank = rank_of<4>(a, c, &R, threadIdx.x);
     route_token<4>(a, blockIdx.x, c, &R, rank, tab);
 }
 
@@ -497,7 +514,7 @@ __global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
         const bool all = slot >= a.slots;   /* the row of groups that routes for the others; one is enough */
         if (all && tile != 0) return;
         const Choice c = choice_of(a, 0, tid);
-        const int rank = rank_of(a, c, &R, tid);
+        const int rank = rank_of<8>(a, c, &R, tid);
         if (all) {
             route_token<8>(a, 0, c, &R, rank, tab);
             return;
@@ -691,42 +708,58 @@ __global__ __launch_bounds__(256) void k_fm_down(Args a) {
 
 /* ---- K3 for few tokens: down and the sum ------------------------------------------
  * A group takes 16 rows of one token's result: the blocks of all its experts' down rows, and of
- * the shared expert's, are dealt to 8 waves, each scaled by its expert's weight as it is added.  A
+ * the shared expert's, are dealt to the waves, each scaled by its expert's weight as it is added.  A
  * matrix that two tokens share is read by both. */
-constexpr int DW = 8;
-constexpr int FEW = 8;
-template <int U>
-__global__ __launch_bounds__(64 * DW) void k_fm_down_few(Args a) {
+__global__ __launch_bounds__(512) void k_fm_down_few(Args a) {
+    constexpr int DW = 8, U = 3;
     __shared__ f32x4 s_sum[DW][64];
     __shared__ const uint8_t *s_ptr[MAXK + 1];
     __shared__ float s_w[MAXK + 1];
     const tlm_hip_moe_desc &d = a.d;
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4;
     args_now(d.D, d.k, d.sd, d.shared_gate_inp, a.h, a.out, a.ws, a.L.ids, a.L.w, a.L.dptr, a.L.sgate, a.L.hid, a.L.shid,
              a.L.nbe, a.L.nbs);
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4;
     const int tile = blockIdx.x, t = blockIdx.y, k = d.k, nbe = a.L.nbe, nbs = a.L.nbs;
+    const uint8_t *ptr = nullptr;
+    float wt = 0.0f;
     if (tid < k) {
-        s_ptr[tid] = ((const uint8_t *const GAS *)(a.ws + a.L.dptr))[t * k + tid];
-        s_w[tid] = ((const GAS float *)(a.ws + a.L.w))[t * k + tid];
+        ptr = ((const uint8_t *const GAS *)(a.ws + a.L.dptr))[t * k + tid];
+        wt = ((const GAS float *)(a.ws + a.L.w))[t * k + tid];
     }
     if (tid == k && nbs) {
-        s_ptr[k] = (const uint8_t *)d.sd;
-        s_w[k] = d.shared_gate_inp ? ((const GAS float *)(a.ws + a.L.sgate))[t] : 1.0f;
+        ptr = (const uint8_t *)d.sd;
+        wt = d.shared_gate_inp ? ((const GAS float *)(a.ws + a.L.sgate))[t] : 1.0f;
     }
-    __syncthreads();
     const int units = k * nbe + nbs, plane = (lane & 15) % 3;
     const size_t code_e = (size_t)fp8_tiles(d.D) * nbe * FP8_UNIT, code_s = (size_t)fp8_tiles(d.D) * nbs * FP8_UNIT;
     const GAS uint16_t *hid = (const GAS uint16_t *)(a.ws + a.L.hid) + ((size_t)t * k * 3 + plane) * nbe * FP8_BLOCK + 16 * g;
     const GAS uint16_t *shid = (const GAS uint16_t *)(a.ws + a.L.shid) + ((size_t)t * 3 + plane) * nbs * FP8_BLOCK + 16 * g;
     f32x4 acc = {0, 0, 0, 0};
+    bf16x8 x[U][4];
+    auto planes = [&](int u0) {   /* they do not wait for the routing */
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int v = u0 + u * DW < units ? u0 + u * DW : units - 1;
+            const int r = v < k * nbe ? v / nbe : k, b = v - r * nbe;
+            const GAS uint16_t *xx = (r < k ? hid + (size_t)r * 3 * nbe * FP8_BLOCK : shid) + b * FP8_BLOCK;
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[u][j] = *(const GAS bf16x8 *)(xx + 64 * (j >> 1) + 8 * (j & 1));
+        }
+    };
+    planes(wave);
+    if (tid <= k) {
+        s_ptr[tid] = ptr;
+        s_w[tid] = wt;
+    }
+    __syncthreads();
     for (int u0 = wave; u0 < units; u0 += DW * U) {
+        if (u0 != wave) planes(u0);
         i32x4 w[U][2];
-        bf16x8 x[U][4];
         float sc[U];
         bool on[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int v = u0 + u * DW < units ? u0 + u * DW : u0;   /* past the end: read again, not added */
+            const int v = u0 + u * DW < units ? u0 + u * DW : units - 1;   /* past the end: read again, not added */
             const int r = v < k * nbe ? v / nbe : k, nb = r < k ? nbe : nbs, b = v - r * nbe;
             const GAS uint8_t *p = (const GAS uint8_t *)s_ptr[r];
             on[u] = u0 + u * DW < units && p != nullptr;   /* a rank without an expert adds nothing: */
@@ -738,9 +771,6 @@ __global__ __launch_bounds__(64 * DW) void k_fm_down_few(Args a) {
             w[u][0] = *(const GAS i32x4 *)(q + lane * 16);
             w[u][1] = *(const GAS i32x4 *)(q + lane * 16 + 1024);
             sc[u] = s_w[r] * *(const GAS float *)z;
-            const GAS uint16_t *xx = (r < k ? hid + (size_t)r * 3 * nbe * FP8_BLOCK : shid) + b * FP8_BLOCK;
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[u][j] = *(const GAS bf16x8 *)(xx + 64 * (j >> 1) + 8 * (j & 1));
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -803,6 +833,18 @@ void spread(Args &a, int run) {
     a.ce = a.by_expert && 2 * a.T * a.d.k > run * a.d.E ? runs : 1;
 }
 
+/* Whether down runs per token (k_fm_down_few) or per expert (k_fm_down, then k_fm_combine).  Per token saves
+ * a launch and the results' way through memory and reads a matrix once for each token that chose
+ * it: while there are no more choices than experts and the matrices read again come to at most 24
+ * MB.  Whole layers, per token against per expert: 2048 x 768, 128 experts top-8: 8 tokens (20 MB)
+ * 70.8 against 74.3 us, 10 (30 MB) 83.6 and 84.5, 16 (71 MB) 115 and 110; 4096 x 1536, 8 tokens (78
+ * MB) 214 and 196; 512 x 256, 32 experts top-4, 8 tokens 19.5 and 22.6; 3000 x 500, 16 experts
+ * top-4, 8 tokens (twice as many choices as experts) 41 and 35. */
+bool by_token(const tlm_hip_moe_desc &d, int64_t T) {
+    const double pairs = (double)T * d.k, again = pairs * (double)(T - 1) * d.k / (2.0 * d.E);
+    return pairs <= d.E && again * (double)d.D * (double)d.de <= 24e6;
+}
+
 int check(const tlm_hip_moe_desc *d, int64_t T) {
     if (!d) return tlmh_seterr(TLM_HIP_EINVAL, "fp8_moe: NULL descriptor");
     if (d->E <= 0 || d->E > MAXE || d->k <= 0 || d->k > MAXK || d->k > d->E)
@@ -863,9 +905,9 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
         spread(a, GT * TPT);
         hipLaunchKernelGGL(k_fm_gateup, dim3((unsigned)wide * 8, (unsigned)(a.slots * a.ce + a.cs)), dim3(64 * NW), 0, s, a);
     }
-    if (T <= FEW) {
+    if (by_token(*d, T)) {
         const dim3 grid((unsigned)fp8_tiles(d->D), (unsigned)T);
-        hipLaunchKernelGGL(k_fm_down_few<3>, grid, dim3(64 * DW), 0, s, a);
+        hipLaunchKernelGGL(k_fm_down_few, grid, dim3(512), 0, s, a);
     } else {
         spread(a, DT * TPT);
         hipLaunchKernelGGL(k_fm_down, dim3((unsigned)((fp8_tiles(d->D) + DM - 1) / DM), (unsigned)(a.slots * a.ce + a.cs)),

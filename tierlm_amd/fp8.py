@@ -25,7 +25,8 @@ _CODES = (E4M3, torch.uint8)
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-_quantize, _matmul, _moe = lib.tlm_hip_fp8_quantize, lib.tlm_hip_fp8_matmul, lib.tlm_hip_fp8_moe
+_pack, _quantize, _matmul, _moe = (lib.tlm_hip_fp8_pack, lib.tlm_hip_fp8_quantize, lib.tlm_hip_fp8_matmul,
+                                   lib.tlm_hip_fp8_moe)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
@@ -35,9 +36,11 @@ def _blocks(n):
 
 def _here(*tensors):
     """The current device's index, on which all the tensors must be."""
-    dev = torch.cuda.current_device() if torch.cuda.is_initialized() or torch.cuda.is_available() else -1
+    dev = tensors[0].get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise ValueError(f"a tensor is on {tensors[0].device}, not on the current HIP device")
     for t in tensors:
-        if t.get_device() != dev or dev < 0:
+        if t.get_device() != dev:
             raise ValueError(f"a tensor is on {t.device}, not on the current HIP device")
     return dev
 
@@ -69,13 +72,17 @@ def pack(W, scale, out=None):
     if W.dtype not in _CODES or not _rows_ok(W) or W.numel() == 0:
         raise ValueError("W must be a 2-D float8_e4m3fn or uint8 tensor with contiguous rows")
     rows, n = W.shape
-    if scale.shape != (_blocks(rows), _blocks(n)) or scale.dtype != torch.float32 or not _rows_ok(scale):
-        raise ValueError(f"scale must be float32 [{_blocks(rows)}, {_blocks(n)}] with contiguous rows")
+    nr, nb = -(-rows // BLOCK), -(-n // BLOCK)
+    if scale.shape != (nr, nb) or scale.dtype != torch.float32 or not _rows_ok(scale):
+        raise ValueError(f"scale must be float32 [{nr}, {nb}] with contiguous rows")
     dev = _here(W, scale)
-    out = _out(out, (packed_bytes(rows, n),), torch.uint8, W, "out")
-    _here(out)
-    check(lib.tlm_hip_fp8_pack(W.data_ptr(), max(W.stride(0), n), scale.data_ptr(), max(scale.stride(0), _blocks(n)),
-                               rows, n, out.data_ptr(), _raw_stream(dev)))
+    out = _out(out, (lib.tlm_hip_fp8_packed_bytes(rows, n),), torch.uint8, W, "out")
+    if out.get_device() != dev or out.data_ptr() % 16:
+        raise ValueError("out must be on the current HIP device, 16-byte aligned")
+    rc = _pack(W.data_ptr(), max(W.stride(0), n), scale.data_ptr(), max(scale.stride(0), nb), rows, n, out.data_ptr(),
+               _raw_stream(dev))
+    if rc:
+        check(rc)
     return out
 
 
