@@ -19,7 +19,7 @@ def test_packed_bytes():
     assert fp8.packed_bytes(17, 129) == 2 * 2 * 2048 + 16
     assert fp8.packed_bytes(257, 640) == 17 * 5 * 2048 + 64          # 3 x 5 scales of 4 bytes, padded to 16
     assert fp8.packed_bytes(151936, 2048) == 151936 * 2048 + 1187 * 16 * 4
-    for rows, n in ((0, 128), (128, 0), (-1, 5), ((1 << 28) + 1, 128), (16, (1 << 22) + 1)):
+    for rows, n in ((0, 128), (128, 0), (-1, 5), ((1 << 25) + 1, 128), (16, (1 << 22) + 1)):
         assert fp8.packed_bytes(rows, n) == 0
 
 
@@ -28,7 +28,7 @@ def test_packed_bytes():
     (EINVAL, (P, 128, P, 1, 16, 128, None)), (EINVAL, (P, 127, P, 1, 16, 128, P)),
     (EINVAL, (P, 256, P, 1, 16, 129, P)), (EINVAL, (P, 128, P, 1, 0, 128, P)), (EINVAL, (P, 128, P, 1, 16, 0, P)),
     (EINVAL, (P, 128, P, 1, 16, 128, HALF)), (EINVAL, (P, 128, ODD, 1, 16, 128, P)),
-    (ERANGE, (P, 1 << 22, P, 1 << 15, 1 << 28, 1 << 22, P))])
+    (ERANGE, (P, 1 << 22, P, 1 << 15, 1 << 25, 1 << 22, P))])
 def test_pack_refuses(want, args):
     assert lib.tlm_hip_fp8_pack(*args, None) == want
     assert b"fp8_pack" in lib.tlm_hip_errmsg()
@@ -53,7 +53,8 @@ def test_quantize_refuses(want, args):
     (EINVAL, (P, 16, 128, P, P, 2, 0, P, 15)), (EINVAL, (HALF, 16, 128, P, P, 1, 0, P, 16)),
     (EINVAL, (P, 16, 128, HALF, P, 1, 0, P, 16)), (EINVAL, (P, 16, 128, P, HALF, 1, 0, P, 16)),
     (EINVAL, (P, 16, 128, P, P, 1, 0, HALF, 16)), (EINVAL, (P, 16, 128, P, P, 1, 2, ODD, 16)),
-    (ERANGE, (P, 16, 128, P, P, 1000001, 0, P, 16)), (0, (None, 16, 128, None, None, 0, 0, None, 16))])
+    (ERANGE, (P, 16, 128, P, P, (1 << 20) + 1, 0, P, 16)),
+    (ERANGE, (P, 1 << 20, 128, P, P, (1 << 15) + 1, 0, P, 1 << 20)), (0, (None, 16, 128, None, None, 0, 0, None, 16))])
 def test_matmul_refuses(want, args):
     assert lib.tlm_hip_fp8_matmul(*args, None) == want
 

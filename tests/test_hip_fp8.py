@@ -248,3 +248,60 @@ def test_linear_streams_and_graph(hip, T):
         got = Y.clone()
         assert torch.equal(got, fp8.matmul(P, rows, n, *fp8.quantize(x))), i
         torch.cuda.synchronize()
+
+
+# (T, rows) at which each size of tile is taken: fp32 results up to 128 x 128, 16-bit ones up to 256 x 256
+TILES = [(100, 5000), (100, 8100), (100, 16300), (250, 16300), (250, 32700), (250, 65300), (33, 66000)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [100, 256, 300, 512, 900])
+@pytest.mark.parametrize("T,rows", TILES)
+def test_matmul_tiles(hip, T, rows, n, dtype):
+    """Every tile size with part tiles of rows and tokens and one to eight blocks of values (the stages'
+    whole and part rounds), the tokens' scales spread over powers of two."""
+    g = gen(T + rows + n)
+    w, s = matrix(g, rows, n)
+    codes, scale = fp8.quantize(randn(g, T, n) * torch.exp2(torch.randint(-6, 7, (T, 1), generator=g, device="cuda")))
+    scale *= 1 + torch.rand(scale.shape, generator=g, device="cuda")      # not powers of two alone
+    check_product(fp8.matmul(fp8.pack(w, s), rows, n, codes, scale, dtype=dtype), w, s, codes, scale, n)
+
+
+@pytest.mark.parametrize("T,rows,n", [(1, 64, 20000), (16, 100, 9000), (20, 64, 8192), (40, 64, 16384), (300, 5000, 2000)])
+def test_matmul_long_rows(hip, T, rows, n):
+    g = gen(T + n)
+    w, s = matrix(g, rows, n)
+    codes, scale = fp8.quantize(randn(g, T, n))
+    for dtype in (torch.float32, torch.bfloat16):
+        check_product(fp8.matmul(fp8.pack(w, s), rows, n, codes, scale, dtype=dtype), w, s, codes, scale, n)
+
+
+def test_repeats_its_bits(hip):
+    g = gen(77)
+    w, s = matrix(g, 3000, 1000)
+    P = fp8.pack(w, s)
+    for T in (1, 20, 64, 200, 1000):
+        codes, scale = fp8.quantize(randn(g, T, 1000))
+        for dtype in (torch.float32, torch.float16):
+            a = fp8.matmul(P, 3000, 1000, codes, scale, dtype=dtype)
+            for _ in range(3):
+                assert torch.equal(a, fp8.matmul(P, 3000, 1000, codes, scale, dtype=dtype))
+
+
+def test_two_calls_at_once(hip):
+    """Products on two streams at a time, each with tensors of its own."""
+    g = gen(78)
+    w, s = matrix(g, 4096, 2048)
+    P = fp8.pack(w, s)
+    xs = [fp8.quantize(randn(g, T, 2048)) for T in (5, 300)]
+    want = [fp8.matmul(P, 4096, 2048, *x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(5):
+        for i, (x, st) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(fp8.matmul(P, 4096, 2048, *x))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(v, want[i]) for v in got[i])

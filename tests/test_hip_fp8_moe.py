@@ -255,3 +255,58 @@ def test_block_refuses(hip):
     with pytest.raises(HipError):
         fp8.MoeBlock(D=256, de=128, E=2, k=3, ffn_norm=c.norm, router_w=c.router_w[:2].contiguous(),
                      expert_ptrs=[m.data_ptr() for ex in c.packed[:2] for m in ex])
+
+
+def test_workspace_grows_under_a_graph(hip):
+    """A graph captured with few tokens still replays after the block has grown for more."""
+    c, g = build(13, 256, 128, 16, 4)
+    h = randn(g, 3, 256)
+    out = torch.empty_like(h)
+    c.block(h, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.block(h, out=out)
+    many = randn(g, 64, 256)
+    c.block(many, out=torch.empty_like(many))
+    for i in range(3):
+        h.copy_(randn(g, 3, 256))
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, c.block(h, out=torch.empty_like(h))), i
+        torch.cuda.synchronize()
+
+
+def test_overlapping_out_is_refused(hip):
+    c, g = build(14, 256, 128, 16, 4)
+    buf = randn(g, 3, 256)
+    with pytest.raises(ValueError):
+        c.block(buf[:2], out=buf[1:])
+
+
+def test_one_matrix_for_two_experts(hip):
+    """Expert pointers may repeat."""
+    c, g = build(15, 256, 128, 8, 3)
+    c.experts[5], c.packed[5] = c.experts[2], c.packed[2]
+    c.block = fp8.MoeBlock(D=256, de=128, E=8, k=3, ffn_norm=c.norm, router_w=c.router_w,
+                           expert_ptrs=[m.data_ptr() for ex in c.packed for m in ex])
+    for T in (1, 30):
+        go(c, g, T)
+
+
+def test_pruned_experts_need_no_matrices(hip):
+    mask = torch.zeros(16, dtype=torch.bool)
+    mask[[0, 3, 7, 15]] = True
+    c, g = build(16, 256, 128, 16, 4, mask=mask)
+    ptrs = [0 if mask[e] else m.data_ptr() for e, ex in enumerate(c.packed) for m in ex]
+    c.block = fp8.MoeBlock(D=256, de=128, E=16, k=4, ffn_norm=c.norm, router_w=c.router_w, expert_ptrs=ptrs,
+                           mask=mask.to("cuda", torch.uint8))
+    for T in (1, 3, 40):
+        go(c, g, T)
+
+
+def test_wide_model(hip):
+    """The longest residual: rows past what the router keeps in registers."""
+    for D, T in ((5000, 3), (16384, 2)):
+        c, g = build(D, D, 64, 6, 2, 48, gate=True)
+        go(c, g, T)

@@ -523,8 +523,8 @@ int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16
 /* Row and length limits keep every launch inside the grid limits; sizes in bytes
  * are 64-bit throughout. */
 static int fp8_dims(const char *who, int64_t rows, int64_t n) {
-    if (rows < 1 || n < 1 || rows > ((int64_t)1 << 28) || n > ((int64_t)1 << 22))
-        return tlmh_seterr(TLM_HIP_EINVAL, "%s: rows=%lld n=%lld outside 1..2^28 and 1..2^22", who, (long long)rows,
+    if (rows < 1 || n < 1 || rows > ((int64_t)1 << 25) || n > ((int64_t)1 << 22))
+        return tlmh_seterr(TLM_HIP_EINVAL, "%s: rows=%lld n=%lld outside 1..2^25 and 1..2^22", who, (long long)rows,
                            (long long)n);
     return TLM_HIP_OK;
 }
@@ -595,8 +595,9 @@ int tlm_hip_fp8_matmul(const void *Wp, int64_t rows, int64_t n, const void *code
     if (!aligned(Wp, 16) || !aligned(codes, 16) || !aligned(scale, 4) || !aligned(Y, (size_t)type_bytes(dt)))
         return tlmh_seterr(TLM_HIP_EINVAL,
                            "fp8_matmul: the matrix and the codes must be 16-byte, scale 4-byte aligned, Y as its type");
-    if (ntok > 1000000)
-        return tlmh_seterr(TLM_HIP_ERANGE, "fp8_matmul: %lld tokens are too many for one launch", (long long)ntok);
+    if (ntok > ((int64_t)1 << 20) || ntok * rows > (int64_t)1 << 35)   /* 2^31 threads in the smallest tiles */
+        return tlmh_seterr(TLM_HIP_ERANGE, "fp8_matmul: %lld tokens of %lld rows are too many for one launch",
+                           (long long)ntok, (long long)rows);
     const MmArgs a = {(const uint8_t *)Wp, (const float *)((const uint8_t *)Wp + fp8_code_bytes(rows, n)),
                       (const uint8_t *)codes, scale, Y, rows, ystride, ntok, (int)fp8_blocks(n), dt,
                       aligned(Y, 4 * (size_t)type_bytes(dt)) && (ystride % 4 == 0 || ntok == 1)};

@@ -137,14 +137,14 @@ class MoeBlock:
     """One routed MoE block of E4M3 matrices for up to 64 tokens a call.  Expert
     e's packed gate / up / down pointers are expert_ptrs[3e .. 3e + 2]; packed
     matrices are the caller's to keep alive, as are the tensors a call is given.
-    The workspace grows to the largest T seen and is one per block, so calls of
-    one block must not overlap (other streams); a block captured into a graph has to
-    run once with its largest T before."""
+    The workspace is one per block and grows with the largest T seen (reserve()
+    sizes it ahead), so calls of one block must not overlap (other streams, two
+    graphs at once)."""
 
     def __init__(self, *, D, de, E, k, ffn_norm, router_w, expert_ptrs, router=0, routed_scale=1.0, eps=1e-6,
                  router_bias=None, mask=None, ds=0, shared=None, shared_gate_inp=None):
-        if len(expert_ptrs) != 3 * E or not all(expert_ptrs):
-            raise ValueError("expert_ptrs must hold 3 E packed matrices")
+        if len(expert_ptrs) != 3 * E or not (all(expert_ptrs) or mask is not None):
+            raise ValueError("expert_ptrs must hold 3 E packed matrices (0 only for experts that the mask prunes)")
         if (ds > 0) != (shared is not None):
             raise ValueError("ds and shared go together")
         for t, shape, dt, what in ((ffn_norm, (D,), torch.float32, "ffn_norm"),
@@ -172,16 +172,20 @@ class MoeBlock:
         self._desc = C.byref(self.desc)
         self.D, self.k = D, k
         check(_moe(self._desc, None, None, 0, None, None, None, None))   # the sizes fit
-        self.workspace, self._room = None, 0
+        self.workspace, self._room, self._earlier = None, 0, []
 
     def reserve(self, T):
-        """Make the workspace large enough for T tokens."""
+        """Make the workspace large enough for T tokens (it at least doubles; a smaller one that a
+        captured graph may hold stays allocated)."""
         if T > self._room:
-            nbytes = int(lib.tlm_hip_fp8_moe_workspace_bytes(self._desc, T))
+            room = min(max(T, 2 * self._room), max(T, MOE_MAX_TOKENS))
+            nbytes = int(lib.tlm_hip_fp8_moe_workspace_bytes(self._desc, room))
             if not nbytes:
                 check(_moe(self._desc, None, None, T, None, None, None, None))
+            if self.workspace is not None:
+                self._earlier.append(self.workspace)
             self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            self._room = T
+            self._room = room
 
     def __call__(self, h, out=None, ids=None, w=None):
         """out = h + MoE(h) for h (f32 [T, D] or [D]), T <= 64; without `out` h itself
@@ -190,8 +194,14 @@ class MoeBlock:
         if h.dtype != torch.float32 or not h.is_contiguous() or h.dim() not in (1, 2) or h.shape[-1] != self.D:
             raise ValueError(f"h must be contiguous float32 [T, {self.D}]")
         T = h.shape[0] if h.dim() == 2 else 1
-        out = h if out is None else _out(out, h.shape, torch.float32, h, "out")
-        dev = _here(h, out)
+        if out is None:
+            out = h
+        else:
+            _out(out, h.shape, torch.float32, h, "out")
+            gap = abs(out.data_ptr() - h.data_ptr())
+            if 0 < gap < 4 * h.numel():
+                raise ValueError("out must be h itself or not overlap it")
+        dev = _here(h, out, self.table)
         pi = pw = None
         if ids is not None:
             _here(_out(ids, (T, self.k), torch.int32, h, "ids"))
