@@ -6,10 +6,12 @@
  *
  * Checked: the device activation quantisers (bytes), the plain-layout matvec
  * and the packed-layout matvec (bits of every row) for F32, Q8_0, Q4_K, Q5_K,
- * Q6_K and Q8_K, the exponential against this host's libm expf, and the
- * matrix cores' float products against v_mul_f32.  Returns the number of
- * failing kernels; bit dt of *mask is set for every dtype whose kernels failed,
- * bit 30 for the exponential, bit 29 for the products. */
+ * Q6_K and Q8_K, the exponential against this host's libm expf, the
+ * matrix cores' float products against v_mul_f32, and the 8-bit floating-point
+ * quantiser (codes and scales) and product (within the roundings of a float sum).
+ * Returns the number of failing kernels; bit dt of *mask is set for every dtype
+ * whose kernels failed, bit 30 for the exponential, bit 29 for the products, bit
+ * 28 for 8-bit floating point. */
 #include "tlm_hip_internal.h"
 #include "tlm_hip_outer.h"
 
@@ -245,6 +247,69 @@ bool outer_ok(uint8_t *dev, uint32_t *s) {
     return ok;
 }
 
+/* an E4M3 code's value, and the code nearest to v (|v| <= 448, ties to even) by search */
+double e4m3(int c) {
+    const int e = (c >> 3) & 15, m = c & 7;
+    const double v = e ? ldexp(8.0 + m, e - 10) : ldexp((double)m, -9);
+    return c & 128 ? -v : v;
+}
+int to_e4m3(double v) {
+    const double a = fabs(v);
+    int best = 0;
+    for (int c = 1; c < 127; c++) {
+        const double d = fabs(e4m3(c) - a), b = fabs(e4m3(best) - a);
+        if (d < b || (d == b && !(c & 1))) best = c;
+    }
+    return best | (signbit(v) ? 128 : 0);
+}
+
+/* 3 tokens and 20 rows of 300 values (part blocks and part tiles); dev: 32 KB */
+bool fp8_ok(uint8_t *dev, uint32_t *s) {
+    constexpr int T = 3, R = 20, N = 300, NB = 3, NP = NB * 128;
+    std::vector<float> x(T * N), sx(T * NB), gs(T * NB), y(T * R);
+    std::vector<uint8_t> w(R * N), cx(T * NP, 0), gc(T * NP);
+    const float sw[NB] = {0.5f, 0.0371f, 3.0f};
+    for (auto &v : x) v = ((float)(st_rng(s) & 0xFFFF) / 32768.0f - 1.0f) * ldexpf(1.0f, (int)(st_rng(s) & 7) - 4);
+    for (auto &c : w) {
+        c = (uint8_t)st_rng(s);
+        if ((c & 127) == 127) c = 0;
+    }
+    for (int t = 0; t < T; t++)
+        for (int b = 0; b < NB; b++) {
+            const int n = N - 128 * b < 128 ? N - 128 * b : 128;
+            double amax = 0.0;
+            for (int i = 0; i < n; i++) amax = fmax(amax, fabs((double)x[t * N + 128 * b + i]));
+            int e = -126;
+            while (amax > ldexp(448.0, e)) e++;
+            sx[t * NB + b] = amax > 0.0 ? ldexpf(1.0f, e) : 0.0f;
+            for (int i = 0; i < n; i++) cx[t * NP + 128 * b + i] = (uint8_t)to_e4m3(ldexp((double)x[t * N + 128 * b + i], -e));
+        }
+    float *dx = (float *)dev, *ds = (float *)(dev + 4096), *dsw = (float *)(dev + 4352), *dy = (float *)(dev + 4608);
+    uint8_t *dc = dev + 8192, *dw = dev + 10240, *dp = dev + 16640;
+    if (hipMemcpy(dx, x.data(), x.size() * 4, hipMemcpyHostToDevice) != hipSuccess ||
+        hipMemcpy(dw, w.data(), w.size(), hipMemcpyHostToDevice) != hipSuccess ||
+        hipMemcpy(dsw, sw, sizeof sw, hipMemcpyHostToDevice) != hipSuccess ||
+        tlm_hip_fp8_quantize(DT_F32, dx, N, N, T, dc, ds, nullptr) != TLM_HIP_OK ||
+        tlm_hip_fp8_pack(dw, N, dsw, NB, R, N, dp, nullptr) != TLM_HIP_OK ||
+        tlm_hip_fp8_matmul(dp, R, N, dc, ds, T, DT_F32, dy, R, nullptr) != TLM_HIP_OK ||
+        hipMemcpy(gc.data(), dc, gc.size(), hipMemcpyDeviceToHost) != hipSuccess ||
+        hipMemcpy(gs.data(), ds, gs.size() * 4, hipMemcpyDeviceToHost) != hipSuccess ||
+        hipMemcpy(y.data(), dy, y.size() * 4, hipMemcpyDeviceToHost) != hipSuccess)
+        return false;
+    if (memcmp(gc.data(), cx.data(), cx.size()) != 0 || memcmp(gs.data(), sx.data(), sx.size() * 4) != 0) return false;
+    for (int t = 0; t < T; t++)
+        for (int r = 0; r < R; r++) {
+            double sum = 0.0, size = 0.0;
+            for (int i = 0; i < N; i++) {
+                const double p = e4m3(cx[t * NP + i]) * e4m3(w[r * N + i]) * (double)sx[t * NB + i / 128] * (double)sw[i / 128];
+                sum += p;
+                size += fabs(p);
+            }
+            if (!(fabs((double)y[t * R + r] - sum) <= (127 + NB + 2) * 0x1p-24 * size)) return false;
+        }
+    return true;
+}
+
 }  // namespace
 
 int tlmh_selftest(int *failed_mask) {
@@ -341,6 +406,10 @@ int tlmh_selftest(int *failed_mask) {
     if (!outer_ok(dev + o_p, &s)) {
         fails++;
         mask |= 1 << 29;
+    }
+    if (!fp8_ok(dev + o_p, &s)) {
+        fails++;
+        mask |= 1 << 28;
     }
     (void)hipDeviceSynchronize();
     (void)hipFree(dev);
