@@ -27,7 +27,7 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 _pack, _quantize, _matmul, _moe = (lib.tlm_hip_fp8_pack, lib.tlm_hip_fp8_quantize, lib.tlm_hip_fp8_matmul,
                                    lib.tlm_hip_fp8_moe)
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _blocks(n):
@@ -37,7 +37,7 @@ def _blocks(n):
 def _here(*tensors):
     """The current device's index, on which all the tensors must be."""
     dev = tensors[0].get_device()
-    if dev < 0 or dev != torch.cuda.current_device():
+    if dev < 0 or dev != _current_device():
         raise ValueError(f"a tensor is on {tensors[0].device}, not on the current HIP device")
     for t in tensors:
         if t.get_device() != dev:
@@ -96,10 +96,16 @@ def quantize(x, codes=None, scale=None):
         raise ValueError("x must be float32, float16 or bfloat16 [T, n] with contiguous rows")
     T, n = x.shape
     nb = -(-n // BLOCK)
-    codes = _out(codes, (T, nb * BLOCK), E4M3, x, "codes")
-    scale = _out(scale, (T, nb), torch.float32, x, "scale")
-    rc = _quantize(dt, x.data_ptr(), x.stride(0), n, T, codes.data_ptr(), scale.data_ptr(),
-                   _raw_stream(_here(x, codes, scale)))
+    dev = _here(x)
+    if codes is None:
+        codes = x.new_empty((T, nb * BLOCK), dtype=E4M3)
+    elif _out(codes, (T, nb * BLOCK), E4M3, x, "codes").get_device() != dev:
+        _here(x, codes)
+    if scale is None:
+        scale = x.new_empty((T, nb)) if dt == 0 else x.new_empty((T, nb), dtype=torch.float32)
+    elif _out(scale, (T, nb), torch.float32, x, "scale").get_device() != dev:
+        _here(x, scale)
+    rc = _quantize(dt, x.data_ptr(), x.stride(0), n, T, codes.data_ptr(), scale.data_ptr(), _raw_stream(dev))
     if rc:
         check(rc)
     return codes, scale
