@@ -11,9 +11,9 @@
  * planes, whose sums are added at the end, smallest first.
  *
  *   K1 router    x, its planes, the router's scores and the selection keys
- *   K1b route    (not for one token) each token's experts and weights
+ *   K1b route    each token's experts and weights
  *   K2 gate/up   16 rows of one expert's gate and up, for all of its tokens: silu(g) * u as
- *                planes; one token routes in this launch
+ *                planes; one token, and few in a small block, route in this launch
  *   K3 down      few tokens: 16 rows of one token's result, all its experts, the sum and the
  *                residual; more: 64 rows of one expert's down for all of its tokens, then
  *                K4 combine  the sum in rank order and the residual
@@ -23,8 +23,8 @@
  *
  * Measured, whole layers: Qwen3-30B-A3B (2048 x 768, 128 experts top-8), one token 22 us (38 MB,
  * of it router 5, gate/up 10, down 7: launches and dependent reads more than bytes), 8
- * tokens 71 us (3.4 TB/s of the experts that they reach), 64 tokens 172; Qwen3-235B-A22B (4096 x
- * 1536), 64 tokens 501 us, 4.75 TB/s, of the 5.1 TB/s that a large copy reaches. */
+ * tokens 68 us (3.6 TB/s of the experts that they reach), 64 tokens 165; Qwen3-235B-A22B (4096 x
+ * 1536), 64 tokens 503 us, 4.75 TB/s, of the 5.1 TB/s that a large copy reaches. */
 #include "tlm_hip_fp8.h"
 
 namespace {
@@ -33,7 +33,7 @@ constexpr int MAXT = TLM_HIP_FP8_MOE_MAX_TOKENS;   /* 64: a token per lane in th
 constexpr int MAXE = 256, MAXK = 32;
 constexpr int NW = 4;              /* waves per group of K2 and K3: the blocks of a row are dealt to them */
 constexpr int TPT = 5;             /* tokens per 16 columns */
-constexpr int GT = 4, DT = 2;      /* column tiles at a time: gate/up, down */
+constexpr int NT = 2;              /* column tiles at a time */
 
 __host__ __device__ inline size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -332,6 +332,7 @@ __global__ __launch_bounds__(256) void k_fm_route(Args a) {
 /* ---- an expert's tokens ------------------------------------------------------ */
 struct List {
     int n, e, cnt[2][4];
+    uint8_t sel[16];
     uint8_t tok[MAXT], rank[MAXT];
 };
 /* Which tokens of which slot a group takes: every `parts`th run from `part` on. */
@@ -396,6 +397,63 @@ __device__ int slot_list(const Args &a, int slot, List *s) {
     return e;
 }
 
+/* The same list from the keys, for the launch that routes itself (T <= ROUTES): the tokens' keys are asked for
+ * before the slot's expert is known, then each token's is ranked by ballots. */
+constexpr int ROUTES = 16;
+constexpr unsigned GROUPS = 1024;
+__device__ int slot_list_keys(const Args &a, int slot, List *s, Route *R) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.d.k, E = a.d.E;
+    if (slot == a.slots) return slot_list(a, slot, s);
+    const GAS uint32_t *key = (const GAS uint32_t *)(a.ws + a.L.key);
+    constexpr int TW = ROUTES / NW, KE = MAXE / 64;
+    uint32_t kf[TW][KE];
+#pragma unroll
+    for (int j = 0; j < TW; j++) {
+        const int t = wave + NW * j;
+#pragma unroll
+        for (int q = 0; q < KE; q++)
+            kf[j][q] = 64 * q < E && t < a.T && lane + 64 * q < E ? key[(size_t)t * E + lane + 64 * q] : 0u;
+    }
+    int e = slot;
+    if (!a.by_expert) {
+        const Choice c = choice_of(a, slot / k, tid);
+        if (tid == 0) s->e = -1;
+        const int rank = rank_of<NW>(a, c, R, tid);
+        if (rank == slot % k) s->e = tid;
+        __syncthreads();
+        e = uniform(s->e);
+        if (e < 0) return -1;
+    }
+#pragma unroll
+    for (int j = 0; j < TW; j++) {
+        const int t = wave + NW * j;
+        uint32_t ke = 0;
+#pragma unroll
+        for (int q = 0; q < KE; q++)
+            if (e >> 6 == q) ke = (uint32_t)__builtin_amdgcn_readlane((int)kf[j][q], e & 63);
+        int rank = 0;
+#pragma unroll
+        for (int q = 0; q < KE; q++)
+            if (64 * q < E)
+                rank += __builtin_popcountll(__ballot(kf[j][q] > ke || (kf[j][q] == ke && lane + 64 * q < e)));
+        if (lane == 0) s->sel[t] = ke && rank < k ? (uint8_t)(rank + 1) : 0;   /* 0 past T: no keys */
+    }
+    __syncthreads();
+    if (wave == 0) {
+        const int sel = lane < a.T ? s->sel[lane < ROUTES ? lane : 0] : 0;
+        const unsigned long long m = __ballot(sel != 0);
+        if (sel) {
+            const int at = __builtin_popcountll(m & ((1ull << lane) - 1));
+            s->tok[at] = (uint8_t)lane;
+            s->rank[at] = (uint8_t)(sel - 1);
+        }
+        if (lane == 0) s->n = __builtin_popcountll(m);
+    }
+    __syncthreads();
+    if (s->n == 0 || (!a.by_expert && s->tok[0] != slot / k)) return -1;
+    return e;
+}
+
 /* ---- 16 rows times up to NT * TPT tokens ------------------------------------- */
 struct Mat {
     const GAS uint8_t *w;          /* the row tile's units */
@@ -410,7 +468,7 @@ __device__ __forceinline__ Mat mat_of(const void *packed, int tile, int64_t rows
 /* This wave's share of the blocks, for NQ column tiles, U blocks in flight; x[q]: this lane's
  * column of planes.  No branch stands between a matrix instruction and the reads of its result: the
  * compiler here has left out the wait on such a path. */
-template <int M, int NQ, int U, int NT>
+template <int M, int NQ, int U>
 __device__ __forceinline__ void run_tiles(const Mat (&m)[M], int nb, int wave, const GAS uint16_t *const (&x)[NT],
                                           f32x4 (&acc)[M][NT]) {
     const int lane = threadIdx.x & 63;
@@ -460,20 +518,16 @@ __device__ __forceinline__ void run_tiles(const Mat (&m)[M], int nb, int wave, c
         }
     }
 }
-template <int M, int NT>
+template <int M>
 __device__ __forceinline__ void run_blocks(const Mat (&m)[M], int nb, int wave, const GAS uint16_t *const (&x)[NT],
                                            int nt, f32x4 (&acc)[M][NT]) {
-    if (nt == 1) run_tiles<M, 1, M == 2 ? 2 : 1, NT>(m, nb, wave, x, acc);
-    else if (nt == 2) run_tiles<M, 2, 1, NT>(m, nb, wave, x, acc);
-    else if constexpr (NT > 2) {
-        if (nt == 3) run_tiles<M, 3, 1, NT>(m, nb, wave, x, acc);
-        else run_tiles<M, 4, 1, NT>(m, nb, wave, x, acc);
-    }
+    if (nt == 1) run_tiles<M, 1, M == 2 ? 2 : 1>(m, nb, wave, x, acc);
+    else run_tiles<M, 2, 1>(m, nb, wave, x, acc);
 }
 
-template <int NT> using Sums = f32x4[NW][NT][64];
+typedef f32x4 Sums[NW][NT][64];
 /* the waves' and planes' sums for row r of the tile and token i of the pass */
-template <int NT> __device__ __forceinline__ float total(const Sums<NT> &s, int r, int i) {
+__device__ __forceinline__ float total(const Sums &s, int r, int i) {
     const int q = i / TPT, l0 = (r >> 2) * 16 + 3 * (i % TPT), v = r & 3;
     float p[3];
 #pragma unroll
@@ -598,22 +652,32 @@ __global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
         for (int j = 0; j < 3; j++) hid[at + (size_t)j * wo] = p[j];
 }
 
-/* More tokens: 16 rows of one expert's gate and up for all of its tokens. */
+/* More tokens: 16 rows of one expert's gate and up for all of its tokens.  KEYS: the routing is not there
+ * yet; the groups find it from the keys, and T groups more do it for the later launches. */
+template <bool KEYS>
 __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
     __shared__ List s;
-    constexpr int NT = GT;
-    __shared__ Sums<NT> s_g, s_u;
+    __shared__ Sums s_g, s_u;
+    static_assert(sizeof(Route) <= sizeof(Sums) && MAXT >= ROUTES, "the routing's tables fit where the sums come");
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    ExpTabLanes tab;
+    tab.load();
+    if (KEYS && (int)blockIdx.y >= a.slots * a.ce + a.cs) {
+        Route *R = (Route *)&s_g;
+        if ((int)blockIdx.x >= a.T) return;
+        const Choice c = choice_of(a, blockIdx.x, tid);
+        const int rank = rank_of<NW>(a, c, R, tid);
+        route_token<NW>(a, blockIdx.x, c, R, rank, tab);
+        return;
+    }
     const Part pt = part_of(a, blockIdx.y);
     const int tile = blockIdx.x, slot = pt.slot;
     const bool shared = slot == a.slots;
     const int64_t rows = shared ? d.ds : d.de;
     const int nbo = shared ? a.L.nbs : a.L.nbe;      /* blocks of the width that this launch makes */
     if (tile >= nbo * 8) return;
-    ExpTabLanes tab;
-    tab.load();
-    const int e = uniform(slot_list(a, slot, &s));
+    const int e = uniform(KEYS ? slot_list_keys(a, slot, &s, (Route *)&s_g) : slot_list(a, slot, &s));
     if (e < 0) return;
     const int n = uniform(s.n);
     uint16_t *hid = (uint16_t *)(a.ws + (shared ? a.L.shid : a.L.hid));
@@ -635,7 +699,7 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
             for (int q = 0; q < NT; q++)
                 x[q] = xp + ((size_t)s.tok[column_index(i0, q, n)] * 3 + column_plane()) * Dp + 16 * (lane >> 4);
             f32x4 acc[2][NT] = {};
-            run_blocks<2, NT>(m, a.L.nbd, wave, x, (left + TPT - 1) / TPT, acc);
+            run_blocks<2>(m, a.L.nbd, wave, x, (left + TPT - 1) / TPT, acc);
 #pragma unroll
             for (int q = 0; q < NT; q++) {
                 s_g[wave][q][lane] = acc[0][q];
@@ -645,7 +709,7 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
         __syncthreads();
         for (int o0 = 0; o0 < left * 16; o0 += 256) {   /* whole waves: the exponential's table is in their lanes */
             const int o = o0 + tid, r = o & 15, i = (o >> 4) < left ? o >> 4 : left - 1;
-            const float v = pad ? 0.0f : silu(total<NT>(s_g, r, i), tab) * total<NT>(s_u, r, i);
+            const float v = pad ? 0.0f : silu(total(s_g, r, i), tab) * total(s_u, r, i);
             uint16_t p[3];
             split3(v, p);
             const int t = s.tok[i0 + i];
@@ -665,8 +729,7 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
 constexpr int DM = 4;
 __global__ __launch_bounds__(256) void k_fm_down(Args a) {
     __shared__ List s;
-    constexpr int NT = DT;
-    __shared__ Sums<NT> s_y;
+    __shared__ Sums s_y;
     const tlm_hip_moe_desc &d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const Part pt = part_of(a, blockIdx.y);
@@ -690,7 +753,7 @@ __global__ __launch_bounds__(256) void k_fm_down(Args a) {
             x[q] = hid + ((size_t)(shared ? t : t * d.k + s.rank[i]) * 3 + column_plane()) * wi + 16 * (lane >> 4);
         }
         f32x4 acc[DM][NT] = {};
-        run_blocks<DM, NT>(m, nb, wave, x, (left + TPT - 1) / TPT, acc);
+        run_blocks<DM>(m, nb, wave, x, (left + TPT - 1) / TPT, acc);
 #pragma unroll
         for (int j = 0; j < DM; j++) {
 #pragma unroll
@@ -699,7 +762,7 @@ __global__ __launch_bounds__(256) void k_fm_down(Args a) {
             for (int o = tid; o < left * 16; o += 256) {
                 const int r = o & 15, i = o >> 4, t = s.tok[i0 + i];
                 const int64_t row = (int64_t)(tile0 + j) * 16 + r;
-                if (row < d.D) eo[(size_t)(shared ? t : t * d.k + s.rank[i0 + i]) * d.D + row] = total<NT>(s_y, r, i);
+                if (row < d.D) eo[(size_t)(shared ? t : t * d.k + s.rank[i0 + i]) * d.D + row] = total(s_y, r, i);
             }
             __syncthreads();
         }
@@ -825,12 +888,13 @@ __global__ __launch_bounds__(256) void k_fm_combine(Args a) {
     a.out[(size_t)t * d.D + i] = a.h[(size_t)t * d.D + i] + acc;
 }
 
-/* The shared expert's tokens go to as many groups as its runs of `run`; an expert's as well where the mean
- * list is over half a run (else most of those groups would find nothing to do). */
-void spread(Args &a, int run) {
-    const int runs = (a.T + run - 1) / run;
+/* The shared expert's tokens go to as many groups as their runs of NT * TPT; an expert's to as many as twice
+ * the mean list has (a longer list's runs wrap round). */
+void spread(Args &a) {
+    constexpr int RUN = NT * TPT;
+    const int runs = (a.T + RUN - 1) / RUN, twice = (2 * a.T * a.d.k + a.d.E * RUN - 1) / (a.d.E * RUN);
     a.cs = a.d.ds > 0 ? runs : 0;
-    a.ce = a.by_expert && 2 * a.T * a.d.k > run * a.d.E ? runs : 1;
+    a.ce = !a.by_expert ? 1 : twice < runs ? twice : runs;
 }
 
 /* Whether down runs per token (k_fm_down_few) or per expert (k_fm_down, then k_fm_combine).  Per token saves
@@ -893,6 +957,7 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     a.T = (int)T;
     a.by_expert = T > 1 && T * d->k >= d->E;
     a.slots = a.by_expert ? d->E : (int)(T * d->k);
+    spread(a);
     const unsigned ny = (unsigned)(a.slots + (d->ds > 0 ? 1 : 0));
     const int wide = a.L.nbe > a.L.nbs ? a.L.nbe : a.L.nbs;
     hipStream_t s = (hipStream_t)stream;
@@ -901,15 +966,22 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     if (T == 1) {
         hipLaunchKernelGGL(k_fm_gateup_one, dim3((unsigned)wide * 8, ny + 1), dim3(512), 0, s, a);
     } else {
-        hipLaunchKernelGGL(k_fm_route, dim3((unsigned)T), dim3(256), 0, s, a);
-        spread(a, GT * TPT);
-        hipLaunchKernelGGL(k_fm_gateup, dim3((unsigned)wide * 8, (unsigned)(a.slots * a.ce + a.cs)), dim3(64 * NW), 0, s, a);
+        const unsigned ys = (unsigned)(a.slots * a.ce + a.cs), xs = (unsigned)wide * 8;
+        /* Routing in the gate/up launch saves one, and each group the work of a rank: worth it up to
+         * 4 groups a compute unit (2048 x 768, 128 experts: 2 tokens, 768 groups, 28.1 against 29.8 us,
+         * 4 tokens, 1536 groups, 44.5 against 43.5, 8 tokens, 3072 groups, 71.7 against 67.9; 1000 x
+         * 300, 32 experts, 8 tokens, 768 groups, 21.5 against 23.8). */
+        if (T <= ROUTES && xs * ys <= GROUPS) {   /* one more row of groups: one a token routes */
+            hipLaunchKernelGGL(k_fm_gateup<true>, dim3(xs > (unsigned)T ? xs : (unsigned)T, ys + 1), dim3(64 * NW), 0, s, a);
+        } else {
+            hipLaunchKernelGGL(k_fm_route, dim3((unsigned)T), dim3(256), 0, s, a);
+            hipLaunchKernelGGL(k_fm_gateup<false>, dim3(xs, ys), dim3(64 * NW), 0, s, a);
+        }
     }
     if (by_token(*d, T)) {
         const dim3 grid((unsigned)fp8_tiles(d->D), (unsigned)T);
         hipLaunchKernelGGL(k_fm_down_few, grid, dim3(512), 0, s, a);
     } else {
-        spread(a, DT * TPT);
         hipLaunchKernelGGL(k_fm_down, dim3((unsigned)((fp8_tiles(d->D) + DM - 1) / DM), (unsigned)(a.slots * a.ce + a.cs)),
                            dim3(64 * NW), 0, s, a);
         hipLaunchKernelGGL(k_fm_combine, dim3((unsigned)((d->D + 255) / 256), (unsigned)T), dim3(256), 0, s, a);
