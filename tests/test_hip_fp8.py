@@ -267,6 +267,24 @@ def test_matmul_tiles(hip, T, rows, n, dtype):
     check_product(fp8.matmul(fp8.pack(w, s), rows, n, codes, scale, dtype=dtype), w, s, codes, scale, n)
 
 
+# (T, rows, n) at which each size of row group is taken: 64 x 64 (long rows), 64 x 32, 32 x 32, 32 x 16 and
+# 16 x 16, few groups and many, short rows and long; then few rows of very many tokens
+GROUPS = [(100, 8200, 4196), (100, 4100, 1100), (30, 16500, 1100), (100, 6500, 1100), (100, 4100, 700),
+          (30, 25000, 300), (100, 2100, 1100), (25, 9000, 1100), (100, 3200, 1100), (30, 4200, 700),
+          (30, 4200, 1100), (16, 16500, 1100), (5, 32800, 1100), (9, 8200, 130), (5, 100, 9000), (16, 40, 700),
+          (5000, 10, 300), (40000, 64, 256), (70000, 16, 130), (70000, 70, 130)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,rows,n", GROUPS)
+def test_matmul_row_groups(hip, T, rows, n, dtype):
+    g = gen(T + rows + n)
+    w, s = matrix(g, rows, n)
+    codes, scale = fp8.quantize(randn(g, T, n) * torch.exp2(torch.randint(-6, 7, (T, 1), generator=g, device="cuda")))
+    scale *= 1 + torch.rand(scale.shape, generator=g, device="cuda")
+    check_product(fp8.matmul(fp8.pack(w, s), rows, n, codes, scale, dtype=dtype), w, s, codes, scale, n)
+
+
 @pytest.mark.parametrize("T,rows,n", [(1, 64, 20000), (16, 100, 9000), (20, 64, 8192), (40, 64, 16384), (300, 5000, 2000)])
 def test_matmul_long_rows(hip, T, rows, n):
     g = gen(T + n)

@@ -157,79 +157,119 @@ __device__ __forceinline__ void store4(const MmArgs &a, int64_t t, int64_t r, f3
             if (r + q < a.rows) y[q] = o[q];
 }
 
-/* ---- product, few tokens ------------------------------------------------------
- * A group takes a row tile and TT token tiles; its KW waves share the blocks of a row, U of
- * them in flight a wave, and add their sums through LDS.  Codes go to the matrix cores as
- * bfloat16 (exact): the weights' bytes bound this, and the 16-bit instructions sum in
- * full floats where the 8-bit ones do not.  More waves rather than more loads a wave:
- * 4096 x 8192, one token 9.9 us with 8 waves of two blocks, 12.0 with 8 of four, 16.8 with 4 of
- * four.  One token: 151936 x 2048 in 46 us (6.8 TB/s), 4096 x 2048 3.8 us. */
-template <int KW, int U, int TT>
+/* ---- product, up to a few hundred tokens -----------------------------------------
+ * A group takes RT row tiles and TT token tiles; its KW waves share the blocks of a row, each with
+ * the next block's loads under way while it computes one, and add their sums through LDS.
+ *   Weights come in the order of the fragments.  Tokens come as rows of whole lines, 8 to an
+ * instruction, and pass through LDS of the wave's own (no barrier) to the order of the fragments, pieces
+ * at piece ^ row % 8, so that neither side meets a bank twice.  Fetched in that order straight from memory,
+ * every quarter of a wave touches 16 lines for 16 bytes each, and those look-ups bound it: 64 tokens
+ * of 4096 x 4096 14.6 us, 512 x 16384 46; now 8.2 and 10.
+ *   EXACT takes the codes as bfloat16 (exact), whose instructions sum in full floats where the 8-bit
+ * ones do not; for few tokens the weights' bytes or the tokens' way through L2 bound either.
+ *   One token: 151936 x 2048 in 45.5 us (6.8 TB/s), 4096 x 4096 5.0, 2048 x 2048 3.5. */
+template <bool EXACT, int KW, int RT, int TT>
 __global__ __launch_bounds__(64 * KW) void k_fp8_rows(MmArgs a) {
-    __shared__ f32x4 s_sum[KW][TT][64];
+    constexpr int XB = TT * FP8_UNIT;   /* a block of the group's tokens */
+    constexpr int PW = XB > RT * TT * 1024 ? XB : RT * TT * 1024;
+    __shared__ __align__(16) uint8_t s_x[KW * PW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4,
               c = lane & 15;
-    const int64_t tile = blockIdx.x;
+    const int tile0 = blockIdx.x * RT, last = (int)fp8_tiles(a.rows) - 1;
     const int64_t t0 = (int64_t)blockIdx.y * TT * 16;
     const int nb = a.nb;
-    const GAS uint8_t *w = (const GAS uint8_t *)a.W + (size_t)tile * nb * FP8_UNIT + lane * 16, *x[TT];
-    const GAS float *sw = (const GAS float *)a.sw + (size_t)(tile / 8) * nb, *sa[TT];
+    const GAS uint8_t *w[RT], *x[TT][2];
+    const GAS float *sw = (const GAS float *)a.sw + (size_t)(tile0 / 8) * nb, *sa[TT];
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+        w[i] = (const GAS uint8_t *)a.W + (size_t)(tile0 + i < last ? tile0 + i : last) * nb * FP8_UNIT + lane * 16;
 #pragma unroll
     for (int j = 0; j < TT; j++) {
         const int64_t t = t0 + 16 * j + c < a.T ? t0 + 16 * j + c : a.T - 1;
-        x[j] = (const GAS uint8_t *)a.x + (size_t)t * nb * FP8_BLOCK + g * 16;
         sa[j] = (const GAS float *)a.sa + t * nb;
-    }
-    f32x4 acc[TT] = {};
-    for (int b0 = wave; b0 < nb; b0 += KW * U) {
-        i32x4 wv[U][2], xv[U][TT][2];
-        float ws[U], xs[U][TT];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int b = b0 + u * KW < nb ? b0 + u * KW : nb - 1;   /* past the end: read again, not added */
-            wv[u][0] = *(const GAS i32x4 *)(w + (size_t)b * FP8_UNIT);
-            wv[u][1] = *(const GAS i32x4 *)(w + (size_t)b * FP8_UNIT + 1024);
-            ws[u] = sw[b];
-#pragma unroll
-            for (int j = 0; j < TT; j++) {
-                xv[u][j][0] = *(const GAS i32x4 *)(x[j] + b * FP8_BLOCK);
-                xv[u][j][1] = *(const GAS i32x4 *)(x[j] + b * FP8_BLOCK + 64);
-                xs[u][j] = sa[j][b];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const bool on = u == 0 || b0 + u * KW < nb;
-            f32x4 p[TT] = {};
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int h = k >> 1, q = 2 * (k & 1);
-                const bf16x8 wf = fp8_to_bf16(wv[u][h][q], wv[u][h][q + 1]);
-#pragma unroll
-                for (int j = 0; j < TT; j++)
-                    p[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, fp8_to_bf16(xv[u][j][h][q], xv[u][j][h][q + 1]),
-                                                                   p[j], 0, 0, 0);
-            }
-#pragma unroll
-            for (int j = 0; j < TT; j++) {
-                const float sc = ws[u] * xs[u][j];
-#pragma unroll
-                for (int v = 0; v < 4; v++) {
-                    const float t = fmaf(p[j][v], sc, acc[j][v]);
-                    acc[j][v] = on ? t : acc[j][v];
-                }
-            }
+        for (int h = 0; h < 2; h++) {
+            const int64_t r = t0 + 16 * j + 8 * h + (lane >> 3);
+            x[j][h] = (const GAS uint8_t *)a.x + (size_t)(r < a.T ? r : a.T - 1) * nb * FP8_BLOCK + 16 * (lane & 7);
         }
     }
+    LAS uint8_t *sx = (LAS uint8_t *)s_x + wave * PW;
+    const int at_w = (lane >> 3) * FP8_BLOCK + 16 * ((lane & 7) ^ (lane >> 3));
+    const int at_r0 = c * FP8_BLOCK + 16 * (g ^ (c & 7)), at_r1 = c * FP8_BLOCK + 16 * ((4 + g) ^ (c & 7));
+    f32x4 acc[RT][TT] = {};
+    struct In {
+        i32x4 w[RT][2], x[TT][2];
+        float ws, xs[TT];
+    };
+    auto load = [&](In &n, int b) {
 #pragma unroll
-    for (int j = 0; j < TT; j++) s_sum[wave][j][lane] = acc[j];
+        for (int j = 0; j < TT; j++) {
+            n.xs[j] = sa[j][b];
+#pragma unroll
+            for (int h = 0; h < 2; h++) n.x[j][h] = *(const GAS i32x4 *)(x[j][h] + b * FP8_BLOCK);
+        }
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) n.w[i][h] = *(const GAS i32x4 *)(w[i] + (size_t)b * FP8_UNIT + 1024 * h);
+        n.ws = sw[b];
+    };
+    auto compute = [&](const In &n) {
+#pragma unroll
+        for (int j = 0; j < TT; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) *(LAS i32x4 *)(sx + j * FP8_UNIT + h * 1024 + at_w) = n.x[j][h];
+        bf16x8 wf[RT][4];
+        if constexpr (EXACT)
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) wf[i][k] = fp8_to_bf16(n.w[i][k >> 1][2 * (k & 1)], n.w[i][k >> 1][2 * (k & 1) + 1]);
+#pragma unroll
+        for (int j = 0; j < TT; j++) {
+            const i32x4 q0 = *(const LAS i32x4 *)(sx + j * FP8_UNIT + at_r0), q1 = *(const LAS i32x4 *)(sx + j * FP8_UNIT + at_r1);
+            f32x4 p[RT] = {};
+            if constexpr (EXACT) {
+                const bf16x8 xf[4] = {fp8_to_bf16(q0[0], q0[1]), fp8_to_bf16(q0[2], q0[3]), fp8_to_bf16(q1[0], q1[1]), fp8_to_bf16(q1[2], q1[3])};
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int i = 0; i < RT; i++) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i][k], xf[k], p[i], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < RT; i++) p[i] = fp8_mfma(fp8_join(n.w[i][0], n.w[i][1]), fp8_join(q0, q1), p[i]);
+            }
+            const float sc = n.ws * n.xs[j];
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) acc[i][j][v] = fmaf(p[i][v], sc, acc[i][j][v]);
+        }
+    };
+    In cur;
+    int b = wave;
+    if (b < nb) {
+        load(cur, b);
+        for (; b + KW < nb; b += KW) {
+            In nxt;
+            load(nxt, b + KW);
+            compute(cur);
+            cur = nxt;
+        }
+        compute(cur);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+        for (int j = 0; j < TT; j++) *(LAS f32x4 *)(sx + (i * TT + j) * 1024 + lane * 16) = acc[i][j];
     __syncthreads();
-    for (int o = threadIdx.x; o < TT * 64; o += 64 * KW) {
-        const int j = o >> 6, l = o & 63;
-        f32x4 s = s_sum[0][j][l];
+    for (int o = threadIdx.x; o < RT * TT * 64; o += 64 * KW) {
+        const int m = o >> 6, i = m / TT, j = m % TT, l = o & 63;
+        const LAS uint8_t *from = (const LAS uint8_t *)s_x + m * 1024 + l * 16;
+        f32x4 s = *(const LAS f32x4 *)from;
 #pragma unroll
-        for (int q = 1; q < KW; q++) s += s_sum[q][j][l];
-        const int64_t t = t0 + 16 * j + (l & 15), r = tile * 16 + 4 * (l >> 4);
+        for (int q = 1; q < KW; q++) s += *(const LAS f32x4 *)(from + q * PW);
+        const int64_t t = t0 + 16 * j + (l & 15), r = (int64_t)(tile0 + i) * 16 + 4 * (l >> 4);
         if (t < a.T && r < a.rows) store4(a, t, r, s);
     }
 }
@@ -472,46 +512,71 @@ template <bool EXACT, int S, int WM, int WN, int TM, int TN> void launch_tile(co
     hipLaunchKernelGGL((k_fp8_tile<EXACT, S, WM, WN, TM, TN>), dim3((unsigned)(mt * nt)), dim3(64 * WM * WN), 0, s, a,
                        (int)mt, (int)nt);
 }
-template <int KW, int U> void launch_rows(const MmArgs &a, hipStream_t s) {
-    const int tt = a.T <= 16 ? 1 : a.T <= 32 ? 2 : 4;
-    const dim3 grid((unsigned)fp8_tiles(a.rows), (unsigned)((a.T + 16 * tt - 1) / (16 * tt)));
-    if (tt == 1) hipLaunchKernelGGL((k_fp8_rows<KW, U, 1>), grid, dim3(64 * KW), 0, s, a);
-    else if (tt == 2) hipLaunchKernelGGL((k_fp8_rows<KW, U, 2>), grid, dim3(64 * KW), 0, s, a);
-    else hipLaunchKernelGGL((k_fp8_rows<KW, 1, 4>), grid, dim3(64 * KW), 0, s, a);
+template <bool EXACT, int KW, int RT, int TT> void launch_rows(const MmArgs &a, hipStream_t s) {
+    const dim3 grid((unsigned)((fp8_tiles(a.rows) + RT - 1) / RT), (unsigned)((a.T + 16 * TT - 1) / (16 * TT)));
+    hipLaunchKernelGGL((k_fp8_rows<EXACT, KW, RT, TT>), grid, dim3(64 * KW), 0, s, a);
 }
 
-/* Which kernel: the row kernel for up to 32 tokens, whose matrix is read once, and for more as long as
- * its groups of 64 tokens do not outnumber the compute units (4096 x 4096, float results: 64 tokens
- * 15.0 us against 17.4 in tiles, 128 tokens 25 against 17; 77 tokens of 1000 x 1111 5.4 against
- * 6.6).  Else the largest tile that still gives every one of the 256 compute units one (16-bit
- * results, 4096 x 4096: 128 tokens 12.6 us in tiles of 32 x 64 and 15.7 in 64 x 64; 256 tokens
- * 22.8 and 15.3; 512 tokens 26.1 in 64 x 64 and 20.9 in 128 x 64; 1024 tokens 37.0 in 128 x 64
- * and 28.1 in 128 x 128; 4096 tokens of 8192 x 4096 175 in 128 x 128 and 139 in 256 x 256).
- * 128 x 128 takes four stages while a unit has one tile (28.1 against 33.2 us with two at 1024
- * tokens), two stages and two groups a unit beyond (25.8 against 30.0 at 2048 x 4096 x 2048). */
+/* Which kernel.  Tiles through LDS once those of 128 x 64 give every one of the 256 compute units one and
+ * there are more than 32 tokens and 64 rows (float results: 64 tokens of 151936 x 2048 83 us against 97 in row
+ * groups, 512 of 4096 x 4096 25 against 27.6, but 256 of them 24 against 15).
+ *   Of the tiles the largest that still gives every unit one (16-bit results: 512 tokens of 4096 x 4096
+ * 26 us in 128 x 128 and 21 in 128 x 64; 1024 tokens 37.0 in 128 x 64 and 28.1 in 128 x 128; 4096 tokens
+ * of 8192 x 4096 175 in 128 x 128 and 139 in 256 x 256) and does not pad the tokens to over 4 / 3 of
+ * what half its width would (64 tokens of 151936 x 2048 107 us in 256 x 256, 75 in 128 x 64; 192 of
+ * 16384 x 2048 17.4 in 128 x 128, 22.7 in 128 x 64).  128 x
+ * 128 takes four stages while a unit has one tile (28.1 against 33.2 us with two at 1024 tokens), two
+ * stages and two groups a unit beyond (25.8 against 30.0 at 2048 x 4096 x 2048).
+ *   Row groups take the largest of 64 x 64, 64 x 32, 32 x 32, 32 x 16 and 16 x 16 with a group for every
+ * unit (4096 x 4096: 32 tokens 6.3 us in 32 x 16, 7.5 in 16 x 16; 128 tokens 10.1 in 64 x 32, 12.3 in
+ * 32 x 32), 64 x 64 only for long rows (512 tokens of 2048 x 2048 9.8 in 64 x 64, 9.1 in 64 x 32; 256 of
+ * 4096 x 4096 15.0 and 16.2).  Few tokens leave the weights' bytes, so that two row tiles a group pay from 9
+ * tokens on or with 4 groups a unit (8192 x 4096: 16 tokens 8.6 us with two, 9.8 with one; 4 tokens 8.7
+ * and 8.1; 151936 x 2048, 4 tokens 46.6 and 52).
+ *   Waves a group: 8 while a unit has about one group, 4 where there are more (64 x 32: 128 tokens of 4096 x
+ * 4096 10.1 us with 8, 11.0 with 4; 192 tokens 15.5 and 14.2); 16 x 16 has 16 for rows of 64 blocks or
+ * more (512 x 16384, one token 7.6 us against 9.8 with 8), 32 x 16 where a unit has two groups or more
+ * (16 tokens of 151936 x 2048 52 against 57.5). */
 void launch_mm(const MmArgs &a, hipStream_t s) {
     constexpr int64_t CUS = 256;
     const bool exact = a.dt == DT_F32;
-    auto count = [&](int m, int n) { return ((a.rows + m - 1) / m) * ((a.T + n - 1) / n); };
-    if (a.T <= 32 || count(16, 64) <= CUS) {
-        if (a.nb <= 4) launch_rows<4, 1>(a, s);
-        else if (a.nb <= 8) launch_rows<8, 1>(a, s);
-        else if (a.nb < 64) launch_rows<8, 2>(a, s);
-        else launch_rows<16, 2>(a, s);
+    auto up = [&](int n) { return (a.T + n - 1) / n; };
+    auto count = [&](int m, int n) { return (a.rows + m - 1) / m * up(n); };
+    auto fits = [&](int m, int n) { return count(m, n) >= CUS && 3 * n * up(n) <= 4 * (n / 2) * up(n / 2); };
+    if (a.T > 32 && (a.rows > 64 || a.T > 65536) && count(128, 64) >= CUS) {
+        if (exact) {
+            if (fits(128, 128)) launch_tile<true, 2, 2, 2, 4, 4>(a, s);
+            else launch_tile<true, 4, 2, 2, 4, 2>(a, s);
+        } else {
+            if (fits(256, 256)) launch_tile<false, 2, 2, 4, 8, 4>(a, s);
+            else if (fits(128, 128) && count(128, 128) >= 2 * CUS) launch_tile<false, 2, 2, 2, 4, 4>(a, s);
+            else if (fits(128, 128)) launch_tile<false, 4, 2, 2, 4, 4>(a, s);
+            else launch_tile<false, 4, 2, 2, 4, 2>(a, s);
+        }
         return;
     }
-    if (exact) {
-        if (count(128, 128) >= CUS) launch_tile<true, 2, 2, 2, 4, 4>(a, s);
-        else if (count(128, 64) >= CUS) launch_tile<true, 4, 2, 2, 4, 2>(a, s);
-        else if (count(64, 64) >= CUS) launch_tile<true, 4, 2, 2, 2, 2>(a, s);
-        else launch_tile<true, 4, 1, 2, 2, 2>(a, s);
+    const int nb = a.nb;
+    auto fills = [&](int m, int n) { return count(m, n) >= CUS && 2 * a.rows > m && 2 * a.T > n; };   /* over half of a group used */
+    if (nb >= 32 && fills(64, 64)) {
+        if (exact) launch_rows<true, 4, 4, 4>(a, s);
+        else launch_rows<false, 4, 4, 4>(a, s);
+    } else if (fills(64, 32)) {
+        const bool few = 2 * count(64, 32) < 3 * CUS && nb >= 8, eight = !exact && a.T > 32;
+        if (few && eight) launch_rows<false, 8, 4, 2>(a, s);
+        else if (few) launch_rows<true, 8, 4, 2>(a, s);
+        else if (eight) launch_rows<false, 4, 4, 2>(a, s);
+        else launch_rows<true, 4, 4, 2>(a, s);
+    } else if (fills(32, 32)) {
+        if (2 * count(32, 32) < 3 * CUS && nb >= 8) launch_rows<true, 8, 2, 2>(a, s);
+        else launch_rows<true, 4, 2, 2>(a, s);
+    } else if (a.rows > 16 && count(32, 16) >= (a.T > 8 ? 3 * CUS / 4 : 4 * CUS)) {
+        if (nb < 8) launch_rows<true, 4, 2, 1>(a, s);
+        else if (count(32, 16) < 2 * CUS) launch_rows<true, 8, 2, 1>(a, s);
+        else launch_rows<true, 16, 2, 1>(a, s);
     } else {
-        if (count(256, 256) >= CUS) launch_tile<false, 2, 2, 4, 8, 4>(a, s);
-        else if (count(128, 128) >= 2 * CUS) launch_tile<false, 2, 2, 2, 4, 4>(a, s);
-        else if (count(128, 128) >= CUS) launch_tile<false, 4, 2, 2, 4, 4>(a, s);
-        else if (count(128, 64) >= CUS) launch_tile<false, 4, 2, 2, 4, 2>(a, s);
-        else if (count(64, 64) >= CUS) launch_tile<false, 4, 2, 2, 2, 2>(a, s);
-        else launch_tile<false, 4, 1, 2, 2, 2>(a, s);
+        if (nb < 8) launch_rows<true, 4, 1, 1>(a, s);
+        else if (nb < 64) launch_rows<true, 8, 1, 1>(a, s);
+        else launch_rows<true, 16, 1, 1>(a, s);
     }
 }
 
