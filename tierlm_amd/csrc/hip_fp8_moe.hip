@@ -75,6 +75,18 @@ struct Args {
     int ce, cs;   /* groups among which an expert's, and the shared expert's, tokens are dealt */
 };
 
+/* A vector's planes: a block of 128 values is 384 bfloat16, in the order of the matrix cores' operands: load
+ * j of 4, group g of 4 lanes' columns, plane, 8 values (64 (j / 2) + 16 g + 8 (j % 2) on).  The
+ * 16 lanes of a quarter wave, five vectors' three planes, then ask for 48 bytes of five lines, not for 16
+ * bytes of fifteen. */
+constexpr int XBLOCK = 3 * FP8_BLOCK;
+__device__ __forceinline__ int plane_at(int i, int plane) {
+    const int g = (i >> 4) & 3, j = 2 * ((i >> 6) & 1) + ((i >> 3) & 1);
+    return (i >> 7) * XBLOCK + ((j * 4 + g) * 3 + plane) * 8 + (i & 7);
+}
+/* this lane's part of a block, load j at 96 j from it */
+__device__ __forceinline__ int plane_lane() { return (int)((threadIdx.x & 63) >> 4) * 24 + (int)((threadIdx.x & 15) % 3) * 8; }
+
 /* a value that all lanes of a wave share, in a scalar register: branches on it are the
  * wave's, and no matrix instruction ends up under a lane mask */
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -169,7 +181,7 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
             for (int j = 0; j < 3; j++) o[j][q] = p[j];
         }
 #pragma unroll
-        for (int j = 0; j < 3; j++) *(u16x4 *)(xp + j * Dp + i) = o[j];
+        for (int j = 0; j < 3; j++) *(u16x4 *)(xp + plane_at(i, j)) = o[j];
     };
 #pragma unroll
     for (int c = 0; c < NC; c++) {
@@ -490,7 +502,7 @@ __device__ __forceinline__ void run_tiles(const Mat (&m)[M], int nb, int wave, c
             for (int q = 0; q < NQ; q++)
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    xv[u][q][j] = *(const GAS bf16x8 *)(x[q] + b * FP8_BLOCK + 64 * (j >> 1) + 8 * (j & 1));
+                    xv[u][q][j] = *(const GAS bf16x8 *)(x[q] + b * XBLOCK + 96 * j);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -542,7 +554,6 @@ __device__ __forceinline__ int column_index(int i0, int q, int n) {
     const int i = i0 + TPT * q + (c < 15 ? c / 3 : 4);
     return i < n ? i : n - 1;
 }
-__device__ __forceinline__ int column_plane() { return (threadIdx.x & 15) % 3; }
 
 /* ---- K2 ----------------------------------------------------------------------- */
 /* One token: every group routes it (all of its loads at once, then a count), so that nothing waits for
@@ -588,7 +599,7 @@ __global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
     f32x4 acc[2] = {};
     if (!pad) {
         const Mat m[2] = {mat_of(shared ? d.sg : s_m[0], tile, rows, nb), mat_of(shared ? d.su : s_m[1], tile, rows, nb)};
-        const GAS uint16_t *x = (const GAS uint16_t *)(a.ws + a.L.xp) + (size_t)column_plane() * nb * FP8_BLOCK + 16 * (lane >> 4);
+        const GAS uint16_t *x = (const GAS uint16_t *)(a.ws + a.L.xp) + plane_lane();
         for (int b0 = wave; b0 < nb; b0 += W * U) {
             i32x4 w[U][2][2];
             float sw[U][2];
@@ -604,7 +615,7 @@ __global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
                         w[u][i][h] = *(const GAS i32x4 *)(m[i].w + (size_t)b * FP8_UNIT + h * 1024 + lane * 16);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; j++) xv[u][j] = *(const GAS bf16x8 *)(x + b * FP8_BLOCK + 64 * (j >> 1) + 8 * (j & 1));
+                for (int j = 0; j < 4; j++) xv[u][j] = *(const GAS bf16x8 *)(x + b * XBLOCK + 96 * j);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
@@ -646,10 +657,10 @@ __global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
     }
     uint16_t p[3];
     split3(silu(g[0] + (g[1] + g[2]), tab) * (u[0] + (u[1] + u[2])), p);   /* 0 in the padding */
-    const size_t at = (size_t)(shared ? 0 : slot) * 3 * wo + tile * 16 + r;
+    const size_t at = (size_t)(shared ? 0 : slot) * 3 * wo;
     if (lane < 16)
 #pragma unroll
-        for (int j = 0; j < 3; j++) hid[at + (size_t)j * wo] = p[j];
+        for (int j = 0; j < 3; j++) hid[at + plane_at(tile * 16 + r, j)] = p[j];
 }
 
 /* More tokens: 16 rows of one expert's gate and up for all of its tokens.  KEYS: the routing is not there
@@ -697,7 +708,7 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
             const GAS uint16_t *x[NT];
 #pragma unroll
             for (int q = 0; q < NT; q++)
-                x[q] = xp + ((size_t)s.tok[column_index(i0, q, n)] * 3 + column_plane()) * Dp + 16 * (lane >> 4);
+                x[q] = xp + (size_t)s.tok[column_index(i0, q, n)] * 3 * Dp + plane_lane();
             f32x4 acc[2][NT] = {};
             run_blocks<2>(m, a.L.nbd, wave, x, (left + TPT - 1) / TPT, acc);
 #pragma unroll
@@ -713,12 +724,10 @@ __global__ __launch_bounds__(256) void k_fm_gateup(Args a) {
             uint16_t p[3];
             split3(v, p);
             const int t = s.tok[i0 + i];
-            const size_t at = (size_t)(shared ? t : t * d.k + s.rank[i0 + i]) * 3 * wo + tile * 16 + r;
-            if (o < left * 16) {
-                hid[at] = p[0];
-                hid[at + wo] = p[1];
-                hid[at + 2 * wo] = p[2];
-            }
+            const size_t at = (size_t)(shared ? t : t * d.k + s.rank[i0 + i]) * 3 * wo;
+            if (o < left * 16)
+#pragma unroll
+                for (int j = 0; j < 3; j++) hid[at + plane_at(tile * 16 + r, j)] = p[j];
         }
         __syncthreads();
     }
@@ -750,7 +759,7 @@ __global__ __launch_bounds__(256) void k_fm_down(Args a) {
 #pragma unroll
         for (int q = 0; q < NT; q++) {
             const int i = column_index(i0, q, n), t = s.tok[i];
-            x[q] = hid + ((size_t)(shared ? t : t * d.k + s.rank[i]) * 3 + column_plane()) * wi + 16 * (lane >> 4);
+            x[q] = hid + (size_t)(shared ? t : t * d.k + s.rank[i]) * 3 * wi + plane_lane();
         }
         f32x4 acc[DM][NT] = {};
         run_blocks<DM>(m, nb, wave, x, (left + TPT - 1) / TPT, acc);
@@ -781,7 +790,7 @@ __global__ __launch_bounds__(512) void k_fm_down_few(Args a) {
     const tlm_hip_moe_desc &d = a.d;
     args_now(d.D, d.k, d.sd, d.shared_gate_inp, a.h, a.out, a.ws, a.L.ids, a.L.w, a.L.dptr, a.L.sgate, a.L.hid, a.L.shid,
              a.L.nbe, a.L.nbs);
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int tile = blockIdx.x, t = blockIdx.y, k = d.k, nbe = a.L.nbe, nbs = a.L.nbs;
     const uint8_t *ptr = nullptr;
     float wt = 0.0f;
@@ -793,10 +802,10 @@ __global__ __launch_bounds__(512) void k_fm_down_few(Args a) {
         ptr = (const uint8_t *)d.sd;
         wt = d.shared_gate_inp ? ((const GAS float *)(a.ws + a.L.sgate))[t] : 1.0f;
     }
-    const int units = k * nbe + nbs, plane = (lane & 15) % 3;
+    const int units = k * nbe + nbs;
     const size_t code_e = (size_t)fp8_tiles(d.D) * nbe * FP8_UNIT, code_s = (size_t)fp8_tiles(d.D) * nbs * FP8_UNIT;
-    const GAS uint16_t *hid = (const GAS uint16_t *)(a.ws + a.L.hid) + ((size_t)t * k * 3 + plane) * nbe * FP8_BLOCK + 16 * g;
-    const GAS uint16_t *shid = (const GAS uint16_t *)(a.ws + a.L.shid) + ((size_t)t * 3 + plane) * nbs * FP8_BLOCK + 16 * g;
+    const GAS uint16_t *hid = (const GAS uint16_t *)(a.ws + a.L.hid) + (size_t)t * k * nbe * XBLOCK + plane_lane();
+    const GAS uint16_t *shid = (const GAS uint16_t *)(a.ws + a.L.shid) + (size_t)t * nbs * XBLOCK + plane_lane();
     f32x4 acc = {0, 0, 0, 0};
     bf16x8 x[U][4];
     auto planes = [&](int u0) {   /* they do not wait for the routing */
@@ -804,9 +813,9 @@ __global__ __launch_bounds__(512) void k_fm_down_few(Args a) {
         for (int u = 0; u < U; u++) {
             const int v = u0 + u * DW < units ? u0 + u * DW : units - 1;
             const int r = v < k * nbe ? v / nbe : k, b = v - r * nbe;
-            const GAS uint16_t *xx = (r < k ? hid + (size_t)r * 3 * nbe * FP8_BLOCK : shid) + b * FP8_BLOCK;
+            const GAS uint16_t *xx = (r < k ? hid + (size_t)r * nbe * XBLOCK : shid) + b * XBLOCK;
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[u][j] = *(const GAS bf16x8 *)(xx + 64 * (j >> 1) + 8 * (j & 1));
+            for (int j = 0; j < 4; j++) x[u][j] = *(const GAS bf16x8 *)(xx + 96 * j);
         }
     };
     planes(wave);
