@@ -21,10 +21,10 @@
  * about 1.4 us, a barrier across the groups of one 6 us and more, so three launches for one
  * token beat two.
  *
- * Measured, whole layers: Qwen3-30B-A3B (2048 x 768, 128 experts top-8), one token 22 us (38 MB,
+ * Measured, whole layers: Qwen3-30B-A3B (2048 x 768, 128 experts top-8), one token 20.6 us (38 MB,
  * of it router 5, gate/up 10, down 7: launches and dependent reads more than bytes), 8
- * tokens 68 us (3.6 TB/s of the experts that they reach), 64 tokens 165; Qwen3-235B-A22B (4096 x
- * 1536), 64 tokens 503 us, 4.75 TB/s, of the 5.1 TB/s that a large copy reaches. */
+ * tokens 60 us (4.0 TB/s of the experts that they reach), 64 tokens 155; Qwen3-235B-A22B (4096 x
+ * 1536), 64 tokens 461-478 us, 5.0-5.2 TB/s, what a large copy reaches. */
 #include "tlm_hip_fp8.h"
 
 namespace {
@@ -412,7 +412,7 @@ __device__ int slot_list(const Args &a, int slot, List *s) {
 /* The same list from the keys, for the launch that routes itself (T <= ROUTES): the tokens' keys are asked for
  * before the slot's expert is known, then each token's is ranked by ballots. */
 constexpr int ROUTES = 16;
-constexpr unsigned GROUPS = 1024;
+constexpr unsigned GROUPS = 1536;
 __device__ int slot_list_keys(const Args &a, int slot, List *s, Route *R) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.d.k, E = a.d.E;
     if (slot == a.slots) return slot_list(a, slot, s);
@@ -477,64 +477,51 @@ __device__ __forceinline__ Mat mat_of(const void *packed, int tile, int64_t rows
             (const GAS float *)(p + fp8_code_bytes(rows, (int64_t)nb * FP8_BLOCK)) + tile / 8 * nb};
 }
 
-/* This wave's share of the blocks, for NQ column tiles, U blocks in flight; x[q]: this lane's
- * column of planes.  No branch stands between a matrix instruction and the reads of its result: the
- * compiler here has left out the wait on such a path. */
-template <int M, int NQ, int U>
+/* This wave's share of the blocks for NQ column tiles; x[q]: this lane's part of its vector's planes.  One block
+ * in flight a wave: with the next one's loads under way too the registers left room for fewer waves
+ * (64 tokens of 2048 x 768, 128 experts 155 us, 167 with two).  No branch stands between a matrix
+ * instruction and the reads of its result: the compiler here has left out the wait on such a path. */
+template <int M, int NQ>
 __device__ __forceinline__ void run_tiles(const Mat (&m)[M], int nb, int wave, const GAS uint16_t *const (&x)[NT],
                                           f32x4 (&acc)[M][NT]) {
     const int lane = threadIdx.x & 63;
-    for (int b0 = wave; b0 < nb; b0 += NW * U) {
-        i32x4 w[U][M][2];
-        float sw[U][M];
-        bf16x8 xv[U][NQ][4];
+    for (int b = wave; b < nb; b += NW) {
+        i32x4 w[M][2];
+        float sw[M];
+        bf16x8 xv[NQ][4];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int b = b0 + u * NW < nb ? b0 + u * NW : nb - 1;   /* past the end: read again, not added */
+        for (int i = 0; i < M; i++) {
+            sw[i] = m[i].sw[b];
+#pragma unroll
+            for (int h = 0; h < 2; h++) w[i][h] = *(const GAS i32x4 *)(m[i].w + (size_t)b * FP8_UNIT + h * 1024 + lane * 16);
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) xv[q][j] = *(const GAS bf16x8 *)(x[q] + b * XBLOCK + 96 * j);
+        f32x4 p[M][NQ] = {};
+#pragma unroll
+        for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int i = 0; i < M; i++) {
-                sw[u][i] = m[i].sw[b];
+                const i32x4 c = w[i][j >> 1];
+                const bf16x8 wv = (j & 1) ? fp8_to_bf16(c[2], c[3]) : fp8_to_bf16(c[0], c[1]);
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-                    w[u][i][h] = *(const GAS i32x4 *)(m[i].w + (size_t)b * FP8_UNIT + h * 1024 + lane * 16);
+                for (int q = 0; q < NQ; q++) p[i][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[q][j], p[i][q], 0, 0, 0);
             }
 #pragma unroll
-            for (int q = 0; q < NQ; q++)
+        for (int q = 0; q < NQ; q++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    xv[u][q][j] = *(const GAS bf16x8 *)(x[q] + b * XBLOCK + 96 * j);
-        }
+            for (int i = 0; i < M; i++)
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const bool on = u == 0 || b0 + u * NW < nb;
-            f32x4 p[M][NQ] = {};
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int i = 0; i < M; i++) {
-                    const i32x4 c = w[u][i][j >> 1];
-                    const bf16x8 wv = (j & 1) ? fp8_to_bf16(c[2], c[3]) : fp8_to_bf16(c[0], c[1]);
-#pragma unroll
-                    for (int q = 0; q < NQ; q++)
-                        p[i][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[u][q][j], p[i][q], 0, 0, 0);
-                }
-#pragma unroll
-            for (int q = 0; q < NQ; q++)
-#pragma unroll
-                for (int i = 0; i < M; i++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        const float t = fmaf(p[i][q][v], sw[u][i], acc[i][q][v]);
-                        acc[i][q][v] = on ? t : acc[i][q][v];
-                    }
-        }
+                for (int v = 0; v < 4; v++) acc[i][q][v] = fmaf(p[i][q][v], sw[i], acc[i][q][v]);
     }
 }
 template <int M>
 __device__ __forceinline__ void run_blocks(const Mat (&m)[M], int nb, int wave, const GAS uint16_t *const (&x)[NT],
                                            int nt, f32x4 (&acc)[M][NT]) {
-    if (nt == 1) run_tiles<M, 1, M == 2 ? 2 : 1>(m, nb, wave, x, acc);
-    else run_tiles<M, 2, 1>(m, nb, wave, x, acc);
+    if (nt == 1) run_tiles<M, 1>(m, nb, wave, x, acc);
+    else run_tiles<M, 2>(m, nb, wave, x, acc);
 }
 
 typedef f32x4 Sums[NW][NT][64];
@@ -907,15 +894,19 @@ void spread(Args &a) {
 }
 
 /* Whether down runs per token (k_fm_down_few) or per expert (k_fm_down, then k_fm_combine).  Per token saves
- * a launch and the results' way through memory and reads a matrix once for each token that chose
- * it: while there are no more choices than experts and the matrices read again come to at most 24
- * MB.  Whole layers, per token against per expert: 2048 x 768, 128 experts top-8: 8 tokens (20 MB)
- * 70.8 against 74.3 us, 10 (30 MB) 83.6 and 84.5, 16 (71 MB) 115 and 110; 4096 x 1536, 8 tokens (78
- * MB) 214 and 196; 512 x 256, 32 experts top-4, 8 tokens 19.5 and 22.6; 3000 x 500, 16 experts
- * top-4, 8 tokens (twice as many choices as experts) 41 and 35. */
-bool by_token(const tlm_hip_moe_desc &d, int64_t T) {
+ * a launch and the results' way through memory, reads a matrix once for each token that chose it and takes 8
+ * waves for a token's 16 rows: while the matrices read again come to at most 100 MB, and all of its groups fit
+ * the chip at once, or there are no more choices than experts and a block for each wave.  Whole layers, per
+ * token against per expert: 2048 x 768, 128 experts top-8: 8 tokens (22 MB) 60.4 against 68.2 us, 16 (94 MB)
+ * 97 and 101, 24 (217 MB) 122 and 118; 4096 x 1536, 6 tokens (47 MB) 151 and 152, 12 (207 MB) 256 and 244;
+ * 1000 x 300, 8 experts top-4, 4 tokens 14.3 and 18.2; more choices than experts and not one round: 3000 x
+ * 500, 16 experts top-4, 8 tokens 32.3 and 30.9; two blocks for 8 waves: 512 x 128, 128 experts top-2, 64
+ * tokens 32.4 and 30.5. */
+bool by_token(const tlm_hip_moe_desc &d, const Layout &L, int64_t T) {
+    if (T == 1) return true;
     const double pairs = (double)T * d.k, again = pairs * (double)(T - 1) * d.k / (2.0 * d.E);
-    return pairs <= d.E && again * (double)d.D * (double)d.de <= 24e6;
+    if (again * (double)d.D * (double)d.de > 100e6) return false;
+    return fp8_tiles(d.D) * T * 8 <= 256 * 16 || (pairs <= d.E && d.k * L.nbe + L.nbs >= 8);
 }
 
 int check(const tlm_hip_moe_desc *d, int64_t T) {
@@ -977,9 +968,9 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     } else {
         const unsigned ys = (unsigned)(a.slots * a.ce + a.cs), xs = (unsigned)wide * 8;
         /* Routing in the gate/up launch saves one, and each group the work of a rank: worth it up to
-         * 4 groups a compute unit (2048 x 768, 128 experts: 2 tokens, 768 groups, 28.1 against 29.8 us,
-         * 4 tokens, 1536 groups, 44.5 against 43.5, 8 tokens, 3072 groups, 71.7 against 67.9; 1000 x
-         * 300, 32 experts, 8 tokens, 768 groups, 21.5 against 23.8). */
+         * 6 groups a compute unit (2048 x 768, 128 experts: 2 tokens, 768 groups, 26.5 against 28.6 us,
+         * 4 tokens, 1536 groups, 40.5 and 40.6, 8 tokens, 3072 groups, 62.8 and 60.6; 1000 x 300, 32
+         * experts, 8 tokens, 768 groups, 18.9 and 21.6). */
         if (T <= ROUTES && xs * ys <= GROUPS) {   /* one more row of groups: one a token routes */
             hipLaunchKernelGGL(k_fm_gateup<true>, dim3(xs > (unsigned)T ? xs : (unsigned)T, ys + 1), dim3(64 * NW), 0, s, a);
         } else {
@@ -987,7 +978,7 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
             hipLaunchKernelGGL(k_fm_gateup<false>, dim3(xs, ys), dim3(64 * NW), 0, s, a);
         }
     }
-    if (by_token(*d, T)) {
+    if (by_token(*d, a.L, T)) {
         const dim3 grid((unsigned)fp8_tiles(d->D), (unsigned)T);
         hipLaunchKernelGGL(k_fm_down_few, grid, dim3(512), 0, s, a);
     } else {
