@@ -21,7 +21,7 @@
  * about 1.4 us, a barrier across the groups of one 6 us and more, so three launches for one
  * token beat two.
  *
- * Measured, whole layers: Qwen3-30B-A3B (2048 x 768, 128 experts top-8), one token 20.6 us (38 MB,
+ * Measured, whole layers: Qwen3-30B-A3B (2048 x 768, 128 experts top-8), one token 19.7 us (38 MB,
  * of it router 5, gate/up 10, down 7: launches and dependent reads more than bytes), 8
  * tokens 60 us (4.0 TB/s of the experts that they reach), 64 tokens 155; Qwen3-235B-A22B (4096 x
  * 1536), 64 tokens 461-478 us, 5.0-5.2 TB/s, what a large copy reaches. */
@@ -545,9 +545,9 @@ __device__ __forceinline__ int column_index(int i0, int q, int n) {
 /* ---- K2 ----------------------------------------------------------------------- */
 /* One token: every group routes it (all of its loads at once, then a count), so that nothing waits for
  * a launch of its own; the last row of groups does it for the later launch and for the caller.
- * 8 waves share the blocks of 16 rows of gate and up, two in flight each. */
+ * 8 waves share the blocks of 16 rows of gate and up. */
 __global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
-    constexpr int W = 8, U = 2;
+    constexpr int W = 8;
     __shared__ __align__(16) Route R;
     __shared__ const void *s_m[2];
     __shared__ f32x4 s_g[W][64], s_u[W][64];
@@ -587,43 +587,46 @@ __global__ __launch_bounds__(512) void k_fm_gateup_one(Args a) {
     if (!pad) {
         const Mat m[2] = {mat_of(shared ? d.sg : s_m[0], tile, rows, nb), mat_of(shared ? d.su : s_m[1], tile, rows, nb)};
         const GAS uint16_t *x = (const GAS uint16_t *)(a.ws + a.L.xp) + plane_lane();
-        for (int b0 = wave; b0 < nb; b0 += W * U) {
-            i32x4 w[U][2][2];
-            float sw[U][2];
-            bf16x8 xv[U][4];
+        struct In {
+            i32x4 w[2][2], x[4];
+            float sw[2];
+        };
+        auto load = [&](In &n, int b) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int b = b0 + u * W < nb ? b0 + u * W : nb - 1;
+            for (int i = 0; i < 2; i++) {
+                n.sw[i] = m[i].sw[b];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    n.w[i][h] = *(const GAS i32x4 *)(m[i].w + (size_t)b * FP8_UNIT + h * 1024 + lane * 16);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) n.x[j] = *(const GAS i32x4 *)(x + b * XBLOCK + 96 * j);
+        };
+        auto compute = [&](const In &n) {
+            f32x4 p[2] = {};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    sw[u][i] = m[i].sw[b];
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        w[u][i][h] = *(const GAS i32x4 *)(m[i].w + (size_t)b * FP8_UNIT + h * 1024 + lane * 16);
+                    const i32x4 c = n.w[i][j >> 1];
+                    p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16((j & 1) ? fp8_to_bf16(c[2], c[3]) : fp8_to_bf16(c[0], c[1]),
+                                                                   __builtin_bit_cast(bf16x8, n.x[j]), p[i], 0, 0, 0);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; j++) xv[u][j] = *(const GAS bf16x8 *)(x + b * XBLOCK + 96 * j);
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) acc[i][v] = fmaf(p[i][v], n.sw[i], acc[i][v]);
+        };
+        if (wave < nb) {   /* the next block's loads are under way while one is computed */
+            In cur;
+            load(cur, wave);
+            for (int b = wave + W; b < nb; b += W) {
+                In nxt;
+                load(nxt, b);
+                compute(cur);
+                cur = nxt;
             }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const bool on = u == 0 || b0 + u * W < nb;
-                f32x4 p[2] = {};
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const i32x4 c = w[u][i][j >> 1];
-                        p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16((j & 1) ? fp8_to_bf16(c[2], c[3]) : fp8_to_bf16(c[0], c[1]),
-                                                                       xv[u][j], p[i], 0, 0, 0);
-                    }
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        const float t = fmaf(p[i][v], sw[u][i], acc[i][v]);
-                        acc[i][v] = on ? t : acc[i][v];
-                    }
-            }
+            compute(cur);
         }
     }
     s_g[wave][lane] = acc[0];
@@ -770,7 +773,7 @@ __global__ __launch_bounds__(256) void k_fm_down(Args a) {
  * the shared expert's, are dealt to the waves, each scaled by its expert's weight as it is added.  A
  * matrix that two tokens share is read by both. */
 __global__ __launch_bounds__(512) void k_fm_down_few(Args a) {
-    constexpr int DW = 8, U = 3;
+    constexpr int DW = 8, U = 2;
     __shared__ f32x4 s_sum[DW][64];
     __shared__ const uint8_t *s_ptr[MAXK + 1];
     __shared__ float s_w[MAXK + 1];
@@ -794,58 +797,72 @@ __global__ __launch_bounds__(512) void k_fm_down_few(Args a) {
     const GAS uint16_t *hid = (const GAS uint16_t *)(a.ws + a.L.hid) + (size_t)t * k * nbe * XBLOCK + plane_lane();
     const GAS uint16_t *shid = (const GAS uint16_t *)(a.ws + a.L.shid) + (size_t)t * nbs * XBLOCK + plane_lane();
     f32x4 acc = {0, 0, 0, 0};
-    bf16x8 x[U][4];
-    auto planes = [&](int u0) {   /* they do not wait for the routing */
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int v = u0 + u * DW < units ? u0 + u * DW : units - 1;
-            const int r = v < k * nbe ? v / nbe : k, b = v - r * nbe;
-            const GAS uint16_t *xx = (r < k ? hid + (size_t)r * nbe * XBLOCK : shid) + b * XBLOCK;
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[u][j] = *(const GAS bf16x8 *)(xx + 96 * j);
-        }
-    };
-    planes(wave);
-    if (tid <= k) {
-        s_ptr[tid] = ptr;
-        s_w[tid] = wt;
-    }
-    __syncthreads();
-    for (int u0 = wave; u0 < units; u0 += DW * U) {
-        if (u0 != wave) planes(u0);
-        i32x4 w[U][2];
+    struct In {
+        i32x4 w[U][2], x[U][4];
         float sc[U];
         bool on[U];
+    };
+    auto planes = [&](In &n, int u0) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int v = u0 + u * DW < units ? u0 + u * DW : units - 1;   /* past the end: read again, not added */
+            const int r = v < k * nbe ? v / nbe : k, b = v - r * nbe;
+            const GAS uint16_t *xx = (r < k ? hid + (size_t)r * nbe * XBLOCK : shid) + b * XBLOCK;
+#pragma unroll
+            for (int j = 0; j < 4; j++) n.x[u][j] = *(const GAS i32x4 *)(xx + 96 * j);
+        }
+    };
+    auto weights = [&](In &n, int u0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int v = u0 + u * DW < units ? u0 + u * DW : units - 1;
             const int r = v < k * nbe ? v / nbe : k, nb = r < k ? nbe : nbs, b = v - r * nbe;
             const GAS uint8_t *p = (const GAS uint8_t *)s_ptr[r];
-            on[u] = u0 + u * DW < units && p != nullptr;   /* a rank without an expert adds nothing: */
+            n.on[u] = u0 + u * DW < units && p != nullptr;   /* a rank without an expert adds nothing: */
             const GAS uint8_t *q = (const GAS uint8_t *)a.ws, *z = q;   /* the workspace (over 2 KB) is read for it */
             if (p) {
                 q = p + ((size_t)tile * nb + b) * FP8_UNIT;
                 z = p + (r < k ? code_e : code_s) + 4 * (tile / 8 * nb + b);
             }
-            w[u][0] = *(const GAS i32x4 *)(q + lane * 16);
-            w[u][1] = *(const GAS i32x4 *)(q + lane * 16 + 1024);
-            sc[u] = s_w[r] * *(const GAS float *)z;
+            n.w[u][0] = *(const GAS i32x4 *)(q + lane * 16);
+            n.w[u][1] = *(const GAS i32x4 *)(q + lane * 16 + 1024);
+            n.sc[u] = s_w[r] * *(const GAS float *)z;
         }
+    };
+    auto compute = [&](const In &n) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             f32x4 p = {0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const i32x4 c = w[u][j >> 1];
+                const i32x4 c = n.w[u][j >> 1];
                 const bf16x8 wv = (j & 1) ? fp8_to_bf16(c[2], c[3]) : fp8_to_bf16(c[0], c[1]);
-                p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, x[u][j], p, 0, 0, 0);
+                p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8, n.x[u][j]), p, 0, 0, 0);
             }
 #pragma unroll
             for (int v = 0; v < 4; v++) {
-                const float f = fmaf(p[v], sc[u], acc[v]);
-                acc[v] = on[u] ? f : acc[v];
+                const float f = fmaf(p[v], n.sc[u], acc[v]);
+                acc[v] = n.on[u] ? f : acc[v];
             }
         }
+    };
+    In cur;
+    planes(cur, wave);   /* they do not wait for the routing */
+    if (tid <= k) {
+        s_ptr[tid] = ptr;
+        s_w[tid] = wt;
+    }
+    __syncthreads();
+    if (wave < units) {   /* the next blocks' loads are under way while some are computed */
+        weights(cur, wave);
+        for (int u0 = wave + DW * U; u0 < units; u0 += DW * U) {
+            In nxt;
+            weights(nxt, u0);
+            planes(nxt, u0);
+            compute(cur);
+            cur = nxt;
+        }
+        compute(cur);
     }
     s_sum[wave][lane] = acc;
     __syncthreads();
