@@ -23,10 +23,10 @@ MOE_MAX_TOKENS = 64             # TLM_HIP_FP8_MOE_MAX_TOKENS
 E4M3 = torch.float8_e4m3fn
 _CODES = (E4M3, torch.uint8)
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-
-
+_U8, _F32 = torch.uint8, torch.float32
 _pack, _quantize, _matmul, _moe = (lib.tlm_hip_fp8_pack, lib.tlm_hip_fp8_quantize, lib.tlm_hip_fp8_matmul,
                                    lib.tlm_hip_fp8_moe)
+_packed_bytes = lib.tlm_hip_fp8_packed_bytes
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
@@ -49,6 +49,8 @@ def _rows_ok(t):
     """2-D with contiguous rows that do not overlap (any row stride)."""
     if t.dim() != 2:
         return False
+    if t.is_contiguous():
+        return True
     s0, s1 = t.stride()
     rows, n = t.shape
     return (s1 == 1 or n == 1) and (s0 >= n or rows <= 1)
@@ -63,7 +65,7 @@ def _out(t, shape, dtype, like, what):
 
 
 def packed_bytes(rows, n):
-    return int(lib.tlm_hip_fp8_packed_bytes(rows, n))
+    return int(_packed_bytes(rows, n))
 
 
 def pack(W, scale, out=None):
@@ -76,7 +78,7 @@ def pack(W, scale, out=None):
     if scale.shape != (nr, nb) or scale.dtype != torch.float32 or not _rows_ok(scale):
         raise ValueError(f"scale must be float32 [{nr}, {nb}] with contiguous rows")
     dev = _here(W, scale)
-    out = _out(out, (lib.tlm_hip_fp8_packed_bytes(rows, n),), torch.uint8, W, "out")
+    out = _out(out, (_packed_bytes(rows, n),), torch.uint8, W, "out")
     if out.get_device() != dev or out.data_ptr() % 16:
         raise ValueError("out must be on the current HIP device, 16-byte aligned")
     rc = _pack(W.data_ptr(), max(W.stride(0), n), scale.data_ptr(), max(scale.stride(0), nb), rows, n, out.data_ptr(),
@@ -115,19 +117,19 @@ def matmul(Wp, rows, n, codes, scale, out=None, dtype=torch.float32):
     """Y[t, r] = packed row r . token t: codes [T, np] and scale [T, np / 128] as
     quantize() gives them; Y [T, rows] of `dtype`, or `out` (rows of any stride)."""
     nb = -(-n // BLOCK)
-    if rows <= 0 or n <= 0 or Wp.dtype != torch.uint8 or not Wp.is_contiguous() or \
-            Wp.numel() < lib.tlm_hip_fp8_packed_bytes(rows, n):
+    if rows <= 0 or n <= 0 or Wp.dtype is not _U8 or not Wp.is_contiguous() or Wp.numel() < _packed_bytes(rows, n):
         raise ValueError(f"Wp is not a packed matrix of {rows} x {n}")
-    if codes.dtype not in _CODES or codes.dim() != 2 or codes.shape[1] != nb * BLOCK or not codes.is_contiguous():
+    shape = codes.shape
+    if codes.dtype not in _CODES or len(shape) != 2 or shape[1] != nb * BLOCK or not codes.is_contiguous():
         raise ValueError(f"codes must be contiguous E4M3 [T, {nb * BLOCK}]")
-    T = codes.shape[0]
-    if scale.shape != (T, nb) or scale.dtype != torch.float32 or not scale.is_contiguous():
+    T = shape[0]
+    if scale.shape != (T, nb) or scale.dtype is not _F32 or not scale.is_contiguous():
         raise ValueError(f"scale must be contiguous float32 [{T}, {nb}]")
     if out is None:
-        if dtype not in _TYPES:
+        dt = _TYPES.get(dtype)
+        if dt is None:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        out = Wp.new_empty((T, rows), dtype=dtype)
-        dt = _TYPES[dtype]
+        out = scale.new_empty((T, rows)) if dt == 0 else scale.new_empty((T, rows), dtype=dtype)
     else:
         dt = _TYPES.get(out.dtype)
         if out.shape != (T, rows) or dt is None or not _rows_ok(out):
