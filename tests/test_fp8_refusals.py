@@ -90,6 +90,9 @@ def test_moe_refuses_calls():
     assert moe(d, h=None) == EINVAL and moe(d, out=None) == EINVAL and moe(d, ws=None) == EINVAL
     assert moe(d, ws=C.c_void_p((1 << 20) + 128)) == EINVAL and moe(d, h=HALF) == EINVAL and moe(d, out=HALF) == EINVAL
     assert moe(d, ids=HALF) == EINVAL and moe(d, w=HALF) == EINVAL
+    assert moe(desc(router_bias=HALF)) == EINVAL and moe(desc(shared_gate_inp=HALF)) == EINVAL
+    for off in (4, 4 * 512 - 4):                                       # out begins inside h, or h inside out
+        assert moe(d, out=C.c_void_p((1 << 20) + off)) == EINVAL and moe(d, h=C.c_void_p((1 << 20) + off)) == EINVAL
     assert moe(d, T=65) == ERANGE and moe(d, T=-1) == ERANGE
     assert moe(d, T=0, h=None, out=None, ws=None) == 0
     assert lib.tlm_hip_fp8_moe(None, P, P, 1, None, None, P, None) == EINVAL

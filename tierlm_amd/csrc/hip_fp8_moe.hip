@@ -961,8 +961,11 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     if ((uintptr_t)workspace & 255u)
         return tlmh_seterr(TLM_HIP_EINVAL, "fp8_moe: workspace must be 256-byte aligned");
     if (((uintptr_t)h | (uintptr_t)out | (uintptr_t)ids | (uintptr_t)w | (uintptr_t)d->ffn_norm |
-         (uintptr_t)d->router_w) & 3u)
+         (uintptr_t)d->router_w | (uintptr_t)d->router_bias | (uintptr_t)d->shared_gate_inp) & 3u)
         return tlmh_seterr(TLM_HIP_EINVAL, "fp8_moe: tensors must be 4-byte aligned");
+    const uintptr_t gap = (uintptr_t)h < (uintptr_t)out ? (uintptr_t)out - (uintptr_t)h : (uintptr_t)h - (uintptr_t)out;
+    if (gap && gap < (size_t)T * (size_t)d->D * 4)   /* a token's group reads h where another's has stored */
+        return tlmh_seterr(TLM_HIP_EINVAL, "fp8_moe: out must be h itself or not overlap it");
     Args a{};
     a.d = *d;
     a.L = layout(*d, T);
