@@ -168,10 +168,10 @@ __device__ __forceinline__ void store4(const MmArgs &a, int64_t t, int64_t r, f3
  * at piece ^ row % 8, so that neither side meets a bank twice.  Fetched in that order straight from memory,
  * every quarter of a wave touches 16 lines for 16 bytes each, and those look-ups bound it: 64 tokens
  * of 4096 x 4096 14.6 us, 512 x 16384 46; now 8.2 and 10.
- *   EXACT takes the codes as bfloat16 (exact), whose instructions sum in full floats where the 8-bit
- * ones do not; for few tokens the weights' bytes or the tokens' way through L2 bound either.
+ *   Codes go to the matrix cores as bfloat16 (exact), whose instructions sum in full floats where the 8-bit
+ * ones do not; the weights' bytes or the tokens' way through L2 bound either.
  *   One token: 151936 x 2048 in 45.5 us (6.8 TB/s), 4096 x 4096 5.0, 2048 x 2048 3.5. */
-template <bool EXACT, int KW, int RT, int TT>
+template <int KW, int RT, int TT>
 __global__ __launch_bounds__(64 * KW) void k_fp8_rows(MmArgs a) {
     constexpr int XB = TT * FP8_UNIT;   /* a block of the group's tokens */
     constexpr int PW = XB > RT * TT * 1024 ? XB : RT * TT * 1024;
@@ -223,25 +223,20 @@ __global__ __launch_bounds__(64 * KW) void k_fp8_rows(MmArgs a) {
 #pragma unroll
             for (int h = 0; h < 2; h++) *(LAS i32x4 *)(sx + j * FP8_UNIT + h * 1024 + at_w) = n.x[j][h];
         bf16x8 wf[RT][4];
-        if constexpr (EXACT)
 #pragma unroll
-            for (int i = 0; i < RT; i++)
+        for (int i = 0; i < RT; i++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) wf[i][k] = fp8_to_bf16(n.w[i][k >> 1][2 * (k & 1)], n.w[i][k >> 1][2 * (k & 1) + 1]);
+            for (int k = 0; k < 4; k++) wf[i][k] = fp8_to_bf16(n.w[i][k >> 1][2 * (k & 1)], n.w[i][k >> 1][2 * (k & 1) + 1]);
 #pragma unroll
         for (int j = 0; j < TT; j++) {
             const i32x4 q0 = *(const LAS i32x4 *)(sx + j * FP8_UNIT + at_r0), q1 = *(const LAS i32x4 *)(sx + j * FP8_UNIT + at_r1);
+            const bf16x8 xf[4] = {fp8_to_bf16(q0[0], q0[1]), fp8_to_bf16(q0[2], q0[3]), fp8_to_bf16(q1[0], q1[1]),
+                                  fp8_to_bf16(q1[2], q1[3])};
             f32x4 p[RT] = {};
-            if constexpr (EXACT) {
-                const bf16x8 xf[4] = {fp8_to_bf16(q0[0], q0[1]), fp8_to_bf16(q0[2], q0[3]), fp8_to_bf16(q1[0], q1[1]), fp8_to_bf16(q1[2], q1[3])};
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+            for (int k = 0; k < 4; k++)
 #pragma unroll
-                    for (int i = 0; i < RT; i++) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i][k], xf[k], p[i], 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int i = 0; i < RT; i++) p[i] = fp8_mfma(fp8_join(n.w[i][0], n.w[i][1]), fp8_join(q0, q1), p[i]);
-            }
+                for (int i = 0; i < RT; i++) p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[i][k], xf[k], p[i], 0, 0, 0);
             const float sc = n.ws * n.xs[j];
 #pragma unroll
             for (int i = 0; i < RT; i++)
@@ -515,71 +510,85 @@ template <bool EXACT, int S, int WM, int WN, int TM, int TN> void launch_tile(co
     hipLaunchKernelGGL((k_fp8_tile<EXACT, S, WM, WN, TM, TN>), dim3((unsigned)(mt * nt)), dim3(64 * WM * WN), 0, s, a,
                        (int)mt, (int)nt);
 }
-template <bool EXACT, int KW, int RT, int TT> void launch_rows(const MmArgs &a, hipStream_t s) {
+template <int KW, int RT, int TT> void launch_rows(const MmArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)((fp8_tiles(a.rows) + RT - 1) / RT), (unsigned)((a.T + 16 * TT - 1) / (16 * TT)));
-    hipLaunchKernelGGL((k_fp8_rows<EXACT, KW, RT, TT>), grid, dim3(64 * KW), 0, s, a);
+    hipLaunchKernelGGL((k_fp8_rows<KW, RT, TT>), grid, dim3(64 * KW), 0, s, a);
 }
 
-/* Which kernel.  Tiles through LDS once those of 128 x 64 give every one of the 256 compute units one and
- * there are more than 32 tokens and 64 rows (float results: 64 tokens of 151936 x 2048 83 us against 97 in row
- * groups, 512 of 4096 x 4096 25 against 27.6, but 256 of them 24 against 15).
- *   Of the tiles the largest that still gives every unit one (16-bit results: 512 tokens of 4096 x 4096
- * 26 us in 128 x 128 and 21 in 128 x 64; 1024 tokens 37.0 in 128 x 64 and 28.1 in 128 x 128; 4096 tokens
- * of 8192 x 4096 175 in 128 x 128 and 139 in 256 x 256) and does not pad the tokens to over 4 / 3 of
- * what half its width would (64 tokens of 151936 x 2048 107 us in 256 x 256, 75 in 128 x 64; 192 of
- * 16384 x 2048 17.4 in 128 x 128, 22.7 in 128 x 64).  128 x
- * 128 takes four stages while a unit has one tile (28.1 against 33.2 us with two at 1024 tokens), two
- * stages and two groups a unit beyond (25.8 against 30.0 at 2048 x 4096 x 2048).
- *   Row groups take the largest of 64 x 64, 64 x 32, 32 x 32, 32 x 16 and 16 x 16 with a group for every
- * unit (4096 x 4096: 32 tokens 6.3 us in 32 x 16, 7.5 in 16 x 16; 128 tokens 10.1 in 64 x 32, 12.3 in
- * 32 x 32), 64 x 64 only for long rows (512 tokens of 2048 x 2048 9.8 in 64 x 64, 9.1 in 64 x 32; 256 of
- * 4096 x 4096 15.0 and 16.2).  Few tokens leave the weights' bytes, so that two row tiles a group pay from 9
- * tokens on or with 4 groups a unit (8192 x 4096: 16 tokens 8.6 us with two, 9.8 with one; 4 tokens 8.7
- * and 8.1; 151936 x 2048, 4 tokens 46.6 and 52).
- *   Waves a group: 8 while a unit has about one group, 4 where there are more (64 x 32: 128 tokens of 4096 x
- * 4096 10.1 us with 8, 11.0 with 4; 192 tokens 15.5 and 14.2); 16 x 16 has 16 for rows of 64 blocks or
- * more (512 x 16384, one token 7.6 us against 9.8 with 8), 32 x 16 where a unit has two groups or more
- * (16 tokens of 151936 x 2048 52 against 57.5). */
+/* Which kernel.  Up to 16 tokens the weights' bytes bound it: row groups of 16 rows, or of 32 that share the
+ * tokens' reads, from 9 tokens on with a group for every compute unit, for fewer with four (8192 x 4096: 16
+ * tokens 8.6 us in groups of 32, 9.8 in 16; 4 tokens 8.7 and 8.1; 151936 x 2048, 4 tokens 46.6 and 52); 16 waves
+ * a group for long rows (512 x 16384, one token 7.6 us against 9.8 with 8; 151936 x 2048, 16 tokens 52 and 57.5).
+ *   More tokens: the kernel whose estimate is least.  With `steps` blocks of a row a wave and q groups on the
+ * fullest unit,  us = start + max(steps * run, q * (group + steps * block)):  run is a step's latency, block its
+ * share of the unit's throughput, group what a group costs besides.  Fitted to 800 sizes, random ones and
+ * multiples of large powers of two, over 17..4096 tokens, 64..60000 rows and 2..128 blocks, weights from memory:
+ * the least estimate's kernel took 2.4% (float results) and 2.9% (16-bit) longer than the fastest of fifteen, in
+ * the geometric mean; the largest kernel with a group for every unit took 9% and 13%.  4096 x 4096: 32 tokens 6.4
+ * us in 32 x 16 and 8.5 in 32 x 32, 128 tokens 10.1 in 64 x 32 and 12.2 in 32 x 32, 512 tokens 21.6 in the tiles of
+ * 128 x 64 and 31 in 128 x 128; 8192 x 4096, 4096 tokens, 16-bit, 137 in 256 x 256 and 175 in 128 x 128. */
+struct Cost {
+    int m, n, waves;   /* rows and tokens of a group; the waves that share a row's blocks */
+    float start, group, run, block;
+};
+enum { ROWS16, ROWS32, SQUARE32, SQUARE32W8, ROWS64, SQUARE64, EXACT64, EXACT128X64, EXACT128X64S4, EXACT128, FAST64, FAST128X64,
+       FAST128, FAST128S4, FAST256, KERNELS };
+constexpr Cost COSTS[KERNELS] = {
+    /* row groups: any result */
+    {16, 16, 8, 2.0f, 0.0f, 0.54f, 0.455f}, {32, 16, 8, 2.0f, 0.0f, 0.66f, 0.69f}, {32, 32, 4, 2.5f, 0.0f, 0.4f, 0.51f},
+    {32, 32, 8, 2.25f, 0.0f, 0.3f, 1.0f}, {64, 32, 8, 1.35f, 0.95f, 1.5f, 1.51f}, {64, 64, 4, 1.7f, 2.0f, 0.05f, 1.34f},
+    /* tiles, exact sums, for float results and up to 32 tokens: two stages, two, four, two */
+    {64, 64, 1, 2.85f, 0.05f, 0.46f, 0.329f}, {128, 64, 1, 3.35f, 0.14f, 0.65f, 0.505f},
+    {128, 64, 1, 2.25f, 1.75f, 0.60f, 0.594f}, {128, 128, 1, 4.25f, 0.0f, 0.95f, 0.829f},
+    /* tiles, the 8-bit matrix instructions: four stages, four, two, four and two.  (The first's latency where
+     * every unit has one and the weights come from memory; fitted, 0.23.) */
+    {64, 64, 1, 2.55f, 0.8f, 0.42f, 0.257f}, {128, 64, 1, 1.8f, 2.45f, 0.44f, 0.421f}, {128, 128, 1, 3.6f, 1.25f, 0.66f, 0.558f},
+    {128, 128, 1, 1.5f, 3.95f, 0.5f, 0.517f}, {256, 256, 1, 0.1f, 8.3f, 1.41f, 1.34f}};
 void launch_mm(const MmArgs &a, hipStream_t s) {
     constexpr int64_t CUS = 256;
-    const bool exact = a.dt == DT_F32;
-    auto up = [&](int n) { return (a.T + n - 1) / n; };
-    auto count = [&](int m, int n) { return (a.rows + m - 1) / m * up(n); };
-    auto fits = [&](int m, int n) { return count(m, n) >= CUS && 3 * n * up(n) <= 4 * (n / 2) * up(n / 2); };
-    if (a.T > 32 && (a.rows > 64 || a.T > 65536) && (count(128, 64) >= CUS || (a.nb >= 32 && count(64, 64) > CUS))) {
-        if (exact) {
-            if (fits(128, 128)) launch_tile<true, 2, 2, 2, 4, 4>(a, s);
-            else launch_tile<true, 4, 2, 2, 4, 2>(a, s);
+    auto count = [&](int m, int n) { return ((a.rows + m - 1) / m) * ((a.T + n - 1) / n); };
+    const int nb = a.nb;
+    if (a.T <= 16) {
+        if (count(32, 16) >= (a.T > 8 ? CUS : 4 * CUS)) {
+            if (nb < 16) launch_rows<8, 2, 1>(a, s);
+            else launch_rows<16, 2, 1>(a, s);
         } else {
-            if (fits(256, 256)) launch_tile<false, 2, 2, 4, 8, 4>(a, s);
-            else if (fits(128, 128) && count(128, 128) >= 2 * CUS) launch_tile<false, 2, 2, 2, 4, 4>(a, s);
-            else if (fits(128, 128)) launch_tile<false, 4, 2, 2, 4, 4>(a, s);
-            else launch_tile<false, 4, 2, 2, 4, 2>(a, s);
+            if (nb < 64) launch_rows<8, 1, 1>(a, s);
+            else launch_rows<16, 1, 1>(a, s);
         }
         return;
     }
-    const int nb = a.nb;
-    auto fills = [&](int m, int n) { return count(m, n) >= CUS && 2 * a.rows > m && 2 * a.T > n; };   /* over half of a group used */
-    if (nb >= 32 && fills(64, 64)) {
-        if (exact) launch_rows<true, 4, 4, 4>(a, s);
-        else launch_rows<false, 4, 4, 4>(a, s);
-    } else if (fills(64, 32)) {
-        const bool few = 2 * count(64, 32) < 3 * CUS && nb >= 8, eight = !exact && a.T > 32;
-        if (few && eight) launch_rows<false, 8, 4, 2>(a, s);
-        else if (few) launch_rows<true, 8, 4, 2>(a, s);
-        else if (eight) launch_rows<false, 4, 4, 2>(a, s);
-        else launch_rows<true, 4, 4, 2>(a, s);
-    } else if (fills(32, 32)) {
-        if (2 * count(32, 32) < 3 * CUS && nb >= 8) launch_rows<true, 8, 2, 2>(a, s);
-        else launch_rows<true, 4, 2, 2>(a, s);
-    } else if (a.rows > 16 && count(32, 16) >= (a.T > 8 ? 3 * CUS / 4 : 4 * CUS)) {
-        if (nb < 8) launch_rows<true, 4, 2, 1>(a, s);
-        else if (count(32, 16) < 2 * CUS) launch_rows<true, 8, 2, 1>(a, s);
-        else launch_rows<true, 16, 2, 1>(a, s);
-    } else {
-        if (nb < 8) launch_rows<true, 4, 1, 1>(a, s);
-        else if (nb < 64) launch_rows<true, 8, 1, 1>(a, s);
-        else launch_rows<true, 16, 1, 1>(a, s);
+    const bool exact = a.dt == DT_F32 || a.T <= 32;
+    int pick = -1;
+    float least = 0.0f;
+    for (int i = 0; i < KERNELS; i++) {
+        if (i > SQUARE64 && (i < FAST64) != exact) continue;
+        const Cost &c = COSTS[i];
+        if (i <= SQUARE64 && a.T > 65535 * (int64_t)c.n) continue;   /* their tokens are the grid's second axis */
+        const float steps = (float)((nb + c.waves - 1) / c.waves), q = (float)((count(c.m, c.n) + CUS - 1) / CUS);
+        const float run = steps * c.run, full = q * (c.group + steps * c.block);
+        const float us = c.start + (run > full ? run : full);
+        if (pick < 0 || us < least) {
+            pick = i;
+            least = us;
+        }
+    }
+    switch (pick) {
+    case ROWS16: launch_rows<8, 1, 1>(a, s); break;
+    case ROWS32: launch_rows<8, 2, 1>(a, s); break;
+    case SQUARE32: launch_rows<4, 2, 2>(a, s); break;
+    case SQUARE32W8: launch_rows<8, 2, 2>(a, s); break;
+    case ROWS64: launch_rows<8, 4, 2>(a, s); break;
+    case SQUARE64: launch_rows<4, 4, 4>(a, s); break;
+    case EXACT64: launch_tile<true, 2, 2, 2, 2, 2>(a, s); break;
+    case EXACT128X64: launch_tile<true, 2, 2, 2, 4, 2>(a, s); break;
+    case EXACT128X64S4: launch_tile<true, 4, 2, 2, 4, 2>(a, s); break;
+    case EXACT128: launch_tile<true, 2, 2, 2, 4, 4>(a, s); break;
+    case FAST64: launch_tile<false, 4, 2, 2, 2, 2>(a, s); break;
+    case FAST128X64: launch_tile<false, 4, 2, 2, 4, 2>(a, s); break;
+    case FAST128: launch_tile<false, 2, 2, 2, 4, 4>(a, s); break;
+    case FAST128S4: launch_tile<false, 4, 2, 2, 4, 4>(a, s); break;
+    default: launch_tile<false, 2, 2, 4, 8, 4>(a, s);
     }
 }
 
