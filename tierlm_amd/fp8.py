@@ -23,7 +23,7 @@ MOE_MAX_TOKENS = 64             # TLM_HIP_FP8_MOE_MAX_TOKENS
 E4M3 = torch.float8_e4m3fn
 _CODES = (E4M3, torch.uint8)
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_U8, _F32 = torch.uint8, torch.float32
+_U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
 _pack, _quantize, _matmul, _moe = (lib.tlm_hip_fp8_pack, lib.tlm_hip_fp8_quantize, lib.tlm_hip_fp8_matmul,
                                    lib.tlm_hip_fp8_moe)
 _packed_bytes = lib.tlm_hip_fp8_packed_bytes
@@ -180,7 +180,8 @@ class MoeBlock:
         self._desc = C.byref(self.desc)
         self.D, self.k = D, k
         check(_moe(self._desc, None, None, 0, None, None, None, None))   # the sizes fit
-        self.workspace, self._room, self._earlier = None, 0, []
+        self._dev = ffn_norm.get_device()
+        self.workspace, self._pws, self._room, self._earlier = None, None, 0, []
 
     def reserve(self, T):
         """Make the workspace large enough for T tokens (it at least doubles; a smaller one that a
@@ -193,34 +194,41 @@ class MoeBlock:
             if self.workspace is not None:
                 self._earlier.append(self.workspace)
             self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            self._pws = self.workspace.data_ptr()
             self._room = room
 
     def __call__(self, h, out=None, ids=None, w=None):
         """out = h + MoE(h) for h (f32 [T, D] or [D]), T <= 64; without `out` h itself
         is updated.  ids (int32) / w (f32), [T, k], receive the routing.  Returns
         out."""
-        if h.dtype != torch.float32 or not h.is_contiguous() or h.dim() not in (1, 2) or h.shape[-1] != self.D:
+        shape = h.shape
+        if h.dtype is not _F32 or not h.is_contiguous() or len(shape) not in (1, 2) or shape[-1] != self.D:
             raise ValueError(f"h must be contiguous float32 [T, {self.D}]")
-        T = h.shape[0] if h.dim() == 2 else 1
+        T = shape[0] if len(shape) == 2 else 1
+        dev, ph = h.get_device(), h.data_ptr()
+        if dev != self._dev or dev != _current_device():
+            _here(h, self.table)
+        po = pi = pw = None
         if out is None:
-            out = h
+            out, po = h, ph
         else:
-            _out(out, h.shape, torch.float32, h, "out")
-            gap = abs(out.data_ptr() - h.data_ptr())
-            if 0 < gap < 4 * h.numel():
+            if out.shape != shape or out.dtype is not _F32 or not out.is_contiguous() or out.get_device() != dev:
+                _here(h, _out(out, shape, _F32, h, "out"))
+            po = out.data_ptr()
+            if po != ph and abs(po - ph) < 4 * T * self.D:
                 raise ValueError("out must be h itself or not overlap it")
-        dev = _here(h, out, self.table)
-        pi = pw = None
         if ids is not None:
-            _here(_out(ids, (T, self.k), torch.int32, h, "ids"))
+            if ids.shape != (T, self.k) or ids.dtype is not _I32 or not ids.is_contiguous() or ids.get_device() != dev:
+                _here(h, _out(ids, (T, self.k), _I32, h, "ids"))
             pi = ids.data_ptr()
         if w is not None:
-            _here(_out(w, (T, self.k), torch.float32, h, "w"))
+            if w.shape != (T, self.k) or w.dtype is not _F32 or not w.is_contiguous() or w.get_device() != dev:
+                _here(h, _out(w, (T, self.k), _F32, h, "w"))
             pw = w.data_ptr()
         if T > self._room:
             self.reserve(T)
         if T:
-            rc = _moe(self._desc, h.data_ptr(), out.data_ptr(), T, pi, pw, self.workspace.data_ptr(), _raw_stream(dev))
+            rc = _moe(self._desc, ph, po, T, pi, pw, self._pws, _raw_stream(dev))
             if rc:
                 check(rc)
         return out
