@@ -250,7 +250,7 @@ def test_linear_streams_and_graph(hip, T):
         torch.cuda.synchronize()
 
 
-# (T, rows) at which each size of tile is taken: fp32 results up to 128 x 128, 16-bit ones up to 256 x 256
+# (T, rows) of large products, whose tiles stream through LDS
 TILES = [(100, 5000), (100, 8100), (100, 16300), (250, 16300), (250, 32700), (250, 65300), (33, 66000)]
 
 
@@ -258,8 +258,8 @@ TILES = [(100, 5000), (100, 8100), (100, 16300), (250, 16300), (250, 32700), (25
 @pytest.mark.parametrize("n", [100, 256, 300, 512, 900])
 @pytest.mark.parametrize("T,rows", TILES)
 def test_matmul_tiles(hip, T, rows, n, dtype):
-    """Every tile size with part tiles of rows and tokens and one to eight blocks of values (the stages'
-    whole and part rounds), the tokens' scales spread over powers of two."""
+    """Part tiles of rows and tokens and one to eight blocks of values (the stages' whole and part rounds), the
+    tokens' scales spread over powers of two."""
     g = gen(T + rows + n)
     w, s = matrix(g, rows, n)
     codes, scale = fp8.quantize(randn(g, T, n) * torch.exp2(torch.randint(-6, 7, (T, 1), generator=g, device="cuda")))
@@ -267,9 +267,12 @@ def test_matmul_tiles(hip, T, rows, n, dtype):
     check_product(fp8.matmul(fp8.pack(w, s), rows, n, codes, scale, dtype=dtype), w, s, codes, scale, n)
 
 
-# (T, rows, n) at which each size of row group is taken: 64 x 64 (long rows), 64 x 32, 32 x 32, 32 x 16 and
-# 16 x 16, few groups and many, short rows and long; then few rows of very many tokens
-GROUPS = [(100, 8200, 4196), (100, 4100, 1100), (30, 16500, 1100), (100, 6500, 1100), (100, 4100, 700),
+# (T, rows, n), one at least for each kernel that the product chooses from (the float results' and the 16-bit
+# ones' differ): few groups and many, short rows and long; then few rows of very many tokens
+GROUPS = [(17, 21, 302), (18, 2101, 308), (17, 4336, 356), (17, 4232, 582), (17, 25365, 303), (18, 8960, 533),
+          (36, 14529, 1677), (34, 12974, 322), (17, 52136, 541), (34, 16717, 2094), (67, 49172, 338), (33, 8290, 626),
+          (33, 18207, 570), (66, 23694, 324), (66, 16901, 1590), (131, 35900, 565), (16, 9000, 2100),
+          (100, 8200, 4196), (100, 4100, 1100), (30, 16500, 1100), (100, 6500, 1100), (100, 4100, 700),
           (30, 25000, 300), (100, 2100, 1100), (25, 9000, 1100), (100, 3200, 1100), (30, 4200, 700),
           (30, 4200, 1100), (16, 16500, 1100), (5, 32800, 1100), (9, 8200, 130), (5, 100, 9000), (16, 40, 700),
           (5000, 10, 300), (40000, 64, 256), (70000, 16, 130), (70000, 70, 130)]

@@ -170,7 +170,7 @@ __device__ __forceinline__ void store4(const MmArgs &a, int64_t t, int64_t r, f3
  * of 4096 x 4096 14.6 us, 512 x 16384 46; now 8.2 and 10.
  *   Codes go to the matrix cores as bfloat16 (exact), whose instructions sum in full floats where the 8-bit
  * ones do not; the weights' bytes or the tokens' way through L2 bound either.
- *   One token: 151936 x 2048 in 45.5 us (6.8 TB/s), 4096 x 4096 5.0, 2048 x 2048 3.5. */
+ *   One token: 151936 x 2048 in 46-52 us (6.0-6.8 TB/s), 4096 x 4096 4.9, 2048 x 2048 3.5. */
 template <int KW, int RT, int TT>
 __global__ __launch_bounds__(64 * KW) void k_fp8_rows(MmArgs a) {
     constexpr int XB = TT * FP8_UNIT;   /* a block of the group's tokens */
@@ -287,9 +287,9 @@ __global__ __launch_bounds__(64 * KW) void k_fp8_rows(MmArgs a) {
  * to the largest of them and cut what lies below 2^-13 of its power of two, about 2^-16 of the
  * result on ordinary data: too much for a float result, an eighth of the rounding of a binary16
  * one, so 16-bit results take the 8-bit instructions and float results EXACT.
- *   4096 tokens, 8192 x 4096: 135 us, 2.03 PFLOP/s for 16-bit results (the matrix pipe is busy
- * 45% of the time; without the loads the same loop takes 106 us), 250 us, 1.1 PFLOP/s
- * for float ones. */
+ *   4096 tokens, 8192 x 4096: 131-137 us, 2.0-2.1 PFLOP/s for 16-bit results (the matrix pipe is busy
+ * 45% of the time; the matrix instructions alone, without loads, LDS reads and most of the fold, take
+ * 108 us), 245 us, 1.1 PFLOP/s for float ones. */
 /* waves a SIMD that the stages' LDS leaves room for, up to two */
 constexpr int tile_waves(int s, int waves, int units) { return waves >= 8 || 2 * s * (units * FP8_UNIT + 256 * waves) <= 160 * 1024 ? 2 : 1; }
 template <bool EXACT, int S, int WM, int WN, int TM, int TN>
@@ -523,7 +523,7 @@ template <int KW, int RT, int TT> void launch_rows(const MmArgs &a, hipStream_t 
  * fullest unit,  us = start + max(steps * run, q * (group + steps * block)):  run is a step's latency, block its
  * share of the unit's throughput, group what a group costs besides.  Fitted to 800 sizes, random ones and
  * multiples of large powers of two, over 17..4096 tokens, 64..60000 rows and 2..128 blocks, weights from memory:
- * the least estimate's kernel took 2.4% (float results) and 2.9% (16-bit) longer than the fastest of fifteen, in
+ * the least estimate's kernel took 2.2% (float results) and 2.9% (16-bit) longer than the fastest of fifteen, in
  * the geometric mean; the largest kernel with a group for every unit took 9% and 13%.  4096 x 4096: 32 tokens 6.4
  * us in 32 x 16 and 8.5 in 32 x 32, 128 tokens 10.1 in 64 x 32 and 12.2 in 32 x 32, 512 tokens 21.6 in the tiles of
  * 128 x 64 and 31 in 128 x 128; 8192 x 4096, 4096 tokens, 16-bit, 137 in 256 x 256 and 175 in 128 x 128. */
@@ -531,12 +531,13 @@ struct Cost {
     int m, n, waves;   /* rows and tokens of a group; the waves that share a row's blocks */
     float start, group, run, block;
 };
-enum { ROWS16, ROWS32, SQUARE32, SQUARE32W8, ROWS64, SQUARE64, EXACT64, EXACT128X64, EXACT128X64S4, EXACT128, FAST64, FAST128X64,
-       FAST128, FAST128S4, FAST256, KERNELS };
+enum { ROWS16, ROWS32, SQUARE32, SQUARE32W8, ROWS64, ROWS64W8, SQUARE64, EXACT64, EXACT128X64, EXACT128X64S4, EXACT128, FAST64,
+       FAST128X64, FAST128, FAST128S4, FAST256, KERNELS };
 constexpr Cost COSTS[KERNELS] = {
     /* row groups: any result */
     {16, 16, 8, 2.0f, 0.0f, 0.54f, 0.455f}, {32, 16, 8, 2.0f, 0.0f, 0.66f, 0.69f}, {32, 32, 4, 2.5f, 0.0f, 0.4f, 0.51f},
-    {32, 32, 8, 2.25f, 0.0f, 0.3f, 1.0f}, {64, 32, 8, 1.35f, 0.95f, 1.5f, 1.51f}, {64, 64, 4, 1.7f, 2.0f, 0.05f, 1.34f},
+    {32, 32, 8, 2.25f, 0.0f, 0.3f, 1.0f}, {64, 32, 4, 2.85f, 0.0f, 0.9f, 0.81f},
+    {64, 32, 8, 1.35f, 0.95f, 1.5f, 1.51f}, {64, 64, 4, 1.7f, 2.0f, 0.05f, 1.34f},
     /* tiles, exact sums, for float results and up to 32 tokens: two stages, two, four, two */
     {64, 64, 1, 2.85f, 0.05f, 0.46f, 0.329f}, {128, 64, 1, 3.35f, 0.14f, 0.65f, 0.505f},
     {128, 64, 1, 2.25f, 1.75f, 0.60f, 0.594f}, {128, 128, 1, 4.25f, 0.0f, 0.95f, 0.829f},
@@ -578,7 +579,8 @@ void launch_mm(const MmArgs &a, hipStream_t s) {
     case ROWS32: launch_rows<8, 2, 1>(a, s); break;
     case SQUARE32: launch_rows<4, 2, 2>(a, s); break;
     case SQUARE32W8: launch_rows<8, 2, 2>(a, s); break;
-    case ROWS64: launch_rows<8, 4, 2>(a, s); break;
+    case ROWS64: launch_rows<4, 4, 2>(a, s); break;
+    case ROWS64W8: launch_rows<8, 4, 2>(a, s); break;
     case SQUARE64: launch_rows<4, 4, 4>(a, s); break;
     case EXACT64: launch_tile<true, 2, 2, 2, 2, 2>(a, s); break;
     case EXACT128X64: launch_tile<true, 2, 2, 2, 4, 2>(a, s); break;
