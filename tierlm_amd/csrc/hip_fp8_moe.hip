@@ -989,7 +989,7 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
         const unsigned ys = (unsigned)(a.slots * a.ce + a.cs), xs = (unsigned)wide * 8;
         /* Routing in the gate/up launch saves one, and each group the work of a rank: worth it up to
          * 6 groups a compute unit (2048 x 768, 128 experts: 2 tokens, 768 groups, 26.5 against 28.6 us,
-         * 4 tokens, 1536 groups, 40.5 and 40.6, 8 tokens, 3072 groups, 62.8 and 60.6; 1000 x 300, 32
+         * 4 tokens, 1536 groups, 40.5 and 40.6, 8 tokens, twice as many, 62.8 and 60.6; 1000 x 300, 32
          * experts, 8 tokens, 768 groups, 18.9 and 21.6). */
         if (T <= ROUTES && xs * ys <= GROUPS) {   /* one more row of groups: one a token routes */
             hipLaunchKernelGGL(k_fm_gateup<true>, dim3(xs > (unsigned)T ? xs : (unsigned)T, ys + 1), dim3(64 * NW), 0, s, a);
