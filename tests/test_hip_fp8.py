@@ -326,3 +326,46 @@ def test_two_calls_at_once(hip):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(v, want[i]) for v in got[i])
+
+
+def test_offsets_past_32_bits(hip):
+    """A matrix, a result and activations of more than 4 GB each: their first, middle and last parts."""
+    g = gen(80)
+    rows, n = 70001, 65500
+    w = torch.randint(0, 120, (rows, n), generator=g, device="cuda", dtype=torch.uint8).view(E4M3)
+    s = torch.exp(0.5 * randn(g, -(-rows // 128), -(-n // 128))) * 0.01
+    P = fp8.pack(w, s)
+    assert P.numel() > 1 << 32
+    for T in (1, 20, 300):
+        codes, scale = fp8.quantize(randn(g, T, n))
+        Y = fp8.matmul(P, rows, n, codes, scale)
+        for r in (0, 34944, 69888):                       # a block of 128 rows from each on
+            e = min(r + 128, rows)
+            check_product(Y[:, r:e], w[r:e], s[r // 128:r // 128 + 1], codes, scale, n)
+    del w, P, Y
+    T, rows, n = 40001, 30003, 128
+    w, s = matrix(g, rows, n)
+    codes, scale = fp8.quantize(randn(g, T, n))
+    Y = fp8.matmul(fp8.pack(w, s), rows, n, codes, scale)
+    assert Y.numel() * 4 > 1 << 32
+    for t in (0, 20000, T - 100):
+        check_product(Y[t:t + 100], w, s, codes[t:t + 100], scale[t:t + 100], n)
+    del Y
+    T, n = 33001, 65536
+    x = torch.randn(T, n, generator=g, device="cuda", dtype=torch.bfloat16)
+    codes, scale = fp8.quantize(x)
+    for t in (0, 16500, T - 3):
+        want, ws = ref_quantize(x[t:t + 3].float())
+        assert np.array_equal(codes[t:t + 3].double().cpu().numpy(), want)
+        assert np.array_equal(scale[t:t + 3].cpu().numpy(), ws.astype(np.float32))
+
+
+def test_most_tokens(hip):
+    """2^20 tokens of a few rows: the second axis of a launch has to hold them."""
+    g = gen(81)
+    T, n = 1 << 20, 130
+    codes, scale = fp8.quantize(randn(g, T, n))
+    for rows in (16, 1):
+        w, s = matrix(g, rows, n)
+        Y = fp8.matmul(fp8.pack(w, s), rows, n, codes, scale)
+        check_product(Y, w, s, codes, scale, n)

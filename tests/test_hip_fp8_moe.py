@@ -141,6 +141,16 @@ def test_block_sizes(hip, D, de, E, k, ds, T, router):
     go(c, g, T)
 
 
+@pytest.mark.parametrize("D,de,E,k,T", [(129, 257, 256, 32, 64), (512, 128, 128, 2, 24), (1024, 256, 128, 4, 10),
+                                        (4096, 512, 16, 4, 14), (1000, 300, 8, 4, 4), (2048, 130, 40, 3, 16),
+                                        (300, 2000, 64, 8, 12), (7, 3, 1, 1, 64)])
+def test_block_launches(hip, D, de, E, k, T):
+    """Each way through the launches: routed in gate/up or before it, down per token or per expert, experts with
+    as many tokens as there are."""
+    c, g = build(D + de + T, D, de, E, k)
+    go(c, g, T)
+
+
 @pytest.mark.parametrize("T", [1, 4, 21, 64])
 def test_crowded_experts(hip, T):
     """Every token near one direction: the same few experts for all of them."""
