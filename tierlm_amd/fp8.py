@@ -94,17 +94,21 @@ def quantize(x, codes=None, scale=None):
     if x.dim() == 1:
         x = x[None]
     dt = _TYPES.get(x.dtype)
-    if dt is None or not _rows_ok(x) or x.shape[1] == 0:
+    if dt is None or not _rows_ok(x):
         raise ValueError("x must be float32, float16 or bfloat16 [T, n] with contiguous rows")
     T, n = x.shape
+    if n == 0:
+        raise ValueError("x must have at least one value a row")
     nb = -(-n // BLOCK)
-    dev = _here(x)
+    dev = x.get_device()
+    if dev < 0 or dev != _current_device():
+        _here(x)
     if codes is None:
-        codes = x.new_empty((T, nb * BLOCK), dtype=E4M3)
+        codes = x.new_empty(T, nb * BLOCK, dtype=E4M3)
     elif _out(codes, (T, nb * BLOCK), E4M3, x, "codes").get_device() != dev:
         _here(x, codes)
     if scale is None:
-        scale = x.new_empty((T, nb)) if dt == 0 else x.new_empty((T, nb), dtype=torch.float32)
+        scale = x.new_empty(T, nb) if dt == 0 else x.new_empty(T, nb, dtype=_F32)
     elif _out(scale, (T, nb), torch.float32, x, "scale").get_device() != dev:
         _here(x, scale)
     rc = _quantize(dt, x.data_ptr(), x.stride(0), n, T, codes.data_ptr(), scale.data_ptr(), _raw_stream(dev))
@@ -129,13 +133,16 @@ def matmul(Wp, rows, n, codes, scale, out=None, dtype=torch.float32):
         dt = _TYPES.get(dtype)
         if dt is None:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        out = scale.new_empty((T, rows)) if dt == 0 else scale.new_empty((T, rows), dtype=dtype)
+        out = scale.new_empty(T, rows) if dt == 0 else scale.new_empty(T, rows, dtype=dtype)
     else:
         dt = _TYPES.get(out.dtype)
         if out.shape != (T, rows) or dt is None or not _rows_ok(out):
             raise ValueError(f"out must be float32, float16 or bfloat16 [{T}, {rows}] with contiguous rows")
-    rc = _matmul(Wp.data_ptr(), rows, n, codes.data_ptr(), scale.data_ptr(), T, dt, out.data_ptr(),
-                 out.stride(0), _raw_stream(_here(Wp, codes, scale, out)))
+    dev = Wp.get_device()
+    if dev < 0 or not dev == codes.get_device() == scale.get_device() == out.get_device() == _current_device():
+        _here(Wp, codes, scale, out)
+    rc = _matmul(Wp.data_ptr(), rows, n, codes.data_ptr(), scale.data_ptr(), T, dt, out.data_ptr(), out.stride(0),
+                 _raw_stream(dev))
     if rc:
         check(rc)
     return out
