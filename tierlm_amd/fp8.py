@@ -75,11 +75,14 @@ def pack(W, scale, out=None):
         raise ValueError("W must be a 2-D float8_e4m3fn or uint8 tensor with contiguous rows")
     rows, n = W.shape
     nr, nb = -(-rows // BLOCK), -(-n // BLOCK)
-    if scale.shape != (nr, nb) or scale.dtype != torch.float32 or not _rows_ok(scale):
+    if scale.shape != (nr, nb) or scale.dtype is not _F32 or not _rows_ok(scale):
         raise ValueError(f"scale must be float32 [{nr}, {nb}] with contiguous rows")
-    dev = _here(W, scale)
-    out = _out(out, (_packed_bytes(rows, n),), torch.uint8, W, "out")
-    if out.get_device() != dev or out.data_ptr() % 16:
+    dev = W.get_device()
+    if dev < 0 or not dev == scale.get_device() == _current_device():
+        _here(W, scale)
+    if out is None:
+        out = W.new_empty(_packed_bytes(rows, n), dtype=_U8)
+    elif _out(out, (_packed_bytes(rows, n),), _U8, W, "out").get_device() != dev or out.data_ptr() % 16:
         raise ValueError("out must be on the current HIP device, 16-byte aligned")
     rc = _pack(W.data_ptr(), max(W.stride(0), n), scale.data_ptr(), max(scale.stride(0), nb), rows, n, out.data_ptr(),
                _raw_stream(dev))
