@@ -32,11 +32,6 @@ __host__ __device__ static inline size_t fp8_code_bytes(int64_t rows, int64_t n)
     return (size_t)fp8_tiles(rows) * (size_t)fp8_blocks(n) * FP8_UNIT;
 }
 
-/* 128 products per element of a 16 x 16 tile: lane l gives 32 codes of row
- * l % 16 of each operand and gets rows 4 (l / 16) + 0..3 of column l % 16 */
-__device__ __forceinline__ f32x4 fp8_mfma(i32x8 a, i32x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
-}
 __device__ __forceinline__ i32x8 fp8_join(i32x4 lo, i32x4 hi) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
