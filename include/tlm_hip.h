@@ -620,7 +620,8 @@ int    tlm_hip_fp8_matmul(const void *Wp, int64_t rows, int64_t n, const void *c
  * [T x k] (device, may be NULL) receive the routing.  Softmax routing selects by
  * the router's scores, sigmoid routing by score + bias, ties to the lower
  * index; where the mask leaves fewer than k experts the ranks behind them get id
- * -1 and weight 0.  workspace: tlm_hip_fp8_moe_workspace_bytes(d, T) bytes,
+ * -1 and weight 0.  An expert with a null pointer among its three in the table
+ * counts as pruned, masked or not.  Packed matrices are 16-byte aligned.  workspace: tlm_hip_fp8_moe_workspace_bytes(d, T) bytes,
  * 256-byte aligned, nothing in it needs to be kept or zeroed; calls that may
  * overlap (other streams) need different workspaces. */
 #define TLM_HIP_FP8_MOE_MAX_TOKENS 64

@@ -129,8 +129,8 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
     extern __shared__ __align__(16) float s_x[];
     __shared__ double s_red[4];
     const tlm_hip_moe_desc &d = a.d;
-    args_now(d.D, d.E, d.ds, d.router, d.eps, d.ffn_norm, d.router_w, d.router_bias, d.mask, d.shared_gate_inp, a.h, a.ws,
-             a.L.xp, a.L.key, a.L.score, a.L.sgate, a.L.nbd);
+    args_now(d.D, d.E, d.ds, d.router, d.eps, d.ffn_norm, d.router_w, d.router_bias, d.mask, d.experts, d.shared_gate_inp,
+             a.h, a.ws, a.L.xp, a.L.key, a.L.score, a.L.sgate, a.L.nbd);
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), t = blockIdx.y;
     const int D = (int)d.D, Dq = (D + 3) & ~3, e = blockIdx.x * 4 + wave;
     const bool live = e < d.E || (e == d.E && d.ds > 0 && d.shared_gate_inp);
@@ -151,6 +151,9 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
     for (int j = 0; j < NV; j++) wv[j] = row4(w, 4 * lane + 256 * j, D);
     ExpTabLanes tab;
     tab.load();
+    /* an expert without all of its matrices cannot be chosen: no launch after this one follows a null pointer */
+    const void *const GAS *mat = (const void *const GAS *)d.experts + 3 * (size_t)(e < d.E ? e : 0);
+    const bool whole = mat[0] && mat[1] && mat[2];
     double ss = 0.0;
 #pragma unroll
     for (int c = 0; c < NC; c++)
@@ -217,7 +220,7 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
     const float score = d.router == 2 ? sig : l;
     const float sel = d.router == 2 && d.router_bias ? score + d.router_bias[e] : score;
     ((float *)(a.ws + a.L.score))[t * d.E + e] = score;
-    ((uint32_t *)(a.ws + a.L.key))[t * d.E + e] = d.mask && d.mask[e] ? 0u : order_key(sel);
+    ((uint32_t *)(a.ws + a.L.key))[t * d.E + e] = !whole || (d.mask && d.mask[e]) ? 0u : order_key(sel);
 }
 
 /* ---- routing ------------------------------------------------------------------
@@ -963,6 +966,8 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     if (((uintptr_t)h | (uintptr_t)out | (uintptr_t)ids | (uintptr_t)w | (uintptr_t)d->ffn_norm |
          (uintptr_t)d->router_w | (uintptr_t)d->router_bias | (uintptr_t)d->shared_gate_inp) & 3u)
         return tlmh_seterr(TLM_HIP_EINVAL, "fp8_moe: tensors must be 4-byte aligned");
+    if (((uintptr_t)d->experts & 7u) || (d->ds > 0 && (((uintptr_t)d->sg | (uintptr_t)d->su | (uintptr_t)d->sd) & 15u)))
+        return tlmh_seterr(TLM_HIP_EINVAL, "fp8_moe: the table must be 8-byte, packed matrices 16-byte aligned");
     const uintptr_t gap = (uintptr_t)h < (uintptr_t)out ? (uintptr_t)out - (uintptr_t)h : (uintptr_t)h - (uintptr_t)out;
     if (gap && gap < (size_t)T * (size_t)d->D * 4)   /* a token's group reads h where another's has stored */
         return tlmh_seterr(TLM_HIP_EINVAL, "fp8_moe: out must be h itself or not overlap it");

@@ -153,7 +153,8 @@ def matmul(Wp, rows, n, codes, scale, out=None, dtype=torch.float32):
 
 class MoeBlock:
     """One routed MoE block of E4M3 matrices for up to 64 tokens a call.  Expert
-    e's packed gate / up / down pointers are expert_ptrs[3e .. 3e + 2]; packed
+    e's packed gate / up / down pointers are expert_ptrs[3e .. 3e + 2], 0 for
+    experts that the mask prunes (they stay pruned where the mask is changed later); packed
     matrices are the caller's to keep alive, as are the tensors a call is given.
     The workspace is one per block and grows with the largest T seen (reserve()
     sizes it ahead), so calls of one block must not overlap (other streams, two
@@ -161,22 +162,25 @@ class MoeBlock:
 
     def __init__(self, *, D, de, E, k, ffn_norm, router_w, expert_ptrs, router=0, routed_scale=1.0, eps=1e-6,
                  router_bias=None, mask=None, ds=0, shared=None, shared_gate_inp=None):
-        if len(expert_ptrs) != 3 * E or not (all(expert_ptrs) or mask is not None):
-            raise ValueError("expert_ptrs must hold 3 E packed matrices (0 only for experts that the mask prunes)")
+        if len(expert_ptrs) != 3 * E or any(p % 16 for p in expert_ptrs):
+            raise ValueError("expert_ptrs must hold 3 E packed matrices, 16-byte aligned")
         if (ds > 0) != (shared is not None):
             raise ValueError("ds and shared go together")
-        for t, shape, dt, what in ((ffn_norm, (D,), torch.float32, "ffn_norm"),
-                                   (router_w, (E, D), torch.float32, "router_w"),
-                                   (router_bias, (E,), torch.float32, "router_bias"), (mask, (E,), torch.uint8, "mask"),
-                                   (shared_gate_inp, (D,), torch.float32, "shared_gate_inp")):
-            if t is not None:
-                _out(t, shape, dt, t, what)
-                _here(t)
+        given = [(t, shape, dt, what) for t, shape, dt, what in (
+            (ffn_norm, (D,), _F32, "ffn_norm"), (router_w, (E, D), _F32, "router_w"), (router_bias, (E,), _F32, "router_bias"),
+            (mask, (E,), _U8, "mask"), (shared_gate_inp, (D,), _F32, "shared_gate_inp")) if t is not None]
+        for t, shape, dt, what in given:
+            _out(t, shape, dt, t, what)
+        if not all(expert_ptrs):
+            pruned = [False] * E if mask is None else mask.tolist()
+            if not all(pruned[i // 3] or p for i, p in enumerate(expert_ptrs)):
+                raise ValueError("expert_ptrs may be 0 only for experts that the mask prunes")
         if shared is not None:
-            if len(shared) != 3 or any(m.numel() < packed_bytes(*rn)
+            if len(shared) != 3 or any(m.dtype is not _U8 or not m.is_contiguous() or m.data_ptr() % 16 or
+                                       m.numel() < packed_bytes(*rn)
                                        for m, rn in zip(shared, ((ds, D), (ds, D), (D, ds)))):
-                raise ValueError("shared must be 3 packed matrices")
-            _here(*shared)
+                raise ValueError("shared must be 3 packed matrices, 16-byte aligned")
+        _here(*(t for t, *_ in given), *(shared or ()))
         self.keep = [ffn_norm, router_w, router_bias, mask, shared, shared_gate_inp]
         self.device = ffn_norm.device
         self.table = torch.tensor(list(expert_ptrs), dtype=torch.int64, device=self.device)
