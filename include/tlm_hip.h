@@ -610,6 +610,10 @@ int    tlm_hip_fp8_quantize(int dt, const void *x, int64_t xstride, int64_t n, i
  * ntok are left as they are.  ntok <= 2^20, ntok * rows <= 2^35. */
 int    tlm_hip_fp8_matmul(const void *Wp, int64_t rows, int64_t n, const void *codes, const float *scale,
                           int64_t ntok, int dt, void *Y, int64_t ystride, void *stream);
+/* The kernel that tlm_hip_fp8_matmul launches for these sizes, by name (rows and
+ * tokens of a group; its waves, or its stages), for profiles and tests.  NULL where
+ * there is no launch. */
+const char *tlm_hip_fp8_matmul_kernel(int64_t rows, int64_t n, int64_t ntok);
 /* A routed MoE block for T tokens of as many sequences (T <=
  * TLM_HIP_FP8_MOE_MAX_TOKENS): out[t] = h[t] + MoE(h[t]) as tlm_hip_moe_layer's block
  * computes it (rmsnorm, router, softmax or sigmoid routing, SwiGLU experts,

@@ -196,6 +196,7 @@ _SIGS = {
     "tlm_hip_fp8_pack": (i32, [vp, sz, vp, i64, i64, i64, vp, vp]),
     "tlm_hip_fp8_quantize": (i32, [i32, vp, i64, i64, i64, vp, vp, vp]),
     "tlm_hip_fp8_matmul": (i32, [vp, i64, i64, vp, vp, i64, i32, vp, i64, vp]),
+    "tlm_hip_fp8_matmul_kernel": (C.c_char_p, [i64, i64, i64]),
     "tlm_hip_fp8_moe_workspace_bytes": (sz, [C.POINTER(MoeDesc), i64]),
     "tlm_hip_fp8_moe": (i32, [C.POINTER(MoeDesc), vp, vp, i64, vp, vp, vp, vp]),
     "tlm_hip_moe_stack_store": (i32, [C.POINTER(MoeDesc), i32, vp, vp, C.POINTER(StackOpts), vp, vp, vp, vp]),

@@ -518,38 +518,40 @@ template <int KW, int RT, int TT> void launch_rows(const MmArgs &a, hipStream_t 
  * geometric mean, and at worst 45%; the largest kernel with a group for every unit took 9%.  4096 x 4096: 32 tokens
  * 6.4 us in 32 x 16 and 8.5 in 32 x 32, 128 tokens 10.1 in 64 x 32 and 12.2 in 32 x 32.  Results of every type take
  * the same kernel: a 16-bit result is the float one's rounding. */
-struct Cost {
-    int m, n, waves;   /* rows and tokens of a group; the waves that share a row's blocks */
+struct Kernel {
+    const char *name;   /* rows and tokens of a group; waves, or stages */
+    void (*launch)(const MmArgs &, hipStream_t);
+    int m, n, waves;    /* rows and tokens of a group; the waves that share a row's blocks */
     float start, group, run, block;
 };
-enum { ROWS16, ROWS32, SQUARE32, SQUARE32W8, ROWS64, ROWS64W8, SQUARE64, TILE64, TILE128X64, TILE128X64S4, TILE128, KERNELS };
-constexpr Cost COSTS[KERNELS] = {
-    /* row groups */
-    {16, 16, 8, 2.0f, 0.0f, 0.54f, 0.455f}, {32, 16, 8, 2.0f, 0.0f, 0.66f, 0.69f}, {32, 32, 4, 2.5f, 0.0f, 0.4f, 0.51f},
-    {32, 32, 8, 2.25f, 0.0f, 0.3f, 1.0f}, {64, 32, 4, 2.85f, 0.0f, 0.9f, 0.81f},
-    {64, 32, 8, 1.35f, 0.95f, 1.5f, 1.51f}, {64, 64, 4, 1.7f, 2.0f, 0.05f, 1.34f},
-    /* tiles: two stages, two, four, two */
-    {64, 64, 1, 2.85f, 0.05f, 0.46f, 0.329f}, {128, 64, 1, 3.35f, 0.14f, 0.65f, 0.505f},
-    {128, 64, 1, 2.25f, 1.75f, 0.60f, 0.594f}, {128, 128, 1, 4.25f, 0.0f, 0.95f, 0.829f}};
-void launch_mm(const MmArgs &a, hipStream_t s) {
+constexpr Kernel KERNELS[] = {
+    {"rows_16x16_w8", launch_rows<8, 1, 1>, 16, 16, 8, 2.0f, 0.0f, 0.54f, 0.455f},
+    {"rows_32x16_w8", launch_rows<8, 2, 1>, 32, 16, 8, 2.0f, 0.0f, 0.66f, 0.69f},
+    {"rows_32x32_w4", launch_rows<4, 2, 2>, 32, 32, 4, 2.5f, 0.0f, 0.4f, 0.51f},
+    {"rows_32x32_w8", launch_rows<8, 2, 2>, 32, 32, 8, 2.25f, 0.0f, 0.3f, 1.0f},
+    {"rows_64x32_w4", launch_rows<4, 4, 2>, 64, 32, 4, 2.85f, 0.0f, 0.9f, 0.81f},
+    {"rows_64x32_w8", launch_rows<8, 4, 2>, 64, 32, 8, 1.35f, 0.95f, 1.5f, 1.51f},
+    {"rows_64x64_w4", launch_rows<4, 4, 4>, 64, 64, 4, 1.7f, 2.0f, 0.05f, 1.34f},
+    {"tile_64x64_s2", launch_tile<2, 2, 2, 2, 2>, 64, 64, 1, 2.85f, 0.05f, 0.46f, 0.329f},
+    {"tile_128x64_s2", launch_tile<2, 2, 2, 4, 2>, 128, 64, 1, 3.35f, 0.14f, 0.65f, 0.505f},
+    {"tile_128x64_s4", launch_tile<4, 2, 2, 4, 2>, 128, 64, 1, 2.25f, 1.75f, 0.60f, 0.594f},
+    {"tile_128x128_s2", launch_tile<2, 2, 2, 4, 4>, 128, 128, 1, 4.25f, 0.0f, 0.95f, 0.829f},
+    /* few tokens of long rows alone */
+    {"rows_16x16_w16", launch_rows<16, 1, 1>, 16, 16, 16},
+    {"rows_32x16_w16", launch_rows<16, 2, 1>, 32, 16, 16}};
+enum { ROWS16 = 0, ROWS32 = 1, TILES = 7, FITTED = 11, ROWS16W16 = 11, ROWS32W16 = 12 };
+const Kernel &choose(int64_t rows, int nb, int64_t T) {
     constexpr int64_t CUS = 256;
-    auto count = [&](int m, int n) { return ((a.rows + m - 1) / m) * ((a.T + n - 1) / n); };
-    const int nb = a.nb;
-    if (a.T <= 16) {
-        if (count(32, 16) >= (a.T > 8 ? CUS : 4 * CUS)) {
-            if (nb < 16) launch_rows<8, 2, 1>(a, s);
-            else launch_rows<16, 2, 1>(a, s);
-        } else {
-            if (nb < 64) launch_rows<8, 1, 1>(a, s);
-            else launch_rows<16, 1, 1>(a, s);
-        }
-        return;
+    auto count = [&](int m, int n) { return ((rows + m - 1) / m) * ((T + n - 1) / n); };
+    if (T <= 16) {
+        if (count(32, 16) >= (T > 8 ? CUS : 4 * CUS)) return KERNELS[nb < 16 ? ROWS32 : ROWS32W16];
+        return KERNELS[nb < 64 ? ROWS16 : ROWS16W16];
     }
     int pick = -1;
     float least = 0.0f;
-    for (int i = 0; i < KERNELS; i++) {
-        const Cost &c = COSTS[i];
-        if (i <= SQUARE64 && a.T > 65535 * (int64_t)c.n) continue;   /* their tokens are the grid's second axis */
+    for (int i = 0; i < FITTED; i++) {
+        const Kernel &c = KERNELS[i];
+        if (i < TILES && T > 65535 * (int64_t)c.n) continue;   /* their tokens are the grid's second axis */
         const float steps = (float)((nb + c.waves - 1) / c.waves), q = (float)((count(c.m, c.n) + CUS - 1) / CUS);
         const float run = steps * c.run, full = q * (c.group + steps * c.block);
         const float us = c.start + (run > full ? run : full);
@@ -558,19 +560,7 @@ void launch_mm(const MmArgs &a, hipStream_t s) {
             least = us;
         }
     }
-    switch (pick) {
-    case ROWS16: launch_rows<8, 1, 1>(a, s); break;
-    case ROWS32: launch_rows<8, 2, 1>(a, s); break;
-    case SQUARE32: launch_rows<4, 2, 2>(a, s); break;
-    case SQUARE32W8: launch_rows<8, 2, 2>(a, s); break;
-    case ROWS64: launch_rows<4, 4, 2>(a, s); break;
-    case ROWS64W8: launch_rows<8, 4, 2>(a, s); break;
-    case SQUARE64: launch_rows<4, 4, 4>(a, s); break;
-    case TILE64: launch_tile<2, 2, 2, 2, 2>(a, s); break;
-    case TILE128X64: launch_tile<2, 2, 2, 4, 2>(a, s); break;
-    case TILE128X64S4: launch_tile<4, 2, 2, 4, 2>(a, s); break;
-    default: launch_tile<2, 2, 2, 4, 4>(a, s);
-    }
+    return KERNELS[pick];
 }
 
 bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
@@ -580,6 +570,7 @@ int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16
 
 /* Row and length limits keep every launch inside the grid limits; sizes in bytes
  * are 64-bit throughout. */
+constexpr int64_t MOST_TOKENS = (int64_t)1 << 20, MOST_RESULTS = (int64_t)1 << 35;   /* 2^31 threads in the smallest tiles */
 static int fp8_dims(const char *who, int64_t rows, int64_t n) {
     if (rows < 1 || n < 1 || rows > ((int64_t)1 << 25) || n > ((int64_t)1 << 22))
         return tlmh_seterr(TLM_HIP_EINVAL, "%s: rows=%lld n=%lld outside 1..2^25 and 1..2^22", who, (long long)rows,
@@ -653,14 +644,23 @@ int tlm_hip_fp8_matmul(const void *Wp, int64_t rows, int64_t n, const void *code
     if (!aligned(Wp, 16) || !aligned(codes, 16) || !aligned(scale, 4) || !aligned(Y, (size_t)type_bytes(dt)))
         return tlmh_seterr(TLM_HIP_EINVAL,
                            "fp8_matmul: the matrix and the codes must be 16-byte, scale 4-byte aligned, Y as its type");
-    if (ntok > ((int64_t)1 << 20) || ntok * rows > (int64_t)1 << 35)   /* 2^31 threads in the smallest tiles */
+    if (ntok > MOST_TOKENS || ntok * rows > MOST_RESULTS)
         return tlmh_seterr(TLM_HIP_ERANGE, "fp8_matmul: %lld tokens of %lld rows are too many for one launch",
                            (long long)ntok, (long long)rows);
     const MmArgs a = {(const uint8_t *)Wp, (const float *)((const uint8_t *)Wp + fp8_code_bytes(rows, n)),
                       (const uint8_t *)codes, scale, Y, rows, ystride, ntok, (int)fp8_blocks(n), dt};
-    hipStream_t s = (hipStream_t)stream;
-    launch_mm(a, s);
+    choose(rows, a.nb, ntok).launch(a, (hipStream_t)stream);
     return tlmh_check(hipGetLastError(), "fp8_matmul launch");
+}
+
+const char *tlm_hip_fp8_matmul_kernel(int64_t rows, int64_t n, int64_t ntok) {
+    if (fp8_dims("fp8_matmul_kernel", rows, n)) return nullptr;
+    if (ntok < 1 || ntok > MOST_TOKENS || ntok * rows > MOST_RESULTS) {
+        tlmh_seterr(TLM_HIP_ERANGE, "fp8_matmul_kernel: no launch for %lld tokens of %lld rows", (long long)ntok,
+                    (long long)rows);
+        return nullptr;
+    }
+    return choose(rows, (int)fp8_blocks(n), ntok).name;
 }
 
 }  // extern "C"

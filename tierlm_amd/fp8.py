@@ -151,6 +151,12 @@ def matmul(Wp, rows, n, codes, scale, out=None, dtype=torch.float32):
     return out
 
 
+def matmul_kernel(rows, n, T):
+    """The name of the kernel that matmul() launches for T tokens (None where there is no launch)."""
+    name = lib.tlm_hip_fp8_matmul_kernel(rows, n, T)
+    return name.decode() if name else None
+
+
 class MoeBlock:
     """One routed MoE block of E4M3 matrices for up to 64 tokens a call.  Expert
     e's packed gate / up / down pointers are expert_ptrs[3e .. 3e + 2], 0 for
