@@ -602,8 +602,10 @@ int    tlm_hip_fp8_quantize(int dt, const void *x, int64_t xstride, int64_t n, i
                             float *scale, void *stream);
 /* Y[t * ystride + r] = sum over the blocks b of scale[t][b] * sw[r / 128][b] *
  * (codes of token t . codes of row r), r < rows, t < ntok, stored as dt (F32,
- * F16 or BF16).  codes / scale as tlm_hip_fp8_quantize writes them (any f32
- * scales; codes past n must be 0).  Products are exact and sums f32 whatever the
+ * F16 or BF16).  codes / scale as tlm_hip_fp8_quantize writes them (codes past n
+ * must be 0); activation scales may be any normal floats or 0, weight scales 0 or of
+ * magnitude 2^-96 to 2^96: the two are not multiplied where their product is no
+ * float.  Infinite and NaN scales poison their tokens and rows.  Products are exact and sums f32 whatever the
  * result's type: an F16 or BF16 result is the F32 result rounded once.  The order
  * of the sums is fixed: a call repeats its bits; another number of tokens may
  * change them.  Elements of Y past rows and rows of Y past
@@ -619,7 +621,8 @@ const char *tlm_hip_fp8_matmul_kernel(int64_t rows, int64_t n, int64_t ntok);
  * computes it (rmsnorm, router, softmax or sigmoid routing, SwiGLU experts,
  * rank-order combine, shared expert), with expert_dt / shared_dt
  * TLM_HIP_DT_FP8 and matrices of tlm_hip_fp8_pack.  Activations stay f32
- * from end to end (no activation quantisation).  Any D <= 16384, widths up
+ * from end to end (no activation quantisation); the sums hold activations and hidden
+ * values of magnitude 2^-110 to 2^110.  Any D <= 16384, widths up
  * to 65536; h and out [T x D] f32, out == h or not overlapping.  ids / w
  * [T x k] (device, may be NULL) receive the routing.  Softmax routing selects by
  * the router's scores, sigmoid routing by score + bias, ties to the lower
