@@ -72,6 +72,7 @@ struct Args {
     float *w;
     uint8_t *ws;
     int T, slots, by_expert;
+    double inv_D;
     int ce, cs;   /* groups among which an expert's, and the shared expert's, tokens are dealt */
 };
 
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
     __shared__ double s_red[4];
     const tlm_hip_moe_desc &d = a.d;
     args_now(d.D, d.E, d.ds, d.router, d.eps, d.ffn_norm, d.router_w, d.router_bias, d.mask, d.experts, d.shared_gate_inp,
-             a.h, a.ws, a.L.xp, a.L.key, a.L.score, a.L.sgate, a.L.nbd);
+             a.h, a.ws, a.inv_D, a.L.xp, a.L.key, a.L.score, a.L.sgate, a.L.nbd);
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), t = blockIdx.y;
     const int D = (int)d.D, Dq = (D + 3) & ~3, e = blockIdx.x * 4 + wave;
     const bool live = e < d.E || (e == d.E && d.ds > 0 && d.shared_gate_inp);
@@ -169,7 +170,18 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
     if (lane == 0) s_red[wave] = ss;
     __syncthreads();
     ss = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
-    const float rn = 1.0f / sqrtf((float)(ss / (double)D) + d.eps);
+    /* The token's factor stays double: rounded, it would be off in the same direction for the whole vector (1.6e-7 of
+     * the result in common, where the elements' own roundings average out), and the mean of large squares is no
+     * float.  The instruction gives 23 bits, a Newton step 45. */
+    const double v = ss * a.inv_D + (double)d.eps;
+    double rn = __builtin_amdgcn_rsq(v);
+    rn = fma(0.5 * rn, fma(-v * rn, rn, 1.0), rn);
+    auto normed = [&](f32x4 h, f32x4 g) {
+        f32x4 x;
+#pragma unroll
+        for (int q = 0; q < 4; q++) x[q] = (float)((double)h[q] * rn) * g[q];
+        return x;
+    };
     const int Dp = a.L.nbd * FP8_BLOCK;
     uint16_t *xp = (uint16_t *)(a.ws + a.L.xp) + (size_t)t * 3 * Dp;
     auto put = [&](int i, f32x4 v) {
@@ -189,9 +201,9 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
 #pragma unroll
     for (int c = 0; c < NC; c++) {
         const int i = 4 * tid + 1024 * c;
-        if (1024 * c < D && i < Dp) put(i, hv[c] * rn * gv[c]);   /* zeros behind D */
+        if (1024 * c < D && i < Dp) put(i, normed(hv[c], gv[c]));   /* zeros behind D */
     }
-    for (int i = 4 * tid + 1024 * NC; i < Dp; i += 1024) put(i, row4(h, i, D) * rn * row4(nw, i, D));
+    for (int i = 4 * tid + 1024 * NC; i < Dp; i += 1024) put(i, normed(row4(h, i, D), row4(nw, i, D)));
     __syncthreads();
     if (!live) return;
     double acc = 0.0;
@@ -981,6 +993,7 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     a.w = w;
     a.ws = (uint8_t *)workspace;
     a.T = (int)T;
+    a.inv_D = 1.0 / (double)d->D;
     a.by_expert = T > 1 && T * d->k >= d->E;
     a.slots = a.by_expert ? d->E : (int)(T * d->k);
     spread(a);
