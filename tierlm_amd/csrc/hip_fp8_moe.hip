@@ -170,7 +170,7 @@ __global__ __launch_bounds__(256) void k_fm_router(Args a) {
     if (lane == 0) s_red[wave] = ss;
     __syncthreads();
     ss = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
-    /* The token's factor stays double: rounded, it would be off in the same direction for the whole vector (1.6e-7 of
+    /* The token's factor stays double: rounded, it would be off in the same direction for the whole vector (1e-7 of
      * the result in common, where the elements' own roundings average out), and the mean of large squares is no
      * float.  The instruction gives 23 bits, a Newton step 45. */
     const double v = ss * a.inv_D + (double)d.eps;
