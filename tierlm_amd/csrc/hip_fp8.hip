@@ -599,6 +599,7 @@ int tlm_hip_fp8_pack(const void *W, size_t row_bytes, const float *scale, int64_
                            (long long)scale_stride, (long long)n);
     if (!aligned(dst, 16) || !aligned(scale, 4))
         return tlmh_seterr(TLM_HIP_EINVAL, "fp8_pack: dst must be 16-byte and scale 4-byte aligned");
+    if (int rc = tlmh_refuse_failed(FAILED_FP8, "fp8_pack")) return rc;
     const int nb = (int)fp8_blocks(n);
     const int64_t pieces = (int64_t)(fp8_code_bytes(rows, n) / 16), ns = fp8_blocks(rows) * nb;
     const int64_t groups = (pieces + ns + 255) / 256;
@@ -627,6 +628,7 @@ int tlm_hip_fp8_quantize(int dt, const void *x, int64_t xstride, int64_t n, int6
     if (ntok > ((int64_t)1 << 26) / nb)
         return tlmh_seterr(TLM_HIP_ERANGE, "fp8_quantize: %lld tokens of %d blocks are too many for one launch",
                            (long long)ntok, nb);
+    if (int rc = tlmh_refuse_failed(FAILED_FP8, "fp8_quantize")) return rc;
     const int64_t blocks = ntok * nb;
     hipStream_t s = (hipStream_t)stream;
     if (dt == DT_F32) launch_quant<float>(x, xstride, n, nb, blocks, codes, scale, s);
@@ -651,6 +653,7 @@ int tlm_hip_fp8_matmul(const void *Wp, int64_t rows, int64_t n, const void *code
     if (ntok > MOST_TOKENS || ntok * rows > MOST_RESULTS)
         return tlmh_seterr(TLM_HIP_ERANGE, "fp8_matmul: %lld tokens of %lld rows are too many for one launch",
                            (long long)ntok, (long long)rows);
+    if (int rc = tlmh_refuse_failed(FAILED_FP8, "fp8_matmul")) return rc;
     const MmArgs a = {(const uint8_t *)Wp, (const float *)((const uint8_t *)Wp + fp8_code_bytes(rows, n)),
                       (const uint8_t *)codes, scale, Y, rows, ystride, ntok, (int)fp8_blocks(n), dt};
     choose(rows, a.nb, ntok).launch(a, (hipStream_t)stream);

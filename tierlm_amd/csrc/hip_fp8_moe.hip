@@ -984,6 +984,7 @@ int tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64
     const uintptr_t gap = (uintptr_t)h < (uintptr_t)out ? (uintptr_t)out - (uintptr_t)h : (uintptr_t)h - (uintptr_t)out;
     if (gap && gap < (size_t)T * (size_t)d->D * 4)   /* a token's group reads h where another's has stored */
         return tlmh_seterr(TLM_HIP_EINVAL, "fp8_moe: out must be h itself or not overlap it");
+    if (int rc = tlmh_refuse_failed(FAILED_FP8, "fp8_moe")) return rc;
     Args a{};
     a.d = *d;
     a.L = layout(*d, T);

@@ -10,8 +10,8 @@
  * matrix cores' float products against v_mul_f32, and the 8-bit floating-point
  * quantiser (codes and scales) and product (within the roundings of a float sum).
  * Returns the number of failing kernels; bit dt of *mask is set for every dtype
- * whose kernels failed, bit 30 for the exponential, bit 29 for the products, bit
- * 28 for 8-bit floating point. */
+ * whose kernels failed, FAILED_EXP for the exponential, FAILED_PRODUCTS for the
+ * products, FAILED_FP8 for 8-bit floating point. */
 #include "tlm_hip_internal.h"
 #include "tlm_hip_outer.h"
 
@@ -400,16 +400,16 @@ int tlmh_selftest(int *failed_mask) {
         for (int i = 0; ok && i < NE; i++) ok = same(ey[i], eg[i]) || (ey[i] != ey[i] && eg[i] != eg[i]);
         if (!ok) {
             fails++;
-            mask |= 1 << 30;
+            mask |= 1 << FAILED_EXP;
         }
     }
     if (!outer_ok(dev + o_p, &s)) {
         fails++;
-        mask |= 1 << 29;
+        mask |= 1 << FAILED_PRODUCTS;
     }
     if (!fp8_ok(dev + o_p, &s)) {
         fails++;
-        mask |= 1 << 28;
+        mask |= 1 << FAILED_FP8;
     }
     (void)hipDeviceSynchronize();
     (void)hipFree(dev);

@@ -6,6 +6,7 @@
  * self-test is refused (NaN results plus an error), never replaced. */
 #include "tlm_hip_internal.h"
 
+#include <atomic>
 #include <math.h>
 #include <mutex>
 #include <stdarg.h>
@@ -37,12 +38,17 @@ int tlmh_check(hipError_t e, const char *what) {
 static std::mutex g_mu;                 /* init + the staging area */
 static int g_device = -1;
 static int g_selftest_failures = 0;
-static int g_failed_mask = 0;           /* bit dt set: that dtype failed its self-test */
+static std::atomic<int> g_failed_mask{0};   /* hip_selftest.hip's mask: bit dt set, that dtype failed its self-test */
 static uint8_t *g_stage = nullptr;      /* device staging for host-pointer entries */
 static size_t g_stage_bytes = 0;
 static hipStream_t g_stage_stream = nullptr;
 
 int tlmh_current_device(void) { return g_device; }
+void tlmh_set_failed(int mask) { g_failed_mask.store(mask, std::memory_order_relaxed); }
+int tlmh_refuse_failed(int bit, const char *who) {
+    if (!((g_failed_mask.load(std::memory_order_relaxed) >> bit) & 1)) return TLM_HIP_OK;
+    return tlmh_seterr(TLM_HIP_EIO, "%s: unavailable, its kernels failed the start-up self-test", who);
+}
 
 /* ---- the workspace of tlm_hip_moe_layer_noalloc ---------------------------
  * A file-scope device array: every GPU the library is initialised on holds its
@@ -83,10 +89,11 @@ int tlm_hip_init(int device) {
     HIPCHK(hipStreamCreateWithFlags(&g_stage_stream, hipStreamNonBlocking));
     g_device = device;
     int mask = 0;
+    tlmh_set_failed(0);   /* the self-test makes the calls that a failure on another device refuses */
     int rc = tlmh_selftest(&mask);
     if (rc < 0) { g_device = -1; return rc; }
     g_selftest_failures = rc;
-    g_failed_mask = mask;
+    tlmh_set_failed(mask);
     return TLM_HIP_OK;
 }
 
