@@ -598,19 +598,20 @@ int    tlm_hip_fp8_pack(const void *W, size_t row_bytes, const float *scale, int
  * are 0), and scales [ntok][np / 128].  A block's scale is the least power of
  * two 2^e, e >= -126, with max |x| <= 448 * 2^e (0 for a block of zeros); each
  * code is x / scale rounded to nearest, ties to even.  An infinity or NaN in a
- * block makes its scale NaN and its codes 0.  codes 16-byte aligned. */
+ * block makes its scale NaN and its codes 0.  codes 16-byte aligned.  At most 2^26
+ * blocks a call (ntok * np / 128; TLM_HIP_ERANGE): longer inputs go in parts. */
 int    tlm_hip_fp8_quantize(int dt, const void *x, int64_t xstride, int64_t n, int64_t ntok, void *codes,
                             float *scale, void *stream);
 /* Y[t * ystride + r] = sum over the blocks b of scale[t][b] * sw[r / 128][b] *
  * (codes of token t . codes of row r), r < rows, t < ntok, stored as dt (F32,
  * F16 or BF16).  codes / scale as tlm_hip_fp8_quantize writes them (codes past n
- * must be 0); activation scales may be any normal floats or 0, weight scales 0 or of
- * magnitude 2^-96 to 2^96: the two are not multiplied where their product is no
- * float.  Infinite and NaN scales poison their tokens and rows.  Products are exact and sums f32 whatever the
- * result's type: an F16 or BF16 result is the F32 result rounded once.  The order
- * of the sums is fixed: a call repeats its bits; another number of tokens may
- * change them.  Elements of Y past rows and rows of Y past
- * ntok are left as they are.  ntok <= 2^20, ntok * rows <= 2^35. */
+ * must be 0); activation scales may be any normal floats or 0, weight scales 0 or
+ * of magnitude 2^-96 to 2^96: their product need not be a float where the result
+ * is.  Infinite and NaN scales poison their tokens and rows.  Products are exact
+ * and sums f32 whatever the result's type: an F16 or BF16 result is the F32 result
+ * rounded once.  The order of the sums is fixed: a call repeats its bits; another
+ * number of tokens may change them.  Y overlaps no input; its elements past rows
+ * and rows past ntok are left as they are.  ntok <= 2^20, ntok * rows <= 2^35. */
 int    tlm_hip_fp8_matmul(const void *Wp, int64_t rows, int64_t n, const void *codes, const float *scale,
                           int64_t ntok, int dt, void *Y, int64_t ystride, void *stream);
 /* The kernel that tlm_hip_fp8_matmul launches for these sizes, by name (rows and
@@ -621,17 +622,18 @@ const char *tlm_hip_fp8_matmul_kernel(int64_t rows, int64_t n, int64_t ntok);
  * TLM_HIP_FP8_MOE_MAX_TOKENS): out[t] = h[t] + MoE(h[t]) as tlm_hip_moe_layer's block
  * computes it (rmsnorm, router, softmax or sigmoid routing, SwiGLU experts,
  * rank-order combine, shared expert), with expert_dt / shared_dt
- * TLM_HIP_DT_FP8 and matrices of tlm_hip_fp8_pack.  Activations stay f32
- * from end to end (no activation quantisation); the sums hold activations and hidden
- * values of magnitude 2^-110 to 2^110.  Any D <= 16384, widths up
- * to 65536; h and out [T x D] f32, out == h or not overlapping.  ids / w
- * [T x k] (device, may be NULL) receive the routing.  Softmax routing selects by
- * the router's scores, sigmoid routing by score + bias, ties to the lower
- * index; where the mask leaves fewer than k experts the ranks behind them get id
- * -1 and weight 0.  An expert with a null pointer among its three in the table
- * counts as pruned, masked or not.  Packed matrices are 16-byte aligned.  workspace: tlm_hip_fp8_moe_workspace_bytes(d, T) bytes,
- * 256-byte aligned, nothing in it needs to be kept or zeroed; calls that may
- * overlap (other streams) need different workspaces. */
+ * TLM_HIP_DT_FP8 and matrices of tlm_hip_fp8_pack (16-byte aligned).  Activations
+ * stay f32 from end to end (no activation quantisation); the sums hold activations
+ * and hidden values of magnitude 2^-110 to 2^110.  Any D <= 16384, widths up to 65536;
+ * h and out [T x D] f32, out == h or not overlapping.  ids / w [T x k] (device,
+ * may be NULL) receive the routing.  Softmax routing selects by the router's scores,
+ * sigmoid routing by score + bias, ties to the lower index; where the mask leaves fewer
+ * than k experts the ranks behind them get id -1 and weight 0.  An expert with a null
+ * pointer among its three in the table counts as pruned, masked or not.  A matrix packed
+ * for other sizes cannot be told from its pointer: the descriptor's sizes are taken on
+ * trust.  workspace: tlm_hip_fp8_moe_workspace_bytes(d, T) bytes, 256-byte aligned,
+ * nothing in it needs to be kept or zeroed; calls that may overlap (other streams,
+ * graphs) need different workspaces. */
 #define TLM_HIP_FP8_MOE_MAX_TOKENS 64
 size_t tlm_hip_fp8_moe_workspace_bytes(const tlm_hip_moe_desc *d, int64_t T);
 int    tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64_t T, int32_t *ids, float *w,

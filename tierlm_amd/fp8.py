@@ -8,8 +8,8 @@ activation quantiser, their product, and a routed MoE block for a few tokens
     Y = fp8.matmul(Wp, rows, n, codes, s)    # [T, rows]
 
 Device memory is torch tensors on the current HIP device; work goes on torch's
-current stream.  Arguments that do not fit raise ValueError before anything
-is launched.
+current stream.  Arguments that do not fit raise ValueError, sizes past a
+call's limits and misaligned memory HipError, before anything is launched.
 """
 import ctypes as C
 
@@ -93,7 +93,8 @@ def pack(W, scale, out=None):
 
 def quantize(x, codes=None, scale=None):
     """x [T, n] (or [n]) -> E4M3 codes [T, np] and f32 scales [T, np / 128], np
-    = n rounded up to 128; rows of x may have any stride."""
+    = n rounded up to 128; rows of x may have any stride.  At most 2^26 blocks of
+    128 a call."""
     if x.dim() == 1:
         x = x[None]
     dt = _TYPES.get(x.dtype)
@@ -164,7 +165,8 @@ class MoeBlock:
     matrices are the caller's to keep alive, as are the tensors a call is given.
     The workspace is one per block and grows with the largest T seen (reserve()
     sizes it ahead), so calls of one block must not overlap (other streams, two
-    graphs at once)."""
+    graphs at once), and the block is kept until its calls are done and as long
+    as a graph that holds one is replayed."""
 
     def __init__(self, *, D, de, E, k, ffn_norm, router_w, expert_ptrs, router=0, routed_scale=1.0, eps=1e-6,
                  router_bias=None, mask=None, ds=0, shared=None, shared_gate_inp=None):
