@@ -605,9 +605,9 @@ int    tlm_hip_fp8_quantize(int dt, const void *x, int64_t xstride, int64_t n, i
 /* Y[t * ystride + r] = sum over the blocks b of scale[t][b] * sw[r / 128][b] *
  * (codes of token t . codes of row r), r < rows, t < ntok, stored as dt (F32,
  * F16 or BF16).  codes / scale as tlm_hip_fp8_quantize writes them (codes past n
- * must be 0); activation scales may be any normal floats or 0, weight scales 0 or
- * of magnitude 2^-96 to 2^96: their product need not be a float where the result
- * is.  Infinite and NaN scales poison their tokens and rows.  Products are exact
+ * must be 0); activation scales are 0 or of magnitude 2^-126 to 2^126, weight scales
+ * 0 or of magnitude 2^-96 to 2^96: their product need not be a float where the
+ * result is.  Infinite and NaN scales poison their tokens and rows.  Products are exact
  * and sums f32 whatever the result's type: an F16 or BF16 result is the F32 result
  * rounded once.  The order of the sums is fixed: a call repeats its bits; another
  * number of tokens may change them.  Y overlaps no input; its elements past rows

@@ -1,5 +1,5 @@
 """Block scales at the ends of the float range: a product of two scales that is no float itself does not
-spoil a result that is one.  Weight scales are between 2^-96 and 2^96, activation scales any normal floats.
+spoil a result that is one.  Weight scales are between 2^-96 and 2^96, activation scales between 2^-126 and 2^126.
 
 Tolerance: (127 + nb + 2) 2^-24 of the sum of magnitudes, and half a subnormal step, 2^-150, for each of the nb
 sums where results end that low."""
