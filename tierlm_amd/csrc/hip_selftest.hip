@@ -8,7 +8,8 @@
  * and the packed-layout matvec (bits of every row) for F32, Q8_0, Q4_K, Q5_K,
  * Q6_K and Q8_K, the exponential against this host's libm expf, the
  * matrix cores' float products against v_mul_f32, and the 8-bit floating-point
- * quantiser (codes and scales) and product (within the roundings of a float sum).
+ * quantiser (codes and scales) and product (within the roundings of a float sum),
+ * at one size, of the row groups.
  * Returns the number of failing kernels; bit dt of *mask is set for every dtype
  * whose kernels failed, FAILED_EXP for the exponential, FAILED_PRODUCTS for the
  * products, FAILED_FP8 for 8-bit floating point. */
