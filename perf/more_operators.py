@@ -91,7 +91,7 @@ def draw(rng):
     heads = _heads(rng)
     H, KV, hd = heads["H"], heads["KV"], heads["hd"]
     if kind == "append":
-        T = _log(rng, 1, min(8192, MOST_APPEND // ((H + 2 * KV) * hd) * 3 // 4))
+        T = _log(rng, 1, min(8192, MOST_APPEND // ((H + 2 * KV) * hd) * 2 // 3))
         B = rng.choice([T if T <= 128 else 1, 1, _log(rng, 1, min(T, 64))])
         past = _log(rng, 1, min(4000, MOST_CACHE // (B * KV * hd))) - 1
         return {"kind": kind, "B": B, "T": T, "past": past, "x": rng.choice(types), **heads}
