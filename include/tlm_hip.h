@@ -602,6 +602,16 @@ int    tlm_hip_fp8_pack(const void *W, size_t row_bytes, const float *scale, int
  * blocks a call (ntok * np / 128; TLM_HIP_ERANGE): longer inputs go in parts. */
 int    tlm_hip_fp8_quantize(int dt, const void *x, int64_t xstride, int64_t n, int64_t ntok, void *codes,
                             float *scale, void *stream);
+/* The residual's addition, the RMS norm and the quantiser in one pass over ntok rows of n values:
+ *   s = h + x, rounded to h's type (x NULL: s = h);  r = 1 / sqrt(mean(s^2) + eps);  y = (s r) w
+ * and the codes [ntok][np] and scales [ntok][np / 128] of y as tlm_hip_fp8_quantize writes them.  The mean is taken in double
+ * and r rounded once to f32; s r and its product with w are f32.  out receives s (out == h with equal strides
+ * updates the residual in place; NULL: s is not stored; otherwise it overlaps no input).  Types: F32, F16 or BF16, x and h
+ * by themselves; w f32.  Rows of any stride and of their type's alignment; codes 16-byte aligned.  ntok <= 2^22 and at
+ * most 2^26 blocks a call (TLM_HIP_ERANGE). */
+int    tlm_hip_fp8_add_rmsnorm(int hdt, const void *h, int64_t hstride, int xdt, const void *x, int64_t xstride,
+                               const float *w, float eps, int64_t n, int64_t ntok, void *out, int64_t ostride,
+                               void *codes, float *scale, void *stream);
 /* Y[t * ystride + r] = sum over the blocks b of scale[t][b] * sw[r / 128][b] *
  * (codes of token t . codes of row r), r < rows, t < ntok, stored as dt (F32,
  * F16 or BF16).  codes / scale as tlm_hip_fp8_quantize writes them (codes past n
@@ -638,6 +648,61 @@ const char *tlm_hip_fp8_matmul_kernel(int64_t rows, int64_t n, int64_t ntok);
 size_t tlm_hip_fp8_moe_workspace_bytes(const tlm_hip_moe_desc *d, int64_t T);
 int    tlm_hip_fp8_moe(const tlm_hip_moe_desc *d, const float *h, float *out, int64_t T, int32_t *ids, float *w,
                        void *workspace, void *stream);
+
+/* ---- paged key-value cache ----------------------------------------------------
+ * Attention for a batch of sequences, each with its own length, over one cache of pages (the reference keeps one
+ * sequence's cache, src/lib/tlm_model.c:402-446; its attention is attn_heads, :683-749).  With the 8-bit calls above this
+ * is the attention half of a layer: tlm_hip_fp8_add_rmsnorm, tlm_hip_fp8_matmul (q | k | v), tlm_hip_kv_append,
+ * tlm_hip_kv_decode or _prompt, tlm_hip_fp8_quantize, tlm_hip_fp8_matmul (o).
+ *
+ * Cache: k and v, each n_pages pages of `page` positions (a power of two from 16 to 4096) for kv_heads heads of head_dim
+ * values (a multiple of 32 up to 256), F16 or BF16, 16-byte aligned.  Pages are [kv_heads][page / 16] blocks of 16
+ * positions, a block of k [head_dim / 16][16 positions][16 values], of v [head_dim][16 positions]; pages can be copied whole.
+ *
+ * Batch: sequence b's position p lies in page tables[b table_stride + p / page].  lens[b] is its length after this call's
+ * rows (positions it has, its own new ones among them); its rows are cu[b] .. cu[b + 1] - 1 of `rows` packed ones (cu
+ * ascending, B + 1 values; NULL: row b alone, rows == B), row i of n at position lens[b] - n + i.  Several sequences may
+ * name one page, as a shared prefix, if none of them appends to it.  tables, lens and cu are device memory that the
+ * kernels read, so a captured graph follows them.  What they may hold: a length of 0 is a padded slot (append writes
+ * nothing, attention gives zeros); a page number outside 0 .. n_pages - 1 names no page, its positions are neither written
+ * nor seen, and so are positions past table_pages pages; a row before position 0 (more rows than positions) is not
+ * written, its query and its attention are zeros.  Rows outside [cu[0], cu[B]) are left as they are.
+ * B <= 2^20, rows * heads <= 2^30, table_pages * page <= 2^30.  The calls keep nothing from one to the next, launch on
+ * `stream` only and may be captured. */
+typedef struct {
+    int32_t dt;                    /* F16 1 or BF16 2 */
+    int32_t kv_heads, head_dim, page;
+    int64_t n_pages;
+    void   *k, *v;
+} tlm_hip_kv_cache;
+typedef struct {
+    int64_t        B, rows;
+    const int32_t *cu, *lens, *tables;
+    int64_t        table_stride;
+    int32_t        table_pages;
+} tlm_hip_kv_batch;
+/* rows of q | k | v ((heads + 2 kv_heads) * head_dim values of dt F32, F16 or BF16, row i at qkv + i qkv_stride): each query
+ * and key head y becomes y r w, r = 1 / sqrt(mean(y^2) + eps), where its norm (f32 [head_dim]) is given; with inv_freq
+ * (double [head_dim / 2]) the pair (y_j, y_{j + head_dim / 2}) is turned by position * inv_freq[j] and multiplied with
+ * rope_scale (the reference's rope(), src/lib/tlm_model.c:721-728); angles are doubles, the rest f32.  Keys and
+ * values go to their pages, rounded once; queries to q [rows][heads][head_dim] in the cache's type (16-byte aligned). */
+int    tlm_hip_kv_append(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int dt, const void *qkv, int64_t qkv_stride,
+                         int heads, const float *q_norm, const float *k_norm, float eps, const double *inv_freq,
+                         float rope_scale, void *q, void *stream);
+/* Attention of one row a sequence (b->cu NULL): out[b][h] = sum_j p_j v_j, p = softmax of scale q . k_j over the positions
+ * j < lens[b], head h with key head h / (heads / kv_heads).  q in the cache's type (row b at q + b q_stride, heads
+ * side by side), out [B][heads][head_dim] of out_dt (F32, F16 or BF16); scale positive.  Sums, maxima and the softmax are
+ * f32, its weights enter the second product rounded to the cache's type.  Sequences are split over their length as the
+ * batch's total asks, in the same way in every call with equal lengths: a call repeats its bits.  workspace:
+ * tlm_hip_kv_decode_workspace_bytes bytes (0: none, by the sizes alone), 256-byte aligned, nothing in it kept or zeroed;
+ * calls that may overlap need different ones. */
+size_t tlm_hip_kv_decode_workspace_bytes(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads);
+int    tlm_hip_kv_decode(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, const void *q, int64_t q_stride, int heads,
+                         float scale, int out_dt, void *out, void *workspace, void *stream);
+/* Attention of packed rows, causal: a row at position p sees the positions 0 .. p of its sequence (cached ones
+ * included).  q and out as above, [rows] for [B]. */
+int    tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, const void *q, int64_t q_stride, int heads,
+                         float scale, int out_dt, void *out, void *stream);
 
 /* ---- reference tier ABI --------------------------------------------------
  * Layout-compatible with tlm_quant_kernels (src/lib/tlm_quant.h:152-166, a

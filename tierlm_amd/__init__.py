@@ -7,5 +7,5 @@ importing fails if the library is not built.
 import torch  # noqa: F401  (before the library, so that both use the HIP runtime that torch brings)
 
 from ._lib import EXPORTS, LIB_PATH, HipError, lib  # noqa: F401
-from . import fp8, quant  # noqa: F401
+from . import fp8, kv, quant  # noqa: F401
 from .moe import MoeBlock, MoeStack  # noqa: F401

@@ -106,6 +106,18 @@ class TensorRef(C.Structure):
                 ("offset", C.c_uint64), ("nbytes", C.c_uint64)]
 
 
+class KvCache(C.Structure):
+    """tlm_hip_kv_cache"""
+    _fields_ = [("dt", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page", C.c_int32),
+                ("n_pages", C.c_int64), ("k", vp), ("v", vp)]
+
+
+class KvBatch(C.Structure):
+    """tlm_hip_kv_batch"""
+    _fields_ = [("B", C.c_int64), ("rows", C.c_int64), ("cu", vp), ("lens", vp), ("tables", vp),
+                ("table_stride", C.c_int64), ("table_pages", C.c_int32)]
+
+
 QDOT = C.CFUNCTYPE(C.c_float, vp, vp, C.c_int64, vp)
 QMV = C.CFUNCTYPE(None, vp, C.c_size_t, vp, vp, C.c_int64, C.c_int64)
 
@@ -195,6 +207,11 @@ _SIGS = {
     "tlm_hip_fp8_packed_bytes": (sz, [i64, i64]),
     "tlm_hip_fp8_pack": (i32, [vp, sz, vp, i64, i64, i64, vp, vp]),
     "tlm_hip_fp8_quantize": (i32, [i32, vp, i64, i64, i64, vp, vp, vp]),
+    "tlm_hip_fp8_add_rmsnorm": (i32, [i32, vp, i64, i32, vp, i64, vp, f32, i64, i64, vp, i64, vp, vp, vp]),
+    "tlm_hip_kv_append": (i32, [C.POINTER(KvCache), C.POINTER(KvBatch), i32, vp, i64, i32, vp, vp, f32, vp, f32, vp, vp]),
+    "tlm_hip_kv_decode_workspace_bytes": (sz, [C.POINTER(KvCache), C.POINTER(KvBatch), i32]),
+    "tlm_hip_kv_decode": (i32, [C.POINTER(KvCache), C.POINTER(KvBatch), vp, i64, i32, f32, i32, vp, vp, vp]),
+    "tlm_hip_kv_prompt": (i32, [C.POINTER(KvCache), C.POINTER(KvBatch), vp, i64, i32, f32, i32, vp, vp]),
     "tlm_hip_fp8_matmul": (i32, [vp, i64, i64, vp, vp, i64, i32, vp, i64, vp]),
     "tlm_hip_fp8_matmul_kernel": (C.c_char_p, [i64, i64, i64]),
     "tlm_hip_fp8_moe_workspace_bytes": (sz, [C.POINTER(MoeDesc), i64]),

@@ -35,34 +35,7 @@ __global__ __launch_bounds__(256) void k_fp8_pack(const uint8_t *__restrict__ W,
     *(u32x4 *)(dst + p * 16) = v;
 }
 
-/* ---- activation quantiser --------------------------------------------------
- * 16 lanes per block of 128 values, 8 values a lane.  scale = 2^e, e the least
- * integer >= -126 with amax <= 448 * 2^e: dividing by it is exact, so the one
- * rounding is the code's, and a floating code loses no relative precision by it. */
-template <class T> __device__ __forceinline__ float ld_f32(const T *p);
-template <> __device__ __forceinline__ float ld_f32<float>(const float *p) { return *p; }
-template <> __device__ __forceinline__ float ld_f32<_Float16>(const _Float16 *p) { return (float)*p; }
-template <> __device__ __forceinline__ float ld_f32<__bf16>(const __bf16 *p) {
-    return __uint_as_float((uint32_t) * (const uint16_t *)p << 16);
-}
-
-/* 8 values from p on, `left` of them in the row; vector loads at any alignment of the
- * elements (this target's memory pipe takes them) */
-template <class T> __device__ __forceinline__ void ld8(float (&v)[8], const T *p, int left) {
-    typedef T T8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-    if (left >= 8) {
-        const T8 q = *(const T8 *)p;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const T e = q[j];
-            v[j] = ld_f32(&e);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = j < left ? ld_f32(p + j) : 0.0f;
-    }
-}
-
+/* ---- activation quantiser: 16 lanes per block of 128 values (fp8_encode) ------ */
 /* U blocks a lane group, their loads in flight together */
 template <class T, int U>
 __global__ __launch_bounds__(256) void k_fp8_quant(const T *__restrict__ x, int64_t xstride, int n, int nb,
@@ -78,29 +51,10 @@ __global__ __launch_bounds__(256) void k_fp8_quant(const T *__restrict__ x, int6
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int blk = blk0 + 16 * u;
-        uint32_t am = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t b = __float_as_uint(v[u][j]) & 0x7FFFFFFFu;   /* order of |v|; NaN and infinity on top */
-            am = b > am ? b : am;
-        }
-        am = group_max_u32<16>(am);
-        /* amax = m 2^x, 1 <= m < 2: e = x - 8 for m <= 1.75, else x - 7 */
-        const int ex = (int)(am >> 23) - 127;
-        int e = (am & 0x7FFFFFu) <= 0x600000u ? ex - 8 : ex - 7;
-        e = e < -126 ? -126 : e;
-        const bool bad = am >= 0x7F800000u;
-        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-        int c0 = 0, c1 = 0;
-        c0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[u][0] * inv, v[u][1] * inv, c0, false);
-        c0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[u][2] * inv, v[u][3] * inv, c0, true);
-        c1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[u][4] * inv, v[u][5] * inv, c1, false);
-        c1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[u][6] * inv, v[u][7] * inv, c1, true);
+        const Fp8Codes c = fp8_encode(v[u]);
         if (blk < blocks) {
-            const u32x2 o = {bad ? 0u : (uint32_t)c0, bad ? 0u : (uint32_t)c1};
-            *(u32x2 *)(codes + (size_t)blk * FP8_BLOCK + 8 * sub) = o;
-            if (sub == 0)
-                scale[blk] = bad ? __uint_as_float(0x7FC00000u) : am ? __uint_as_float((uint32_t)(127 + e) << 23) : 0.0f;
+            *(u32x2 *)(codes + (size_t)blk * FP8_BLOCK + 8 * sub) = c.codes;
+            if (sub == 0) scale[blk] = c.scale;
         }
     }
 }

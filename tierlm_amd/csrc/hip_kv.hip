@@ -1,0 +1,638 @@
+/* hip_kv.hip - the paged key-value cache: appending a batch's rows, and the attention of one new token a
+ * sequence (the reference's attn_heads, src/lib/tlm_model.c:683-749, for many sequences over pages of 16-bit keys and
+ * values).  Layout and work items: tlm_hip_kv.h; prompts: hip_kv_prompt.hip. */
+#include "tlm_hip_kv.h"
+
+namespace {
+
+bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
+
+/* ---- append ------------------------------------------------------------------
+ * A group per block of 16 positions and key head: its up to 16 new rows of that head's G queries, key and value.  16 lanes
+ * hold a vector: lane s the pairs j = M s .. M s + M - 1 and their partners at hd / 2 + j (M = hd / 32), so the norm is one
+ * 16-lane sum and the rotation stays in the lane, and a lane's angles serve every vector of its row.  Values are
+ * turned over in registers (8 rows of one value to 16 bytes): the cache's block is written as whole pieces.
+ * Bound by memory; what a decode step's few rows take is the launch. */
+struct AppendArgs {
+    KvView c;
+    const void *x;
+    int64_t xstride;
+    void *q, *k, *v;
+    const float *qw, *kw;
+    const double *freq;
+    float eps, rope_scale;
+    int G;
+};
+
+template <class X> __device__ __forceinline__ float to_f32(X v) { return (float)v; }
+
+template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
+    constexpr int HD = 32 * M;
+    const KvView &c = a.c;
+    const int tid = threadIdx.x;
+    const KvItem it = kv_find(c.B, (int)blockIdx.x, [&](int b) {
+        const KvRows r = kv_rows(c, b);
+        return (int)kv_append_items(r.n, kv_len(c, b));
+    });
+    if (it.b < 0) return;
+    const int kvh = blockIdx.y, G = a.G, H = G * c.heads;
+    const KvRows r = kv_rows(c, it.b);
+    const int64_t p0 = kv_len(c, it.b) - r.n;                   /* position of the first new row */
+    const int64_t blk = kv_floor16(p0) + it.i;
+    const int64_t lo = blk * KV_BLOCK > p0 ? blk * KV_BLOCK : p0;
+    const int64_t end = blk * KV_BLOCK + KV_BLOCK, hi = end < p0 + r.n ? end : p0 + r.n;
+    const int n = (int)(hi - lo);
+    const X *x = (const X *)a.x + (r.first + lo - p0) * a.xstride;    /* the block's first row */
+    T *q = (T *)a.q + (r.first + lo - p0) * (int64_t)H * HD;
+    int64_t at = -1;
+    if (blk >= 0 && (blk >> c.sh) < c.table_pages)
+        at = kv_block(c, c.tables[it.b * c.table_stride + (blk >> c.sh)], blk, kvh);
+
+    /* queries and key: 16 lane groups, gpt of them to a row */
+    const int sub = tid & 15, grp = tid >> 4;
+    const int gpt = n == 1 ? 16 : n == 2 ? 8 : n <= 4 ? 4 : n <= 8 ? 2 : 1;
+    const int t = grp / gpt;
+    if (t < n) {
+        float cs[M], sn[M];
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            cs[m] = 1.0f;
+            sn[m] = 0.0f;
+        }
+        if (a.freq) {
+            /* the angle in double, less whole turns (2 pi as a sum of two doubles): a far position's fraction of a turn
+             * keeps its bits, and sine and cosine are of a float in [-pi, pi] */
+            const double pos = (double)(lo + t);
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+                const double ang = pos * a.freq[M * sub + m];
+                const double turns = rint(ang * 0.15915494309189535);
+                const double rem = __builtin_fma(-turns, 2.4492935982947064e-16, __builtin_fma(-turns, 6.283185307179586, ang));
+                float s, co;
+                sincosf((float)rem, &s, &co);
+                cs[m] = co * a.rope_scale;
+                sn[m] = s * a.rope_scale;
+            }
+        }
+        const X *row = x + t * a.xstride;
+        const bool written = lo + t >= 0;
+        for (int j = grp % gpt; j <= G; j += gpt) {             /* queries of the head's group, then its key */
+            const X *src = row + (int64_t)(j < G ? kvh * G + j : H + kvh) * HD + M * sub;
+            float u[M], w[M];
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+                u[m] = to_f32(src[m]);
+                w[m] = to_f32(src[HD / 2 + m]);
+            }
+            const float *nw = j < G ? a.qw : a.kw;
+            if (nw) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int m = 0; m < M; m++) ss = fmaf(u[m], u[m], fmaf(w[m], w[m], ss));
+                ss += dpp_f32<DPP_XOR1>(ss);
+                ss += dpp_f32<DPP_XOR2>(ss);
+                ss += dpp_f32<DPP_HALF_MIRROR>(ss);
+                ss += dpp_f32<DPP_MIRROR>(ss);
+                const float f = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
+#pragma unroll
+                for (int m = 0; m < M; m++) {
+                    u[m] = u[m] * f * nw[M * sub + m];
+                    w[m] = w[m] * f * nw[HD / 2 + M * sub + m];
+                }
+            }
+            T lo_[M], hi_[M];
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+                lo_[m] = (T)fmaf(u[m], cs[m], -(w[m] * sn[m]));
+                hi_[m] = (T)fmaf(w[m], cs[m], u[m] * sn[m]);
+                if (!written) lo_[m] = hi_[m] = (T)0.0f;
+            }
+            if (j < G) {
+                T *o = q + (int64_t)t * H * HD + (int64_t)(kvh * G + j) * HD + M * sub;
+#pragma unroll
+                for (int m = 0; m < M; m++) {
+                    o[m] = lo_[m];
+                    o[HD / 2 + m] = hi_[m];
+                }
+            } else if (at >= 0) {
+                T *o = (T *)a.k + at;
+                const int p = (int)(lo + t - blk * KV_BLOCK);
+#pragma unroll
+                for (int m = 0; m < M; m++) {
+                    o[kv_key_at(p, M * sub + m)] = lo_[m];
+                    o[kv_key_at(p, HD / 2 + M * sub + m)] = hi_[m];
+                }
+            }
+        }
+    }
+    if (at < 0) return;
+    /* values: a thread per value and half block */
+    const X *src = x + (int64_t)(H + c.heads + kvh) * HD;
+    const int first = (int)(lo - blk * KV_BLOCK), last = first + n;
+    T *o = (T *)a.v + at;
+    for (int i = tid; i < 2 * HD; i += 256) {
+        const int d = i >> 1, p0h = (i & 1) * 8;
+        if (p0h >= last || p0h + 8 <= first) continue;
+        T e[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int p = p0h + j;
+            e[j] = p >= first && p < last ? (T)to_f32(src[(p - first) * a.xstride + d]) : (T)0.0f;
+        }
+        if (p0h >= first && p0h + 8 <= last) {
+            typename KvType<T>::x8 w;
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = e[j];
+            *(typename KvType<T>::x8 *)(o + kv_value_at(p0h, d)) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (p0h + j >= first && p0h + j < last) o[kv_value_at(p0h + j, d)] = e[j];
+        }
+    }
+}
+
+/* ---- decode --------------------------------------------------------------------
+ * out = sum_j p_j v_j / sum_j p_j, p_j = 2^(scale log2(e) q . k_j - m), one pass over the cache with the running maximum m.
+ * A group takes one run of a sequence's positions for one key head and up to 16 NC of its queries; its NW waves take tiles
+ * of 32 positions in turn, straight from memory into the matrix cores' operands (no LDS on the way), the next tile's
+ * loads in flight, and merge their sums through LDS at the end.  The bytes of the cache bound it.
+ *
+ * Runs: the lengths are the device's, so every group works the split out for itself: W items for B sequences, the run
+ * length such that W suffices whatever the lengths are (kv_run); a long sequence among short ones is split as far as the
+ * total asks.  Sequences of one run are written at once; the others' sums go to the workspace, item w's at w, and k_kv_join
+ * adds a sequence's in order. */
+struct DecodeArgs {
+    KvView c;
+    const void *q, *k, *v;
+    void *out;
+    float *part, *ml;        /* [W][heads][HD] sums, [W][heads][2] maximum and weight */
+    int64_t qstride;
+    float scale2;            /* scale log2(e) */
+    int G, W, out_dt;
+    int64_t run;             /* > 0: no split, every sequence is one run */
+};
+
+__device__ __forceinline__ void store_out(void *out, int dt, int64_t i, const float (&v)[4]) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef __bf16 b4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef f32x4 f4 __attribute__((aligned(4)));
+    if (dt == DT_F32) *(f4 *)((float *)out + i) = f4{v[0], v[1], v[2], v[3]};
+    else if (dt == DT_F16) *(h4 *)((_Float16 *)out + i) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    else *(b4 *)((__bf16 *)out + i) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+}
+
+/* the run length of a batch (W > B), the same in every group */
+__device__ __forceinline__ int64_t decode_run(const KvView &c, int W) {
+    const int64_t cap = kv_cap(c);
+    double sum = 0.0;   /* exact: whole numbers below 2^53 */
+    for (int b = wave_lane(); b < c.B; b += 64) {
+        const int64_t len = kv_len(c, b);
+        sum += (double)(len < cap ? len : cap);
+    }
+    return kv_run((int64_t)wave_sum_f64(sum), W, c.B, 128);
+}
+
+template <class T, int HD, int NC, int NW>
+__global__ __launch_bounds__(NW * 64, HD *NC <= 128 ? 2 : 1) void k_kv_decode(DecodeArgs a) {
+    typedef typename KvType<T>::x8 x8;
+    constexpr int KS = HD / 32, DT = HD / 16;    /* steps of the first product, result tiles of the second */
+    constexpr int LD = HD + 4;                   /* a merged column in LDS: 16 lanes' float4 on all banks */
+    __shared__ float s_o[NW / 2][NC * 16 * LD], s_ml[NW / 2][NC * 16 * 2];
+    const KvView &c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = kv_uniform(tid >> 6), col = lane & 15, g = lane >> 4;
+    const int64_t cap = kv_cap(c), run = a.run > 0 ? a.run : decode_run(c, a.W);
+    auto length = [&](int b) {
+        const int64_t len = kv_len(c, b);
+        return len < cap ? len : cap;
+    };
+    KvItem it;
+    if (a.run > 0) it = {(int)blockIdx.x, 0, 1, (int)blockIdx.x};
+    else it = kv_find(c.B, (int)blockIdx.x, [&](int b) { return (int)kv_decode_items(length(b), run); });
+    if (it.b < 0) return;
+    const int kvh = blockIdx.y, col0 = blockIdx.z * NC * 16, ncol = a.G - col0 < NC * 16 ? a.G - col0 : NC * 16;
+    const int32_t *table = c.tables + it.b * c.table_stride;
+    const int len = (int)length(it.b);
+    const int begin = (int)(it.i * run), stop = len - begin < run ? len : (int)(begin + run);
+    const int tiles = (stop - begin + 31) / 32;     /* 0: an empty sequence */
+
+    /* queries: column col, values 32 ks + 8 g .. + 7 */
+    x8 qf[NC][KS];
+#pragma unroll
+    for (int n = 0; n < NC; n++)
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int h = n * 16 + col;
+            u32x4 v = {0, 0, 0, 0};
+            if (h < ncol)
+                v = kv_load8((const T *)a.q + it.b * a.qstride + (int64_t)(kvh * a.G + col0 + h) * HD + 32 * ks + 8 * g);
+            qf[n][ks] = kv_bits<x8>(v);
+        }
+
+    /* A tile's two blocks: row i of key tile t is position 8 (i / 4) + 4 t + i % 4 (block i / 8), so that a lane's scores are
+     * the positions 8 g .. 8 g + 7 (block g / 2), which are its operand of the second product. */
+    const int krow = 8 * (col >> 2) + (col & 3);
+    const int koff = kv_key_at(krow & 15, 0) + (g >> 1) * 256 + (g & 1) * 8;   /* + 64 t (four positions) + 512 ks */
+    const int voff = kv_value_at(0, col) + (g & 1) * 8;                        /* + 256 dt */
+    struct Tile {
+        u32x4 k[2][KS], v[DT];
+        int ok;          /* bit i: block i is a page's */
+    };
+    /* the wave's page numbers, 32 of its tiles at a time: lane 2 i + j holds block j of its i-th tile */
+    int pages = 0;
+    auto names = [&](int i0) {
+        const int blk = begin / KV_BLOCK + 2 * (wave + NW * (i0 + (lane >> 1))) + (lane & 1);
+        const int lastb = (stop - 1) / KV_BLOCK;
+        pages = blk <= lastb ? table[blk >> c.sh] : -1;
+    };
+    auto load = [&](Tile &t, int i) {
+        const int b0 = begin / KV_BLOCK + 2 * (wave + NW * i);
+        int64_t o0 = kv_block(c, __builtin_amdgcn_readlane(pages, 2 * (i & 31)), b0, kvh);
+        int64_t o1 = kv_block(c, __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1), b0 + 1, kvh);
+        t.ok = (o0 >= 0 ? 1 : 0) | (o1 >= 0 ? 2 : 0);
+        o0 = o0 < 0 ? 0 : o0;    /* block 0 is inside the cache; what it holds is masked */
+        o1 = o1 < 0 ? 0 : o1;
+        const GAS T *k = (const GAS T *)a.k + ((col & 8) ? o1 : o0) + koff;
+        const GAS T *v = (const GAS T *)a.v + (g >= 2 ? o1 : o0) + voff;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            t.k[0][ks] = *(const GAS u32x4 *)(k + 512 * ks);
+            t.k[1][ks] = *(const GAS u32x4 *)(k + 512 * ks + 64);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) t.v[dt] = *(const GAS u32x4 *)(v + 256 * dt);
+    };
+
+    f32x4 o[NC][DT];
+    float m[NC], l[NC];
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) o[n][dt] = f32x4{0, 0, 0, 0};
+    }
+    auto compute = [&](Tile &t, int i) {
+        const int p0 = begin + 32 * (wave + NW * i) + 8 * g;     /* the lane's first position */
+        const bool whole = p0 - 8 * g + 32 <= stop && t.ok == 3;
+        const int left = ((t.ok >> (g >> 1)) & 1) ? stop - p0 : 0;
+        if (!whole) {    /* what a masked place holds may be anything, and 0 times it not 0 */
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    t.v[dt][w] &= (2 * w < left ? 0xFFFFu : 0u) | (2 * w + 1 < left ? 0xFFFF0000u : 0u);
+        }
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            f32x4 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                s[u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) s[u] = KvType<T>::mma(kv_bits<x8>(t.k[u][ks]), qf[n][ks], s[u]);
+            }
+            float z[8];
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                z[j] = s[j >> 2][j & 3] * a.scale2;
+                if (!whole && j >= left) z[j] = -INFINITY;
+                top = fmaxf(top, z[j]);
+            }
+            if (__any(top > m[n] + KV_SLACK)) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                /* each column by its own scores: another's do not show in its bits */
+                const float to = top > m[n] + KV_SLACK ? top : m[n], f = to == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - to);
+                m[n] = to;
+                l[n] *= f;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[n][dt] *= f;
+            }
+            /* before any score is above -infinity the maximum is taken as 0 */
+            const float base = (m[n] == -INFINITY ? 0.0f : m[n]) - KvType<T>::SHIFT;
+            x8 p;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float e = __builtin_amdgcn_exp2f(z[j] - base);
+                l[n] += e;
+                p[j] = (T)e;   /* 8 (bf16) or 11 bits of a weight in [0, 1]: as the values it is multiplied with have */
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) o[n][dt] = KvType<T>::mma(kv_bits<x8>(t.v[dt]), p, o[n][dt]);
+        }
+    };
+    const int mine = (tiles - wave + NW - 1) / NW;      /* this wave's tiles */
+    if (mine > 0) {
+        Tile ta, tb;
+        names(0);
+        load(ta, 0);
+        for (int i = 0; i < mine; i += 2) {
+            if (i + 1 < mine) load(tb, i + 1);
+            compute(ta, i);
+            if (i + 2 < mine) {
+                if (((i + 2) & 31) == 0) names(i + 2);
+                load(ta, i + 2);
+            }
+            if (i + 1 < mine) compute(tb, i + 1);
+        }
+    }
+    /* the lanes of a column hold different positions' weights */
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        l[n] += __shfl_xor(l[n], 16, 64);
+        l[n] += __shfl_xor(l[n], 32, 64);
+    }
+    /* merge the waves, half of them at a time, always in the same order */
+#pragma unroll
+    for (int half = NW / 2; half >= 1; half >>= 1) {
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+                    *(f32x4 *)&s_o[wave - half][(n * 16 + col) * LD + 16 * dt + 4 * g] = o[n][dt];
+                if (g == 0) {
+                    s_ml[wave - half][(n * 16 + col) * 2] = m[n];
+                    s_ml[wave - half][(n * 16 + col) * 2 + 1] = l[n];
+                }
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                const float om = s_ml[wave][(n * 16 + col) * 2], ol = s_ml[wave][(n * 16 + col) * 2 + 1];
+                const float to = fmaxf(m[n], om), base = to == -INFINITY ? 0.0f : to;
+                const float fm = __builtin_amdgcn_exp2f(m[n] - base), fo = __builtin_amdgcn_exp2f(om - base);
+                m[n] = to;
+                l[n] = l[n] * fm + ol * fo;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    const f32x4 w = *(const f32x4 *)&s_o[wave][(n * 16 + col) * LD + 16 * dt + 4 * g];
+                    o[n][dt] = o[n][dt] * fm + w * fo;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (wave > 0) return;
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        const int h = n * 16 + col;
+        if (h >= ncol) continue;
+        const int64_t head = kvh * a.G + col0 + h, H = (int64_t)a.G * c.heads;
+        if (it.n == 1) {
+            const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];     /* no position at all: zeros */
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                const float v[4] = {o[n][dt][0] * inv, o[n][dt][1] * inv, o[n][dt][2] * inv, o[n][dt][3] * inv};
+                store_out(a.out, a.out_dt, (it.b * H + head) * HD + 16 * dt + 4 * g, v);
+            }
+        } else {
+            const int64_t w = (int64_t)blockIdx.x * H + head;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) *(f32x4 *)(a.part + w * HD + 16 * dt + 4 * g) = o[n][dt];
+            if (g == 0) {
+                a.ml[2 * w] = m[n];
+                a.ml[2 * w + 1] = l[n];
+            }
+        }
+    }
+}
+
+/* The sums of a sequence of several runs, one group a sequence and head: four lanes' values a thread, the runs dealt to the
+ * threads' rows, added through LDS in a fixed order. */
+template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a) {
+    constexpr int L4 = HD / 4, R = 256 / L4;
+    __shared__ float s_o[R][HD], s_l[R], s_m[4];
+    const KvView &c = a.c;
+    const int64_t cap = kv_cap(c), run = decode_run(c, a.W);
+    const int b = blockIdx.x, head = blockIdx.y, H = a.G * c.heads, tid = threadIdx.x;
+    auto items = [&](int b) {
+        const int64_t len = kv_len(c, b);
+        return (int)kv_decode_items(len < cap ? len : cap, run);
+    };
+    const int n = items(b);
+    if (n == 1) return;
+    int before = 0;
+    for (int i = wave_lane(); i < b; i += 64) before += items(i);
+    before = (int)wave_sum_f64((double)before);
+    const int64_t w0 = (int64_t)before * H + head;
+    float top = -INFINITY;
+    for (int i = tid; i < n; i += 256) top = fmaxf(top, a.ml[2 * (w0 + (int64_t)i * H)]);
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if ((tid & 63) == 0) s_m[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    const float base = top == -INFINITY ? 0.0f : top;
+    const int r = tid / L4, e = tid % L4 * 4;
+    if (r < R) {
+        f32x4 o = {0, 0, 0, 0};
+        float l = 0.0f;
+#pragma unroll 4
+        for (int i = r; i < n; i += R) {
+            const int64_t w = w0 + (int64_t)i * H;
+            const float f = __builtin_amdgcn_exp2f(a.ml[2 * w] - base);
+            l += a.ml[2 * w + 1] * f;
+            o += *(const f32x4 *)(a.part + w * HD + e) * f;
+        }
+        *(f32x4 *)&s_o[r][e] = o;
+        if (e == 0) s_l[r] = l;
+    }
+    __syncthreads();
+    if (tid >= L4) return;
+    f32x4 o = {0, 0, 0, 0};
+    float l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        o += *(const f32x4 *)&s_o[i][e];
+        l += s_l[i];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    store_out(a.out, a.out_dt, ((int64_t)b * H + head) * HD + e, v);
+}
+
+/* ---- launches -------------------------------------------------------------- */
+template <class X, class T, int M> void append_m(const AppendArgs &a, dim3 grid, hipStream_t s) {
+    hipLaunchKernelGGL((k_kv_append<X, T, M>), grid, dim3(256), 0, s, a);
+}
+template <class X, class T> void append_hd(const AppendArgs &a, dim3 grid, hipStream_t s) {
+    static void (*const by_width[8])(const AppendArgs &, dim3, hipStream_t) = {
+        append_m<X, T, 1>, append_m<X, T, 2>, append_m<X, T, 3>, append_m<X, T, 4>,
+        append_m<X, T, 5>, append_m<X, T, 6>, append_m<X, T, 7>, append_m<X, T, 8>};
+    by_width[a.c.hd / 32 - 1](a, grid, s);
+}
+template <class T> void append_x(int xdt, const AppendArgs &a, dim3 grid, hipStream_t s) {
+    if (xdt == DT_F32) append_hd<float, T>(a, grid, s);
+    else if (xdt == DT_F16) append_hd<_Float16, T>(a, grid, s);
+    else append_hd<__bf16, T>(a, grid, s);
+}
+
+/* Up to this many positions a sequence, by its table, every sequence is one group of eight waves and one launch */
+constexpr int64_t DECODE_WHOLE = 2048;
+/* Items that fill the chip: four groups of four waves a compute unit */
+constexpr int64_t DECODE_GROUPS = 1024;
+
+struct DecodePlan {
+    int64_t run;
+    int W, nc, z;
+};
+DecodePlan decode_plan(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads) {
+    const int G = heads / c->kv_heads, nc = G <= 16 ? 1 : G <= 32 || c->head_dim > 128 ? 2 : 4, z = (G + nc * 16 - 1) / (nc * 16);
+    const int64_t cap = (int64_t)b->table_pages * c->page;
+    if (cap <= DECODE_WHOLE) return {cap, (int)b->B, nc, z};
+    int64_t W = DECODE_GROUPS / ((int64_t)c->kv_heads * z);
+    W = W > 2 * b->B ? W : 2 * b->B;
+    return {0, (int)W, nc, z};
+}
+size_t decode_bytes(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads) {
+    const DecodePlan p = decode_plan(c, b, heads);
+    return p.run ? 0 : (size_t)p.W * heads * (c->head_dim + 4) * 4;
+}
+
+template <class T, int HD, int NC> void decode_nc(const DecodeArgs &a, const DecodePlan &p, hipStream_t s) {
+    const dim3 grid((unsigned)p.W, (unsigned)a.c.heads, (unsigned)p.z);
+    if (p.run) {
+        constexpr int NW = NC == 1 && HD <= 128 ? 8 : 4;   /* eight waves leave a wave 256 registers */
+        hipLaunchKernelGGL((k_kv_decode<T, HD, NC, NW>), grid, dim3(NW * 64), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((k_kv_decode<T, HD, NC, 4>), grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_kv_join<HD>), dim3((unsigned)a.c.B, (unsigned)(a.G * a.c.heads)), dim3(256), 0, s, a);
+    }
+}
+template <class T, int HD> void decode_hd(const DecodeArgs &a, const DecodePlan &p, hipStream_t s) {
+    if (p.nc == 1) decode_nc<T, HD, 1>(a, p, s);
+    else if (p.nc == 2) decode_nc<T, HD, 2>(a, p, s);
+    else if constexpr (HD <= 128) decode_nc<T, HD, 4>(a, p, s);
+}
+template <class T> void decode(const DecodeArgs &a, const DecodePlan &p, hipStream_t s) {
+    static void (*const by_width[8])(const DecodeArgs &, const DecodePlan &, hipStream_t) = {
+        decode_hd<T, 32>, decode_hd<T, 64>, decode_hd<T, 96>, decode_hd<T, 128>,
+        decode_hd<T, 160>, decode_hd<T, 192>, decode_hd<T, 224>, decode_hd<T, 256>};
+    by_width[a.c.hd / 32 - 1](a, p, s);
+}
+
+} // namespace
+
+/* What all three calls ask of a cache and a batch; *v is filled for the kernels */
+int kv_check(const char *who, const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads, KvView *v) {
+    if (!c || !b) return tlmh_seterr(TLM_HIP_EINVAL, "%s: NULL argument", who);
+    if (c->dt != DT_F16 && c->dt != DT_BF16)
+        return tlmh_seterr(TLM_HIP_EUNSUP, "%s: cache of dtype %d (F16 and BF16 only)", who, c->dt);
+    if (c->head_dim < 32 || c->head_dim > 256 || c->head_dim % 32)
+        return tlmh_seterr(TLM_HIP_EUNSUP, "%s: head_dim %d is not a multiple of 32 up to 256", who, c->head_dim);
+    if (c->page < KV_BLOCK || c->page > 4096 || (c->page & (c->page - 1)))
+        return tlmh_seterr(TLM_HIP_EINVAL, "%s: page of %d positions (a power of two from 16 to 4096)", who, c->page);
+    if (c->kv_heads < 1 || c->kv_heads > 4096 || heads < 1 || heads > 65536 || heads % c->kv_heads)
+        return tlmh_seterr(TLM_HIP_EINVAL, "%s: %d heads on %d key heads", who, heads, c->kv_heads);
+    if (c->n_pages < 1 || c->n_pages > 0x7FFFFFFF)
+        return tlmh_seterr(TLM_HIP_EINVAL, "%s: %lld pages", who, (long long)c->n_pages);
+    if (b->B < 0 || b->rows < 0 || (!b->cu && b->rows != b->B))
+        return tlmh_seterr(TLM_HIP_EINVAL, "%s: %lld rows of %lld sequences", who, (long long)b->rows, (long long)b->B);
+    if (b->B > (1 << 20) || b->rows * heads > ((int64_t)1 << 30))
+        return tlmh_seterr(TLM_HIP_ERANGE, "%s: %lld rows of %lld sequences are too many for one launch", who,
+                           (long long)b->rows, (long long)b->B);
+    if (b->table_pages < 1 || (int64_t)b->table_pages * c->page > (1 << 30))
+        return tlmh_seterr(TLM_HIP_EINVAL, "%s: tables of %d pages (1 to 2^30 positions)", who, b->table_pages);
+    if (b->B > 1 && b->table_stride < b->table_pages)
+        return tlmh_seterr(TLM_HIP_EINVAL, "%s: table stride %lld below %d", who, (long long)b->table_stride, b->table_pages);
+    if (b->B > 0 && b->rows > 0) {
+        if (!c->k || !c->v || !b->lens || !b->tables) return tlmh_seterr(TLM_HIP_EINVAL, "%s: NULL argument", who);
+        if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(b->lens, 4) || !aligned(b->tables, 4) || !aligned(b->cu, 4))
+            return tlmh_seterr(TLM_HIP_EINVAL, "%s: keys and values must be 16-byte, lens, tables and cu 4-byte aligned", who);
+    }
+    int sh = 0;
+    while ((KV_BLOCK << sh) < c->page) sh++;
+    *v = {b->tables, b->lens, b->cu, b->table_stride, b->rows, (int32_t)b->B, b->table_pages, (int32_t)c->n_pages,
+          c->kv_heads, sh, c->head_dim};
+    return TLM_HIP_OK;
+}
+
+extern "C" {
+
+int tlm_hip_kv_append(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int dt, const void *qkv, int64_t qkv_stride,
+                      int heads, const float *q_norm, const float *k_norm, float eps, const double *inv_freq,
+                      float rope_scale, void *q, void *stream) {
+    AppendArgs a;
+    if (int rc = kv_check("kv_append", c, b, heads, &a.c)) return rc;
+    if (!type_bytes(dt)) return tlmh_seterr(TLM_HIP_EUNSUP, "kv_append: dtype %d (F32, F16 and BF16 only)", dt);
+    if (!(eps >= 0.0f) || eps > 3.0e38f) return tlmh_seterr(TLM_HIP_EINVAL, "kv_append: eps must be finite and not negative");
+    if (b->B == 0 || b->rows == 0) return TLM_HIP_OK;
+    if (!qkv || !q) return tlmh_seterr(TLM_HIP_EINVAL, "kv_append: NULL argument");
+    const int64_t width = (int64_t)(heads + 2 * c->kv_heads) * c->head_dim;
+    if (qkv_stride < width && b->rows > 1)
+        return tlmh_seterr(TLM_HIP_EINVAL, "kv_append: row stride %lld below %lld", (long long)qkv_stride, (long long)width);
+    if (!aligned(qkv, (size_t)type_bytes(dt)) || !aligned(q, 16) || !aligned(q_norm, 4) || !aligned(k_norm, 4) ||
+        !aligned(inv_freq, 8))
+        return tlmh_seterr(TLM_HIP_EINVAL, "kv_append: qkv must have its type's alignment, q 16, the norms 4, inv_freq 8 "
+                           "bytes");
+    const int64_t items = kv_append_most(b->rows, b->B);
+    if (items > (1 << 23))
+        return tlmh_seterr(TLM_HIP_ERANGE, "kv_append: %lld rows of %lld sequences are too many for one launch",
+                           (long long)b->rows, (long long)b->B);
+    a.x = qkv;
+    a.xstride = qkv_stride;
+    a.q = q;
+    a.k = c->k;
+    a.v = c->v;
+    a.qw = q_norm;
+    a.kw = k_norm;
+    a.freq = inv_freq;
+    a.eps = eps;
+    a.rope_scale = rope_scale;
+    a.G = heads / c->kv_heads;
+    const dim3 grid((unsigned)items, (unsigned)c->kv_heads);
+    if (c->dt == DT_F16) append_x<_Float16>(dt, a, grid, (hipStream_t)stream);
+    else append_x<__bf16>(dt, a, grid, (hipStream_t)stream);
+    return tlmh_check(hipGetLastError(), "kv_append launch");
+}
+
+size_t tlm_hip_kv_decode_workspace_bytes(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads) {
+    KvView v;
+    if (kv_check("kv_decode_workspace_bytes", c, b, heads, &v)) return 0;
+    return decode_bytes(c, b, heads);
+}
+
+int tlm_hip_kv_decode(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, const void *q, int64_t q_stride, int heads,
+                      float scale, int out_dt, void *out, void *workspace, void *stream) {
+    DecodeArgs a;
+    if (int rc = kv_check("kv_decode", c, b, heads, &a.c)) return rc;
+    if (b->cu) return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: one row a sequence (cu must be NULL)");
+    if (!type_bytes(out_dt)) return tlmh_seterr(TLM_HIP_EUNSUP, "kv_decode: dtype %d (F32, F16 and BF16 only)", out_dt);
+    if (!(scale > 0.0f) || scale > 3.0e38f) return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: scale must be finite and positive");
+    if (b->B == 0) return TLM_HIP_OK;
+    if (!q || !out) return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: NULL argument");
+    if (q_stride < (int64_t)heads * c->head_dim && b->B > 1)
+        return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: row stride %lld below %lld", (long long)q_stride,
+                           (long long)heads * c->head_dim);
+    if (!aligned(q, 2) || !aligned(out, (size_t)type_bytes(out_dt)))
+        return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: q and out must have their type's alignment");
+    const DecodePlan p = decode_plan(c, b, heads);
+    if ((int64_t)p.W * c->kv_heads * p.z > (1 << 22))
+        return tlmh_seterr(TLM_HIP_ERANGE, "kv_decode: %lld sequences of %d heads are too many for one launch",
+                           (long long)b->B, heads);
+    if (!p.run && (!workspace || !aligned(workspace, 256)))
+        return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: needs a workspace of %zu bytes, 256-byte aligned", decode_bytes(c, b, heads));
+    a.q = q;
+    a.k = c->k;
+    a.v = c->v;
+    a.out = out;
+    a.part = (float *)workspace;
+    a.ml = p.run ? nullptr : a.part + (size_t)p.W * heads * c->head_dim;
+    a.qstride = q_stride;
+    a.scale2 = scale * 1.44269504088896341f;
+    a.G = heads / c->kv_heads;
+    a.W = p.W;
+    a.out_dt = out_dt;
+    a.run = p.run;
+    if (c->dt == DT_F16) decode<_Float16>(a, p, (hipStream_t)stream);
+    else decode<__bf16>(a, p, (hipStream_t)stream);
+    return tlmh_check(hipGetLastError(), "kv_decode launch");
+}
+
+} // extern "C"

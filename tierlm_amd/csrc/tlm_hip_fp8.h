@@ -36,6 +36,60 @@ __device__ __forceinline__ i32x8 fp8_join(i32x4 lo, i32x4 hi) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+template <class T> __device__ __forceinline__ float ld_f32(const T *p);
+template <> __device__ __forceinline__ float ld_f32<float>(const float *p) { return *p; }
+template <> __device__ __forceinline__ float ld_f32<_Float16>(const _Float16 *p) { return (float)*p; }
+template <> __device__ __forceinline__ float ld_f32<__bf16>(const __bf16 *p) {
+    return __uint_as_float((uint32_t) * (const uint16_t *)p << 16);
+}
+
+/* 8 values from p on, `left` of them in the row; vector loads at any alignment of the
+ * elements (this target's memory pipe takes them) */
+template <class T> __device__ __forceinline__ void ld8(float (&v)[8], const T *p, int left) {
+    typedef T T8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    if (left >= 8) {
+        const T8 q = *(const T8 *)p;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const T e = q[j];
+            v[j] = ld_f32(&e);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = j < left ? ld_f32(p + j) : 0.0f;
+    }
+}
+
+/* A block of 128 values held by 16 lanes, 8 a lane: this lane's codes and the block's scale.
+ * scale = 2^e, e the least integer >= -126 with amax <= 448 * 2^e: dividing by it is exact, so the one
+ * rounding is the code's, and a floating code loses no relative precision by it. */
+struct Fp8Codes {
+    u32x2 codes;
+    float scale;
+};
+__device__ __forceinline__ Fp8Codes fp8_encode(const float (&v)[8]) {
+    uint32_t am = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;   /* order of |v|; NaN and infinity on top */
+        am = b > am ? b : am;
+    }
+    am = group_max_u32<16>(am);
+    /* amax = m 2^x, 1 <= m < 2: e = x - 8 for m <= 1.75, else x - 7 */
+    const int ex = (int)(am >> 23) - 127;
+    int e = (am & 0x7FFFFFu) <= 0x600000u ? ex - 8 : ex - 7;
+    e = e < -126 ? -126 : e;
+    const bool bad = am >= 0x7F800000u;
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    int c0 = 0, c1 = 0;
+    c0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, c0, false);
+    c0 = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, c0, true);
+    c1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, c1, false);
+    c1 = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, c1, true);
+    return {{bad ? 0u : (uint32_t)c0, bad ? 0u : (uint32_t)c1},
+            bad ? __uint_as_float(0x7FC00000u) : am ? __uint_as_float((uint32_t)(127 + e) << 23) : 0.0f};
+}
+
 /* eight codes times a power of two (1 / 2^100 to 2^100) as bfloat16: exact (E4M3 has 4 significant
  * bits, from 2^-9 to 448) */
 __device__ __forceinline__ bf16x8 fp8_to_bf16(int lo, int hi, float pow2 = 1.0f) {

@@ -1,0 +1,173 @@
+/* tlm_hip_kv.h - the paged key-value cache: where a position lies, which work a group takes.
+ *
+ * A page holds P positions (a power of two >= 16) of every key head, as blocks of 16 positions.  Block
+ * (page, head, i) of 16 * head_dim elements is number (page * heads + head) * (P / 16) + i of either array:
+ *   keys    [head_dim / 16][16 positions][16 values]
+ *   values  [head_dim][16 positions]
+ * Both are the order in which the matrix cores take their operands: S^T = K Q^T contracts over values, O^T = V^T P^T over
+ * positions, and a lane's operand is 8 consecutive elements of the contracted axis.  So every fragment is 16-byte pieces
+ * of one contiguous kilobyte, from memory or LDS, with no transposition and no bank conflict, and the scores' result
+ * lanes (one query each) hold the very positions that the second product's operand wants.
+ *
+ * Plain C++ but for the last part: the CPU tests compile it without HIP.  Included by .hip files. */
+#ifndef TLM_HIP_KV_H
+#define TLM_HIP_KV_H
+
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#include "tlm_hip_internal.h"
+#define TLM_HD __host__ __device__ __forceinline__
+#else
+#define TLM_HD inline
+#endif
+
+constexpr int KV_BLOCK = 16;      /* positions of a block */
+
+/* What the kernels know of a cache and its batch.  Lengths, row bounds and tables are the device's: they are held to
+ * their limits where they are used, and what lies outside holds nothing. */
+struct KvView {
+    const int32_t *tables, *lens, *cu;   /* cu: null, a row a sequence */
+    int64_t table_stride;
+    int64_t rows;
+    int32_t B, table_pages, n_pages, heads;
+    int32_t sh;                          /* log2 of a page's blocks */
+    int32_t hd;
+};
+
+/* rows of sequence b (first, count) inside [0, rows) whatever cu holds */
+struct KvRows {
+    int64_t first, n;
+};
+TLM_HD KvRows kv_rows(const KvView &c, int b) {
+    if (!c.cu) return {b, b < c.rows ? 1 : 0};
+    int64_t lo = c.cu[b], hi = c.cu[b + 1];
+    lo = lo < 0 ? 0 : lo > c.rows ? c.rows : lo;
+    hi = hi < lo ? lo : hi > c.rows ? c.rows : hi;
+    return {lo, hi - lo};
+}
+/* positions of sequence b after this call's rows (negative lengths are zero) */
+TLM_HD int64_t kv_len(const KvView &c, int b) { return c.lens[b] < 0 ? 0 : c.lens[b]; }
+/* positions that its table can name */
+TLM_HD int64_t kv_cap(const KvView &c) { return ((int64_t)c.table_pages << c.sh) * KV_BLOCK; }
+
+/* Element offset of block `blk` (16 positions) of a sequence's head: -1 where the table names no page of the cache. */
+TLM_HD int64_t kv_block(const KvView &c, int32_t page, int64_t blk, int head) {
+    if ((uint32_t)page >= (uint32_t)c.n_pages) return -1;
+    const int64_t at = (((int64_t)page * c.heads + head) << c.sh) + (blk & (((int64_t)1 << c.sh) - 1));
+    return at * (KV_BLOCK * c.hd);
+}
+/* Key value e / value value e of position p (mod 16) inside a block */
+TLM_HD int kv_key_at(int p, int e) { return e / 16 * 256 + p * 16 + e % 16; }
+TLM_HD int kv_value_at(int p, int e) { return e * 16 + p; }
+
+/* ---- append: an item is a block of 16 positions of a sequence ------------- */
+/* First position of a sequence's new rows (negative if it has more rows than positions), and the blocks they touch */
+TLM_HD int64_t kv_floor16(int64_t p) { return p >= 0 ? p / 16 : -((15 - p) / 16); }
+TLM_HD int64_t kv_append_items(int64_t n, int64_t len) {
+    return n > 0 ? kv_floor16(len - 1) - kv_floor16(len - n) + 1 : 0;
+}
+/* as many items as any lengths of B sequences with `rows` rows give */
+TLM_HD int64_t kv_append_most(int64_t rows, int64_t B) {
+    const int64_t used = rows < B ? rows : B;   /* sequences that can have a row; n rows touch at most (n + 14) / 16 + 1 */
+    return (rows + 14 * used) / 16 + used;
+}
+
+/* ---- decode: an item is a run of a sequence's positions ------------------- */
+/* With W items for B sequences (W > B) and `total` positions: the run length that W items suffice for, a multiple of unit.
+ * Sum of ceil(len / c) over the sequences (at least one each) <= total / c + B <= W. */
+TLM_HD int64_t kv_run(int64_t total, int64_t W, int64_t B, int64_t unit) {
+    const int64_t c = (total + (W - B) - 1) / (W - B);
+    return c < unit ? unit : (c + unit - 1) / unit * unit;
+}
+TLM_HD int64_t kv_decode_items(int64_t len, int64_t run) { return len <= run ? 1 : (len + run - 1) / run; }
+
+/* ---- prompt: an item is a tile of a sequence's (token, head) rows ---------- */
+TLM_HD int64_t kv_prompt_items(int64_t n, int64_t group, int64_t tile) { return (n * group + tile - 1) / tile; }
+TLM_HD int64_t kv_prompt_most(int64_t rows, int64_t B, int64_t group, int64_t tile) {
+    const int64_t used = rows < B ? rows : B;
+    return (rows * group - used) / tile + used;   /* sum of ceil(x_b / tile), x_b >= 1 */
+}
+
+#ifdef __HIPCC__
+/* constant memory: what no launch under way writes; uniform reads go through the scalar cache */
+#define CAS __attribute__((address_space(4)))
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+/* 16-bit types of cache and queries and their matrix instructions */
+template <class T> struct KvType;
+template <> struct KvType<__bf16> {
+    typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+    static constexpr uint32_t EXP = 0x7F80u;      /* all ones: an infinity or NaN */
+    static constexpr float SHIFT = 0.0f;
+    static __device__ __forceinline__ f32x4 mma(x8 a, x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mma(x8 a, x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct KvType<_Float16> {
+    typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+    static constexpr uint32_t EXP = 0x7C00u;
+    /* probabilities are held times 2^8: with at most 2^6 over the running maximum they stay finite, and those that a long
+     * context leaves near 2^-20 stay out of the subnormals */
+    static constexpr float SHIFT = 8.0f;
+    static __device__ __forceinline__ f32x4 mma(x8 a, x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mma(x8 a, x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+/* How far (in powers of two) scores may rise over the maximum that the running sums are scaled by before those are
+ * scaled anew: the probabilities stay finite in either type and in the float sums, and most tiles scale nothing */
+constexpr float KV_SLACK = 6.0f;
+
+template <class V> __device__ __forceinline__ V kv_bits(u32x4 v) { return __builtin_bit_cast(V, v); }
+
+/* 8 consecutive elements at any alignment of the type */
+template <class T> __device__ __forceinline__ u32x4 kv_load8(const T *p) {
+    typedef u32x4 any __attribute__((aligned(2)));
+    return *(const any *)p;
+}
+
+__device__ __forceinline__ int kv_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+/* sum of the lanes up to this one */
+__device__ __forceinline__ int kv_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);    /* row_shr 1, 2, 4, 8: inside 16 lanes */
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   /* lanes 15 and 47 to the rows behind them */
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   /* lane 31 to the upper half */
+    return v;
+}
+
+/* Which sequence item w belongs to, and its number there, by a scan over the sequences' item counts, 64 a round (each
+ * wave by itself).  b < 0: there are fewer items.  before: the items of the sequences before it.  Every field is uniform. */
+struct KvItem {
+    int b, i, n, before;
+};
+template <class Count> __device__ __forceinline__ KvItem kv_find(int B, int w, const Count &count) {
+    const int lane = wave_lane();
+    int before = 0;
+    for (int b0 = 0; b0 < B; b0 += 64) {
+        const int mine = b0 + lane < B ? count(b0 + lane) : 0, upto = kv_scan(mine);
+        const uint64_t in = __ballot(before + upto > w);
+        if (in) {
+            const int l = __builtin_ctzll(in);
+            const int n = __builtin_amdgcn_readlane(mine, l), u = __builtin_amdgcn_readlane(upto, l);
+            const int i = w - (before + u - n);
+            /* row bounds that overlap can add up past an int */
+            return {i >= 0 && i < n ? b0 + l : -1, i, n, before + u - n};
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return {-1, 0, 0, before};
+}
+#endif
+
+#endif

@@ -1,10 +1,11 @@
 """8-bit floating point on device tensors: E4M3 matrices with a scale per 128 x
 128 block (the reference's FP8 weights, src/lib/tlm_quant.c:761-776), the
-activation quantiser, their product, and a routed MoE block for a few tokens
-(tlm_hip_fp8_*).
+activation quantiser (alone, or behind a residual's addition and its RMS norm), their
+product, and a routed MoE block for a few tokens (tlm_hip_fp8_*).
 
     Wp = fp8.pack(W, scale)                  # once: W [rows, n] float8_e4m3fn, scale [rows/128, n/128]
     codes, s = fp8.quantize(x)               # x [T, n] float32, float16 or bfloat16
+    codes, s = fp8.add_rmsnorm(h, x, w)      # h += x, then the codes of rmsnorm(h) w
     Y = fp8.matmul(Wp, rows, n, codes, s)    # [T, rows]
 
 Device memory is torch tensors on the current HIP device; work goes on torch's
@@ -26,6 +27,7 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _U8, _I32, _F32 = torch.uint8, torch.int32, torch.float32
 _pack, _quantize, _matmul, _moe = (lib.tlm_hip_fp8_pack, lib.tlm_hip_fp8_quantize, lib.tlm_hip_fp8_matmul,
                                    lib.tlm_hip_fp8_moe)
+_add_rmsnorm = lib.tlm_hip_fp8_add_rmsnorm
 _packed_bytes = lib.tlm_hip_fp8_packed_bytes
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
@@ -116,6 +118,53 @@ def quantize(x, codes=None, scale=None):
     elif _out(scale, (T, nb), torch.float32, x, "scale").get_device() != dev:
         _here(x, scale)
     rc = _quantize(dt, x.data_ptr(), x.stride(0), n, T, codes.data_ptr(), scale.data_ptr(), _raw_stream(dev))
+    if rc:
+        check(rc)
+    return codes, scale
+
+
+def add_rmsnorm(h, x, weight, eps=1e-6, out=None, codes=None, scale=None):
+    """s = h + x (x None: h), rounded to h's dtype and stored in `out` (without it in h itself, the residual updated
+    in place); returns the codes and scales of rmsnorm(s) weight as quantize() gives them.  h and x [T, n],
+    float32, float16 or bfloat16 each by itself, rows of any stride; weight float32 [n].  `out` is h or overlaps
+    neither."""
+    hdt = _TYPES.get(h.dtype)
+    if hdt is None or not _rows_ok(h):
+        raise ValueError("h must be float32, float16 or bfloat16 [T, n] with contiguous rows")
+    T, n = h.shape
+    if n == 0:
+        raise ValueError("h must have at least one value a row")
+    dev, px, xdt, xstride = h.get_device(), None, 0, 0
+    here = dev >= 0 and dev == weight.get_device() == _current_device()
+    if x is not None:
+        xdt = _TYPES.get(x.dtype)
+        if xdt is None or x.shape != h.shape or not _rows_ok(x):
+            raise ValueError(f"x must be float32, float16 or bfloat16 [{T}, {n}] with contiguous rows")
+        px, xstride, here = x.data_ptr(), max(x.stride(0), n), here and x.get_device() == dev
+    if weight.shape != (n,) or weight.dtype is not _F32 or not weight.is_contiguous():
+        raise ValueError(f"weight must be contiguous float32 [{n}]")
+    stride, ostride = max(h.stride(0), n), 0
+    if out is None:
+        po, ostride = (None if x is None else h.data_ptr()), stride
+    else:
+        if out.shape != h.shape or out.dtype is not h.dtype or not _rows_ok(out):
+            raise ValueError(f"out must be {h.dtype} [{T}, {n}] with contiguous rows")
+        po, ostride, here = out.data_ptr(), max(out.stride(0), n), here and out.get_device() == dev
+        if po == h.data_ptr() and ostride != stride and T > 1:
+            raise ValueError("out must be h itself or not overlap it")
+    nb = -(-n // BLOCK)
+    if codes is None:
+        codes = torch.empty(T, nb * BLOCK, dtype=E4M3, device=h.device)
+    else:
+        here = _out(codes, (T, nb * BLOCK), E4M3, h, "codes").get_device() == dev and here
+    if scale is None:
+        scale = torch.empty(T, nb, dtype=_F32, device=h.device)
+    else:
+        here = _out(scale, (T, nb), _F32, h, "scale").get_device() == dev and here
+    if not here:
+        _here(*(t for t in (h, x, weight, out, codes, scale) if t is not None))
+    rc = _add_rmsnorm(hdt, h.data_ptr(), stride, xdt, px, xstride, weight.data_ptr(), eps, n, T, po, ostride,
+                      codes.data_ptr(), scale.data_ptr(), _raw_stream(dev))
     if rc:
         check(rc)
     return codes, scale
