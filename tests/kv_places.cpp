@@ -70,23 +70,28 @@ int main() {
                 CHECK(kv_append_items(a, a + len) + kv_append_items(b, b + 15 - len % 16) <= most);
             }
 
-    /* decode: the runs cover a sequence, and W items are enough */
-    for (int64_t B = 1; B < 6; B++)
-        for (int64_t W = 2 * B; W < 20; W += 3)
-            for (int trial = 0; trial < 200; trial++) {
-                std::vector<int64_t> len(B);
-                int64_t total = 0, items = 0;
-                for (auto &l : len) total += l = (trial * 7919 + (&l - len.data()) * 104729) % 5000 * (trial % 3 == 0 ? 1 : (&l - len.data()) == 0);
-                const int64_t run = kv_run(total, W, B, 128);
-                CHECK(run > 0 && run % 128 == 0);
-                for (auto l : len) {
-                    const int64_t n = kv_decode_items(l, run);
-                    CHECK(n >= 1 && n * run >= l && (n == 1 || (n - 1) * run < l));
-                    items += n;
-                }
-                CHECK(items <= W);
+    /* decode: the workers' shares cover the units in order, in parts that differ by one at most; a unit's worker is found,
+     * and no worker needs more than the two places it has */
+    CHECK(kv_units(0) == 1 && kv_units(1) == 1 && kv_units(128) == 1 && kv_units(129) == 2 && kv_units(1 << 30) == 1 << 23);
+    for (int W = 1; W < 40; W++)
+        for (int U = 1; U < 200; U++) {
+            const KvShares s = kv_shares(U, W);
+            CHECK(kv_share(s, 0) == 0 && kv_share(s, W) == U);
+            for (int w = 0; w < W; w++) {
+                const int n = kv_share(s, w + 1) - kv_share(s, w);
+                CHECK(n == U / W || n == U / W + 1);
+                for (int x = kv_share(s, w); x < kv_share(s, w + 1); x++) CHECK(kv_worker(s, x) == w);
             }
-    CHECK(kv_run((int64_t)1 << 50, 3, 1, 128) == (int64_t)1 << 49);
+            for (int step = 1; step < 30; step += 4) {       /* sequences of step units */
+                std::set<int> slots;
+                for (int a = 0; a < U; a += step) {
+                    const int b = a + step < U ? a + step : U, w0 = kv_worker(s, a), n = kv_worker(s, b - 1) - w0 + 1;
+                    for (int i = 0; i < n && n > 1; i++) CHECK(slots.insert(kv_slot(w0 + i, i == 0)).second);
+                }
+                CHECK(slots.empty() || (*slots.begin() >= 0 && *slots.rbegin() < 2 * W));
+            }
+        }
+    CHECK(kv_share(kv_shares((1 << 30) - 1, 512), 512) == (1 << 30) - 1 && kv_worker(kv_shares((1 << 30) - 1, 512), (1 << 30) - 2) == 511);
 
     /* prompt: as many tiles as the launch allows for */
     for (int a = 0; a < 60; a++)

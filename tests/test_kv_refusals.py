@@ -81,9 +81,9 @@ def test_refuses_more():
 
 
 def test_workspace():
-    """None up to 2048 positions of table; beyond, it must be there and aligned."""
+    """None up to 512 positions of table; beyond, it must be there and aligned."""
     c = C.byref(cache())
-    small, wide = batch(table_pages=128, table_stride=128), batch(table_pages=129, table_stride=129)
+    small, wide = batch(table_pages=32, table_stride=32), batch(table_pages=33, table_stride=33)
     ws = lib.tlm_hip_kv_decode_workspace_bytes
     assert ws(c, C.byref(small), 8) == 0
     assert ws(c, C.byref(wide), 8) > 0 and ws(c, C.byref(wide), 7) == 0

@@ -155,23 +155,25 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
 
 /* ---- decode --------------------------------------------------------------------
  * out = sum_j p_j v_j / sum_j p_j, p_j = 2^(scale log2(e) q . k_j - m), one pass over the cache with the running maximum m.
- * A group takes one run of a sequence's positions for one key head and up to 16 NC of its queries; its NW waves take tiles
+ * A group takes a part of a sequence's positions for one key head and up to 16 NC of its queries; its NW waves take tiles
  * of 32 positions in turn, straight from memory into the matrix cores' operands (no LDS on the way), the next tile's
  * loads in flight, and merge their sums through LDS at the end.  The bytes of the cache bound it.
  *
- * Runs: the lengths are the device's, so every group works the split out for itself: W items for B sequences, the run
- * length such that W suffices whatever the lengths are (kv_run); a long sequence among short ones is split as far as the
- * total asks.  Sequences of one run are written at once; the others' sums go to the workspace, item w's at w, and k_kv_join
- * adds a sequence's in order. */
+ * Shares: the lengths are the device's, so every group works its share out for itself.  All sequences' positions lie end
+ * to end in units of 128, and W workers a key head take equal parts of that line, across the sequences' ends: however
+ * uneven the lengths are, the groups that fill the chip once end together.  A sequence inside one share is written at
+ * once; the parts of the others go to the workspace, and k_kv_join adds a sequence's in order.  Where the tables are short
+ * (DECODE_WHOLE) each sequence is a group's and one launch does. */
 struct DecodeArgs {
     KvView c;
     const void *q, *k, *v;
     void *out;
-    float *part, *ml;        /* [W][heads][HD] sums, [W][heads][2] maximum and weight */
+    float *part, *ml;        /* [2 W][heads][HD] sums, [2 W][heads][2] maximum and weight */
     int64_t qstride;
     float scale2;            /* scale log2(e) */
     int G, W, out_dt;
-    int64_t run;             /* > 0: no split, every sequence is one run */
+    int whole;               /* 1: worker b has sequence b */
+    int hb;                  /* heads of a group of the join */
 };
 
 __device__ __forceinline__ void store_out(void *out, int dt, int64_t i, const float (&v)[4]) {
@@ -183,15 +185,15 @@ __device__ __forceinline__ void store_out(void *out, int dt, int64_t i, const fl
     else *(b4 *)((__bf16 *)out + i) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
 }
 
-/* the run length of a batch (W > B), the same in every group */
-__device__ __forceinline__ int64_t decode_run(const KvView &c, int W) {
-    const int64_t cap = kv_cap(c);
-    double sum = 0.0;   /* exact: whole numbers below 2^53 */
-    for (int b = wave_lane(); b < c.B; b += 64) {
-        const int64_t len = kv_len(c, b);
-        sum += (double)(len < cap ? len : cap);
-    }
-    return kv_run((int64_t)wave_sum_f64(sum), W, c.B, 128);
+__device__ __forceinline__ int decode_len(const KvView &c, int b) {
+    const int64_t len = kv_len(c, b), cap = kv_cap(c);
+    return (int)(len < cap ? len : cap);
+}
+/* the batch's shares, the same in every group */
+__device__ __forceinline__ KvShares decode_shares(const KvView &c, int W) {
+    int sum = 0;
+    for (int b = wave_lane(); b < c.B; b += 64) sum += kv_units(decode_len(c, b));
+    return kv_shares(__builtin_amdgcn_readlane(kv_scan(sum), 63), W);
 }
 
 template <class T, int HD, int NC, int NW>
@@ -202,19 +204,27 @@ __global__ __launch_bounds__(NW * 64, HD *NC <= 128 ? 2 : 1) void k_kv_decode(De
     __shared__ float s_o[NW / 2][NC * 16 * LD], s_ml[NW / 2][NC * 16 * 2];
     const KvView &c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = kv_uniform(tid >> 6), col = lane & 15, g = lane >> 4;
-    const int64_t cap = kv_cap(c), run = a.run > 0 ? a.run : decode_run(c, a.W);
-    auto length = [&](int b) {
-        const int64_t len = kv_len(c, b);
-        return len < cap ? len : cap;
-    };
-    KvItem it;
-    if (a.run > 0) it = {(int)blockIdx.x, 0, 1, (int)blockIdx.x};
-    else it = kv_find(c.B, (int)blockIdx.x, [&](int b) { return (int)kv_decode_items(length(b), run); });
-    if (it.b < 0) return;
-    const int kvh = blockIdx.y, col0 = blockIdx.z * NC * 16, ncol = a.G - col0 < NC * 16 ? a.G - col0 : NC * 16;
-    const int32_t *table = c.tables + it.b * c.table_stride;
-    const int len = (int)length(it.b);
-    const int begin = (int)(it.i * run), stop = len - begin < run ? len : (int)(begin + run);
+    const int worker = blockIdx.x, kvh = blockIdx.y;
+    const int col0 = blockIdx.z * NC * 16, ncol = a.G - col0 < NC * 16 ? a.G - col0 : NC * 16;
+    int b, first, left;     /* the sequence, its first unit here, units of the share that are left */
+    if (a.whole) {
+        b = worker;
+        first = 0;
+        left = 1 << 30;
+    } else {
+        const KvShares sh = decode_shares(c, a.W);
+        const int at = kv_share(sh, worker);
+        left = kv_share(sh, worker + 1) - at;
+        if (left == 0) return;
+        const KvItem it = kv_find(c.B, at, [&](int i) { return kv_units(decode_len(c, i)); });
+        if (it.b < 0) return;
+        b = it.b;
+        first = it.i;
+    }
+    for (;;) {
+    const int32_t *table = c.tables + b * c.table_stride;
+    const int len = decode_len(c, b), units = kv_units(len), take = units - first < left ? units - first : left;
+    const int begin = first * KV_UNIT, stop = len - begin < take * KV_UNIT ? len : begin + take * KV_UNIT;
     const int tiles = (stop - begin + 31) / 32;     /* 0: an empty sequence */
 
     /* queries: column col, values 32 ks + 8 g .. + 7 */
@@ -226,7 +236,7 @@ __global__ __launch_bounds__(NW * 64, HD *NC <= 128 ? 2 : 1) void k_kv_decode(De
             const int h = n * 16 + col;
             u32x4 v = {0, 0, 0, 0};
             if (h < ncol)
-                v = kv_load8((const T *)a.q + it.b * a.qstride + (int64_t)(kvh * a.G + col0 + h) * HD + 32 * ks + 8 * g);
+                v = kv_load8((const T *)a.q + b * a.qstride + (int64_t)(kvh * a.G + col0 + h) * HD + 32 * ks + 8 * g);
             qf[n][ks] = kv_bits<x8>(v);
         }
 
@@ -378,79 +388,86 @@ __global__ __launch_bounds__(NW * 64, HD *NC <= 128 ? 2 : 1) void k_kv_decode(De
         }
         __syncthreads();
     }
-    if (wave > 0) return;
+    if (wave == 0) {
 #pragma unroll
-    for (int n = 0; n < NC; n++) {
-        const int h = n * 16 + col;
-        if (h >= ncol) continue;
-        const int64_t head = kvh * a.G + col0 + h, H = (int64_t)a.G * c.heads;
-        if (it.n == 1) {
-            const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];     /* no position at all: zeros */
+        for (int n = 0; n < NC; n++) {
+            const int h = n * 16 + col;
+            if (h >= ncol) continue;
+            const int64_t head = kvh * a.G + col0 + h, H = (int64_t)a.G * c.heads;
+            if (take == units) {
+                const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];     /* no position at all: zeros */
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                const float v[4] = {o[n][dt][0] * inv, o[n][dt][1] * inv, o[n][dt][2] * inv, o[n][dt][3] * inv};
-                store_out(a.out, a.out_dt, (it.b * H + head) * HD + 16 * dt + 4 * g, v);
-            }
-        } else {
-            const int64_t w = (int64_t)blockIdx.x * H + head;
+                for (int dt = 0; dt < DT; dt++) {
+                    const float v[4] = {o[n][dt][0] * inv, o[n][dt][1] * inv, o[n][dt][2] * inv, o[n][dt][3] * inv};
+                    store_out(a.out, a.out_dt, (b * H + head) * HD + 16 * dt + 4 * g, v);
+                }
+            } else {
+                const int64_t w = kv_slot(worker, first == 0) * H + head;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) *(f32x4 *)(a.part + w * HD + 16 * dt + 4 * g) = o[n][dt];
-            if (g == 0) {
-                a.ml[2 * w] = m[n];
-                a.ml[2 * w + 1] = l[n];
+                for (int dt = 0; dt < DT; dt++) *(f32x4 *)(a.part + w * HD + 16 * dt + 4 * g) = o[n][dt];
+                if (g == 0) {
+                    a.ml[2 * w] = m[n];
+                    a.ml[2 * w + 1] = l[n];
+                }
             }
         }
+    }
+    left -= take;
+    if (a.whole || left == 0) return;
+    if (++b >= c.B) return;
+    first = 0;
     }
 }
 
-/* The sums of a sequence of several runs, one group a sequence and head: four lanes' values a thread, the runs dealt to the
- * threads' rows, added through LDS in a fixed order. */
+/* The sums of the sequences that several workers share: a group per sequence and hb heads, HD / 4 threads a row, the
+ * workers' parts dealt to a head's rows, each with a maximum of its own, the rows added through LDS in a fixed order. */
 template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a) {
-    constexpr int L4 = HD / 4, R = 256 / L4;
-    __shared__ float s_o[R][HD], s_l[R], s_m[4];
+    constexpr int L4 = HD / 4, ROWS = 256 / L4;
+    __shared__ float s_o[ROWS][HD], s_ml[ROWS][2];
     const KvView &c = a.c;
-    const int64_t cap = kv_cap(c), run = decode_run(c, a.W);
-    const int b = blockIdx.x, head = blockIdx.y, H = a.G * c.heads, tid = threadIdx.x;
-    auto items = [&](int b) {
-        const int64_t len = kv_len(c, b);
-        return (int)kv_decode_items(len < cap ? len : cap, run);
-    };
-    const int n = items(b);
-    if (n == 1) return;
+    const int b = blockIdx.x, H = a.G * c.heads, tid = threadIdx.x;
+    const KvShares sh = decode_shares(c, a.W);
     int before = 0;
-    for (int i = wave_lane(); i < b; i += 64) before += items(i);
-    before = (int)wave_sum_f64((double)before);
-    const int64_t w0 = (int64_t)before * H + head;
-    float top = -INFINITY;
-    for (int i = tid; i < n; i += 256) top = fmaxf(top, a.ml[2 * (w0 + (int64_t)i * H)]);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    if ((tid & 63) == 0) s_m[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    const float base = top == -INFINITY ? 0.0f : top;
-    const int r = tid / L4, e = tid % L4 * 4;
-    if (r < R) {
-        f32x4 o = {0, 0, 0, 0};
-        float l = 0.0f;
+    for (int i = wave_lane(); i < b; i += 64) before += kv_units(decode_len(c, i));
+    before = __builtin_amdgcn_readlane(kv_scan(before), 63);
+    const int units = kv_units(decode_len(c, b));
+    const int w0 = kv_worker(sh, before), n = kv_worker(sh, before + units - 1) - w0 + 1;
+    if (n == 1) return;
+    const int R = ROWS / a.hb, row = tid / L4, e = tid % L4 * 4, hd = row / R, r = row % R;
+    const int head = blockIdx.y * a.hb + hd;
+    f32x4 o = {0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    if (hd < a.hb && head < H) {
 #pragma unroll 4
         for (int i = r; i < n; i += R) {
-            const int64_t w = w0 + (int64_t)i * H;
-            const float f = __builtin_amdgcn_exp2f(a.ml[2 * w] - base);
-            l += a.ml[2 * w + 1] * f;
-            o += *(const f32x4 *)(a.part + w * HD + e) * f;
+            const int64_t w = (int64_t)kv_slot(w0 + i, i == 0) * H + head;
+            const float mi = a.ml[2 * w], li = a.ml[2 * w + 1];
+            const f32x4 oi = *(const f32x4 *)(a.part + w * HD + e);
+            const float to = fmaxf(m, mi), base = to == -INFINITY ? 0.0f : to;
+            const float f = __builtin_amdgcn_exp2f(m - base), fi = __builtin_amdgcn_exp2f(mi - base);
+            o = o * f + oi * fi;
+            l = l * f + li * fi;
+            m = to;
         }
-        *(f32x4 *)&s_o[r][e] = o;
-        if (e == 0) s_l[r] = l;
+    }
+    if (row < ROWS) {
+        *(f32x4 *)&s_o[row][e] = o;
+        if (e == 0) {
+            s_ml[row][0] = m;
+            s_ml[row][1] = l;
+        }
     }
     __syncthreads();
-    if (tid >= L4) return;
-    f32x4 o = {0, 0, 0, 0};
-    float l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-        o += *(const f32x4 *)&s_o[i][e];
-        l += s_l[i];
+    if (r > 0 || hd >= a.hb || head >= H) return;
+    float top = m;
+    for (int i = 1; i < R; i++) top = fmaxf(top, s_ml[row + i][0]);
+    const float base = top == -INFINITY ? 0.0f : top, f = __builtin_amdgcn_exp2f(m - base);
+    o *= f;
+    l *= f;
+    for (int i = 1; i < R; i++) {
+        const float fi = __builtin_amdgcn_exp2f(s_ml[row + i][0] - base);
+        o += *(const f32x4 *)&s_o[row + i][e] * fi;
+        l += s_ml[row + i][1] * fi;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
@@ -474,35 +491,35 @@ template <class T> void append_x(int xdt, const AppendArgs &a, dim3 grid, hipStr
 }
 
 /* Up to this many positions a sequence, by its table, every sequence is one group of eight waves and one launch */
-constexpr int64_t DECODE_WHOLE = 2048;
-/* Items that fill the chip: four groups of four waves a compute unit */
-constexpr int64_t DECODE_GROUPS = 1024;
+constexpr int64_t DECODE_WHOLE = 512;
 
 struct DecodePlan {
-    int64_t run;
-    int W, nc, z;
+    int whole, W, nc, z, hb;
 };
 DecodePlan decode_plan(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads) {
     const int G = heads / c->kv_heads, nc = G <= 16 ? 1 : G <= 32 || c->head_dim > 128 ? 2 : 4, z = (G + nc * 16 - 1) / (nc * 16);
     const int64_t cap = (int64_t)b->table_pages * c->page;
-    if (cap <= DECODE_WHOLE) return {cap, (int)b->B, nc, z};
-    int64_t W = DECODE_GROUPS / ((int64_t)c->kv_heads * z);
-    W = W > 2 * b->B ? W : 2 * b->B;
-    return {0, (int)W, nc, z};
+    if (cap <= DECODE_WHOLE) return {1, (int)b->B, nc, z, 0};
+    /* as many groups as the chip holds at once */
+    const int slots = 256 * (c->head_dim * nc <= 64 ? 4 : c->head_dim * nc <= 128 ? 2 : 1), W = slots / (c->kv_heads * z);
+    /* the join: about 1024 groups, a head each if there are fewer */
+    const int64_t hb = b->B * heads / 1024;
+    const int rows = 256 / (c->head_dim / 4);
+    return {0, W < 1 ? 1 : W, nc, z, (int)(hb < 1 ? 1 : hb > rows ? rows : hb)};
 }
 size_t decode_bytes(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads) {
     const DecodePlan p = decode_plan(c, b, heads);
-    return p.run ? 0 : (size_t)p.W * heads * (c->head_dim + 4) * 4;
+    return p.whole ? 0 : (size_t)2 * p.W * heads * (c->head_dim + 4) * 4;
 }
 
 template <class T, int HD, int NC> void decode_nc(const DecodeArgs &a, const DecodePlan &p, hipStream_t s) {
     const dim3 grid((unsigned)p.W, (unsigned)a.c.heads, (unsigned)p.z);
-    if (p.run) {
+    if (p.whole) {
         constexpr int NW = NC == 1 && HD <= 128 ? 8 : 4;   /* eight waves leave a wave 256 registers */
         hipLaunchKernelGGL((k_kv_decode<T, HD, NC, NW>), grid, dim3(NW * 64), 0, s, a);
     } else {
         hipLaunchKernelGGL((k_kv_decode<T, HD, NC, 4>), grid, dim3(256), 0, s, a);
-        hipLaunchKernelGGL((k_kv_join<HD>), dim3((unsigned)a.c.B, (unsigned)(a.G * a.c.heads)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_kv_join<HD>), dim3((unsigned)a.c.B, (unsigned)((a.G * a.c.heads + p.hb - 1) / p.hb)), dim3(256), 0, s, a);
     }
 }
 template <class T, int HD> void decode_hd(const DecodeArgs &a, const DecodePlan &p, hipStream_t s) {
@@ -528,7 +545,7 @@ int kv_check(const char *who, const tlm_hip_kv_cache *c, const tlm_hip_kv_batch 
         return tlmh_seterr(TLM_HIP_EUNSUP, "%s: head_dim %d is not a multiple of 32 up to 256", who, c->head_dim);
     if (c->page < KV_BLOCK || c->page > 4096 || (c->page & (c->page - 1)))
         return tlmh_seterr(TLM_HIP_EINVAL, "%s: page of %d positions (a power of two from 16 to 4096)", who, c->page);
-    if (c->kv_heads < 1 || c->kv_heads > 4096 || heads < 1 || heads > 65536 || heads % c->kv_heads)
+    if (c->kv_heads < 1 || c->kv_heads > 4096 || heads < 1 || heads > 16384 || heads % c->kv_heads)
         return tlmh_seterr(TLM_HIP_EINVAL, "%s: %d heads on %d key heads", who, heads, c->kv_heads);
     if (c->n_pages < 1 || c->n_pages > 0x7FFFFFFF)
         return tlmh_seterr(TLM_HIP_EINVAL, "%s: %lld pages", who, (long long)c->n_pages);
@@ -572,7 +589,7 @@ int tlm_hip_kv_append(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int 
         return tlmh_seterr(TLM_HIP_EINVAL, "kv_append: qkv must have its type's alignment, q 16, the norms 4, inv_freq 8 "
                            "bytes");
     const int64_t items = kv_append_most(b->rows, b->B);
-    if (items > (1 << 23))
+    if (items * c->kv_heads > (1 << 23))
         return tlmh_seterr(TLM_HIP_ERANGE, "kv_append: %lld rows of %lld sequences are too many for one launch",
                            (long long)b->rows, (long long)b->B);
     a.x = qkv;
@@ -613,23 +630,26 @@ int tlm_hip_kv_decode(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, cons
     if (!aligned(q, 2) || !aligned(out, (size_t)type_bytes(out_dt)))
         return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: q and out must have their type's alignment");
     const DecodePlan p = decode_plan(c, b, heads);
-    if ((int64_t)p.W * c->kv_heads * p.z > (1 << 22))
+    /* the batch's units are counted in an int; groups of a launch */
+    if (b->B * (((int64_t)b->table_pages * c->page + KV_UNIT - 1) / KV_UNIT) >= (1 << 30) ||
+        (int64_t)p.W * c->kv_heads * p.z > (1 << 22) || b->B * heads > (1 << 23))
         return tlmh_seterr(TLM_HIP_ERANGE, "kv_decode: %lld sequences of %d heads are too many for one launch",
                            (long long)b->B, heads);
-    if (!p.run && (!workspace || !aligned(workspace, 256)))
+    if (!p.whole && (!workspace || !aligned(workspace, 256)))
         return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: needs a workspace of %zu bytes, 256-byte aligned", decode_bytes(c, b, heads));
     a.q = q;
     a.k = c->k;
     a.v = c->v;
     a.out = out;
     a.part = (float *)workspace;
-    a.ml = p.run ? nullptr : a.part + (size_t)p.W * heads * c->head_dim;
+    a.ml = p.whole ? nullptr : a.part + (size_t)2 * p.W * heads * c->head_dim;
     a.qstride = q_stride;
     a.scale2 = scale * 1.44269504088896341f;
     a.G = heads / c->kv_heads;
     a.W = p.W;
     a.out_dt = out_dt;
-    a.run = p.run;
+    a.whole = p.whole;
+    a.hb = p.hb;
     if (c->dt == DT_F16) decode<_Float16>(a, p, (hipStream_t)stream);
     else decode<__bf16>(a, p, (hipStream_t)stream);
     return tlmh_check(hipGetLastError(), "kv_decode launch");

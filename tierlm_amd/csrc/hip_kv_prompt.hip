@@ -46,8 +46,8 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(Prompt
     __shared__ int s_odd;                    /* first tile whose product left values out */
     const KvView &c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = kv_uniform(tid >> 6), col = lane & 31, h = lane >> 5;
-    const int kvh = blockIdx.x, G = a.G;
-    const KvItem it = kv_find(c.B, (int)blockIdx.y, [&](int b) {
+    const int kvh = (int)(blockIdx.x % (uint32_t)c.heads), G = a.G;
+    const KvItem it = kv_find(c.B, (int)(blockIdx.x / (uint32_t)c.heads), [&](int b) {
         return (int)kv_prompt_items(kv_rows(c, b).n, G, 32 * NW);
     });
     if (it.b < 0) return;
@@ -265,10 +265,11 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(Prompt
         }
 }
 
+constexpr int TILE = 128;    /* rows of a group */
+
 template <class T, int HD> void launch(const PromptArgs &a, int64_t B, hipStream_t s) {
-    constexpr int NW = 4;
-    const dim3 grid((unsigned)a.c.heads, (unsigned)kv_prompt_most(a.c.rows, B, a.G, 32 * NW));
-    hipLaunchKernelGGL((k_kv_prompt<T, HD, NW>), grid, dim3(NW * 64), 0, s, a);
+    const dim3 grid((unsigned)(kv_prompt_most(a.c.rows, B, a.G, TILE) * a.c.heads));
+    hipLaunchKernelGGL((k_kv_prompt<T, HD, TILE / 32>), grid, dim3(TILE * 2), 0, s, a);
 }
 template <class T> void prompt(const PromptArgs &a, int64_t B, hipStream_t s) {
     static void (*const by_width[8])(const PromptArgs &, int64_t, hipStream_t) = {
@@ -294,6 +295,9 @@ extern "C" int tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_bat
                            (long long)heads * c->head_dim);
     if (!aligned(q, 2) || !aligned(out, (size_t)type_bytes(out_dt)))
         return tlmh_seterr(TLM_HIP_EINVAL, "kv_prompt: q and out must have their type's alignment");
+    if (kv_prompt_most(b->rows, b->B, heads / c->kv_heads, TILE) * c->kv_heads > (1 << 23))
+        return tlmh_seterr(TLM_HIP_ERANGE, "kv_prompt: %lld rows of %lld sequences are too many for one launch",
+                           (long long)b->rows, (long long)b->B);
     a.q = q;
     a.k = c->k;
     a.v = c->v;

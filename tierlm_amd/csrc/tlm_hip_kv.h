@@ -73,14 +73,23 @@ TLM_HD int64_t kv_append_most(int64_t rows, int64_t B) {
     return (rows + 14 * used) / 16 + used;
 }
 
-/* ---- decode: an item is a run of a sequence's positions ------------------- */
-/* With W items for B sequences (W > B) and `total` positions: the run length that W items suffice for, a multiple of unit.
- * Sum of ceil(len / c) over the sequences (at least one each) <= total / c + B <= W. */
-TLM_HD int64_t kv_run(int64_t total, int64_t W, int64_t B, int64_t unit) {
-    const int64_t c = (total + (W - B) - 1) / (W - B);
-    return c < unit ? unit : (c + unit - 1) / unit * unit;
+/* ---- decode: the batch's positions end to end in units of 128, dealt to W workers in equal shares ------------ */
+constexpr int KV_UNIT = 128;
+/* units of a sequence (an empty one has one too: its zeros are written) */
+TLM_HD int kv_units(int64_t len) { return len <= KV_UNIT ? 1 : (int)((len + KV_UNIT - 1) / KV_UNIT); }
+/* U units: the first U mod W workers take U / W + 1 of them, the others U / W */
+struct KvShares {
+    int q, r;
+};
+TLM_HD KvShares kv_shares(int U, int W) { return {U / W, U % W}; }
+TLM_HD int kv_share(KvShares s, int w) { return w * s.q + (w < s.r ? w : s.r); }     /* worker w's first unit */
+TLM_HD int kv_worker(KvShares s, int x) {                                            /* unit x's worker */
+    const int big = s.r * (s.q + 1);
+    return x < big ? x / (s.q + 1) : s.r + (x - big) / s.q;
 }
-TLM_HD int64_t kv_decode_items(int64_t len, int64_t run) { return len <= run ? 1 : (len + run - 1) / run; }
+/* Where worker w leaves its sums of a sequence that it does not have to itself: one that began with an earlier worker, or
+ * one that begins here (a worker has at most one of each) */
+TLM_HD int kv_slot(int w, bool begins) { return 2 * w + (begins ? 1 : 0); }
 
 /* ---- prompt: an item is a tile of a sequence's (token, head) rows ---------- */
 TLM_HD int64_t kv_prompt_items(int64_t n, int64_t group, int64_t tile) { return (n * group + tile - 1) / tile; }
