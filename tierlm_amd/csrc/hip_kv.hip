@@ -11,7 +11,7 @@ int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16
 /* ---- append ------------------------------------------------------------------
  * A group per block of 16 positions and key head: its up to 16 new rows of that head's G queries, key and value.  16 lanes
  * hold a vector: lane s the pairs j = M s .. M s + M - 1 and their partners at hd / 2 + j (M = hd / 32), so the norm is one
- * 16-lane sum and the rotation stays in the lane, and a lane's angles serve every vector of its row.  Values are
+ * 16-lane sum and the rotation stays in the lane.  Values are
  * turned over in registers (8 rows of one value to 16 bytes): the cache's block is written as whole pieces.
  * Bound by memory; what a decode step's few rows take is the launch. */
 struct AppendArgs {
@@ -27,8 +27,34 @@ struct AppendArgs {
 
 template <class X> __device__ __forceinline__ float to_f32(X v) { return (float)v; }
 
+/* M consecutive elements at any alignment of the type */
+template <int M, class X> __device__ __forceinline__ void load_m(float *v, const X *p) {
+    if constexpr (M == 2 || M == 4 || M == 8) {
+        typedef X XM __attribute__((ext_vector_type(M), aligned(sizeof(X))));
+        const XM x = *(const XM *)p;
+#pragma unroll
+        for (int m = 0; m < M; m++) v[m] = to_f32((X)x[m]);
+    } else {
+#pragma unroll
+        for (int m = 0; m < M; m++) v[m] = to_f32(p[m]);
+    }
+}
+template <int M, class T> __device__ __forceinline__ void store_m(T *p, const float *v) {
+    if constexpr (M == 2 || M == 4 || M == 8) {
+        typedef T TM __attribute__((ext_vector_type(M), aligned(sizeof(T))));
+        TM x;
+#pragma unroll
+        for (int m = 0; m < M; m++) x[m] = (T)v[m];
+        *(TM *)p = x;
+    } else {
+#pragma unroll
+        for (int m = 0; m < M; m++) p[m] = (T)v[m];
+    }
+}
+
 template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     constexpr int HD = 32 * M;
+    __shared__ float s_cs[KV_BLOCK][HD / 2 + 4], s_sn[KV_BLOCK][HD / 2 + 4];
     const KvView &c = a.c;
     const int tid = threadIdx.x;
     const KvItem it = kv_find(c.B, (int)blockIdx.x, [&](int b) {
@@ -49,106 +75,140 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
     if (blk >= 0 && (blk >> c.sh) < c.table_pages)
         at = kv_block(c, c.tables[it.b * c.table_stride + (blk >> c.sh)], blk, kvh);
 
-    /* queries and key: 16 lane groups, gpt of them to a row */
+    /* sine and cosine of the block's rows, once.  The angle is a double, less whole turns (2 pi as a sum of two
+     * doubles): a far position's fraction of a turn keeps its bits, and the functions take a float in [-pi, pi]. */
+    if (a.freq) {
+        for (int i = tid; i < n * (HD / 2); i += 256) {
+            const int t = i / (HD / 2), j = i % (HD / 2);
+            const double ang = (double)(lo + t) * a.freq[j], turns = rint(ang * 0.15915494309189535);
+            const double rem = __builtin_fma(-turns, 2.4492935982947064e-16, __builtin_fma(-turns, 6.283185307179586, ang));
+            float s, co;
+            sincosf((float)rem, &s, &co);
+            s_cs[t][j] = co * a.rope_scale;
+            s_sn[t][j] = s * a.rope_scale;
+        }
+        __syncthreads();
+    }
+
+    /* norm and rotation of the pairs (u, w) of row t */
     const int sub = tid & 15, grp = tid >> 4;
-    const int gpt = n == 1 ? 16 : n == 2 ? 8 : n <= 4 ? 4 : n <= 8 ? 2 : 1;
-    const int t = grp / gpt;
-    if (t < n) {
-        float cs[M], sn[M];
+    auto turn = [&](float (&u)[M], float (&w)[M], const float (&nw)[2 * M], bool norm, int t) {
+        if (norm) {
+            float ss = 0.0f;
 #pragma unroll
-        for (int m = 0; m < M; m++) {
-            cs[m] = 1.0f;
-            sn[m] = 0.0f;
+            for (int m = 0; m < M; m++) ss = fmaf(u[m], u[m], fmaf(w[m], w[m], ss));
+            ss += dpp_f32<DPP_XOR1>(ss);
+            ss += dpp_f32<DPP_XOR2>(ss);
+            ss += dpp_f32<DPP_HALF_MIRROR>(ss);
+            ss += dpp_f32<DPP_MIRROR>(ss);
+            const float f = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));
+#pragma unroll
+            for (int m = 0; m < M; m++) {
+                u[m] = u[m] * f * nw[m];
+                w[m] = w[m] * f * nw[M + m];
+            }
         }
         if (a.freq) {
-            /* the angle in double, less whole turns (2 pi as a sum of two doubles): a far position's fraction of a turn
-             * keeps its bits, and sine and cosine are of a float in [-pi, pi] */
-            const double pos = (double)(lo + t);
 #pragma unroll
             for (int m = 0; m < M; m++) {
-                const double ang = pos * a.freq[M * sub + m];
-                const double turns = rint(ang * 0.15915494309189535);
-                const double rem = __builtin_fma(-turns, 2.4492935982947064e-16, __builtin_fma(-turns, 6.283185307179586, ang));
-                float s, co;
-                sincosf((float)rem, &s, &co);
-                cs[m] = co * a.rope_scale;
-                sn[m] = s * a.rope_scale;
+                const float c = s_cs[t][M * sub + m], s = s_sn[t][M * sub + m], y = u[m];
+                u[m] = fmaf(y, c, -(w[m] * s));
+                w[m] = fmaf(w[m], c, y * s);
             }
         }
-        const X *row = x + t * a.xstride;
-        const bool written = lo + t >= 0;
-        for (int j = grp % gpt; j <= G; j += gpt) {             /* queries of the head's group, then its key */
-            const X *src = row + (int64_t)(j < G ? kvh * G + j : H + kvh) * HD + M * sub;
-            float u[M], w[M];
+        if (lo + t < 0) {
+#pragma unroll
+            for (int m = 0; m < M; m++) u[m] = w[m] = 0.0f;
+        }
+    };
+    auto weights = [&](float (&nw)[2 * M], const float *p) {
+        if (!p) return;
+        load_m<M>(nw, p + M * sub);
+        load_m<M>(nw + M, p + HD / 2 + M * sub);
+    };
+    /* queries row by row as they lie in memory: 16 lane groups, two vectors of each in flight */
+    {
+        float nw[2 * M], u0[M], w0[M], u1[M], w1[M];
+        weights(nw, a.qw);
+        struct At {
+            int t, j;
+        };
+        const int dt = 16 / G, dj = 16 % G;
+        auto next = [&](At p) {
+            p.t += dt;
+            p.j += dj;
+            if (p.j >= G) {
+                p.j -= G;
+                p.t++;
+            }
+            return p;
+        };
+        const X *src = x + (int64_t)kvh * G * HD + M * sub;
+        T *dst = q + (int64_t)kvh * G * HD + M * sub;
+        auto load = [&](float (&u)[M], float (&w)[M], At p) {
+            if (p.t >= n) return;
+            const X *v = src + p.t * a.xstride + p.j * HD;
+            load_m<M>(u, v);
+            load_m<M>(w, v + HD / 2);
+        };
+        auto finish = [&](float (&u)[M], float (&w)[M], At p) {
+            if (p.t >= n) return;
+            turn(u, w, nw, a.qw != nullptr, p.t);
+            T *o = dst + (int64_t)p.t * H * HD + p.j * HD;
+            store_m<M>(o, u);
+            store_m<M>(o + HD / 2, w);
+        };
+        At p = {grp / G, grp % G}, p1 = next(p);
+        load(u0, w0, p);
+        while (p.t < n) {
+            load(u1, w1, p1);
+            finish(u0, w0, p);
+            p = next(p1);
+            load(u0, w0, p);
+            finish(u1, w1, p1);
+            p1 = next(p);
+        }
+    }
+    /* keys, a lane group a row */
+    if (at >= 0 && grp < n) {
+        float nw[2 * M], u[M], w[M];
+        weights(nw, a.kw);
+        const X *src = x + grp * a.xstride + (int64_t)(H + kvh) * HD + M * sub;
+        load_m<M>(u, src);
+        load_m<M>(w, src + HD / 2);
+        turn(u, w, nw, a.kw != nullptr, grp);
+        T *o = (T *)a.k + at;
+        const int pos = (int)(lo + grp - blk * KV_BLOCK);
+        if constexpr (16 % M == 0) {    /* M values of one piece */
+            store_m<M>(o + kv_key_at(pos, M * sub), u);
+            store_m<M>(o + kv_key_at(pos, HD / 2 + M * sub), w);
+        } else {
 #pragma unroll
             for (int m = 0; m < M; m++) {
-                u[m] = to_f32(src[m]);
-                w[m] = to_f32(src[HD / 2 + m]);
-            }
-            const float *nw = j < G ? a.qw : a.kw;
-            if (nw) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int m = 0; m < M; m++) ss = fmaf(u[m], u[m], fmaf(w[m], w[m], ss));
-                ss += dpp_f32<DPP_XOR1>(ss);
-                ss += dpp_f32<DPP_XOR2>(ss);
-                ss += dpp_f32<DPP_HALF_MIRROR>(ss);
-                ss += dpp_f32<DPP_MIRROR>(ss);
-                const float f = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
-#pragma unroll
-                for (int m = 0; m < M; m++) {
-                    u[m] = u[m] * f * nw[M * sub + m];
-                    w[m] = w[m] * f * nw[HD / 2 + M * sub + m];
-                }
-            }
-            T lo_[M], hi_[M];
-#pragma unroll
-            for (int m = 0; m < M; m++) {
-                lo_[m] = (T)fmaf(u[m], cs[m], -(w[m] * sn[m]));
-                hi_[m] = (T)fmaf(w[m], cs[m], u[m] * sn[m]);
-                if (!written) lo_[m] = hi_[m] = (T)0.0f;
-            }
-            if (j < G) {
-                T *o = q + (int64_t)t * H * HD + (int64_t)(kvh * G + j) * HD + M * sub;
-#pragma unroll
-                for (int m = 0; m < M; m++) {
-                    o[m] = lo_[m];
-                    o[HD / 2 + m] = hi_[m];
-                }
-            } else if (at >= 0) {
-                T *o = (T *)a.k + at;
-                const int p = (int)(lo + t - blk * KV_BLOCK);
-#pragma unroll
-                for (int m = 0; m < M; m++) {
-                    o[kv_key_at(p, M * sub + m)] = lo_[m];
-                    o[kv_key_at(p, HD / 2 + M * sub + m)] = hi_[m];
-                }
+                o[kv_key_at(pos, M * sub + m)] = (T)u[m];
+                o[kv_key_at(pos, HD / 2 + M * sub + m)] = (T)w[m];
             }
         }
     }
     if (at < 0) return;
-    /* values: a thread per value and half block */
+    /* values: a thread per value and half block.  (Read ahead of the angles they take the registers of a wave a SIMD and
+     * the queries' loads wait behind them: 8192 rows 75 -> 82 us.) */
     const X *src = x + (int64_t)(H + c.heads + kvh) * HD;
     const int first = (int)(lo - blk * KV_BLOCK), last = first + n;
     T *o = (T *)a.v + at;
     for (int i = tid; i < 2 * HD; i += 256) {
-        const int d = i >> 1, p0h = (i & 1) * 8;
-        if (p0h >= last || p0h + 8 <= first) continue;
-        T e[8];
+        const int d = i % HD, half = i / HD * 8;
+        if (half >= last || half + 8 <= first) continue;
+        float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int p = p0h + j;
-            e[j] = p >= first && p < last ? (T)to_f32(src[(p - first) * a.xstride + d]) : (T)0.0f;
-        }
-        if (p0h >= first && p0h + 8 <= last) {
-            typename KvType<T>::x8 w;
-#pragma unroll
-            for (int j = 0; j < 8; j++) w[j] = e[j];
-            *(typename KvType<T>::x8 *)(o + kv_value_at(p0h, d)) = w;
+        for (int j = 0; j < 8; j++)
+            v[j] = half + j >= first && half + j < last ? to_f32(src[(half + j - first) * a.xstride + d]) : 0.0f;
+        if (half >= first && half + 8 <= last) {
+            store_m<8>(o + kv_value_at(half, d), v);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (p0h + j >= first && p0h + j < last) o[kv_value_at(p0h + j, d)] = e[j];
+                if (half + j >= first && half + j < last) o[kv_value_at(half + j, d)] = (T)v[j];
         }
     }
 }
@@ -172,7 +232,6 @@ struct DecodeArgs {
     int64_t qstride;
     float scale2;            /* scale log2(e) */
     int G, W, out_dt;
-    int whole;               /* 1: worker b has sequence b */
     int hb;                  /* heads of a group of the join */
 };
 
@@ -189,14 +248,48 @@ __device__ __forceinline__ int decode_len(const KvView &c, int b) {
     const int64_t len = kv_len(c, b), cap = kv_cap(c);
     return (int)(len < cap ? len : cap);
 }
-/* the batch's shares, the same in every group */
-__device__ __forceinline__ KvShares decode_shares(const KvView &c, int W) {
-    int sum = 0;
-    for (int b = wave_lane(); b < c.B; b += 64) sum += kv_units(decode_len(c, b));
-    return kv_shares(__builtin_amdgcn_readlane(kv_scan(sum), 63), W);
-}
+/* The batch's lengths and shares, the same in every group.  Up to 64 sequences are read once, a lane each: what follows
+ * waits for one read of memory. */
+struct DecodeBatch {
+    const KvView &c;
+    int mine, upto;       /* B <= 64: lane b's length, and the units up to its sequence's end */
+    KvShares sh;
+    __device__ __forceinline__ DecodeBatch(const KvView &c_, int W) : c(c_), mine(0), upto(0) {
+        const int lane = wave_lane();
+        int sum = 0;
+        if (few()) {
+            if (lane < c.B) {
+                mine = decode_len(c, lane);
+                sum = kv_units(mine);
+            }
+        } else {
+            for (int b = lane; b < c.B; b += 64) sum += kv_units(decode_len(c, b));
+        }
+        upto = kv_scan(sum);
+        sh = kv_shares(__builtin_amdgcn_readlane(upto, 63), W);
+    }
+    __device__ __forceinline__ bool few() const { return c.B <= 64; }
+    __device__ __forceinline__ int len(int b) const {
+        return few() ? __builtin_amdgcn_readlane(mine, b) : kv_uniform(decode_len(c, b));
+    }
+    /* the sequence of unit x, and x's number in it; b < 0: there is none */
+    __device__ __forceinline__ KvItem find(int x) const {
+        if (!few()) return kv_find(c.B, x, [&](int b) { return kv_units(decode_len(c, b)); });
+        const uint64_t in = __ballot(wave_lane() < c.B && upto > x);
+        if (!in) return {-1, 0, 0, 0};
+        const int b = __builtin_ctzll(in), n = kv_units(len(b)), u = __builtin_amdgcn_readlane(upto, b);
+        return {b, x - (u - n), n, u - n};
+    }
+    /* units of the sequences before b */
+    __device__ __forceinline__ int before(int b) const {
+        if (few()) return __builtin_amdgcn_readlane(upto, b) - kv_units(len(b));
+        int sum = 0;
+        for (int i = wave_lane(); i < b; i += 64) sum += kv_units(decode_len(c, i));
+        return __builtin_amdgcn_readlane(kv_scan(sum), 63);
+    }
+};
 
-template <class T, int HD, int NC, int NW>
+template <class T, int HD, int NC, int NW, bool WHOLE>
 __global__ __launch_bounds__(NW * 64, HD *NC <= 128 ? 2 : 1) void k_kv_decode(DecodeArgs a) {
     typedef typename KvType<T>::x8 x8;
     constexpr int KS = HD / 32, DT = HD / 16;    /* steps of the first product, result tiles of the second */
@@ -206,24 +299,9 @@ __global__ __launch_bounds__(NW * 64, HD *NC <= 128 ? 2 : 1) void k_kv_decode(De
     const int tid = threadIdx.x, lane = tid & 63, wave = kv_uniform(tid >> 6), col = lane & 15, g = lane >> 4;
     const int worker = blockIdx.x, kvh = blockIdx.y;
     const int col0 = blockIdx.z * NC * 16, ncol = a.G - col0 < NC * 16 ? a.G - col0 : NC * 16;
-    int b, first, left;     /* the sequence, its first unit here, units of the share that are left */
-    if (a.whole) {
-        b = worker;
-        first = 0;
-        left = 1 << 30;
-    } else {
-        const KvShares sh = decode_shares(c, a.W);
-        const int at = kv_share(sh, worker);
-        left = kv_share(sh, worker + 1) - at;
-        if (left == 0) return;
-        const KvItem it = kv_find(c.B, at, [&](int i) { return kv_units(decode_len(c, i)); });
-        if (it.b < 0) return;
-        b = it.b;
-        first = it.i;
-    }
-    for (;;) {
+    auto part = [&](int b, int len, int first, int left) {
     const int32_t *table = c.tables + b * c.table_stride;
-    const int len = decode_len(c, b), units = kv_units(len), take = units - first < left ? units - first : left;
+    const int units = kv_units(len), take = units - first < left ? units - first : left;
     const int begin = first * KV_UNIT, stop = len - begin < take * KV_UNIT ? len : begin + take * KV_UNIT;
     const int tiles = (stop - begin + 31) / 32;     /* 0: an empty sequence */
 
@@ -412,10 +490,18 @@ __global__ __launch_bounds__(NW * 64, HD *NC <= 128 ? 2 : 1) void k_kv_decode(De
             }
         }
     }
-    left -= take;
-    if (a.whole || left == 0) return;
-    if (++b >= c.B) return;
-    first = 0;
+    return take;
+    };
+    if (WHOLE) {
+        part(worker, kv_uniform(decode_len(c, worker)), 0, 1 << 30);
+    } else {
+        const DecodeBatch batch(c, a.W);
+        const int at = kv_share(batch.sh, worker);
+        int left = kv_share(batch.sh, worker + 1) - at;
+        if (left == 0) return;
+        const KvItem it = batch.find(at);
+        if (it.b < 0) return;
+        for (int b = it.b, first = it.i; left > 0 && b < c.B; b++, first = 0) left -= part(b, batch.len(b), first, left);
     }
 }
 
@@ -426,12 +512,9 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a)
     __shared__ float s_o[ROWS][HD], s_ml[ROWS][2];
     const KvView &c = a.c;
     const int b = blockIdx.x, H = a.G * c.heads, tid = threadIdx.x;
-    const KvShares sh = decode_shares(c, a.W);
-    int before = 0;
-    for (int i = wave_lane(); i < b; i += 64) before += kv_units(decode_len(c, i));
-    before = __builtin_amdgcn_readlane(kv_scan(before), 63);
-    const int units = kv_units(decode_len(c, b));
-    const int w0 = kv_worker(sh, before), n = kv_worker(sh, before + units - 1) - w0 + 1;
+    const DecodeBatch batch(c, a.W);
+    const int before = batch.before(b), w0 = kv_worker(batch.sh, before);
+    const int n = kv_worker(batch.sh, before + kv_units(batch.len(b)) - 1) - w0 + 1;
     if (n == 1) return;
     const int R = ROWS / a.hb, row = tid / L4, e = tid % L4 * 4, hd = row / R, r = row % R;
     const int head = blockIdx.y * a.hb + hd;
@@ -516,10 +599,11 @@ template <class T, int HD, int NC> void decode_nc(const DecodeArgs &a, const Dec
     const dim3 grid((unsigned)p.W, (unsigned)a.c.heads, (unsigned)p.z);
     if (p.whole) {
         constexpr int NW = NC == 1 && HD <= 128 ? 8 : 4;   /* eight waves leave a wave 256 registers */
-        hipLaunchKernelGGL((k_kv_decode<T, HD, NC, NW>), grid, dim3(NW * 64), 0, s, a);
+        hipLaunchKernelGGL((k_kv_decode<T, HD, NC, NW, true>), grid, dim3(NW * 64), 0, s, a);
     } else {
-        hipLaunchKernelGGL((k_kv_decode<T, HD, NC, 4>), grid, dim3(256), 0, s, a);
-        hipLaunchKernelGGL((k_kv_join<HD>), dim3((unsigned)a.c.B, (unsigned)((a.G * a.c.heads + p.hb - 1) / p.hb)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_kv_decode<T, HD, NC, 4, false>), grid, dim3(256), 0, s, a);
+        const dim3 join((unsigned)a.c.B, (unsigned)((a.G * a.c.heads + p.hb - 1) / p.hb));
+        hipLaunchKernelGGL((k_kv_join<HD>), join, dim3(256), 0, s, a);
     }
 }
 template <class T, int HD> void decode_hd(const DecodeArgs &a, const DecodePlan &p, hipStream_t s) {
@@ -648,7 +732,6 @@ int tlm_hip_kv_decode(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, cons
     a.G = heads / c->kv_heads;
     a.W = p.W;
     a.out_dt = out_dt;
-    a.whole = p.whole;
     a.hb = p.hb;
     if (c->dt == DT_F16) decode<_Float16>(a, p, (hipStream_t)stream);
     else decode<__bf16>(a, p, (hipStream_t)stream);
