@@ -84,6 +84,20 @@ def test_prompt_heads(hip, hd, heads, kv_heads):
     check_prompt(Batch(F16 if hd % 64 else BF16, heads, kv_heads, hd, 32, [90, 7], [150, 7], seed=hd + heads))
 
 
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_prompt_many_groups(hip, hd, dtype):
+    """Enough rows to fill the chip: 128 of them a group, their positions in one piece."""
+    check_prompt(Batch(dtype, 208, 16, hd, 64, [200, 0, 151, 1], [200, 3, 300, 70], seed=hd))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompt_few_groups(hip, hd):
+    """As many groups as take 64 rows, and as few as take 32."""
+    for heads, kv_heads, n in ((64, 4, 200), (16, 2, 40)):
+        check_prompt(Batch(BF16, heads, kv_heads, hd, 16, [n], [n + 333], seed=hd))
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256, 1024])
 def test_prompt_pages(hip, page):
     check_prompt(Batch(BF16, 8, 2, 128, page, [300, 77], [1300, 77], seed=page))
@@ -132,12 +146,12 @@ def test_decode_and_prompt_agree(hip):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_masked_places_may_hold_anything(hip, dtype):
     """Infinities and NaN behind a row's position leave its bits alone; rows that see them get them."""
-    for first, n in ((0, 150), (70, 40)):
-        b = Batch(dtype, 8, 2, 64, 16, [n], [first + n], seed=9)
+    for first, n, H, KV in ((0, 150, 8, 2), (70, 40, 8, 2), (0, 300, 64, 2), (90, 200, 416, 16)):   # 32, 64, 128 rows a group
+        b = Batch(dtype, H, KV, 64, 16, [n], [first + n], seed=9)
         want = kv.prompt(b.q, b.cache, b.tables, b.lens, b.cu, dtype=F32)
         for where, value in ((first + 20, math.inf), (first + n - 1, math.nan), (first + n // 2, -math.inf)):
             for which in "kv":
-                c = Batch(dtype, 8, 2, 64, 16, [n], [first + n], seed=9)
+                c = Batch(dtype, H, KV, 64, 16, [n], [first + n], seed=9)
                 k, v = c.k[0].clone(), c.v[0].clone()
                 (k if which == "k" else v)[where, :, 5] = value
                 c.put(0, k, v)

@@ -24,42 +24,50 @@ __device__ __forceinline__ void store_out(void *out, int dt, int64_t i, const fl
     else *(b4 *)((__bf16 *)out + i) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
 }
 
-/* A group takes 32 NW rows of one sequence and key head, a row being a (token, query head of the group) pair: the heads
- * that share keys lie side by side, so a tile of few tokens wastes little of the causal border.  A wave holds 32 rows as the
- * columns of S^T = K Q^T and of O^T = V^T P^T (32 x 32 x 16 products).  Keys and values come 64 positions at a time by direct
- * loads into LDS, in units of a kilobyte that are one operand each, two stages: the next 64 are under way while these are
- * used.
+/* What a page number outside the cache stands for: its positions are masked, and a finite value times weight 0 is 0 */
+__device__ const u32x4 kv_nothing[KV_BLOCK * 256 * 2 / 16] = {};
+
+/* A group of four waves takes 32 RG rows of one sequence and key head (RG = 4 / SG), a row being a (token, query head of
+ * the group) pair: the heads that share keys lie side by side, so a tile of few tokens wastes little of the causal border.
+ * A wave holds 32 rows as the columns of S^T = K Q^T and of O^T = V^T P^T (32 x 32 x 16 products), and takes every SG-th
+ * stage of 32 TP positions; the SG waves of the same rows add their sums through LDS at the end.  RG waves share a stage: keys
+ * and values come by direct loads into LDS, in units of a kilobyte that are one operand each; the next stage is under way
+ * while this one is used.
  *
  * Row i of a key operand is position 8 h + 4 u + e of its block for i = 8 u + 4 h + e: a lane's scores are then 8
  * consecutive positions a block, its operand of the second product.
  *
- * A masked place's value may be infinite or NaN, and its weight 0 does not silence it: in tiles with a border the values that
- * are not finite leave LDS, and rows that see them get them at the end, value by value (rare).
- */
-template <class T, int HD, int NW>
-__global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(PromptArgs a) {
+ * A masked place's value may be infinite or NaN, and its weight 0 does not silence it: in stages with a border the values
+ * that are not finite leave LDS, and rows that see them get them at the end, value by value (rare). */
+template <class T, int HD, int SG, int TP>
+__global__ __launch_bounds__(256, HD > 128 || (SG == 4 && HD > 64) ? 1 : 2) void k_kv_prompt(PromptArgs a) {
     typedef typename KvType<T>::x8 x8;
+    constexpr int RG = 4 / SG, ROWS = 32 * RG;
     constexpr int KS = HD / 16, DT = HD / 32;
-    constexpr int UNITS = 4 * KS;            /* of a stage: 2 KS of keys, 4 DT of values */
-    static_assert(NW == 4, "how a stage is dealt");
-    __shared__ __attribute__((aligned(1024))) uint8_t s_buf[2][UNITS * 1024];
-    __shared__ int s_odd;                    /* first tile whose product left values out */
+    constexpr int POS = 32 * TP, BLOCKS = 2 * TP;      /* positions of a stage */
+    constexpr int UNITS = 2 * TP * KS;                 /* of a stage: TP KS of keys, BLOCKS DT of values */
+    constexpr int ALL = (1 << BLOCKS) - 1;
+    /* two objects: reads of one stage do not wait for the loads into the other */
+    __shared__ __attribute__((aligned(1024))) uint8_t s_even[SG * UNITS * 1024], s_odds[SG * UNITS * 1024];
+    __shared__ int s_odd;                    /* first stage whose product left values out */
+    __shared__ float s_ml[2 * RG][2][32];    /* SG > 1 */
     const KvView &c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = kv_uniform(tid >> 6), col = lane & 31, h = lane >> 5;
+    const int rg = wave % RG, sg = wave / RG;
     const int kvh = (int)(blockIdx.x % (uint32_t)c.heads), G = a.G;
     const KvItem it = kv_find(c.B, (int)(blockIdx.x / (uint32_t)c.heads), [&](int b) {
-        return (int)kv_prompt_items(kv_rows(c, b).n, G, 32 * NW);
+        return (int)kv_prompt_items(kv_rows(c, b).n, G, ROWS);
     });
     if (it.b < 0) return;
     const KvRows rows = kv_rows(c, it.b);
     const int64_t len = kv_len(c, it.b), cap = kv_cap(c);
-    const int nrow = (int)(rows.n * G), row0 = (it.n - 1 - it.i) * 32 * NW;    /* the longest first */
+    const int nrow = (int)(rows.n * G), row0 = (it.n - 1 - it.i) * ROWS;    /* the longest first */
     const int64_t p0 = len - rows.n;
     const int present = (int)(len < cap ? len : cap);
     const int32_t *table = c.tables + it.b * c.table_stride;
 
     /* the lane's row, its last visible position (-1: none) */
-    const int row = row0 + 32 * wave + col, token = row / G;
+    const int row = row0 + 32 * rg + col, token = row / G;
     const bool real = row < nrow;
     auto limit = [&](int token) {
         const int64_t p = p0 + token;
@@ -67,62 +75,83 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(Prompt
     };
     const int lim = real ? limit(token) : -1;
     auto last_of = [&](int r) { return limit((r < nrow ? r : nrow - 1) / G); };
-    const int end = last_of(row0 + 32 * NW - 1) + 1;             /* positions that the group needs */
-    const int gfirst = limit(row0 / G), wfirst = limit((row0 + 32 * wave) / G), wend = row0 + 32 * wave < nrow ? last_of(row0 + 32 * wave + 31) + 1 : 0;
-    const int tiles = (end + 63) / 64;
+    const int end = last_of(row0 + ROWS - 1) + 1;             /* positions that the group needs */
+    const int gfirst = limit(row0 / G), wfirst = limit((row0 + 32 * rg) / G);
+    const int wend = row0 + 32 * rg < nrow ? last_of(row0 + 32 * rg + 31) + 1 : 0;
+    const int tiles = (end + POS - 1) / POS;
 
     const int64_t H = (int64_t)G * c.heads;
-    const int64_t mine = (rows.first + token) * 1;
     x8 qf[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) {
         u32x4 v = {0, 0, 0, 0};
-        if (real) v = kv_load8((const T *)a.q + mine * a.qstride + (int64_t)(kvh * G + row - token * G) * HD + 16 * ks + 8 * h);
+        if (real)
+            v = kv_load8((const T *)a.q + (rows.first + token) * a.qstride + (int64_t)(kvh * G + row - token * G) * HD +
+                         16 * ks + 8 * h);
         qf[ks] = kv_bits<x8>(v);
     }
 
-    /* A stage's units: wave 0 and 1 load the keys of 32 positions each (KS units of 16 values), wave 2 and 3 the values of
-     * two blocks each (DT units of 32 values).  Every wave looks its own two blocks' pages up, and whether all four are there. */
     const int i16 = col & 15, krow = 8 * ((i16 >> 2) & 1) + 4 * (i16 >> 3) + (i16 & 3);
-    const bool kwave = wave < 2;
-    const int off = kwave ? kv_key_at(krow, 0) + 8 * h : kv_value_at(0, col) + 8 * h, step = kwave ? 256 : 512;
-    const GAS T *const src = (const GAS T *)(kwave ? a.k : a.v) + off;
+    const int koff = kv_key_at(krow, 0) + 8 * h, voff = kv_value_at(0, col) + 8 * h;
     const int lastb = end > 0 ? (end - 1) / KV_BLOCK : 0;
     struct Pages {
-        int p0, p1, p2, p3;
+        int p[BLOCKS];
     };
     auto pages = [&](int tile) {
         const CAS int32_t *t = (const CAS int32_t *)table;
-        auto one = [&](int s) {
-            const int blk = 4 * tile + s;
-            return t[(blk < lastb ? blk : lastb) >> c.sh];
-        };
-        return Pages{one(0), one(1), one(2), one(3)};
-    };
-    struct Blocks {
-        int64_t b0, b1;   /* this wave's */
-        int ok;           /* bit s: block s is a page's */
-    };
-    auto blocks = [&](Pages p, int tile) {
-        auto at = [&](int page, int s) {
-            const int blk = 4 * tile + s;
-            const int64_t at = kv_block(c, page, blk < lastb ? blk : lastb, kvh);
-            return at >= 0 ? at : 0;      /* inside the cache; masked */
-        };
-        const uint32_t n = (uint32_t)c.n_pages;
-        const int ok = ((uint32_t)p.p0 < n ? 1 : 0) | ((uint32_t)p.p1 < n ? 2 : 0) | ((uint32_t)p.p2 < n ? 4 : 0) |
-                       ((uint32_t)p.p3 < n ? 8 : 0);
-        const int w = wave & 1;
-        return Blocks{at(w ? p.p2 : p.p0, 2 * w), at(w ? p.p3 : p.p1, 2 * w + 1), ok};
-    };
-    auto load = [&](Blocks n, uint8_t *to) {
-        const GAS T *p0 = src + (kwave && (col & 16) ? n.b1 : n.b0);
-        const GAS T *p1 = kwave ? p0 + 256 * DT : src + n.b1;
-        to += wave * KS * 1024;
+        Pages n;
 #pragma unroll
-        for (int j = 0; j < KS; j++)
-            __builtin_amdgcn_global_load_lds((const GAS void *)((j < DT ? p0 : p1) + step * (j < DT ? j : j - DT)),
-                                             (LAS void *)(to + j * 1024), 16, 0, 0);
+        for (int s = 0; s < BLOCKS; s++) {
+            const int blk = BLOCKS * tile + s;
+            n.p[s] = t[(blk < lastb ? blk : lastb) >> c.sh];
+        }
+        return n;
+    };
+    /* Puts a stage's loads under way; bit s of the result: block s is a page's.  RG waves share the units in order (keys: half t
+     * of the positions, 16 values ks; values: block s, 32 values dt): 4 take a quarter each, 2 the keys or the values. */
+    auto load = [&](const Pages &n, int tile, uint8_t *to) {
+        auto at = [&](const void *base, int s) {
+            const int blk = BLOCKS * tile + s;
+            const int64_t at = kv_block(c, n.p[s], blk < lastb ? blk : lastb, kvh);
+            return at >= 0 ? (const GAS T *)base + at : (const GAS T *)kv_nothing;
+        };
+        int here = 0;
+#pragma unroll
+        for (int s = 0; s < BLOCKS; s++) here |= (uint32_t)n.p[s] < (uint32_t)c.n_pages ? 1 << s : 0;
+        auto put = [&](const GAS T *src, int u) {
+            __builtin_amdgcn_global_load_lds((const GAS void *)src, (LAS void *)(to + u * 1024), 16, 0, 0);
+        };
+        auto keys = [&](int t, int ks0, int count) {
+            const GAS T *b0 = at(a.k, 2 * t), *b1 = at(a.k, 2 * t + 1), *src = (col & 16 ? b1 : b0) + koff;
+#pragma unroll
+            for (int j = 0; j < count; j++) put(src + 256 * (ks0 + j), t * KS + ks0 + j);
+        };
+        auto values = [&](int s) {
+            const GAS T *src = at(a.v, s) + voff;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) put(src + 512 * dt, TP * KS + s * DT + dt);
+        };
+        if (RG == 4 && TP == 2) {
+            if (rg == 0) keys(0, 0, KS);
+            else if (rg == 1) keys(1, 0, KS);
+            else if (rg == 2) values(0), values(1);
+            else values(2), values(3);
+        } else if (RG == 4) {
+            if (rg == 0) keys(0, 0, DT);
+            else if (rg == 1) keys(0, DT, DT);
+            else if (rg == 2) values(0);
+            else values(1);
+        } else {
+            if (RG == 1 || rg == 0) {
+                keys(0, 0, KS);
+                if (TP == 2) keys(1, 0, KS);
+            }
+            if (RG == 1 || rg == 1) {
+                values(0), values(1);
+                if (TP == 2) values(2), values(3);
+            }
+        }
+        return here;
     };
 
     f32x16 o[DT];
@@ -132,64 +161,64 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(Prompt
     if (tid == 0) s_odd = tiles;
 
     int ok = 0;
-    Pages next = {0, 0, 0, 0};
+    Pages next = {};
     if (tiles > 0) {
-        const Blocks n = blocks(pages(0), 0);
-        load(n, s_buf[0]);
-        ok = n.ok;
-        next = pages(1);
+        ok = load(pages(sg), sg, s_even + sg * UNITS * 1024);
+        next = pages(SG + sg);
     }
-    for (int tile = 0; tile < tiles; tile++) {
+    auto step = [&](int i, uint8_t *stage, uint8_t *other) {
         __builtin_amdgcn_s_waitcnt(0);      /* this stage's own loads; the barrier brings the other waves' */
         __syncthreads();
-        uint8_t *buf = s_buf[tile & 1];
-        const int here = ok;
-        if (tile + 1 < tiles) {
-            const Blocks n = blocks(next, tile + 1);
-            load(n, s_buf[(tile + 1) & 1]);
-            ok = n.ok;
-        }
-        if (tile * 64 + 63 > gfirst || here != 15) {
-            /* a border: no value that is masked for some row may disturb its product.  Wave w cleans block w. */
-            const int left = ((here >> wave) & 1) ? present - (tile * 64 + 16 * wave + 8 * h) : 0;
+        const int tile = SG * i + sg, base = tile * POS, here = ok;
+        uint8_t *buf = stage + sg * UNITS * 1024;
+        if (SG * (i + 1) < tiles) ok = load(next, tile + SG, other + sg * UNITS * 1024);
+        if ((SG * i + SG) * POS - 1 > gfirst) {
+            /* a border: no value that is masked for some row may disturb its product.  The waves of a stage share its blocks. */
+            constexpr int EACH = BLOCKS >= RG ? BLOCKS / RG : 1;
             bool odd = false;
+            if (rg * EACH < BLOCKS) {
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) {
-                u32x4 *at = (u32x4 *)(buf + (2 * KS + wave * DT + dt) * 1024 + lane * 16);
-                u32x4 v = *at;
+                for (int e = 0; e < EACH; e++) {
+                    const int s = rg * EACH + e, left = present - (base + 16 * s + 8 * h);
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    constexpr uint32_t E = KvType<T>::EXP;
-                    const uint32_t there = (2 * w < left ? 0xFFFFu : 0u) | (2 * w + 1 < left ? 0xFFFF0000u : 0u), x = v[w] & there;
-                    const uint32_t finite = ((x & E) == E ? 0u : 0xFFFFu) | ((x & (E << 16)) == E << 16 ? 0u : 0xFFFF0000u);
-                    odd |= finite != 0xFFFFFFFFu;
-                    v[w] = x & finite;
+                    for (int dt = 0; dt < DT; dt++) {
+                        u32x4 *at = (u32x4 *)(buf + (TP * KS + s * DT + dt) * 1024 + lane * 16);
+                        u32x4 v = *at;
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            constexpr uint32_t E = KvType<T>::EXP;
+                            const uint32_t there = (2 * w < left ? 0xFFFFu : 0u) | (2 * w + 1 < left ? 0xFFFF0000u : 0u);
+                            const uint32_t x = v[w] & there;
+                            const uint32_t finite =
+                                ((x & E) == E ? 0u : 0xFFFFu) | ((x & (E << 16)) == E << 16 ? 0u : 0xFFFF0000u);
+                            odd |= finite != 0xFFFFFFFFu;
+                            v[w] = x & finite;
+                        }
+                        *at = v;
+                    }
                 }
-                *at = v;
             }
             if (__any(odd) && lane == 0) atomicMin(&s_odd, tile);
             __syncthreads();
         }
-        const int base = tile * 64;
         if (base >= wend) {
-            next = pages(tile + 2);
-            continue;
+            next = pages(tile + 2 * SG);
+            return;
         }
-        const uint8_t *kb = buf + lane * 16, *vb = buf + 2 * KS * 1024 + lane * 16;
-        f32x16 s[2];
+        const uint8_t *kb = buf + lane * 16, *vb = buf + TP * KS * 1024 + lane * 16;
+        f32x16 s[TP];
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            s[t] = f32x16{0};
+        for (int t = 0; t < TP; t++) s[t] = f32x16{0};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-                s[t] = KvType<T>::mma(*(const x8 *)(kb + (t * KS + ks) * 1024), qf[ks], s[t]);
-        }
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int t = 0; t < TP; t++) s[t] = KvType<T>::mma(*(const x8 *)(kb + (t * KS + ks) * 1024), qf[ks], s[t]);
         __builtin_amdgcn_sched_barrier(0);
-        next = pages(tile + 2);    /* scalar loads: behind the reads of LDS, which one counter waits for too */
-        const bool whole = base + 63 <= wfirst && here == 15;
+        next = pages(tile + 2 * SG);    /* scalar loads: behind the reads of LDS, which one counter waits for too */
+        const bool whole = base + POS - 1 <= wfirst && here == ALL;
         if (!whole) {
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+            for (int t = 0; t < TP; t++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int p = base + 32 * t + 16 * (r >> 3) + 8 * h + (r & 7);
@@ -199,7 +228,7 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(Prompt
         }
         float top = s[0][0];
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < TP; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[t][r]);
         top *= a.scale2;
@@ -213,9 +242,9 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(Prompt
             for (int dt = 0; dt < DT; dt++) o[dt] *= f;
         }
         const float sub = (m == -INFINITY ? 0.0f : m) - KvType<T>::SHIFT;
-        x8 p[4];
+        x8 p[BLOCKS];
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < TP; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const float e = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale2, -sub));
@@ -223,18 +252,57 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(Prompt
                 p[2 * t + (r >> 3)][r & 7] = (T)e;    /* as many bits as the values it is multiplied with */
             }
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++)
+        for (int ks = 0; ks < BLOCKS; ks++)
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++)
+            for (int dt = 0; dt < DT; dt++)
                 o[dt] = KvType<T>::mma(*(const x8 *)(vb + (ks * DT + dt) * 1024), p[ks], o[dt]);
+    };
+    for (int i = 0; SG * i < tiles; i += 2) {
+        step(i, s_even, s_odds);
+        if (SG * (i + 1) < tiles) step(i + 1, s_odds, s_even);
     }
+    l += __shfl_xor(l, 32, 64);
     __syncthreads();
+    /* the splits' sums, half of them at a time, always in the same order */
+#pragma unroll
+    for (int half = SG / 2; half >= 1; half >>= 1) {
+        f32x4 *const at = (f32x4 *)(s_even) + ((sg & (half - 1)) * RG + rg) * DT * 4 * 64 + lane;
+        float(*const ml)[32] = s_ml[(sg & (half - 1)) * RG + rg];
+        if (sg >= half && sg < 2 * half) {
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    at[(dt * 4 + r) * 64] = f32x4{o[dt][4 * r], o[dt][4 * r + 1], o[dt][4 * r + 2], o[dt][4 * r + 3]};
+            if (h == 0) {
+                ml[0][col] = m;
+                ml[1][col] = l;
+            }
+        }
+        __syncthreads();
+        if (sg < half) {
+            const float om = ml[0][col], ol = ml[1][col], to = fmaxf(m, om), base = to == -INFINITY ? 0.0f : to;
+            const float fm = __builtin_amdgcn_exp2f(m - base), fo = __builtin_amdgcn_exp2f(om - base);
+            m = to;
+            l = l * fm + ol * fo;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const f32x4 w = at[(dt * 4 + r) * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[dt][4 * r + e] = o[dt][4 * r + e] * fm + w[e] * fo;
+                }
+        }
+        __syncthreads();
+    }
+    if (sg > 0) return;
     const int odd_from = kv_uniform(s_odd);
     if (odd_from < tiles) {
-        /* Rows that see a value that is not finite, from the first tile that left one out; where a later tile had it in its
+        /* Rows that see a value that is not finite, from the first stage that left one out; where a later stage had it in its
          * product it is added once more, which changes nothing. */
 #pragma unroll 1
-        for (int blk = 4 * odd_from; blk <= (wend - 1) / KV_BLOCK; blk++) {
+        for (int blk = BLOCKS * odd_from; blk <= (wend - 1) / KV_BLOCK; blk++) {
             const int64_t at = kv_block(c, table[blk >> c.sh], blk, kvh);
             if (at < 0) continue;
             const uint16_t *v = (const uint16_t *)a.v + at + 64 * h;
@@ -252,7 +320,6 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(Prompt
             }
         }
     }
-    l += __shfl_xor(l, 32, 64);
     if (!real) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;    /* a row that sees nothing: zeros */
     const int64_t at = ((rows.first + token) * H + kvh * G + (row - token * G)) * HD;
@@ -265,11 +332,26 @@ __global__ __launch_bounds__(NW * 64, HD <= 128 ? 2 : 1) void k_kv_prompt(Prompt
         }
 }
 
-constexpr int TILE = 128;    /* rows of a group */
+/* Rows of a group: 128 where that many groups fill the chip twice (two fit a compute unit); else 64, the positions dealt to
+ * two waves, or 32 and four, while all groups still run at once (one a unit, two up to 64 wide): a stage takes a lone wave
+ * about a microsecond whatever its rows.  us with 128 / 64 / 32 rows, 32 heads on 4 of 128: 4096 tokens 156 / 178 / 395,
+ * 2048 59 / 58 / 129, 1024 30 / 24 / 48, 512 19 / 15 / 21, 256 13.3 / 10.6 / 11.2; 128 behind 8000 176 / 117 / 80; 8 heads on 2
+ * of 64, 2048 tokens: 39 / 26 / 22. */
+int split_of(int64_t rows, int64_t B, int group, int kv_heads, int hd) {
+    const int64_t groups = kv_prompt_most(rows, B, group, 128) * kv_heads;
+    return groups > 512 ? 1 : groups > (hd <= 64 ? 128 : 64) ? 2 : 4;
+}
 
+template <class T, int HD, int SG, int TP> void launch_sg(const PromptArgs &a, int64_t B, hipStream_t s) {
+    const dim3 grid((unsigned)(kv_prompt_most(a.c.rows, B, a.G, 128 / SG) * a.c.heads));
+    hipLaunchKernelGGL((k_kv_prompt<T, HD, SG, TP>), grid, dim3(256), 0, s, a);
+}
 template <class T, int HD> void launch(const PromptArgs &a, int64_t B, hipStream_t s) {
-    const dim3 grid((unsigned)(kv_prompt_most(a.c.rows, B, a.G, TILE) * a.c.heads));
-    hipLaunchKernelGGL((k_kv_prompt<T, HD, TILE / 32>), grid, dim3(TILE * 2), 0, s, a);
+    const int sg = split_of(a.c.rows, B, a.G, a.c.heads, HD);
+    if (sg == 1) return launch_sg<T, HD, 1, 2>(a, B, s);
+    if constexpr (HD <= 128)     /* wider, four stages twice are more than the LDS */
+        if (sg == 4) return launch_sg<T, HD, 4, 1>(a, B, s);
+    launch_sg<T, HD, 2, HD <= 64 ? 2 : 1>(a, B, s);
 }
 template <class T> void prompt(const PromptArgs &a, int64_t B, hipStream_t s) {
     static void (*const by_width[8])(const PromptArgs &, int64_t, hipStream_t) = {
@@ -295,7 +377,7 @@ extern "C" int tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_bat
                            (long long)heads * c->head_dim);
     if (!aligned(q, 2) || !aligned(out, (size_t)type_bytes(out_dt)))
         return tlmh_seterr(TLM_HIP_EINVAL, "kv_prompt: q and out must have their type's alignment");
-    if (kv_prompt_most(b->rows, b->B, heads / c->kv_heads, TILE) * c->kv_heads > (1 << 23))
+    if (kv_prompt_most(b->rows, b->B, heads / c->kv_heads, 128) * c->kv_heads > (1 << 23))
         return tlmh_seterr(TLM_HIP_ERANGE, "kv_prompt: %lld rows of %lld sequences are too many for one launch",
                            (long long)b->rows, (long long)b->B);
     a.q = q;

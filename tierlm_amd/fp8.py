@@ -154,11 +154,11 @@ def add_rmsnorm(h, x, weight, eps=1e-6, out=None, codes=None, scale=None):
             raise ValueError("out must be h itself or not overlap it")
     nb = -(-n // BLOCK)
     if codes is None:
-        codes = torch.empty(T, nb * BLOCK, dtype=E4M3, device=h.device)
+        codes = h.new_empty((T, nb * BLOCK), dtype=E4M3)
     else:
         here = _out(codes, (T, nb * BLOCK), E4M3, h, "codes").get_device() == dev and here
     if scale is None:
-        scale = torch.empty(T, nb, dtype=_F32, device=h.device)
+        scale = weight.new_empty((T, nb))
     else:
         here = _out(scale, (T, nb), _F32, h, "scale").get_device() == dev and here
     if not here:

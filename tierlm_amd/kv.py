@@ -55,6 +55,7 @@ class Cache:
         self._dev = self.k.get_device()
         self._c = KvCache(_CACHE[dtype], kv_heads, head_dim, page, n_pages, self.k.data_ptr(), self.v.data_ptr())
         self._ref = C.byref(self._c)
+        self._workspace = {}        # bytes of a decode's workspace by its sizes
 
     def keys(self, pages):
         """The keys of these pages (a list, or an int tensor), end to end: [kv_heads, positions, head_dim]."""
@@ -119,7 +120,7 @@ def append(cache, qkv, heads, tables, lens, cu=None, *, q_norm=None, k_norm=None
         if t is not None and (t.shape != (n,) or t.dtype is not ty or not t.is_contiguous()):
             raise ValueError(f"{what} must be contiguous {ty} [{n}]")
     if out is None:
-        out = torch.empty(T, heads, hd, dtype=cache.dtype, device=cache.k.device)
+        out = cache.k.new_empty((T, heads, hd))
     elif out.shape != (T, heads, hd) or out.dtype is not cache.dtype or not out.is_contiguous() or \
             out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous {cache.dtype} [{T}, {heads}, {hd}], 16-byte aligned")
@@ -151,8 +152,11 @@ def _queries(q, cache, scale, out, dtype):
     elif not 0.0 < scale < math.inf:
         raise ValueError("scale must be finite and positive")
     if out is None:
-        out = torch.empty(T, heads, hd, dtype=q.dtype if dtype is None else dtype, device=q.device)
-        if out.dtype not in _TYPES:
+        if dtype is None:
+            out = q.new_empty(q.shape)
+        elif dtype in _TYPES:
+            out = q.new_empty(q.shape, dtype=dtype)
+        else:
             raise ValueError("dtype must be float32, float16 or bfloat16")
     elif out.shape != q.shape or out.dtype not in _TYPES or not out.is_contiguous():
         raise ValueError(f"out must be contiguous float32, float16 or bfloat16 {tuple(q.shape)}")
@@ -166,8 +170,13 @@ def decode(q, cache, tables, lens, *, scale=None, out=None, dtype=None):
     stride, heads, scale, out = _queries(q, cache, scale, out, dtype)
     b = _batch(cache, q.shape[0], tables, lens, None, (q, out))
     ref = C.byref(b)
-    nbytes = lib.tlm_hip_kv_decode_workspace_bytes(cache._ref, ref, heads)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    key = (b.B, heads, b.table_pages)
+    nbytes = cache._workspace.get(key)
+    if nbytes is None:
+        if len(cache._workspace) >= 4096:
+            cache._workspace.clear()
+        nbytes = cache._workspace[key] = lib.tlm_hip_kv_decode_workspace_bytes(cache._ref, ref, heads)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = _decode(cache._ref, ref, q.data_ptr(), stride, heads, scale, _TYPES[out.dtype], out.data_ptr(),
                  ws.data_ptr() if nbytes else None, _raw_stream(cache._dev))
     if rc:
