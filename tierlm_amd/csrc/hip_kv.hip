@@ -290,7 +290,7 @@ struct DecodeBatch {
 };
 
 template <class T, int HD, int NC, int NW, bool WHOLE>
-__global__ __launch_bounds__(NW * 64, HD *NC <= 128 ? 2 : 1) void k_kv_decode(DecodeArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeArgs a) {
     typedef typename KvType<T>::x8 x8;
     constexpr int KS = HD / 32, DT = HD / 16;    /* steps of the first product, result tiles of the second */
     constexpr int LD = HD + 4;                   /* a merged column in LDS: 16 lanes' float4 on all banks */
@@ -583,8 +583,11 @@ DecodePlan decode_plan(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int
     const int G = heads / c->kv_heads, nc = G <= 16 ? 1 : G <= 32 || c->head_dim > 128 ? 2 : 4, z = (G + nc * 16 - 1) / (nc * 16);
     const int64_t cap = (int64_t)b->table_pages * c->page;
     if (cap <= DECODE_WHOLE) return {1, (int)b->B, nc, z, 0};
-    /* as many groups as the chip holds at once */
-    const int slots = 256 * (c->head_dim * nc <= 64 ? 4 : c->head_dim * nc <= 128 ? 2 : 1), W = slots / (c->kv_heads * z);
+    /* A group a compute unit: four waves with two tiles each on their way keep the memory busy, and fewer shares are fewer
+     * parts to join.  256 groups / 512 (1024 up to 64 wide): one sequence of 131071, 32 heads on 4 of 128, 52.7 / 55.1 us; 64
+     * of up to 8192, 64 on 4, 113 / 118; 60000, 8 on 2 of 64, 13.8 / 18.3; 240 groups 53.6, 114, 14.2; 256 of eight waves
+     * 53.6, 116, 14.1. */
+    const int W = 256 / (c->kv_heads * z);
     /* the join: about 1024 groups, a head each if there are fewer */
     const int64_t hb = b->B * heads / 1024;
     const int rows = 256 / (c->head_dim / 4);
