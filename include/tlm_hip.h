@@ -46,7 +46,8 @@ enum {
  * start-up self-test of every HIP kernel against the library's built-in
  * scalar rule on fixed data (src/lib/tlm_quant.c:950-1056).  A kernel that
  * fails is counted and its dtype is refused: by the host-pointer tier entries, and
- * 8-bit floating point by every tlm_hip_fp8_* call that launches (TLM_HIP_EIO).
+ * 8-bit floating point by every tlm_hip_fp8_* call that launches, the paged cache by
+ * every tlm_hip_kv_* one (TLM_HIP_EIO).
  * Idempotent for the same device.  TLM_HIP_EUNSUP when no GPU is present. */
 int         tlm_hip_init(int device);
 void        tlm_hip_shutdown(void);

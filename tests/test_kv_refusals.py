@@ -164,3 +164,44 @@ def test_places(tmp_path):
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover=all",
                     os.path.join(HERE, "kv_places.cpp"), "-o", exe], check=True)
     assert subprocess.run([exe], check=True, capture_output=True, text=True).stdout == "ok\n"
+
+
+@pytest.fixture
+def failed():
+    if torch.cuda.is_available():
+        pytest.skip("addresses that a launch would follow")
+    note = getattr(lib, "_Z15tlmh_set_failedi")           # tlmh_set_failed(int), of the library's own start
+    note.argtypes, note.restype = [C.c_int], None
+    yield note
+    note(0)
+
+
+def test_a_failed_self_test_refuses_the_calls(failed):
+    c, b = C.byref(cache()), C.byref(batch())
+    calls = {"kv_append": lambda: lib.tlm_hip_kv_append(c, b, 0, P, 768, 8, None, None, 1e-6, None, 1.0, P, None),
+             "kv_decode": lambda: lib.tlm_hip_kv_decode(c, b, P, 512, 8, 0.1, 2, P, P, None),
+             "kv_prompt": lambda: lib.tlm_hip_kv_prompt(c, b, P, 512, 8, 0.1, 2, P, None)}
+    norm = lambda: lib.tlm_hip_fp8_add_rmsnorm(0, P, 128, 2, P, 128, P, 1e-6, 128, 2, P, 128, P, P, None)   # noqa: E731
+    failed(1 << 27)
+    for name, call in calls.items():
+        assert call() == -1 and name.encode() in lib.tlm_hip_errmsg() and b"self-test" in lib.tlm_hip_errmsg()
+    norm()
+    assert b"self-test" not in lib.tlm_hip_errmsg()
+    failed(1 << 28)
+    assert norm() == -1 and b"self-test" in lib.tlm_hip_errmsg()
+    calls["kv_decode"]()                                   # no device: another error
+    assert b"self-test" not in lib.tlm_hip_errmsg()
+
+
+def test_struct_layout(tmp_path):
+    """The C structs as the compiler lays them out."""
+    src = tmp_path / "s.c"
+    src.write_text('''#include <stdio.h>
+#include "tlm_hip.h"
+int main(void) { printf("%zu %zu %zu %zu %zu\\n", sizeof(tlm_hip_kv_cache), offsetof(tlm_hip_kv_cache, v),
+                        sizeof(tlm_hip_kv_batch), offsetof(tlm_hip_kv_batch, tables), offsetof(tlm_hip_kv_batch, table_pages));
+                 return 0; }''')
+    exe = str(tmp_path / "s")
+    subprocess.run(["gcc", "-I", os.path.join(os.path.dirname(HERE), "include"), str(src), "-o", exe], check=True)
+    got = [int(v) for v in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [C.sizeof(KvCache), KvCache.v.offset, C.sizeof(KvBatch), KvBatch.tables.offset, KvBatch.table_pages.offset]

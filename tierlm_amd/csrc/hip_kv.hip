@@ -675,6 +675,7 @@ int tlm_hip_kv_append(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int 
         !aligned(inv_freq, 8))
         return tlmh_seterr(TLM_HIP_EINVAL, "kv_append: qkv must have its type's alignment, q 16, the norms 4, inv_freq 8 "
                            "bytes");
+    if (int rc = tlmh_refuse_failed(FAILED_KV, "kv_append")) return rc;
     const int64_t items = kv_append_most(b->rows, b->B);
     if (items * c->kv_heads > (1 << 23))
         return tlmh_seterr(TLM_HIP_ERANGE, "kv_append: %lld rows of %lld sequences are too many for one launch",
@@ -724,6 +725,7 @@ int tlm_hip_kv_decode(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, cons
                            (long long)b->B, heads);
     if (!p.whole && (!workspace || !aligned(workspace, 256)))
         return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: needs a workspace of %zu bytes, 256-byte aligned", decode_bytes(c, b, heads));
+    if (int rc = tlmh_refuse_failed(FAILED_KV, "kv_decode")) return rc;
     a.q = q;
     a.k = c->k;
     a.v = c->v;

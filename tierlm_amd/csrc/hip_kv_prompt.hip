@@ -380,6 +380,7 @@ extern "C" int tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_bat
     if (kv_prompt_most(b->rows, b->B, heads / c->kv_heads, 128) * c->kv_heads > (1 << 23))
         return tlmh_seterr(TLM_HIP_ERANGE, "kv_prompt: %lld rows of %lld sequences are too many for one launch",
                            (long long)b->rows, (long long)b->B);
+    if (int rc = tlmh_refuse_failed(FAILED_KV, "kv_prompt")) return rc;
     a.q = q;
     a.k = c->k;
     a.v = c->v;

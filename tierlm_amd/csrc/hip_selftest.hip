@@ -12,7 +12,7 @@
  * at one size, of the row groups.
  * Returns the number of failing kernels; bit dt of *mask is set for every dtype
  * whose kernels failed, FAILED_EXP for the exponential, FAILED_PRODUCTS for the
- * products, FAILED_FP8 for 8-bit floating point. */
+ * products, FAILED_FP8 for 8-bit floating point, FAILED_KV for the paged cache. */
 #include "tlm_hip_internal.h"
 #include "tlm_hip_outer.h"
 
@@ -264,6 +264,22 @@ int to_e4m3(double v) {
     return best | (signbit(v) ? 128 : 0);
 }
 
+/* the quantiser's codes and scales of T rows of n values, by search */
+void h_fp8(const float *x, int T, int n, uint8_t *codes, float *scale) {
+    const int nb = (n + 127) / 128, np = nb * 128;
+    memset(codes, 0, (size_t)T * np);
+    for (int t = 0; t < T; t++)
+        for (int b = 0; b < nb; b++) {
+            const int m = n - 128 * b < 128 ? n - 128 * b : 128;
+            double amax = 0.0;
+            for (int i = 0; i < m; i++) amax = fmax(amax, fabs((double)x[t * n + 128 * b + i]));
+            int e = -126;
+            while (amax > ldexp(448.0, e)) e++;
+            scale[t * nb + b] = amax > 0.0 ? ldexpf(1.0f, e) : 0.0f;
+            for (int i = 0; i < m; i++) codes[t * np + 128 * b + i] = (uint8_t)to_e4m3(ldexp((double)x[t * n + 128 * b + i], -e));
+        }
+}
+
 /* 3 tokens and 20 rows of 300 values (part blocks and part tiles); dev: 32 KB */
 bool fp8_ok(uint8_t *dev, uint32_t *s) {
     constexpr int T = 3, R = 20, N = 300, NB = 3, NP = NB * 128;
@@ -275,16 +291,7 @@ bool fp8_ok(uint8_t *dev, uint32_t *s) {
         c = (uint8_t)st_rng(s);
         if ((c & 127) == 127) c = 0;
     }
-    for (int t = 0; t < T; t++)
-        for (int b = 0; b < NB; b++) {
-            const int n = N - 128 * b < 128 ? N - 128 * b : 128;
-            double amax = 0.0;
-            for (int i = 0; i < n; i++) amax = fmax(amax, fabs((double)x[t * N + 128 * b + i]));
-            int e = -126;
-            while (amax > ldexp(448.0, e)) e++;
-            sx[t * NB + b] = amax > 0.0 ? ldexpf(1.0f, e) : 0.0f;
-            for (int i = 0; i < n; i++) cx[t * NP + 128 * b + i] = (uint8_t)to_e4m3(ldexp((double)x[t * N + 128 * b + i], -e));
-        }
+    h_fp8(x.data(), T, N, cx.data(), sx.data());
     float *dx = (float *)dev, *ds = (float *)(dev + 4096), *dsw = (float *)(dev + 4352), *dy = (float *)(dev + 4608);
     uint8_t *dc = dev + 8192, *dw = dev + 10240, *dp = dev + 16640;
     if (hipMemcpy(dx, x.data(), x.size() * 4, hipMemcpyHostToDevice) != hipSuccess ||
@@ -308,7 +315,166 @@ bool fp8_ok(uint8_t *dev, uint32_t *s) {
             }
             if (!(fabs((double)y[t * R + r] - sum) <= (127 + NB + 2) * 0x1p-24 * size)) return false;
         }
-    return true;
+    /* the norm in front of the quantiser: 2 x, x itself added, times some positive weights */
+    std::vector<float> h(T * N), v(T * N), nw(N), x2(x), gh(T * N);
+    for (int i = 0; i < N; i++) nw[i] = 0.5f + (float)(i % 7) * 0.125f;
+    for (auto &e : x2) e *= 2.0f;
+    for (int t = 0; t < T; t++) {
+        double sum = 0.0;
+        for (int i = 0; i < N; i++) {
+            h[t * N + i] = x2[t * N + i] + x[t * N + i];
+            sum += (double)h[t * N + i] * (double)h[t * N + i];
+        }
+        const float r = (float)(1.0 / sqrt(sum / N + 0x1p-20));
+        for (int i = 0; i < N; i++) v[t * N + i] = (h[t * N + i] * r) * nw[i];
+    }
+    h_fp8(v.data(), T, N, cx.data(), sx.data());
+    float *dh = (float *)(dev + 10240), *dn = (float *)dp;
+    if (hipMemcpy(dh, x2.data(), x2.size() * 4, hipMemcpyHostToDevice) != hipSuccess ||
+        hipMemcpy(dn, nw.data(), nw.size() * 4, hipMemcpyHostToDevice) != hipSuccess ||
+        tlm_hip_fp8_add_rmsnorm(DT_F32, dh, N, DT_F32, dx, N, dn, 0x1p-20f, N, T, dh, N, dc, ds, nullptr) != TLM_HIP_OK ||
+        hipMemcpy(gc.data(), dc, gc.size(), hipMemcpyDeviceToHost) != hipSuccess ||
+        hipMemcpy(gs.data(), ds, gs.size() * 4, hipMemcpyDeviceToHost) != hipSuccess ||
+        hipMemcpy(gh.data(), dh, gh.size() * 4, hipMemcpyDeviceToHost) != hipSuccess)
+        return false;
+    return memcmp(gh.data(), h.data(), h.size() * 4) == 0 && memcmp(gc.data(), cx.data(), cx.size()) == 0 &&
+           memcmp(gs.data(), sx.data(), sx.size() * 4) == 0;
+}
+
+/* a value rounded to F16 or BF16 (nothing here is past their range), and one read back */
+double to_half(int dt, double v) {
+    if (v == 0.0) return 0.0;
+    int e;
+    frexp(v, &e);
+    const int bits = dt == DT_F16 ? 11 : 8, least = dt == DT_F16 ? -24 : -133;
+    const int unit = e - bits < least ? least : e - bits;
+    return ldexp(nearbyint(ldexp(v, -unit)), unit);
+}
+double from_half(int dt, uint16_t h) {
+    if (dt == DT_F16) return h_f16(h);
+    const uint32_t u = (uint32_t)h << 16;
+    float f;
+    memcpy(&f, &u, 4);
+    return f;
+}
+
+/* The paged cache: two sequences (19 rows, and 3 behind 20 positions that a first call appended) of 4 heads on 2 of 32,
+ * with norms and rotation; their attention as prompts, and of the last rows alone, whole and in shares (a wide table). */
+bool kv_ok(uint32_t *s) {
+    constexpr int H = 4, KV = 2, HD = 32, PAGE = 16, PAGES = 5, WIDE = 40, ROW = (H + 2 * KV) * HD, B = 2, FIRST = 20, T = 22;
+    const int n[B] = {19, 3}, len[B] = {19, 23}, table[B][3] = {{4, 1, -1}, {0, 3, -1}};
+    const size_t cache = (size_t)PAGES * KV * PAGE * HD * 2, ws = (size_t)2 * 256 * H * (HD + 4) * 4;
+    const size_t o_k = ((size_t)(FIRST + T) * ROW * 4 + 255) & ~(size_t)255, o_v = o_k + cache, o_q = o_v + cache,
+                 o_y = o_q + 16384, o_i = o_y + 16384, o_w = o_i + 4096;
+    std::vector<float> x((FIRST + T) * ROW), norm(2 * HD), gy(T * H * HD), gd(B * H * HD);
+    std::vector<double> freq(HD / 2);
+    std::vector<int32_t> ints(8 + B * WIDE, -1);
+    std::vector<uint16_t> gq(T * H * HD);
+    for (auto &e : x) e = (float)(st_rng(s) & 0xFFFF) / 16384.0f - 2.0f;
+    for (auto &e : norm) e = 0.5f + (float)(st_rng(s) & 0xFF) / 256.0f;
+    for (int j = 0; j < HD / 2; j++) freq[j] = pow(1e4, -2.0 * j / HD);
+    const int32_t head[8] = {0, n[0], T, len[0], len[1], 0, FIRST, FIRST};   /* cu, lens; the first call's cu and length */
+    for (int i = 0; i < 8; i++) ints[i] = head[i];
+    for (int b = 0; b < B; b++)
+        for (int i = 0; i < 3; i++) ints[8 + b * WIDE + i] = table[b][i];
+    uint8_t *dev = nullptr;
+    if (hipMalloc((void **)&dev, o_w + ws) != hipSuccess) return false;
+    const int32_t *di = (const int32_t *)(dev + o_i);
+    double *df = (double *)(dev + o_i + 1024);
+    float *dn = (float *)(dev + o_i + 2048), *dx = (float *)dev;
+    void *q = dev + o_q, *y = dev + o_y;
+    bool ok = hipMemcpy(dx, x.data(), x.size() * 4, hipMemcpyHostToDevice) == hipSuccess &&
+              hipMemcpy(dev + o_i, ints.data(), ints.size() * 4, hipMemcpyHostToDevice) == hipSuccess &&
+              hipMemcpy(df, freq.data(), freq.size() * 8, hipMemcpyHostToDevice) == hipSuccess &&
+              hipMemcpy(dn, norm.data(), norm.size() * 4, hipMemcpyHostToDevice) == hipSuccess;
+    /* a head's row with its norm, turned to position pos */
+    auto turned = [&](const float *src, const float *w, int pos, double *o) {
+        double ss = 0.0;
+        for (int i = 0; i < HD; i++) ss += (double)src[i] * src[i];
+        const double r = 1.0 / sqrt(ss / HD + 1e-6);
+        for (int j = 0; j < HD / 2; j++) {
+            const double a = src[j] * r * w[j], d = src[HD / 2 + j] * r * w[HD / 2 + j], ang = pos * freq[j];
+            o[j] = a * cos(ang) - d * sin(ang);
+            o[HD / 2 + j] = d * cos(ang) + a * sin(ang);
+        }
+    };
+    for (int dt : {DT_F16, DT_BF16}) {
+        const double half = dt == DT_F16 ? 0x1p-11 : 0x1p-8;
+        const tlm_hip_kv_cache c = {dt, KV, HD, PAGE, PAGES, dev + o_k, dev + o_v};
+        const tlm_hip_kv_batch first = {1, FIRST, di + 5, di + 7, di + 8 + WIDE, WIDE, 3}, b = {B, T, di, di + 3, di + 8, WIDE, 3};
+        ok = ok && tlm_hip_kv_append(&c, &first, DT_F32, dx, ROW, H, dn, dn + HD, 1e-6f, df, 1.0f, q, nullptr) == TLM_HIP_OK &&
+             tlm_hip_kv_append(&c, &b, DT_F32, dx + FIRST * ROW, ROW, H, dn, dn + HD, 1e-6f, df, 1.0f, q, nullptr) == TLM_HIP_OK &&
+             tlm_hip_kv_prompt(&c, &b, q, H * HD, H, 0.25f, DT_F32, y, nullptr) == TLM_HIP_OK &&
+             hipMemcpy(gq.data(), q, gq.size() * 2, hipMemcpyDeviceToHost) == hipSuccess &&
+             hipMemcpy(gy.data(), y, gy.size() * 4, hipMemcpyDeviceToHost) == hipSuccess;
+        if (!ok) break;
+        std::vector<double> k[B], v[B];
+        for (int i = 0; i < B; i++) {
+            k[i].resize(len[i] * KV * HD);
+            v[i].resize(len[i] * KV * HD);
+            for (int p = 0; p < len[i]; p++) {
+                const float *row = x.data() + (i == 0 ? FIRST + p : p < FIRST ? p : FIRST + n[0] + p - FIRST) * ROW;
+                for (int h = 0; h < KV; h++) {
+                    double *o = &k[i][(p * KV + h) * HD];
+                    turned(row + (H + h) * HD, norm.data() + HD, p, o);
+                    for (int e = 0; e < HD; e++) {
+                        o[e] = to_half(dt, o[e]);
+                        v[i][(p * KV + h) * HD + e] = to_half(dt, row[(H + KV + h) * HD + e]);
+                    }
+                }
+            }
+        }
+        /* Row t of the call, at position p of sequence i.  A query is within a half step of its definition, f32 roundings beside it.
+         * A key next to the border of two steps may be the other one here: a step (two half ones) of each product of a score, so a
+         * weight is off by twice the largest score's steps; and each weight is rounded once. */
+        auto check = [&](const float *got, int i, int t, int p) {
+            for (int h = 0; h < H; h++) {
+                double qv[HD], e[32], top = -1e300, sum = 0.0, size = 0.0;
+                turned(x.data() + (FIRST + t) * ROW + h * HD, norm.data(), p, qv);
+                for (int d = 0; d < HD; d++) {
+                    const double g = from_half(dt, gq[(t * H + h) * HD + d]);
+                    ok = ok && fabs(g - qv[d]) <= half * fabs(qv[d]) + 1e-5;
+                    qv[d] = g;
+                }
+                for (int j = 0; j <= p; j++) {
+                    double mag = e[j] = 0.0;
+                    for (int d = 0; d < HD; d++) {
+                        const double u = qv[d] * k[i][(j * KV + h / 2) * HD + d] * 0.25;
+                        e[j] += u;
+                        mag += fabs(u);
+                    }
+                    top = fmax(top, e[j]);
+                    size = fmax(size, mag);
+                }
+                for (int j = 0; j <= p; j++) sum += e[j] = exp(e[j] - top);
+                for (int d = 0; d < HD; d++) {
+                    double o = 0.0, mag = 0.0;
+                    for (int j = 0; j <= p; j++) {
+                        const double u = e[j] / sum * v[i][(j * KV + h / 2) * HD + d];
+                        o += u;
+                        mag += fabs(u);
+                    }
+                    ok = ok && fabs(got[h * HD + d] - o) <= mag * (half * (1.0 + 4.0 * size) + 1e-5) + 1e-6;
+                }
+            }
+        };
+        for (int i = 0, t = 0; i < B; i++)
+            for (int r = 0; r < n[i]; r++, t++) check(&gy[t * H * HD], i, t, len[i] - n[i] + r);
+        /* the last row of each sequence: rows n[0] - 1 and n[0] + n[1] - 1 */
+        for (int pages : {3, WIDE}) {
+            const tlm_hip_kv_batch last = {B, B, nullptr, di + 3, di + 8, WIDE, pages};
+            ok = ok && tlm_hip_kv_decode_workspace_bytes(&c, &last, H) <= ws &&
+                 tlm_hip_kv_decode(&c, &last, (const uint16_t *)q + (n[0] - 1) * H * HD, n[1] * H * HD, H, 0.25f, DT_F32, y,
+                                   dev + o_w, nullptr) == TLM_HIP_OK &&
+                 hipMemcpy(gd.data(), y, gd.size() * 4, hipMemcpyDeviceToHost) == hipSuccess;
+            if (!ok) break;
+            check(&gd[0], 0, n[0] - 1, len[0] - 1);
+            check(&gd[H * HD], 1, T - 1, len[1] - 1);
+        }
+    }
+    (void)hipDeviceSynchronize();
+    (void)hipFree(dev);
+    return ok;
 }
 
 }  // namespace
@@ -411,6 +577,10 @@ int tlmh_selftest(int *failed_mask) {
     if (!fp8_ok(dev + o_p, &s)) {
         fails++;
         mask |= 1 << FAILED_FP8;
+    }
+    if (!kv_ok(&s)) {
+        fails++;
+        mask |= 1 << FAILED_KV;
     }
     (void)hipDeviceSynchronize();
     (void)hipFree(dev);

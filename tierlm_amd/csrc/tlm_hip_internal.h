@@ -29,7 +29,7 @@ enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2, DT_Q8_0 = 8, DT_Q4_K = 12, DT_Q5_K =
 int tlmh_seterr(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 int tlmh_check(hipError_t e, const char *what);
 /* the self-test's mask: bit dt for a dtype's kernels, and these */
-enum { FAILED_FP8 = 28, FAILED_PRODUCTS = 29, FAILED_EXP = 30 };
+enum { FAILED_KV = 27, FAILED_FP8 = 28, FAILED_PRODUCTS = 29, FAILED_EXP = 30 };
 void tlmh_set_failed(int mask);
 /* TLM_HIP_OK, or the error of a call whose kernels failed the self-test */
 int tlmh_refuse_failed(int bit, const char *who);
