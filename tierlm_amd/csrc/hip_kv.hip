@@ -709,7 +709,7 @@ int tlm_hip_kv_decode(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, cons
     if (int rc = kv_check("kv_decode", c, b, heads, &a.c)) return rc;
     if (b->cu) return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: one row a sequence (cu must be NULL)");
     if (!type_bytes(out_dt)) return tlmh_seterr(TLM_HIP_EUNSUP, "kv_decode: dtype %d (F32, F16 and BF16 only)", out_dt);
-    if (!(scale > 0.0f) || scale > 3.0e38f) return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: scale must be finite and positive");
+    if (!(scale > 0.0f) || scale > 2.0e38f) return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: scale must be finite and positive");
     if (b->B == 0) return TLM_HIP_OK;
     if (!q || !out) return tlmh_seterr(TLM_HIP_EINVAL, "kv_decode: NULL argument");
     if (q_stride < (int64_t)heads * c->head_dim && b->B > 1)

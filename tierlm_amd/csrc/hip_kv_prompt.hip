@@ -369,7 +369,7 @@ extern "C" int tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_bat
     PromptArgs a;
     if (int rc = kv_check("kv_prompt", c, b, heads, &a.c)) return rc;
     if (!type_bytes(out_dt)) return tlmh_seterr(TLM_HIP_EUNSUP, "kv_prompt: dtype %d (F32, F16 and BF16 only)", out_dt);
-    if (!(scale > 0.0f) || scale > 3.0e38f) return tlmh_seterr(TLM_HIP_EINVAL, "kv_prompt: scale must be finite and positive");
+    if (!(scale > 0.0f) || scale > 2.0e38f) return tlmh_seterr(TLM_HIP_EINVAL, "kv_prompt: scale must be finite and positive");
     if (b->B == 0 || b->rows == 0) return TLM_HIP_OK;
     if (!q || !out) return tlmh_seterr(TLM_HIP_EINVAL, "kv_prompt: NULL argument");
     if (q_stride < (int64_t)heads * c->head_dim && b->rows > 1)

@@ -128,29 +128,29 @@ def add_rmsnorm(h, x, weight, eps=1e-6, out=None, codes=None, scale=None):
     in place); returns the codes and scales of rmsnorm(s) weight as quantize() gives them.  h and x [T, n],
     float32, float16 or bfloat16 each by itself, rows of any stride; weight float32 [n].  `out` is h or overlaps
     neither."""
+    shape = h.shape
     hdt = _TYPES.get(h.dtype)
-    if hdt is None or not _rows_ok(h):
+    if hdt is None or len(shape) != 2 or not _rows_ok(h):
         raise ValueError("h must be float32, float16 or bfloat16 [T, n] with contiguous rows")
-    T, n = h.shape
+    T, n = shape
     if n == 0:
         raise ValueError("h must have at least one value a row")
-    dev, px, xdt, xstride = h.get_device(), None, 0, 0
+    dev, po, px, xdt, xstride = h.get_device(), None, None, 0, 0
     here = dev >= 0 and dev == weight.get_device() == _current_device()
+    stride = ostride = max(h.stride(0), n)
     if x is not None:
         xdt = _TYPES.get(x.dtype)
-        if xdt is None or x.shape != h.shape or not _rows_ok(x):
+        if xdt is None or x.shape != shape or not _rows_ok(x):
             raise ValueError(f"x must be float32, float16 or bfloat16 [{T}, {n}] with contiguous rows")
-        px, xstride, here = x.data_ptr(), max(x.stride(0), n), here and x.get_device() == dev
+        px, xstride, po = x.data_ptr(), max(x.stride(0), n), h.data_ptr()
+        here = here and x.get_device() == dev
     if weight.shape != (n,) or weight.dtype is not _F32 or not weight.is_contiguous():
         raise ValueError(f"weight must be contiguous float32 [{n}]")
-    stride, ostride = max(h.stride(0), n), 0
-    if out is None:
-        po, ostride = (None if x is None else h.data_ptr()), stride
-    else:
-        if out.shape != h.shape or out.dtype is not h.dtype or not _rows_ok(out):
+    if out is not None:
+        if out.shape != shape or out.dtype is not h.dtype or not _rows_ok(out):
             raise ValueError(f"out must be {h.dtype} [{T}, {n}] with contiguous rows")
         po, ostride, here = out.data_ptr(), max(out.stride(0), n), here and out.get_device() == dev
-        if po == h.data_ptr() and ostride != stride and T > 1:
+        if ostride != stride and T > 1 and po == h.data_ptr():
             raise ValueError("out must be h itself or not overlap it")
     nb = -(-n // BLOCK)
     if codes is None:

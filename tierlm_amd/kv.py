@@ -35,8 +35,9 @@ class Cache:
 
     .k [n_pages, kv_heads, page / 16, head_dim / 16, 16, 16] holds value 16 i + j of the block's position p at
     [..., i, p, j], .v [n_pages, kv_heads, page / 16, head_dim, 16] value d at [..., d, p].  Pages may be copied
-    (cache.k[dst] = cache.k[src]); keys() and values() give them as [kv_heads, positions, head_dim].  The
-    memory is not cleared: a position is read once its sequence's length covers it."""
+    (cache.k[dst] = cache.k[src]); the two tensors themselves stay the cache's.  keys() and values() give pages as
+    [kv_heads, positions, head_dim].  The memory is not cleared: a position is read once its sequence's length
+    covers it."""
 
     def __init__(self, n_pages, kv_heads, head_dim, page=64, dtype=torch.bfloat16, device=None):
         if dtype not in _CACHE:
@@ -50,12 +51,20 @@ class Cache:
         if device is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.n_pages, self.kv_heads, self.head_dim, self.page, self.dtype = n_pages, kv_heads, head_dim, page, dtype
-        self.k = torch.empty(n_pages, kv_heads, page // 16, head_dim // 16, 16, 16, dtype=dtype, device=device)
-        self.v = torch.empty(n_pages, kv_heads, page // 16, head_dim, 16, dtype=dtype, device=device)
-        self._dev = self.k.get_device()
-        self._c = KvCache(_CACHE[dtype], kv_heads, head_dim, page, n_pages, self.k.data_ptr(), self.v.data_ptr())
+        self._k = torch.empty(n_pages, kv_heads, page // 16, head_dim // 16, 16, 16, dtype=dtype, device=device)
+        self._v = torch.empty(n_pages, kv_heads, page // 16, head_dim, 16, dtype=dtype, device=device)
+        self._dev = self._k.get_device()
+        self._c = KvCache(_CACHE[dtype], kv_heads, head_dim, page, n_pages, self._k.data_ptr(), self._v.data_ptr())
         self._ref = C.byref(self._c)
         self._workspace = {}        # bytes of a decode's workspace by its sizes
+
+    @property
+    def k(self):
+        return self._k
+
+    @property
+    def v(self):
+        return self._v
 
     def keys(self, pages):
         """The keys of these pages (a list, or an int tensor), end to end: [kv_heads, positions, head_dim]."""
@@ -75,12 +84,13 @@ def rope_frequencies(head_dim, theta, device=None):
 
 def _batch(cache, rows, tables, lens, cu, others):
     """The C batch, once its tensors fit."""
-    B = lens.shape[0] if lens.dim() == 1 else -1
-    if lens.dtype is not _I32 or B < 0 or not lens.is_contiguous():
+    shape, pages = lens.shape, tables.shape
+    if len(shape) != 1 or lens.dtype is not _I32 or not lens.is_contiguous():
         raise ValueError("lens must be contiguous int32 [B]")
-    if tables.dtype is not _I32 or tables.dim() != 2 or tables.shape[0] != B or not _rows_ok(tables) or \
-            tables.shape[1] < 1:
+    B = shape[0]
+    if len(pages) != 2 or pages[0] != B or pages[1] < 1 or tables.dtype is not _I32 or not _rows_ok(tables):
         raise ValueError(f"tables must be int32 [{B}, pages] with contiguous rows")
+    pages = pages[1]
     pcu = None
     dev = cache._dev
     if cu is None:
@@ -95,10 +105,20 @@ def _batch(cache, rows, tables, lens, cu, others):
     if dev < 0 or not dev == lens.get_device() == tables.get_device() == _current_device():
         _here(cache.k, lens, tables)
     for t in others:
-        if t is not None and t.get_device() != dev:
+        if t.get_device() != dev:
             _here(cache.k, t)
-    return KvBatch(B, rows, pcu, lens.data_ptr(), tables.data_ptr(), max(tables.stride(0), tables.shape[1]),
-                   tables.shape[1])
+    return KvBatch(B, rows, pcu, lens.data_ptr(), tables.data_ptr(), max(tables.stride(0), pages), pages)
+
+
+def _vector(t, n, dtype, what, dev):
+    """The address of a contiguous vector (None: null)."""
+    if t is None:
+        return None
+    if t.shape != (n,) or t.dtype is not dtype or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous {dtype} [{n}]")
+    if t.get_device() != dev:
+        raise ValueError(f"{what} is on {t.device}, not on the cache's device")
+    return t.data_ptr()
 
 
 def append(cache, qkv, heads, tables, lens, cu=None, *, q_norm=None, k_norm=None, eps=1e-6, inv_freq=None,
@@ -107,28 +127,24 @@ def append(cache, qkv, heads, tables, lens, cu=None, *, q_norm=None, k_norm=None
     the query and key heads (q_norm, k_norm: float32 [head_dim]), rotary positions (inv_freq: float64 [head_dim / 2],
     pairs j and j + head_dim / 2), keys and values to their pages.  Returns the queries, [T, heads,
     head_dim] of the cache's dtype."""
-    hd = cache.head_dim
+    hd, dev, shape = cache.head_dim, cache._dev, qkv.shape
     dt = _TYPES.get(qkv.dtype)
     if heads < 1 or heads % cache.kv_heads:
         raise ValueError(f"heads must be a multiple of the cache's {cache.kv_heads}")
     width = (heads + 2 * cache.kv_heads) * hd
-    if dt is None or qkv.dim() != 2 or qkv.shape[1] != width or not _rows_ok(qkv):
+    if dt is None or len(shape) != 2 or shape[1] != width or not _rows_ok(qkv):
         raise ValueError(f"qkv must be float32, float16 or bfloat16 [T, {width}] with contiguous rows")
-    T = qkv.shape[0]
-    for t, n, ty, what in ((q_norm, hd, _F32, "q_norm"), (k_norm, hd, _F32, "k_norm"),
-                           (inv_freq, hd // 2, _F64, "inv_freq")):
-        if t is not None and (t.shape != (n,) or t.dtype is not ty or not t.is_contiguous()):
-            raise ValueError(f"{what} must be contiguous {ty} [{n}]")
+    T = shape[0]
+    pq, pk = _vector(q_norm, hd, _F32, "q_norm", dev), _vector(k_norm, hd, _F32, "k_norm", dev)
+    pf = _vector(inv_freq, hd // 2, _F64, "inv_freq", dev)
     if out is None:
-        out = cache.k.new_empty((T, heads, hd))
+        out = cache._k.new_empty((T, heads, hd))
     elif out.shape != (T, heads, hd) or out.dtype is not cache.dtype or not out.is_contiguous() or \
             out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous {cache.dtype} [{T}, {heads}, {hd}], 16-byte aligned")
-    b = _batch(cache, T, tables, lens, cu, (qkv, out, q_norm, k_norm, inv_freq))
-    rc = _append(cache._ref, C.byref(b), dt, qkv.data_ptr(), max(qkv.stride(0), width), heads,
-                 q_norm.data_ptr() if q_norm is not None else None, k_norm.data_ptr() if k_norm is not None else None,
-                 eps, inv_freq.data_ptr() if inv_freq is not None else None, rope_scale, out.data_ptr(),
-                 _raw_stream(cache._dev))
+    b = _batch(cache, T, tables, lens, cu, (qkv, out))
+    rc = _append(cache._ref, C.byref(b), dt, qkv.data_ptr(), max(qkv.stride(0), width), heads, pq, pk, eps, pf,
+                 rope_scale, out.data_ptr(), _raw_stream(dev))
     if rc:
         check(rc)
     return out
@@ -136,9 +152,10 @@ def append(cache, qkv, heads, tables, lens, cu=None, *, q_norm=None, k_norm=None
 
 def _queries(q, cache, scale, out, dtype):
     """Row stride and heads of q, the scale and the result."""
-    if q.dtype is not cache.dtype or q.dim() != 3 or q.shape[2] != cache.head_dim:
+    shape = q.shape
+    if q.dtype is not cache.dtype or len(shape) != 3 or shape[2] != cache.head_dim:
         raise ValueError(f"q must be {cache.dtype} [T, heads, {cache.head_dim}]")
-    T, heads, hd = q.shape
+    T, heads, hd = shape
     if heads < 1 or heads % cache.kv_heads:
         raise ValueError(f"q's heads must be a multiple of the cache's {cache.kv_heads}")
     stride = heads * hd
@@ -153,24 +170,24 @@ def _queries(q, cache, scale, out, dtype):
         raise ValueError("scale must be finite and positive")
     if out is None:
         if dtype is None:
-            out = q.new_empty(q.shape)
+            out = q.new_empty(shape)
         elif dtype in _TYPES:
-            out = q.new_empty(q.shape, dtype=dtype)
+            out = q.new_empty(shape, dtype=dtype)
         else:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-    elif out.shape != q.shape or out.dtype not in _TYPES or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous float32, float16 or bfloat16 {tuple(q.shape)}")
-    return stride, heads, scale, out
+    elif out.shape != shape or out.dtype not in _TYPES or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous float32, float16 or bfloat16 {tuple(shape)}")
+    return T, stride, heads, scale, out
 
 
 def decode(q, cache, tables, lens, *, scale=None, out=None, dtype=None):
     """Attention of one new token a sequence: q [B, heads, head_dim] of the cache's dtype (rows of any stride) over
     the lens[b] positions of sequence b -> [B, heads, head_dim] of `dtype` (q's without it).  scale: 1 /
     sqrt(head_dim) without it."""
-    stride, heads, scale, out = _queries(q, cache, scale, out, dtype)
-    b = _batch(cache, q.shape[0], tables, lens, None, (q, out))
+    T, stride, heads, scale, out = _queries(q, cache, scale, out, dtype)
+    b = _batch(cache, T, tables, lens, None, (q, out))
     ref = C.byref(b)
-    key = (b.B, heads, b.table_pages)
+    key = (T, heads, tables.shape[1])
     nbytes = cache._workspace.get(key)
     if nbytes is None:
         if len(cache._workspace) >= 4096:
@@ -187,8 +204,8 @@ def decode(q, cache, tables, lens, *, scale=None, out=None, dtype=None):
 def prompt(q, cache, tables, lens, cu, *, scale=None, out=None, dtype=None):
     """Causal attention of packed rows: row i of sequence b's n sees its positions up to lens[b] - n + i, cached
     ones included.  q [T, heads, head_dim] -> [T, heads, head_dim]; rows outside cu's are left as they are."""
-    stride, heads, scale, out = _queries(q, cache, scale, out, dtype)
-    b = _batch(cache, q.shape[0], tables, lens, cu, (q, out))
+    T, stride, heads, scale, out = _queries(q, cache, scale, out, dtype)
+    b = _batch(cache, T, tables, lens, cu, (q, out))
     rc = _prompt(cache._ref, C.byref(b), q.data_ptr(), stride, heads, scale, _TYPES[out.dtype], out.data_ptr(),
                  _raw_stream(cache._dev))
     if rc:
