@@ -40,7 +40,7 @@ __device__ const u32x4 kv_nothing[KV_BLOCK * 256 * 2 / 16] = {};
  * A masked place's value may be infinite or NaN, and its weight 0 does not silence it: in stages with a border the values
  * that are not finite leave LDS, and rows that see them get them at the end, value by value (rare). */
 template <class T, int HD, int SG, int TP>
-__global__ __launch_bounds__(256, HD > 128 || (SG == 4 && HD > 64) ? 1 : 2) void k_kv_prompt(PromptArgs a) {
+__global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) ? 1 : 2) void k_kv_prompt(PromptArgs a) {
     typedef typename KvType<T>::x8 x8;
     constexpr int RG = 4 / SG, ROWS = 32 * RG;
     constexpr int KS = HD / 16, DT = HD / 32;
@@ -348,7 +348,7 @@ template <class T, int HD, int SG, int TP> void launch_sg(const PromptArgs &a, i
 }
 template <class T, int HD> void launch(const PromptArgs &a, int64_t B, hipStream_t s) {
     const int sg = split_of(a.c.rows, B, a.G, a.c.heads, HD);
-    if (sg == 1) return launch_sg<T, HD, 1, 2>(a, B, s);
+    if (sg == 1) return launch_sg<T, HD, 1, HD <= 128 ? 2 : 1>(a, B, s);
     if constexpr (HD <= 128)     /* wider, four stages twice are more than the LDS */
         if (sg == 4) return launch_sg<T, HD, 4, 1>(a, B, s);
     launch_sg<T, HD, 2, HD <= 64 ? 2 : 1>(a, B, s);
