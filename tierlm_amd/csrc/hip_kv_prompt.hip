@@ -332,14 +332,15 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
         }
 }
 
-/* Rows of a group: 128 where that many groups fill the chip twice (two fit a compute unit); else 64, the positions dealt to
- * two waves, or 32 and four, while all groups still run at once (one a unit, two up to 64 wide): a stage takes a lone wave
- * about a microsecond whatever its rows.  us with 128 / 64 / 32 rows, 32 heads on 4 of 128: 4096 tokens 156 / 178 / 395,
- * 2048 59 / 58 / 129, 1024 30 / 24 / 48, 512 19 / 15 / 21, 256 13.3 / 10.6 / 11.2; 128 behind 8000 176 / 117 / 80; 8 heads on 2
- * of 64, 2048 tokens: 39 / 26 / 22. */
+/* Rows of a group: 128 where that many groups fill the chip (two fit a compute unit; past 128 wide, where of those with 64
+ * rows only one does, from half as many on); else 64, the positions dealt to two waves, or 32 and four, while all groups
+ * still run at once: a stage takes a lone wave about a microsecond whatever its rows.  us with 128 / 64 / 32 rows, 32 heads on
+ * 4 of 128: 4096 tokens 156 / 178 / 395, 2048 59 / 58 / 129, 1024 30 / 24 / 48, 512 19 / 15 / 21, 256 13.3 / 10.6 / 11.2; 128
+ * behind 8000 176 / 117 / 80; 8 heads on 2 of 64, 2048 tokens 39 / 26 / 22; 16 on 2 of 256, 4096 tokens 219 / 259, 2048
+ * 104 / 77. */
 int split_of(int64_t rows, int64_t B, int group, int kv_heads, int hd) {
     const int64_t groups = kv_prompt_most(rows, B, group, 128) * kv_heads;
-    return groups > 512 ? 1 : groups > (hd <= 64 ? 128 : 64) ? 2 : 4;
+    return groups > (hd <= 128 ? 512 : 256) ? 1 : groups > (hd <= 64 ? 128 : 64) ? 2 : 4;
 }
 
 template <class T, int HD, int SG, int TP> void launch_sg(const PromptArgs &a, int64_t B, hipStream_t s) {
