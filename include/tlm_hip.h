@@ -686,13 +686,14 @@ typedef struct {
  * and key head y becomes y r w, r = 1 / sqrt(mean(y^2) + eps), where its norm (f32 [head_dim]) is given; with inv_freq
  * (double [head_dim / 2]) the pair (y_j, y_{j + head_dim / 2}) is turned by position * inv_freq[j] and multiplied with
  * rope_scale (the reference's rope(), src/lib/tlm_model.c:721-728); angles are doubles, the rest f32.  Keys and
- * values go to their pages, rounded once; queries to q [rows][heads][head_dim] in the cache's type (16-byte aligned). */
+ * values go to their pages, rounded once; queries to q [rows][heads][head_dim] in the cache's type (16-byte aligned,
+ * overlapping no input).  Two rows of a batch never have one place: no page is appended to by two sequences. */
 int    tlm_hip_kv_append(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int dt, const void *qkv, int64_t qkv_stride,
                          int heads, const float *q_norm, const float *k_norm, float eps, const double *inv_freq,
                          float rope_scale, void *q, void *stream);
 /* Attention of one row a sequence (b->cu NULL): out[b][h] = sum_j p_j v_j, p = softmax of scale q . k_j over the positions
  * j < lens[b], head h with key head h / (heads / kv_heads).  q in the cache's type (row b at q + b q_stride, heads
- * side by side), out [B][heads][head_dim] of out_dt (F32, F16 or BF16); scale positive.  Sums, maxima and the softmax are
+ * side by side), out [B][heads][head_dim] of out_dt (F32, F16 or BF16), overlapping no input; scale positive.  Sums, maxima and the softmax are
  * f32, its weights enter the second product rounded to the cache's type.  Sequences are split over their length as the
  * batch's total asks, in the same way in every call with equal lengths: a call repeats its bits.  workspace:
  * tlm_hip_kv_decode_workspace_bytes bytes (0: none, by the sizes alone), 256-byte aligned, nothing in it kept or zeroed;

@@ -63,6 +63,19 @@ def test_against_the_quantiser(hip, hdt, xdt, T, n):
     assert same(codes, want[0]) and same(scale, want[1])
 
 
+@pytest.mark.parametrize("n", [700, 20000])
+def test_sum_not_stored(hip, n):
+    """The C call without a place for the sum: h stays, the codes are those of the sum."""
+    from tierlm_amd import lib
+    h, x, w = inputs(3, n, F16, BF16, seed=n)
+    s, y = steps(h, x, w)
+    want, keep = fp8.quantize(y), h.clone()
+    codes, scale = torch.empty_like(want[0]), torch.empty_like(want[1])
+    rc = lib.tlm_hip_fp8_add_rmsnorm(1, h.data_ptr(), n, 2, x.data_ptr(), n, w.data_ptr(), EPS, n, 3, None, 0,
+                                     codes.data_ptr(), scale.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and same(h, keep) and same(codes, want[0]) and same(scale, want[1])
+
+
 @pytest.mark.parametrize("n", [100, 2048, 20000])
 def test_definition(hip, n):
     """64 bits: r, s r and y are off by at most 2^-24 each of themselves (three roundings), the code by half its step."""

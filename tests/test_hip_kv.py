@@ -62,6 +62,13 @@ def test_decode_many_sequences(hip):
         check_decode(Batch(F16, 4, 2, 32, 16, [1] * 300, lens, seed=3, width=width))
 
 
+@pytest.mark.parametrize("B,heads,kv_heads,hd", [(70, 36, 2, 96), (300, 64, 4, 64), (64, 40, 8, 128), (40, 60, 3, 224)])
+def test_decode_split_many_heads(hip, B, heads, kv_heads, hd):
+    """Sequences of several shares, their heads joined several a group."""
+    lens = [(997 * i) % 1400 if i % 9 else 1 + i for i in range(B)]
+    check_decode(Batch(BF16, heads, kv_heads, hd, 32, [1] * B, lens, seed=B, width=50))
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("scale", [1e-6, 0.25, 3.0])
 def test_decode_scale_and_type(hip, dtype, scale):
@@ -103,8 +110,9 @@ def test_prompt_pages(hip, page):
     check_prompt(Batch(BF16, 8, 2, 128, page, [300, 77], [1300, 77], seed=page))
 
 
-def test_prompt_many_sequences(hip):
-    new = [(7 * i) % 13 for i in range(200)]
+@pytest.mark.parametrize("B", [64, 65, 200, 257, 700])
+def test_prompt_many_sequences(hip, B):
+    new = [(7 * i) % 13 for i in range(B)]
     check_prompt(Batch(F16, 4, 2, 32, 16, new, [n + i % 40 for i, n in enumerate(new)], seed=5))
 
 

@@ -114,6 +114,27 @@ def test_parts(hip, norms, rope):
     check(BF16, BF16, 8, 2, 128, 64, [33, 2], [40, 2], norms=norms, rope=rope, rope_scale=1.0 if not rope else 1.3)
 
 
+@pytest.mark.parametrize("which", ["q", "k"])
+def test_one_norm(hip, which):
+    """The other heads pass as they are."""
+    b = Batch(F16, 4, 2, 64, 16, [20], [30], seed=11)
+    g = gen(12)
+    x, w = torch.randn(20, 8 * 64, generator=g, device="cuda"), 1 + 0.1 * torch.randn(64, generator=g, device="cuda")
+    qn, kn = (w, None) if which == "q" else (None, w)
+    q = kv.append(b.cache, x, 4, b.tables, b.lens, b.cu, q_norm=qn, k_norm=kn)
+    wq, wk, _, tol = reference(x, 4, 2, 64, torch.arange(10, 30, device="cuda"), qn, kn, 1e-6, None, 1.0)
+    k = b.cache.keys(b.tables_list[0])[:, 10:30].transpose(0, 1)
+    for got, want, t in ((q, wq, tol[:, :4]), (k, wk, tol[:, 4:])):
+        assert ((got.double() - want).abs() <= t + (want.abs() + t) * 2.0 ** -11 + 2.0 ** -25).all()
+    plain = k if which == "q" else q
+    assert torch.equal(plain, (x[:, 256:384] if which == "q" else x[:, :256]).reshape(20, -1, 64).to(F16))
+
+
+@pytest.mark.parametrize("B", [3, 64, 65, 300])
+def test_many_sequences(hip, B):
+    check(F16, F32, 4, 2, 32, 16, [(5 * i) % 7 for i in range(B)], [(5 * i) % 7 + (i * 3) % 20 for i in range(B)], seed=B)
+
+
 def test_a_row_a_sequence(hip):
     check(BF16, F32, 32, 4, 128, 64, [1] * 70, [1 + 13 * i for i in range(70)], cu=False)
 

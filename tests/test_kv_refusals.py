@@ -35,7 +35,7 @@ BAD = [
     (EINVAL, dict(n_pages=0), {}, {}), (EINVAL, dict(n_pages=1 << 31), {}, {}), (EINVAL, dict(k=None), {}, {}),
     (EINVAL, dict(v=None), {}, {}), (EINVAL, dict(k=P + 8), {}, {}), (EINVAL, dict(v=P + 2), {}, {}),
     (EINVAL, {}, dict(B=-1), {}), (EINVAL, {}, dict(rows=-1), {}), (EINVAL, {}, dict(rows=4), {}),
-    (ERANGE, {}, dict(B=(1 << 20) + 1, rows=(1 << 20) + 1), {}), (ERANGE, {}, dict(rows=1 << 28, cu=P), {}),
+    (ERANGE, {}, dict(B=(1 << 20) + 1, rows=(1 << 20) + 1), {}), (ERANGE, {}, dict(rows=1 << 28, cu=P), {}), (ERANGE, {}, dict(rows=1 << 62, cu=P), {}),
     (EINVAL, {}, dict(table_pages=0), {}), (EINVAL, {}, dict(table_pages=(1 << 26) + 1, table_stride=1 << 27), {}),
     (EINVAL, {}, dict(table_stride=3), {}), (EINVAL, {}, dict(lens=None), {}), (EINVAL, {}, dict(tables=None), {}),
     (EINVAL, {}, dict(lens=P + 2), {}), (EINVAL, {}, dict(tables=P + 1), {}),

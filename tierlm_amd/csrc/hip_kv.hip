@@ -57,10 +57,12 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
     __shared__ float s_cs[KV_BLOCK][HD / 2 + 4], s_sn[KV_BLOCK][HD / 2 + 4];
     const KvView &c = a.c;
     const int tid = threadIdx.x;
-    const KvItem it = kv_find(c.B, (int)blockIdx.x, [&](int b) {
-        const KvRows r = kv_rows(c, b);
-        return (int)kv_append_items(r.n, kv_len(c, b));
-    });
+    KvItem it = {(int)blockIdx.x, 0, 1, 0};     /* a row a sequence: a block each */
+    if (c.cu)
+        it = kv_find(c.B, (int)blockIdx.x, [&](int b) {
+            const KvRows r = kv_rows(c, b);
+            return (int)kv_append_items(r.n, kv_len(c, b));
+        });
     if (it.b < 0) return;
     const int kvh = blockIdx.y, G = a.G, H = G * c.heads;
     const KvRows r = kv_rows(c, it.b);
@@ -263,6 +265,7 @@ struct DecodeBatch {
                 sum = kv_units(mine);
             }
         } else {
+#pragma unroll 4
             for (int b = lane; b < c.B; b += 64) sum += kv_units(decode_len(c, b));
         }
         upto = kv_scan(sum);
@@ -284,6 +287,7 @@ struct DecodeBatch {
     __device__ __forceinline__ int before(int b) const {
         if (few()) return __builtin_amdgcn_readlane(upto, b) - kv_units(len(b));
         int sum = 0;
+#pragma unroll 4
         for (int i = wave_lane(); i < b; i += 64) sum += kv_units(decode_len(c, i));
         return __builtin_amdgcn_readlane(kv_scan(sum), 63);
     }
@@ -638,7 +642,7 @@ int kv_check(const char *who, const tlm_hip_kv_cache *c, const tlm_hip_kv_batch 
         return tlmh_seterr(TLM_HIP_EINVAL, "%s: %lld pages", who, (long long)c->n_pages);
     if (b->B < 0 || b->rows < 0 || (!b->cu && b->rows != b->B))
         return tlmh_seterr(TLM_HIP_EINVAL, "%s: %lld rows of %lld sequences", who, (long long)b->rows, (long long)b->B);
-    if (b->B > (1 << 20) || b->rows * heads > ((int64_t)1 << 30))
+    if (b->B > (1 << 20) || b->rows > ((int64_t)1 << 30) || b->rows * heads > ((int64_t)1 << 30))
         return tlmh_seterr(TLM_HIP_ERANGE, "%s: %lld rows of %lld sequences are too many for one launch", who,
                            (long long)b->rows, (long long)b->B);
     if (b->table_pages < 1 || (int64_t)b->table_pages * c->page > (1 << 30))
@@ -676,7 +680,7 @@ int tlm_hip_kv_append(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int 
         return tlmh_seterr(TLM_HIP_EINVAL, "kv_append: qkv must have its type's alignment, q 16, the norms 4, inv_freq 8 "
                            "bytes");
     if (int rc = tlmh_refuse_failed(FAILED_KV, "kv_append")) return rc;
-    const int64_t items = kv_append_most(b->rows, b->B);
+    const int64_t items = b->cu ? kv_append_most(b->rows, b->B) : b->B;
     if (items * c->kv_heads > (1 << 23))
         return tlmh_seterr(TLM_HIP_ERANGE, "kv_append: %lld rows of %lld sequences are too many for one launch",
                            (long long)b->rows, (long long)b->B);

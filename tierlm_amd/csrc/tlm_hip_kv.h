@@ -67,7 +67,7 @@ TLM_HD int64_t kv_floor16(int64_t p) { return p >= 0 ? p / 16 : -((15 - p) / 16)
 TLM_HD int64_t kv_append_items(int64_t n, int64_t len) {
     return n > 0 ? kv_floor16(len - 1) - kv_floor16(len - n) + 1 : 0;
 }
-/* as many items as any lengths of B sequences with `rows` rows give */
+/* as many items as any lengths of B sequences with `rows` rows give (without cu a sequence is an item) */
 TLM_HD int64_t kv_append_most(int64_t rows, int64_t B) {
     const int64_t used = rows < B ? rows : B;   /* sequences that can have a row; n rows touch at most (n + 14) / 16 + 1 */
     return (rows + 14 * used) / 16 + used;
@@ -163,19 +163,34 @@ struct KvItem {
 template <class Count> __device__ __forceinline__ KvItem kv_find(int B, int w, const Count &count) {
     const int lane = wave_lane();
     int before = 0;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-        const int mine = b0 + lane < B ? count(b0 + lane) : 0, upto = kv_scan(mine);
+    auto scan = [&](int b0, int mine, KvItem &it) {
+        const int upto = kv_scan(mine);
         const uint64_t in = __ballot(before + upto > w);
         if (in) {
             const int l = __builtin_ctzll(in);
             const int n = __builtin_amdgcn_readlane(mine, l), u = __builtin_amdgcn_readlane(upto, l);
             const int i = w - (before + u - n);
             /* row bounds that overlap can add up past an int */
-            return {i >= 0 && i < n ? b0 + l : -1, i, n, before + u - n};
+            it = {i >= 0 && i < n ? b0 + l : -1, i, n, before + u - n};
+            return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
+        return false;
+    };
+    KvItem it = {-1, 0, 0, 0};
+    if (B <= 64) {
+        scan(0, lane < B ? count(lane) : 0, it);
+        return it;
     }
-    return {-1, 0, 0, before};
+    for (int b0 = 0; b0 < B; b0 += 256) {     /* four rounds' reads at once */
+        int mine[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) mine[u] = b0 + 64 * u + lane < B ? count(b0 + 64 * u + lane) : 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (scan(b0 + 64 * u, mine[u], it)) return it;
+    }
+    return it;
 }
 #endif
 
