@@ -18,7 +18,7 @@ class Batch:
     """Sequences of new[b] rows and lens[b] positions with pages dealt at random; the cache's content random
     everywhere, NaN where no sequence has a position."""
 
-    def __init__(self, dtype, heads, kv_heads, hd, page, new, lens, seed=0, spare=1, width=None):
+    def __init__(self, dtype, heads, kv_heads, hd, page, new, lens, seed=0, spare=1, width=None, last=False):
         g = gen(seed)
         self.heads, self.new, self.lens_list = heads, list(new), list(lens)
         B = len(lens)
@@ -26,6 +26,8 @@ class Batch:
         n_pages = sum(need) + spare
         self.cache = kv.Cache(n_pages, kv_heads, hd, page=page, dtype=dtype)
         perm = torch.randperm(n_pages, generator=torch.Generator().manual_seed(seed + 1)).tolist()
+        if last:                     # the cache's last pages
+            perm = list(range(n_pages))
         self.tables_list = [[perm.pop() for _ in range(m)] for m in need]
         width = width or max(max(need), 1)
         t = torch.full((B, width), -1, dtype=torch.int32)

@@ -320,3 +320,62 @@ def test_streams_and_graphs(hip):
         for o, n in zip(outs, lens):
             assert torch.equal(o, kv.decode(b.q, b.cache, b.tables, n)), i
         assert torch.equal(y, want_p)
+
+
+def test_far_pages(hip):
+    """Pages past 2^31 elements and 2^32 bytes of a cache; decode whole and in shares, prompt."""
+    lens = [300, 70]
+    for width in (None, 40):
+        b = Batch(BF16, 16, 8, 256, 64, [1, 1], lens, seed=20, spare=20000, width=width, last=True)
+        assert min(b.tables_list[0]) * b.cache.k[0].numel() > 2 ** 31
+        check_decode(b)
+        del b
+    b = Batch(BF16, 16, 8, 256, 64, [50, 70], lens, seed=21, spare=20000, last=True)
+    check_prompt(b)
+    # and appended there: what a second cache of few pages gets
+    x = torch.randn(120, 32 * 256, generator=gen(22), device="cuda")
+    q = kv.append(b.cache, x, 16, b.tables, b.lens, b.cu)
+    c = Batch(BF16, 16, 8, 256, 64, [50, 70], lens, seed=21)
+    assert torch.equal(q, kv.append(c.cache, x, 16, c.tables, c.lens, c.cu))
+    for i, n in enumerate(lens):
+        for a in ("keys", "values"):
+            assert torch.equal(getattr(b.cache, a)(b.tables_list[i])[:, :n], getattr(c.cache, a)(c.tables_list[i])[:, :n])
+
+
+def test_rows_past_32_bits(hip):
+    """A batch whose queries, rows and results pass 2^31 elements: 1400 sequences of 100 rows of 64 heads of 256."""
+    B, n, H, hd = 1400, 100, 64, 256
+    cache = kv.Cache(B * 7, 1, hd, page=16, dtype=BF16)
+    tables = torch.arange(B * 7, dtype=torch.int32, device="cuda").view(B, 7)
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    cu = (torch.arange(B + 1, device="cuda") * n).to(torch.int32)
+    x = torch.randn(B * n, (H + 2) * hd, generator=gen(23), device="cuda", dtype=BF16)
+    q = kv.append(cache, x, H, tables, lens, cu)
+    assert torch.equal(q.view(B * n, -1), x[:, :H * hd])
+    y = kv.prompt(q, cache, tables, lens, cu)
+    last = torch.empty(B, H, hd, dtype=BF16, device="cuda")
+    kv.decode(q[n - 1::n], cache, tables, lens, out=last)
+    for b in (0, 700, B - 1):
+        k, v = cache.keys(tables[b].tolist())[:, :n].transpose(0, 1), cache.values(tables[b].tolist())[:, :n].transpose(0, 1)
+        assert torch.equal(k.reshape(n, hd), x[b * n:(b + 1) * n, H * hd:(H + 1) * hd])
+        want, tol = reference(q[b * n:(b + 1) * n], k, v, 1 / 16, 0)
+        close(y[b * n:(b + 1) * n], want, tol)
+        close(last[b:b + 1], want[-1:], tol[-1:])
+
+
+def test_two_streams_at_once(hip):
+    """Decodes of one cache on two streams at a time, each with a workspace of its own."""
+    b = Batch(BF16, 32, 4, 128, 64, [1] * 5, [3000, 40, 700, 2, 1500], seed=24, width=60)
+    c = Batch(BF16, 32, 4, 128, 64, [1] * 5, [3000, 40, 700, 2, 1500], seed=24, width=60)
+    lens2 = torch.tensor([100, 40, 699, 0, 1499], dtype=torch.int32, device="cuda")
+    want = [kv.decode(c.q, c.cache, c.tables, n) for n in (c.lens, lens2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for s, n, o in zip(streams, (b.lens, lens2), outs):
+            with torch.cuda.stream(s):
+                o.append(kv.decode(b.q, b.cache, b.tables, n))
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(w, y) for y in o)
