@@ -45,7 +45,8 @@ def same(a, b):
 
 @pytest.mark.parametrize("hdt", [F32, F16, BF16])
 @pytest.mark.parametrize("xdt", [F32, F16, BF16])
-@pytest.mark.parametrize("T,n", [(1, 1), (3, 127), (2, 512), (5, 513), (7, 1111), (1, 2048), (3, 2049), (2, 5000), (2, 8192),
+@pytest.mark.parametrize("T,n", [(1, 1), (3, 127), (2, 512), (5, 513), (7, 1111), (1, 2048), (3, 1024), (3, 1025), (3, 2049), (2, 4096), (2, 4097), (2, 5000), (2, 6144), (3, 6145),
+                                 (2, 8192), (2, 8193),
                                  (3, 9001), (1, 16384), (2, 16385), (1, 40000)])
 def test_against_the_quantiser(hip, hdt, xdt, T, n):
     h, x, w = inputs(T, n, hdt, xdt, seed=n)

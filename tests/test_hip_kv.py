@@ -58,7 +58,7 @@ def test_decode_split(hip, hd, heads, kv_heads, lens):
 def test_decode_many_sequences(hip):
     """More sequences than a wave scans at once, split and not."""
     lens = [(37 * i) % 191 for i in range(300)]
-    for width in (12, 200):
+    for width in (12, 40, 64, 65, 200):
         check_decode(Batch(F16, 4, 2, 32, 16, [1] * 300, lens, seed=3, width=width))
 
 

@@ -9,11 +9,13 @@ bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
 
 /* ---- append ------------------------------------------------------------------
- * A group per block of 16 positions and key head: its up to 16 new rows of that head's G queries, key and value.  16 lanes
- * hold a vector: lane s the pairs j = M s .. M s + M - 1 and their partners at hd / 2 + j (M = hd / 32), so the norm is one
- * 16-lane sum and the rotation stays in the lane.  Values are
- * turned over in registers (8 rows of one value to 16 bytes): the cache's block is written as whole pieces.
- * Bound by memory; what a decode step's few rows take is the launch. */
+ * A group per block of 16 positions and key head: its up to 16 new rows of that head's G queries, key and value.  16
+ * lanes hold a vector: lane s the pairs j = M s .. M s + M - 1 and their partners at hd / 2 + j (M = hd / 32), so the norm is
+ * one 16-lane sum and the rotation stays in the lane.  Vectors go in the order of memory, 16 heads of a row at a time (a
+ * row a lane group: 87 us for what takes 75), and values are turned over in registers (8 rows of one value to 16 bytes),
+ * so the cache's block is written as whole pieces.
+ * 8192 rows of 64 + 8 heads of 128, bf16: 75 us, 4.0 TB/s (63 us from an idle device); 61 rows of a decode step 5.5 us, a chain
+ * of four reads and a launch. */
 struct AppendArgs {
     KvView c;
     const void *x;
@@ -219,13 +221,15 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
  * out = sum_j p_j v_j / sum_j p_j, p_j = 2^(scale log2(e) q . k_j - m), one pass over the cache with the running maximum m.
  * A group takes a part of a sequence's positions for one key head and up to 16 NC of its queries; its NW waves take tiles
  * of 32 positions in turn, straight from memory into the matrix cores' operands (no LDS on the way), the next tile's
- * loads in flight, and merge their sums through LDS at the end.  The bytes of the cache bound it.
+ * loads in flight, and merge their sums through LDS at the end.  The bytes of the cache bound it: 64 sequences of up to 8192,
+ * 64 heads on 4 of 128, in 102 us (5.4 TB/s, some of it from the memory-side cache; a copy 5.14), one of 131071, 32 on 4, in 48.
  *
  * Shares: the lengths are the device's, so every group works its share out for itself.  All sequences' positions lie end
  * to end in units of 128, and W workers a key head take equal parts of that line, across the sequences' ends: however
  * uneven the lengths are, the groups that fill the chip once end together.  A sequence inside one share is written at
  * once; the parts of the others go to the workspace, and k_kv_join adds a sequence's in order.  Where the tables are short
- * (DECODE_WHOLE) each sequence is a group's and one launch does. */
+ * (DECODE_WHOLE) each sequence is a group's and one launch does.  With a fixed number of splits a sequence the 64 ragged ones
+ * took 129 us instead of 113 with their join. */
 struct DecodeArgs {
     KvView c;
     const void *q, *k, *v;
@@ -304,197 +308,197 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
     const int worker = blockIdx.x, kvh = blockIdx.y;
     const int col0 = blockIdx.z * NC * 16, ncol = a.G - col0 < NC * 16 ? a.G - col0 : NC * 16;
     auto part = [&](int b, int len, int first, int left) {
-    const int32_t *table = c.tables + b * c.table_stride;
-    const int units = kv_units(len), take = units - first < left ? units - first : left;
-    const int begin = first * KV_UNIT, stop = len - begin < take * KV_UNIT ? len : begin + take * KV_UNIT;
-    const int tiles = (stop - begin + 31) / 32;     /* 0: an empty sequence */
+        const int32_t *table = c.tables + b * c.table_stride;
+        const int units = kv_units(len), take = units - first < left ? units - first : left;
+        const int begin = first * KV_UNIT, stop = len - begin < take * KV_UNIT ? len : begin + take * KV_UNIT;
+        const int tiles = (stop - begin + 31) / 32;     /* 0: an empty sequence */
 
-    /* queries: column col, values 32 ks + 8 g .. + 7 */
-    x8 qf[NC][KS];
+        /* queries: column col, values 32 ks + 8 g .. + 7 */
+        x8 qf[NC][KS];
 #pragma unroll
-    for (int n = 0; n < NC; n++)
+        for (int n = 0; n < NC; n++)
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const int h = n * 16 + col;
-            u32x4 v = {0, 0, 0, 0};
-            if (h < ncol)
-                v = kv_load8((const T *)a.q + b * a.qstride + (int64_t)(kvh * a.G + col0 + h) * HD + 32 * ks + 8 * g);
-            qf[n][ks] = kv_bits<x8>(v);
-        }
+            for (int ks = 0; ks < KS; ks++) {
+                const int h = n * 16 + col;
+                u32x4 v = {0, 0, 0, 0};
+                if (h < ncol)
+                    v = kv_load8((const T *)a.q + b * a.qstride + (int64_t)(kvh * a.G + col0 + h) * HD + 32 * ks + 8 * g);
+                qf[n][ks] = kv_bits<x8>(v);
+            }
 
-    /* A tile's two blocks: row i of key tile t is position 8 (i / 4) + 4 t + i % 4 (block i / 8), so that a lane's scores are
-     * the positions 8 g .. 8 g + 7 (block g / 2), which are its operand of the second product. */
-    const int krow = 8 * (col >> 2) + (col & 3);
-    const int koff = kv_key_at(krow & 15, 0) + (g >> 1) * 256 + (g & 1) * 8;   /* + 64 t (four positions) + 512 ks */
-    const int voff = kv_value_at(0, col) + (g & 1) * 8;                        /* + 256 dt */
-    struct Tile {
-        u32x4 k[2][KS], v[DT];
-        int ok;          /* bit i: block i is a page's */
-    };
-    /* the wave's page numbers, 32 of its tiles at a time: lane 2 i + j holds block j of its i-th tile */
-    int pages = 0;
-    auto names = [&](int i0) {
-        const int blk = begin / KV_BLOCK + 2 * (wave + NW * (i0 + (lane >> 1))) + (lane & 1);
-        const int lastb = (stop - 1) / KV_BLOCK;
-        pages = blk <= lastb ? table[blk >> c.sh] : -1;
-    };
-    auto load = [&](Tile &t, int i) {
-        const int b0 = begin / KV_BLOCK + 2 * (wave + NW * i);
-        int64_t o0 = kv_block(c, __builtin_amdgcn_readlane(pages, 2 * (i & 31)), b0, kvh);
-        int64_t o1 = kv_block(c, __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1), b0 + 1, kvh);
-        t.ok = (o0 >= 0 ? 1 : 0) | (o1 >= 0 ? 2 : 0);
-        o0 = o0 < 0 ? 0 : o0;    /* block 0 is inside the cache; what it holds is masked */
-        o1 = o1 < 0 ? 0 : o1;
-        const GAS T *k = (const GAS T *)a.k + ((col & 8) ? o1 : o0) + koff;
-        const GAS T *v = (const GAS T *)a.v + (g >= 2 ? o1 : o0) + voff;
+        /* A tile's two blocks: row i of key tile t is position 8 (i / 4) + 4 t + i % 4 (block i / 8), so that a lane's scores are
+         * the positions 8 g .. 8 g + 7 (block g / 2), which are its operand of the second product. */
+        const int krow = 8 * (col >> 2) + (col & 3);
+        const int koff = kv_key_at(krow & 15, 0) + (g >> 1) * 256 + (g & 1) * 8;   /* + 64 t (four positions) + 512 ks */
+        const int voff = kv_value_at(0, col) + (g & 1) * 8;                        /* + 256 dt */
+        struct Tile {
+            u32x4 k[2][KS], v[DT];
+            int ok;          /* bit i: block i is a page's */
+        };
+        /* the wave's page numbers, 32 of its tiles at a time: lane 2 i + j holds block j of its i-th tile */
+        int pages = 0;
+        auto names = [&](int i0) {
+            const int blk = begin / KV_BLOCK + 2 * (wave + NW * (i0 + (lane >> 1))) + (lane & 1);
+            const int lastb = (stop - 1) / KV_BLOCK;
+            pages = blk <= lastb ? table[blk >> c.sh] : -1;
+        };
+        auto load = [&](Tile &t, int i) {
+            const int b0 = begin / KV_BLOCK + 2 * (wave + NW * i);
+            int64_t o0 = kv_block(c, __builtin_amdgcn_readlane(pages, 2 * (i & 31)), b0, kvh);
+            int64_t o1 = kv_block(c, __builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1), b0 + 1, kvh);
+            t.ok = (o0 >= 0 ? 1 : 0) | (o1 >= 0 ? 2 : 0);
+            o0 = o0 < 0 ? 0 : o0;    /* block 0 is inside the cache; what it holds is masked */
+            o1 = o1 < 0 ? 0 : o1;
+            const GAS T *k = (const GAS T *)a.k + ((col & 8) ? o1 : o0) + koff;
+            const GAS T *v = (const GAS T *)a.v + (g >= 2 ? o1 : o0) + voff;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            t.k[0][ks] = *(const GAS u32x4 *)(k + 512 * ks);
-            t.k[1][ks] = *(const GAS u32x4 *)(k + 512 * ks + 64);
-        }
+            for (int ks = 0; ks < KS; ks++) {
+                t.k[0][ks] = *(const GAS u32x4 *)(k + 512 * ks);
+                t.k[1][ks] = *(const GAS u32x4 *)(k + 512 * ks + 64);
+            }
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) t.v[dt] = *(const GAS u32x4 *)(v + 256 * dt);
-    };
+            for (int dt = 0; dt < DT; dt++) t.v[dt] = *(const GAS u32x4 *)(v + 256 * dt);
+        };
 
-    f32x4 o[NC][DT];
-    float m[NC], l[NC];
-#pragma unroll
-    for (int n = 0; n < NC; n++) {
-        m[n] = -INFINITY;
-        l[n] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) o[n][dt] = f32x4{0, 0, 0, 0};
-    }
-    auto compute = [&](Tile &t, int i) {
-        const int p0 = begin + 32 * (wave + NW * i) + 8 * g;     /* the lane's first position */
-        const bool whole = p0 - 8 * g + 32 <= stop && t.ok == 3;
-        const int left = ((t.ok >> (g >> 1)) & 1) ? stop - p0 : 0;
-        if (!whole) {    /* what a masked place holds may be anything, and 0 times it not 0 */
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                for (int w = 0; w < 4; w++)
-                    t.v[dt][w] &= (2 * w < left ? 0xFFFFu : 0u) | (2 * w + 1 < left ? 0xFFFF0000u : 0u);
-        }
+        f32x4 o[NC][DT];
+        float m[NC], l[NC];
 #pragma unroll
         for (int n = 0; n < NC; n++) {
-            f32x4 s[2];
+            m[n] = -INFINITY;
+            l[n] = 0.0f;
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                s[u] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++) s[u] = KvType<T>::mma(kv_bits<x8>(t.k[u][ks]), qf[n][ks], s[u]);
-            }
-            float z[8];
-            float top = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                z[j] = s[j >> 2][j & 3] * a.scale2;
-                if (!whole && j >= left) z[j] = -INFINITY;
-                top = fmaxf(top, z[j]);
-            }
-            if (__any(top > m[n] + KV_SLACK)) {
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                /* each column by its own scores: another's do not show in its bits */
-                const float to = top > m[n] + KV_SLACK ? top : m[n], f = to == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - to);
-                m[n] = to;
-                l[n] *= f;
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++) o[n][dt] *= f;
-            }
-            /* before any score is above -infinity the maximum is taken as 0 */
-            const float base = (m[n] == -INFINITY ? 0.0f : m[n]) - KvType<T>::SHIFT;
-            x8 p;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float e = __builtin_amdgcn_exp2f(z[j] - base);
-                l[n] += e;
-                p[j] = (T)e;   /* 8 (bf16) or 11 bits of a weight in [0, 1]: as the values it is multiplied with have */
-            }
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) o[n][dt] = KvType<T>::mma(kv_bits<x8>(t.v[dt]), p, o[n][dt]);
+            for (int dt = 0; dt < DT; dt++) o[n][dt] = f32x4{0, 0, 0, 0};
         }
-    };
-    const int mine = (tiles - wave + NW - 1) / NW;      /* this wave's tiles */
-    if (mine > 0) {
-        Tile ta, tb;
-        names(0);
-        load(ta, 0);
-        for (int i = 0; i < mine; i += 2) {
-            if (i + 1 < mine) load(tb, i + 1);
-            compute(ta, i);
-            if (i + 2 < mine) {
-                if (((i + 2) & 31) == 0) names(i + 2);
-                load(ta, i + 2);
-            }
-            if (i + 1 < mine) compute(tb, i + 1);
-        }
-    }
-    /* the lanes of a column hold different positions' weights */
-#pragma unroll
-    for (int n = 0; n < NC; n++) {
-        l[n] += __shfl_xor(l[n], 16, 64);
-        l[n] += __shfl_xor(l[n], 32, 64);
-    }
-    /* merge the waves, half of them at a time, always in the same order */
-#pragma unroll
-    for (int half = NW / 2; half >= 1; half >>= 1) {
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-            for (int n = 0; n < NC; n++) {
+        auto compute = [&](Tile &t, int i) {
+            const int p0 = begin + 32 * (wave + NW * i) + 8 * g;     /* the lane's first position */
+            const bool whole = p0 - 8 * g + 32 <= stop && t.ok == 3;
+            const int left = ((t.ok >> (g >> 1)) & 1) ? stop - p0 : 0;
+            if (!whole) {    /* what a masked place holds may be anything, and 0 times it not 0 */
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++)
-                    *(f32x4 *)&s_o[wave - half][(n * 16 + col) * LD + 16 * dt + 4 * g] = o[n][dt];
-                if (g == 0) {
-                    s_ml[wave - half][(n * 16 + col) * 2] = m[n];
-                    s_ml[wave - half][(n * 16 + col) * 2 + 1] = l[n];
-                }
+#pragma unroll
+                    for (int w = 0; w < 4; w++)
+                        t.v[dt][w] &= (2 * w < left ? 0xFFFFu : 0u) | (2 * w + 1 < left ? 0xFFFF0000u : 0u);
             }
-        }
-        __syncthreads();
-        if (wave < half) {
 #pragma unroll
             for (int n = 0; n < NC; n++) {
-                const float om = s_ml[wave][(n * 16 + col) * 2], ol = s_ml[wave][(n * 16 + col) * 2 + 1];
-                const float to = fmaxf(m[n], om), base = to == -INFINITY ? 0.0f : to;
-                const float fm = __builtin_amdgcn_exp2f(m[n] - base), fo = __builtin_amdgcn_exp2f(om - base);
-                m[n] = to;
-                l[n] = l[n] * fm + ol * fo;
+                f32x4 s[2];
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    const f32x4 w = *(const f32x4 *)&s_o[wave][(n * 16 + col) * LD + 16 * dt + 4 * g];
-                    o[n][dt] = o[n][dt] * fm + w * fo;
+                for (int u = 0; u < 2; u++) {
+                    s[u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) s[u] = KvType<T>::mma(kv_bits<x8>(t.k[u][ks]), qf[n][ks], s[u]);
                 }
+                float z[8];
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    z[j] = s[j >> 2][j & 3] * a.scale2;
+                    if (!whole && j >= left) z[j] = -INFINITY;
+                    top = fmaxf(top, z[j]);
+                }
+                if (__any(top > m[n] + KV_SLACK)) {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    /* each column by its own scores: another's do not show in its bits */
+                    const float to = top > m[n] + KV_SLACK ? top : m[n], f = to == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - to);
+                    m[n] = to;
+                    l[n] *= f;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) o[n][dt] *= f;
+                }
+                /* before any score is above -infinity the maximum is taken as 0 */
+                const float base = (m[n] == -INFINITY ? 0.0f : m[n]) - KvType<T>::SHIFT;
+                x8 p;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float e = __builtin_amdgcn_exp2f(z[j] - base);
+                    l[n] += e;
+                    p[j] = (T)e;   /* 8 (bf16) or 11 bits of a weight in [0, 1]: as the values it is multiplied with have */
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[n][dt] = KvType<T>::mma(kv_bits<x8>(t.v[dt]), p, o[n][dt]);
+            }
+        };
+        const int mine = (tiles - wave + NW - 1) / NW;      /* this wave's tiles */
+        if (mine > 0) {
+            Tile ta, tb;
+            names(0);
+            load(ta, 0);
+            for (int i = 0; i < mine; i += 2) {
+                if (i + 1 < mine) load(tb, i + 1);
+                compute(ta, i);
+                if (i + 2 < mine) {
+                    if (((i + 2) & 31) == 0) names(i + 2);
+                    load(ta, i + 2);
+                }
+                if (i + 1 < mine) compute(tb, i + 1);
             }
         }
-        __syncthreads();
-    }
-    if (wave == 0) {
+        /* the lanes of a column hold different positions' weights */
 #pragma unroll
         for (int n = 0; n < NC; n++) {
-            const int h = n * 16 + col;
-            if (h >= ncol) continue;
-            const int64_t head = kvh * a.G + col0 + h, H = (int64_t)a.G * c.heads;
-            if (take == units) {
-                const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];     /* no position at all: zeros */
+            l[n] += __shfl_xor(l[n], 16, 64);
+            l[n] += __shfl_xor(l[n], 32, 64);
+        }
+        /* merge the waves, half of them at a time, always in the same order */
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    const float v[4] = {o[n][dt][0] * inv, o[n][dt][1] * inv, o[n][dt][2] * inv, o[n][dt][3] * inv};
-                    store_out(a.out, a.out_dt, (b * H + head) * HD + 16 * dt + 4 * g, v);
+        for (int half = NW / 2; half >= 1; half >>= 1) {
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int n = 0; n < NC; n++) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+                        *(f32x4 *)&s_o[wave - half][(n * 16 + col) * LD + 16 * dt + 4 * g] = o[n][dt];
+                    if (g == 0) {
+                        s_ml[wave - half][(n * 16 + col) * 2] = m[n];
+                        s_ml[wave - half][(n * 16 + col) * 2 + 1] = l[n];
+                    }
                 }
-            } else {
-                const int64_t w = kv_slot(worker, first == 0) * H + head;
+            }
+            __syncthreads();
+            if (wave < half) {
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) *(f32x4 *)(a.part + w * HD + 16 * dt + 4 * g) = o[n][dt];
-                if (g == 0) {
-                    a.ml[2 * w] = m[n];
-                    a.ml[2 * w + 1] = l[n];
+                for (int n = 0; n < NC; n++) {
+                    const float om = s_ml[wave][(n * 16 + col) * 2], ol = s_ml[wave][(n * 16 + col) * 2 + 1];
+                    const float to = fmaxf(m[n], om), base = to == -INFINITY ? 0.0f : to;
+                    const float fm = __builtin_amdgcn_exp2f(m[n] - base), fo = __builtin_amdgcn_exp2f(om - base);
+                    m[n] = to;
+                    l[n] = l[n] * fm + ol * fo;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+                        const f32x4 w = *(const f32x4 *)&s_o[wave][(n * 16 + col) * LD + 16 * dt + 4 * g];
+                        o[n][dt] = o[n][dt] * fm + w * fo;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (wave == 0) {
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                const int h = n * 16 + col;
+                if (h >= ncol) continue;
+                const int64_t head = kvh * a.G + col0 + h, H = (int64_t)a.G * c.heads;
+                if (take == units) {
+                    const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];     /* no position at all: zeros */
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+                        const float v[4] = {o[n][dt][0] * inv, o[n][dt][1] * inv, o[n][dt][2] * inv, o[n][dt][3] * inv};
+                        store_out(a.out, a.out_dt, (b * H + head) * HD + 16 * dt + 4 * g, v);
+                    }
+                } else {
+                    const int64_t w = kv_slot(worker, first == 0) * H + head;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) *(f32x4 *)(a.part + w * HD + 16 * dt + 4 * g) = o[n][dt];
+                    if (g == 0) {
+                        a.ml[2 * w] = m[n];
+                        a.ml[2 * w + 1] = l[n];
+                    }
                 }
             }
         }
-    }
-    return take;
+        return take;
     };
     if (WHOLE) {
         part(worker, kv_uniform(decode_len(c, worker)), 0, 1 << 30);
@@ -510,7 +514,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
 }
 
 /* The sums of the sequences that several workers share: a group per sequence and hb heads, HD / 4 threads a row, the
- * workers' parts dealt to a head's rows, each with a maximum of its own, the rows added through LDS in a fixed order. */
+ * workers' parts dealt to a head's rows, each with a maximum of its own, the rows added through LDS in a fixed order.  4 to
+ * 5 us whatever the sizes: a launch and two reads after each other (1024 threads a group, or a group for 32 values: the same). */
 template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a) {
     constexpr int L4 = HD / 4, ROWS = 256 / L4;
     __shared__ float s_o[ROWS][HD], s_ml[ROWS][2];
@@ -577,16 +582,22 @@ template <class T> void append_x(int xdt, const AppendArgs &a, dim3 grid, hipStr
     else append_hd<__bf16, T>(a, grid, s);
 }
 
-/* Up to this many positions a sequence, by its table, every sequence is one group of eight waves and one launch */
+/* A sequence a group of eight waves and one launch, where the tables are as short as this; twice as long where there are groups
+ * for every compute unit.  us whole / in shares, 32 heads on 4 of 128: one sequence of 500 8.1 / 8.8, of 1000 10.3 / 8.8; 64 of
+ * 500 16.1 / 18.0, of 1000 24.8 / 27.1, of up to 1000 18.9 / 21.6; 256 of 1000 104 / 103; 300 of 8 on 2 of 64 5.3 / 8.1. */
 constexpr int64_t DECODE_WHOLE = 512;
 
 struct DecodePlan {
     int whole, W, nc, z, hb;
 };
 DecodePlan decode_plan(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads) {
-    const int G = heads / c->kv_heads, nc = G <= 16 ? 1 : G <= 32 || c->head_dim > 128 ? 2 : 4, z = (G + nc * 16 - 1) / (nc * 16);
+    /* Columns of 16 queries a group.  A key head with more queries has a group for every 16, which read the cache again from
+     * the caches nearer by; narrow heads, whose tiles are little to read, take 32.  us with 16 / 32 / 64 a group: 48 sequences of up
+     * to 8192 with 64 heads on 1 of 128 36.6 / 36.5 / 44.9, 40 on 2 of 128 55 / 55, 128 on 4 of 64 55 / 46; one of 30000
+     * with 64 on 1 of 128 14.6 / 17.8 / 24.8, 64 on 2 of 256 22.5 / 28.4. */
+    const int G = heads / c->kv_heads, nc = G > 16 && c->head_dim <= 64 ? 2 : 1, z = (G + nc * 16 - 1) / (nc * 16);
     const int64_t cap = (int64_t)b->table_pages * c->page;
-    if (cap <= DECODE_WHOLE) return {1, (int)b->B, nc, z, 0};
+    if (cap <= DECODE_WHOLE || (cap <= 2 * DECODE_WHOLE && b->B * c->kv_heads * z >= 256)) return {1, (int)b->B, nc, z, 0};
     /* A group a compute unit: four waves with two tiles each on their way keep the memory busy, and fewer shares are fewer
      * parts to join.  256 groups / 512 (1024 up to 64 wide): one sequence of 131071, 32 heads on 4 of 128, 52.7 / 55.1 us; 64
      * of up to 8192, 64 on 4, 113 / 118; 60000, 8 on 2 of 64, 13.8 / 18.3; 240 groups 53.6, 114, 14.2; 256 of eight waves
@@ -614,9 +625,9 @@ template <class T, int HD, int NC> void decode_nc(const DecodeArgs &a, const Dec
     }
 }
 template <class T, int HD> void decode_hd(const DecodeArgs &a, const DecodePlan &p, hipStream_t s) {
-    if (p.nc == 1) decode_nc<T, HD, 1>(a, p, s);
-    else if (p.nc == 2) decode_nc<T, HD, 2>(a, p, s);
-    else if constexpr (HD <= 128) decode_nc<T, HD, 4>(a, p, s);
+    if constexpr (HD <= 64)
+        if (p.nc == 2) return decode_nc<T, HD, 2>(a, p, s);
+    decode_nc<T, HD, 1>(a, p, s);
 }
 template <class T> void decode(const DecodeArgs &a, const DecodePlan &p, hipStream_t s) {
     static void (*const by_width[8])(const DecodeArgs &, const DecodePlan &, hipStream_t) = {
