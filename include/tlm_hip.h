@@ -702,9 +702,11 @@ size_t tlm_hip_kv_decode_workspace_bytes(const tlm_hip_kv_cache *c, const tlm_hi
 int    tlm_hip_kv_decode(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, const void *q, int64_t q_stride, int heads,
                          float scale, int out_dt, void *out, void *workspace, void *stream);
 /* Attention of packed rows, causal: a row at position p sees the positions 0 .. p of its sequence (cached ones
- * included).  q and out as above, [rows] for [B]. */
+ * included).  q and out as above, [rows] for [B].  workspace: tlm_hip_kv_prompt_workspace_bytes bytes (0: none, by the sizes
+ * alone: few rows over far-reaching tables have their positions split), as tlm_hip_kv_decode's. */
+size_t tlm_hip_kv_prompt_workspace_bytes(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads);
 int    tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, const void *q, int64_t q_stride, int heads,
-                         float scale, int out_dt, void *out, void *stream);
+                         float scale, int out_dt, void *out, void *workspace, void *stream);
 
 /* ---- reference tier ABI --------------------------------------------------
  * Layout-compatible with tlm_quant_kernels (src/lib/tlm_quant.h:152-166, a

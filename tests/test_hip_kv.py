@@ -105,6 +105,21 @@ def test_prompt_few_groups(hip, hd):
         check_prompt(Batch(BF16, heads, kv_heads, hd, 16, [n], [n + 333], seed=hd))
 
 
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("new,lens,width", [
+    ([16], [4000], 63), ([1], [2100], 63), ([5, 0, 40, 1], [3000, 4, 40, 0], 60), ([100], [1500], 64), ([3] * 9, [2047] * 9, 200),
+    ([2, 30], [130, 300], 400)])
+def test_prompt_parts(hip, hd, new, lens, width):
+    """Few rows over far-reaching tables: positions split over groups and joined; short sequences among them."""
+    check_prompt(Batch(BF16 if hd % 64 else F16, 16, 2, hd, 64, new, lens, seed=hd, width=width))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompt_parts_of_more_rows(hip, hd):
+    """64 rows a group, two parts or more."""
+    check_prompt(Batch(BF16, 32, 2, hd, 64, [290 if hd < 256 else 150], [3000], seed=hd))
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256, 1024])
 def test_prompt_pages(hip, page):
     check_prompt(Batch(BF16, 8, 2, 128, page, [300, 77], [1300, 77], seed=page))
@@ -154,7 +169,8 @@ def test_decode_and_prompt_agree(hip):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_masked_places_may_hold_anything(hip, dtype):
     """Infinities and NaN behind a row's position leave its bits alone; rows that see them get them."""
-    for first, n, H, KV in ((0, 150, 8, 2), (70, 40, 8, 2), (0, 300, 64, 2), (90, 200, 416, 16)):   # 32, 64, 128 rows a group
+    # 32 rows a group, 64 and 128, and parts
+    for first, n, H, KV in ((0, 150, 8, 2), (70, 40, 8, 2), (0, 300, 64, 2), (90, 200, 416, 16), (2300, 40, 8, 2)):
         b = Batch(dtype, H, KV, 64, 16, [n], [first + n], seed=9)
         want = kv.prompt(b.q, b.cache, b.tables, b.lens, b.cu, dtype=F32)
         for where, value in ((first + 20, math.inf), (first + n - 1, math.nan), (first + n // 2, -math.inf)):

@@ -56,7 +56,7 @@ def test_refuses(call, want, ck, bk, ak):
     elif call == "decode":
         rc = lib.tlm_hip_kv_decode(c, b, a["x"], a["stride"], a["heads"], 0.1, a["dt"], a["out"], P, None)
     else:
-        rc = lib.tlm_hip_kv_prompt(c, b, a["x"], a["stride"], a["heads"], 0.1, a["dt"], a["out"], None)
+        rc = lib.tlm_hip_kv_prompt(c, b, a["x"], a["stride"], a["heads"], 0.1, a["dt"], a["out"], P, None)
     if call == "decode" and "cu" in bk:
         want = EINVAL if "rows" not in bk else want
     assert rc == want, lib.tlm_hip_errmsg()
@@ -76,7 +76,7 @@ def test_refuses_more():
     assert lib.tlm_hip_kv_append(c, b, 0, P, 768, 8, None, None, 0.0, None, 1.0, P + 8, None) == EINVAL
     for scale in (0.0, -1.0, float("nan"), float("inf")):
         assert lib.tlm_hip_kv_decode(c, b, P, 512, 8, scale, 2, P, P, None) == EINVAL
-        assert lib.tlm_hip_kv_prompt(c, b, P, 512, 8, scale, 2, P, None) == EINVAL
+        assert lib.tlm_hip_kv_prompt(c, b, P, 512, 8, scale, 2, P, P, None) == EINVAL
     assert lib.tlm_hip_kv_decode(c, C.byref(batch(cu=P)), P, 512, 8, 0.1, 2, P, P, None) == EINVAL
 
 
@@ -90,13 +90,21 @@ def test_workspace():
     for p in (None, P + 16):
         assert lib.tlm_hip_kv_decode(c, C.byref(wide), P, 512, 8, 0.1, 2, P, p, None) == EINVAL
         assert b"workspace" in lib.tlm_hip_errmsg()
+    ws = lib.tlm_hip_kv_prompt_workspace_bytes
+    small, wide = batch(cu=P, table_pages=127, table_stride=127), batch(cu=P, table_pages=128, table_stride=128)
+    assert ws(c, C.byref(small), 8) == 0 and ws(c, C.byref(wide), 8) > 0 and ws(c, C.byref(wide), 7) == 0
+    assert ws(c, C.byref(batch(cu=P, rows=1 << 20, table_pages=128, table_stride=128)), 8) == 0      # rows enough
+    assert ws(c, C.byref(batch(cu=P, rows=0, table_pages=128, table_stride=128)), 8) == 0
+    for p in (None, P + 16):
+        assert lib.tlm_hip_kv_prompt(c, C.byref(wide), P, 512, 8, 0.1, 2, P, p, None) == EINVAL
+        assert b"workspace" in lib.tlm_hip_errmsg()
 
 
 def test_nothing_to_do():
     c = C.byref(cache())
     for b in (batch(B=0, rows=0, lens=None, tables=None), batch(B=2, rows=0, cu=P, lens=None, tables=None)):
         assert lib.tlm_hip_kv_append(c, C.byref(b), 0, None, 768, 8, None, None, 1e-6, None, 1.0, None, None) == 0
-        assert lib.tlm_hip_kv_prompt(c, C.byref(b), None, 512, 8, 0.1, 2, None, None) == 0
+        assert lib.tlm_hip_kv_prompt(c, C.byref(b), None, 512, 8, 0.1, 2, None, None, None) == 0
     b = batch(B=0, rows=0, lens=None, tables=None)
     assert lib.tlm_hip_kv_decode(c, C.byref(b), None, 512, 8, 0.1, 2, None, None, None) == 0
 
@@ -180,7 +188,7 @@ def test_a_failed_self_test_refuses_the_calls(failed):
     c, b = C.byref(cache()), C.byref(batch())
     calls = {"kv_append": lambda: lib.tlm_hip_kv_append(c, b, 0, P, 768, 8, None, None, 1e-6, None, 1.0, P, None),
              "kv_decode": lambda: lib.tlm_hip_kv_decode(c, b, P, 512, 8, 0.1, 2, P, P, None),
-             "kv_prompt": lambda: lib.tlm_hip_kv_prompt(c, b, P, 512, 8, 0.1, 2, P, None)}
+             "kv_prompt": lambda: lib.tlm_hip_kv_prompt(c, b, P, 512, 8, 0.1, 2, P, P, None)}
     norm = lambda: lib.tlm_hip_fp8_add_rmsnorm(0, P, 128, 2, P, 128, P, 1e-6, 128, 2, P, 128, P, P, None)   # noqa: E731
     failed(1 << 27)
     for name, call in calls.items():

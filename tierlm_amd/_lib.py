@@ -211,7 +211,8 @@ _SIGS = {
     "tlm_hip_kv_append": (i32, [C.POINTER(KvCache), C.POINTER(KvBatch), i32, vp, i64, i32, vp, vp, f32, vp, f32, vp, vp]),
     "tlm_hip_kv_decode_workspace_bytes": (sz, [C.POINTER(KvCache), C.POINTER(KvBatch), i32]),
     "tlm_hip_kv_decode": (i32, [C.POINTER(KvCache), C.POINTER(KvBatch), vp, i64, i32, f32, i32, vp, vp, vp]),
-    "tlm_hip_kv_prompt": (i32, [C.POINTER(KvCache), C.POINTER(KvBatch), vp, i64, i32, f32, i32, vp, vp]),
+    "tlm_hip_kv_prompt_workspace_bytes": (sz, [C.POINTER(KvCache), C.POINTER(KvBatch), i32]),
+    "tlm_hip_kv_prompt": (i32, [C.POINTER(KvCache), C.POINTER(KvBatch), vp, i64, i32, f32, i32, vp, vp, vp]),
     "tlm_hip_fp8_matmul": (i32, [vp, i64, i64, vp, vp, i64, i32, vp, i64, vp]),
     "tlm_hip_fp8_matmul_kernel": (C.c_char_p, [i64, i64, i64]),
     "tlm_hip_fp8_moe_workspace_bytes": (sz, [C.POINTER(MoeDesc), i64]),

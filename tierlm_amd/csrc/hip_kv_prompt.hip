@@ -11,8 +11,9 @@ struct PromptArgs {
     const void *q, *k, *v;
     void *out;
     int64_t qstride;
+    float *part, *ml;        /* parts > 1: [tile and key head][parts][rows][HD] sums, [..][2] maximum and weight */
     float scale2;            /* scale log2(e) */
-    int G, out_dt;
+    int G, out_dt, parts;
 };
 
 __device__ __forceinline__ void store_out(void *out, int dt, int64_t i, const float (&v)[4]) {
@@ -27,6 +28,35 @@ __device__ __forceinline__ void store_out(void *out, int dt, int64_t i, const fl
 /* What a page number outside the cache stands for: its positions are masked, and a finite value times weight 0 is 0 */
 __device__ const u32x4 kv_nothing[KV_BLOCK * 256 * 2 / 16] = {};
 
+/* Tile w of `tile` (token, head) rows: its sequence, its first row and what its rows see */
+struct PromptTile {
+    int b, nrow, row0, present, end;
+    KvRows rows;
+    int64_t p0;
+    __device__ __forceinline__ int limit(int token) const {      /* last position that a token sees (-1: none) */
+        const int64_t p = p0 + token;
+        return (int)(p < 0 ? -1 : p < present ? p : present - 1);
+    }
+    __device__ __forceinline__ int last_of(int r, int G) const { return limit((r < nrow ? r : nrow - 1) / G); }
+    __device__ __forceinline__ PromptTile(const KvView &c, int G, int w, int tile) {
+        const KvItem it = kv_find(c.B, w, [&](int b) { return (int)kv_prompt_items(kv_rows(c, b).n, G, tile); });
+        b = it.b;
+        if (b < 0) return;
+        rows = kv_rows(c, b);
+        const int64_t len = kv_len(c, b), cap = kv_cap(c);
+        nrow = (int)(rows.n * G);
+        row0 = (it.n - 1 - it.i) * tile;      /* the longest first */
+        p0 = len - rows.n;
+        present = (int)(len < cap ? len : cap);
+        end = last_of(row0 + tile - 1, G) + 1;
+    }
+};
+/* stages of each of `parts` parts: a whole number for every wave */
+__device__ __forceinline__ int prompt_part(int tiles, int parts, int sg) {
+    const int per = (tiles + parts - 1) / parts;
+    return per < sg ? sg : (per + sg - 1) / sg * sg;
+}
+
 /* A group of four waves takes 32 RG rows of one sequence and key head (RG = 4 / SG), a row being a (token, query head of
  * the group) pair: the heads that share keys lie side by side, so a tile of few tokens wastes little of the causal border.
  * A wave holds 32 rows as the columns of S^T = K Q^T and of O^T = V^T P^T (32 x 32 x 16 products), and takes every SG-th
@@ -39,7 +69,7 @@ __device__ const u32x4 kv_nothing[KV_BLOCK * 256 * 2 / 16] = {};
  *
  * A masked place's value may be infinite or NaN, and its weight 0 does not silence it: in stages with a border the values
  * that are not finite leave LDS, and rows that see them get them at the end, value by value (rare). */
-template <class T, int HD, int SG, int TP>
+template <class T, int HD, int SG, int TP, bool PARTS>
 __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) ? 1 : 2) void k_kv_prompt(PromptArgs a) {
     typedef typename KvType<T>::x8 x8;
     constexpr int RG = 4 / SG, ROWS = 32 * RG;
@@ -54,31 +84,25 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
     const KvView &c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = kv_uniform(tid >> 6), col = lane & 31, h = lane >> 5;
     const int rg = wave % RG, sg = wave / RG;
-    const int kvh = (int)(blockIdx.x % (uint32_t)c.heads), G = a.G;
-    const KvItem it = kv_find(c.B, (int)(blockIdx.x / (uint32_t)c.heads), [&](int b) {
-        return (int)kv_prompt_items(kv_rows(c, b).n, G, ROWS);
-    });
-    if (it.b < 0) return;
-    const KvRows rows = kv_rows(c, it.b);
-    const int64_t len = kv_len(c, it.b), cap = kv_cap(c);
-    const int nrow = (int)(rows.n * G), row0 = (it.n - 1 - it.i) * ROWS;    /* the longest first */
-    const int64_t p0 = len - rows.n;
-    const int present = (int)(len < cap ? len : cap);
-    const int32_t *table = c.tables + it.b * c.table_stride;
+    const int kvh = (int)(blockIdx.x % (uint32_t)c.heads), G = a.G, y = (int)(blockIdx.x / (uint32_t)c.heads);
+    const int w = PARTS ? y / a.parts : y, mypart = PARTS ? y % a.parts : 0;
+    const PromptTile pt(c, G, w, ROWS);
+    if (pt.b < 0) return;
+    const KvRows &rows = pt.rows;
+    const int nrow = pt.nrow, row0 = pt.row0, present = pt.present;
+    const int32_t *table = c.tables + pt.b * c.table_stride;
 
     /* the lane's row, its last visible position (-1: none) */
     const int row = row0 + 32 * rg + col, token = row / G;
     const bool real = row < nrow;
-    auto limit = [&](int token) {
-        const int64_t p = p0 + token;
-        return (int)(p < 0 ? -1 : p < present ? p : present - 1);
-    };
-    const int lim = real ? limit(token) : -1;
-    auto last_of = [&](int r) { return limit((r < nrow ? r : nrow - 1) / G); };
-    const int end = last_of(row0 + ROWS - 1) + 1;             /* positions that the group needs */
-    const int gfirst = limit(row0 / G), wfirst = limit((row0 + 32 * rg) / G);
-    const int wend = row0 + 32 * rg < nrow ? last_of(row0 + 32 * rg + 31) + 1 : 0;
+    const int lim = real ? pt.limit(token) : -1;
+    const int end = pt.end;                                   /* positions that the group needs */
+    const int gfirst = pt.limit(row0 / G), wfirst = pt.limit((row0 + 32 * rg) / G);
+    const int wend = row0 + 32 * rg < nrow ? pt.last_of(row0 + 32 * rg + 31, G) + 1 : 0;
     const int tiles = (end + POS - 1) / POS;
+    const int per = PARTS ? prompt_part(tiles, a.parts, SG) : tiles;
+    const int t0 = mypart * per, t1 = tiles - t0 < per ? tiles : t0 + per;     /* this group's stages */
+    if (PARTS && mypart > 0 && t0 >= tiles) return;
 
     const int64_t H = (int64_t)G * c.heads;
     x8 qf[KS];
@@ -162,17 +186,17 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
 
     int ok = 0;
     Pages next = {};
-    if (tiles > 0) {
-        ok = load(pages(sg), sg, s_even + sg * UNITS * 1024);
-        next = pages(SG + sg);
+    if (t0 < t1) {
+        ok = load(pages(t0 + sg), t0 + sg, s_even + sg * UNITS * 1024);
+        next = pages(t0 + SG + sg);
     }
     auto step = [&](int i, uint8_t *stage, uint8_t *other) {
         __builtin_amdgcn_s_waitcnt(0);      /* this stage's own loads; the barrier brings the other waves' */
         __syncthreads();
-        const int tile = SG * i + sg, base = tile * POS, here = ok;
+        const int tile = t0 + SG * i + sg, base = tile * POS, here = ok;
         uint8_t *buf = stage + sg * UNITS * 1024;
-        if (SG * (i + 1) < tiles) ok = load(next, tile + SG, other + sg * UNITS * 1024);
-        if ((SG * i + SG) * POS - 1 > gfirst) {
+        if (t0 + SG * (i + 1) < t1) ok = load(next, tile + SG, other + sg * UNITS * 1024);
+        if ((t0 + SG * i + SG) * POS - 1 > gfirst) {
             /* a border: no value that is masked for some row may disturb its product.  The waves of a stage share its blocks. */
             constexpr int EACH = BLOCKS >= RG ? BLOCKS / RG : 1;
             bool odd = false;
@@ -257,9 +281,9 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
             for (int dt = 0; dt < DT; dt++)
                 o[dt] = KvType<T>::mma(*(const x8 *)(vb + (ks * DT + dt) * 1024), p[ks], o[dt]);
     };
-    for (int i = 0; SG * i < tiles; i += 2) {
+    for (int i = 0; t0 + SG * i < t1; i += 2) {
         step(i, s_even, s_odds);
-        if (SG * (i + 1) < tiles) step(i + 1, s_odds, s_even);
+        if (t0 + SG * (i + 1) < t1) step(i + 1, s_odds, s_even);
     }
     l += __shfl_xor(l, 32, 64);
     __syncthreads();
@@ -302,7 +326,7 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
         /* Rows that see a value that is not finite, from the first stage that left one out; where a later stage had it in its
          * product it is added once more, which changes nothing. */
 #pragma unroll 1
-        for (int blk = BLOCKS * odd_from; blk <= (wend - 1) / KV_BLOCK; blk++) {
+        for (int blk = BLOCKS * odd_from; blk < BLOCKS * t1 && blk <= (wend - 1) / KV_BLOCK; blk++) {
             const int64_t at = kv_block(c, table[blk >> c.sh], blk, kvh);
             if (at < 0) continue;
             const uint16_t *v = (const uint16_t *)a.v + at + 64 * h;
@@ -321,6 +345,20 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
         }
     }
     if (!real) return;
+    if (PARTS && tiles > per) {
+        const int64_t at = (((int64_t)w * c.heads + kvh) * a.parts + mypart) * ROWS + 32 * rg + col;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                *(f32x4 *)(a.part + at * HD + 32 * dt + 8 * r + 4 * h) =
+                    f32x4{o[dt][4 * r], o[dt][4 * r + 1], o[dt][4 * r + 2], o[dt][4 * r + 3]};
+        if (h == 0) {
+            a.ml[2 * at] = m;
+            a.ml[2 * at + 1] = l;
+        }
+        return;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;    /* a row that sees nothing: zeros */
     const int64_t at = ((rows.first + token) * H + kvh * G + (row - token * G)) * HD;
 #pragma unroll
@@ -332,32 +370,87 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
         }
 }
 
+/* The parts of a tile's rows, in order: a group a tile and key head, HD / 4 threads a row. */
+template <int HD, int SG, int TP> __global__ __launch_bounds__(256) void k_kv_prompt_join(PromptArgs a) {
+    constexpr int ROWS = 128 / SG, L4 = HD / 4, EACH = 256 / L4;
+    const KvView &c = a.c;
+    const int kvh = (int)(blockIdx.x % (uint32_t)c.heads), w = (int)(blockIdx.x / (uint32_t)c.heads), G = a.G;
+    const PromptTile pt(c, G, w, ROWS);
+    if (pt.b < 0) return;
+    const int tiles = (pt.end + 32 * TP - 1) / (32 * TP), per = prompt_part(tiles, a.parts, SG), n = (tiles + per - 1) / per;
+    if (n <= 1) return;
+    const int e = threadIdx.x % L4 * 4, r0 = threadIdx.x / L4;
+    if (r0 >= EACH) return;
+    const int64_t H = (int64_t)G * c.heads, at0 = ((int64_t)w * c.heads + kvh) * a.parts * ROWS;
+    for (int r = r0; r < ROWS && pt.row0 + r < pt.nrow; r += EACH) {
+        f32x4 o = {0, 0, 0, 0};
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+            const int64_t at = at0 + (int64_t)i * ROWS + r;
+            const float mi = a.ml[2 * at], li = a.ml[2 * at + 1];
+            const f32x4 oi = *(const f32x4 *)(a.part + at * HD + e);
+            const float to = fmaxf(m, mi), base = to == -INFINITY ? 0.0f : to;
+            const float f = __builtin_amdgcn_exp2f(m - base), fi = __builtin_amdgcn_exp2f(mi - base);
+            o = o * f + oi * fi;
+            l = l * f + li * fi;
+            m = to;
+        }
+        const int row = pt.row0 + r, token = row / G;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        store_out(a.out, a.out_dt, ((pt.rows.first + token) * H + kvh * G + (row - token * G)) * HD + e, v);
+    }
+}
+
 /* Rows of a group: 128 where that many groups fill the chip (two fit a compute unit; past 128 wide, where of those with 64
  * rows only one does, from half as many on); else 64, the positions dealt to two waves, or 32 and four, while all groups
  * still run at once: a stage takes a lone wave about a microsecond whatever its rows.  us with 128 / 64 / 32 rows, 32 heads on
  * 4 of 128: 4096 tokens 156 / 178 / 395, 2048 59 / 58 / 129, 1024 30 / 24 / 48, 512 19 / 15 / 21, 256 13.3 / 10.6 / 11.2; 128
  * behind 8000 176 / 117 / 80; 8 heads on 2 of 64, 2048 tokens 39 / 26 / 22; 16 on 2 of 256, 4096 tokens 219 / 259, 2048
- * 104 / 77. */
-int split_of(int64_t rows, int64_t B, int group, int kv_heads, int hd) {
-    const int64_t groups = kv_prompt_most(rows, B, group, 128) * kv_heads;
-    return groups > (hd <= 128 ? 512 : 256) ? 1 : groups > (hd <= 64 ? 128 : 64) ? 2 : 4;
+ * 104 / 77.
+ * Where even those leave units idle and the tables reach far (the lengths are the device's), the positions of each tile go to
+ * several groups, at least 512 each, and a second launch joins them. */
+struct PromptPlan {
+    int sg, parts;
+    int64_t tiles;      /* of all key heads */
+};
+PromptPlan prompt_plan(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads) {
+    const int group = heads / c->kv_heads, hd = c->head_dim;
+    const int64_t groups = kv_prompt_most(b->rows, b->B, group, 128) * c->kv_heads;
+    int sg = groups > (hd <= 128 ? 512 : 256) ? 1 : groups > (hd <= 64 ? 128 : 64) ? 2 : 4;
+    if (sg == 4 && hd > 128) sg = 2;      /* four stages twice are more than the LDS */
+    const int64_t tiles = kv_prompt_most(b->rows, b->B, group, 128 / sg) * c->kv_heads, cap = (int64_t)b->table_pages * c->page;
+    const int64_t room = (sg == 4 ? (hd <= 64 ? 512 : 256) : hd <= 128 ? 512 : 256) / tiles, reach = cap / 512;
+    int64_t parts = sg == 1 || reach < 4 ? 1 : room < reach ? room : reach;
+    parts = parts > 16 ? 16 : parts;
+    return {sg, parts < 1 ? 1 : (int)parts, tiles};
+}
+size_t prompt_bytes(const PromptPlan &p, int hd) {
+    return p.parts == 1 ? 0 : (size_t)p.tiles * p.parts * (128 / p.sg) * (hd + 2) * 4;
 }
 
-template <class T, int HD, int SG, int TP> void launch_sg(const PromptArgs &a, int64_t B, hipStream_t s) {
-    const dim3 grid((unsigned)(kv_prompt_most(a.c.rows, B, a.G, 128 / SG) * a.c.heads));
-    hipLaunchKernelGGL((k_kv_prompt<T, HD, SG, TP>), grid, dim3(256), 0, s, a);
+template <class T, int HD, int SG, int TP> void launch_sg(const PromptArgs &a, const PromptPlan &p, hipStream_t s) {
+    if constexpr (SG > 1) {
+        if (p.parts > 1) {
+            hipLaunchKernelGGL((k_kv_prompt<T, HD, SG, TP, true>), dim3((unsigned)(p.tiles * p.parts)), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_kv_prompt_join<HD, SG, TP>), dim3((unsigned)p.tiles), dim3(256), 0, s, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((k_kv_prompt<T, HD, SG, TP, false>), dim3((unsigned)p.tiles), dim3(256), 0, s, a);
 }
-template <class T, int HD> void launch(const PromptArgs &a, int64_t B, hipStream_t s) {
-    const int sg = split_of(a.c.rows, B, a.G, a.c.heads, HD);
-    if (sg == 1) return launch_sg<T, HD, 1, HD <= 128 ? 2 : 1>(a, B, s);
-    if constexpr (HD <= 128)     /* wider, four stages twice are more than the LDS */
-        if (sg == 4) return launch_sg<T, HD, 4, 1>(a, B, s);
-    launch_sg<T, HD, 2, HD <= 64 ? 2 : 1>(a, B, s);
+template <class T, int HD> void launch(const PromptArgs &a, const PromptPlan &p, hipStream_t s) {
+    if (p.sg == 1) return launch_sg<T, HD, 1, HD <= 128 ? 2 : 1>(a, p, s);
+    if constexpr (HD <= 128)
+        if (p.sg == 4) return launch_sg<T, HD, 4, 1>(a, p, s);
+    launch_sg<T, HD, 2, HD <= 64 ? 2 : 1>(a, p, s);
 }
-template <class T> void prompt(const PromptArgs &a, int64_t B, hipStream_t s) {
-    static void (*const by_width[8])(const PromptArgs &, int64_t, hipStream_t) = {
-        launch<T, 32>, launch<T, 64>, launch<T, 96>, launch<T, 128>, launch<T, 160>, launch<T, 192>, launch<T, 224>, launch<T, 256>};
-    by_width[a.c.hd / 32 - 1](a, B, s);
+template <class T> void prompt(const PromptArgs &a, const PromptPlan &p, hipStream_t s) {
+    static void (*const by_width[8])(const PromptArgs &, const PromptPlan &, hipStream_t) = {
+        launch<T, 32>, launch<T, 64>, launch<T, 96>, launch<T, 128>,
+        launch<T, 160>, launch<T, 192>, launch<T, 224>, launch<T, 256>};
+    by_width[a.c.hd / 32 - 1](a, p, s);
 }
 
 bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
@@ -365,8 +458,16 @@ int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16
 
 } // namespace
 
-extern "C" int tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, const void *q, int64_t q_stride,
-                                 int heads, float scale, int out_dt, void *out, void *stream) {
+extern "C" {
+
+size_t tlm_hip_kv_prompt_workspace_bytes(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads) {
+    KvView v;
+    if (kv_check("kv_prompt_workspace_bytes", c, b, heads, &v) || b->B == 0 || b->rows == 0) return 0;
+    return prompt_bytes(prompt_plan(c, b, heads), c->head_dim);
+}
+
+int tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, const void *q, int64_t q_stride, int heads,
+                      float scale, int out_dt, void *out, void *workspace, void *stream) {
     PromptArgs a;
     if (int rc = kv_check("kv_prompt", c, b, heads, &a.c)) return rc;
     if (!type_bytes(out_dt)) return tlmh_seterr(TLM_HIP_EUNSUP, "kv_prompt: dtype %d (F32, F16 and BF16 only)", out_dt);
@@ -381,6 +482,10 @@ extern "C" int tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_bat
     if (kv_prompt_most(b->rows, b->B, heads / c->kv_heads, 128) * c->kv_heads > (1 << 23))
         return tlmh_seterr(TLM_HIP_ERANGE, "kv_prompt: %lld rows of %lld sequences are too many for one launch",
                            (long long)b->rows, (long long)b->B);
+    const PromptPlan p = prompt_plan(c, b, heads);
+    const size_t need = prompt_bytes(p, c->head_dim);
+    if (need && (!workspace || !aligned(workspace, 256)))
+        return tlmh_seterr(TLM_HIP_EINVAL, "kv_prompt: needs a workspace of %zu bytes, 256-byte aligned", need);
     if (int rc = tlmh_refuse_failed(FAILED_KV, "kv_prompt")) return rc;
     a.q = q;
     a.k = c->k;
@@ -390,7 +495,12 @@ extern "C" int tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_bat
     a.scale2 = scale * 1.44269504088896341f;
     a.G = heads / c->kv_heads;
     a.out_dt = out_dt;
-    if (c->dt == DT_F16) prompt<_Float16>(a, b->B, (hipStream_t)stream);
-    else prompt<__bf16>(a, b->B, (hipStream_t)stream);
+    a.parts = p.parts;
+    a.part = (float *)workspace;
+    a.ml = need ? a.part + (size_t)p.tiles * p.parts * (128 / p.sg) * c->head_dim : nullptr;
+    if (c->dt == DT_F16) prompt<_Float16>(a, p, (hipStream_t)stream);
+    else prompt<__bf16>(a, p, (hipStream_t)stream);
     return tlmh_check(hipGetLastError(), "kv_prompt launch");
 }
+
+} // extern "C"

@@ -404,7 +404,7 @@ bool kv_ok(uint32_t *s) {
         const tlm_hip_kv_batch first = {1, FIRST, di + 5, di + 7, di + 8 + WIDE, WIDE, 3}, b = {B, T, di, di + 3, di + 8, WIDE, 3};
         ok = ok && tlm_hip_kv_append(&c, &first, DT_F32, dx, ROW, H, dn, dn + HD, 1e-6f, df, 1.0f, q, nullptr) == TLM_HIP_OK &&
              tlm_hip_kv_append(&c, &b, DT_F32, dx + FIRST * ROW, ROW, H, dn, dn + HD, 1e-6f, df, 1.0f, q, nullptr) == TLM_HIP_OK &&
-             tlm_hip_kv_prompt(&c, &b, q, H * HD, H, 0.25f, DT_F32, y, nullptr) == TLM_HIP_OK &&
+             tlm_hip_kv_prompt(&c, &b, q, H * HD, H, 0.25f, DT_F32, y, nullptr, nullptr) == TLM_HIP_OK &&
              hipMemcpy(gq.data(), q, gq.size() * 2, hipMemcpyDeviceToHost) == hipSuccess &&
              hipMemcpy(gy.data(), y, gy.size() * 4, hipMemcpyDeviceToHost) == hipSuccess;
         if (!ok) break;

@@ -26,6 +26,7 @@ from .fp8 import _current_device, _here, _raw_stream, _rows_ok
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _CACHE = {torch.float16: 1, torch.bfloat16: 2}
 _I32, _F32, _F64 = torch.int32, torch.float32, torch.float64
+_decode_bytes, _prompt_bytes = lib.tlm_hip_kv_decode_workspace_bytes, lib.tlm_hip_kv_prompt_workspace_bytes
 _append, _decode, _prompt = lib.tlm_hip_kv_append, lib.tlm_hip_kv_decode, lib.tlm_hip_kv_prompt
 
 
@@ -56,7 +57,7 @@ class Cache:
         self._dev = self._k.get_device()
         self._c = KvCache(_CACHE[dtype], kv_heads, head_dim, page, n_pages, self._k.data_ptr(), self._v.data_ptr())
         self._ref = C.byref(self._c)
-        self._workspace = {}        # bytes of a decode's workspace by its sizes
+        self._sizes = {}            # bytes of a workspace by the call's sizes
 
     @property
     def k(self):
@@ -180,6 +181,16 @@ def _queries(q, cache, scale, out, dtype):
     return T, stride, heads, scale, out
 
 
+def _workspace(cache, q, call, ref, key):
+    """A call's own workspace (None: it needs none) from torch's allocator, which orders its reuse on the stream."""
+    nbytes = cache._sizes.get(key)
+    if nbytes is None:
+        if len(cache._sizes) >= 4096:
+            cache._sizes.clear()
+        nbytes = cache._sizes[key] = call(cache._ref, ref, key[1])
+    return q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
 def decode(q, cache, tables, lens, *, scale=None, out=None, dtype=None):
     """Attention of one new token a sequence: q [B, heads, head_dim] of the cache's dtype (rows of any stride) over
     the lens[b] positions of sequence b -> [B, heads, head_dim] of `dtype` (q's without it).  scale: 1 /
@@ -187,15 +198,9 @@ def decode(q, cache, tables, lens, *, scale=None, out=None, dtype=None):
     T, stride, heads, scale, out = _queries(q, cache, scale, out, dtype)
     b = _batch(cache, T, tables, lens, None, (q, out))
     ref = C.byref(b)
-    key = (T, heads, tables.shape[1])
-    nbytes = cache._workspace.get(key)
-    if nbytes is None:
-        if len(cache._workspace) >= 4096:
-            cache._workspace.clear()
-        nbytes = cache._workspace[key] = lib.tlm_hip_kv_decode_workspace_bytes(cache._ref, ref, heads)
-    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    ws = _workspace(cache, q, _decode_bytes, ref, (T, heads, b.table_pages))
     rc = _decode(cache._ref, ref, q.data_ptr(), stride, heads, scale, _TYPES[out.dtype], out.data_ptr(),
-                 ws.data_ptr() if nbytes else None, _raw_stream(cache._dev))
+                 None if ws is None else ws.data_ptr(), _raw_stream(cache._dev))
     if rc:
         check(rc)
     return out
@@ -206,8 +211,10 @@ def prompt(q, cache, tables, lens, cu, *, scale=None, out=None, dtype=None):
     ones included.  q [T, heads, head_dim] -> [T, heads, head_dim]; rows outside cu's are left as they are."""
     T, stride, heads, scale, out = _queries(q, cache, scale, out, dtype)
     b = _batch(cache, T, tables, lens, cu, (q, out))
-    rc = _prompt(cache._ref, C.byref(b), q.data_ptr(), stride, heads, scale, _TYPES[out.dtype], out.data_ptr(),
-                 _raw_stream(cache._dev))
+    ref = C.byref(b)
+    ws = _workspace(cache, q, _prompt_bytes, ref, (T, heads, b.table_pages, b.B))
+    rc = _prompt(cache._ref, ref, q.data_ptr(), stride, heads, scale, _TYPES[out.dtype], out.data_ptr(),
+                 None if ws is None else ws.data_ptr(), _raw_stream(cache._dev))
     if rc:
         check(rc)
     return out
