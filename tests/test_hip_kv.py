@@ -191,6 +191,29 @@ def test_masked_places_may_hold_anything(hip, dtype):
                     assert torch.isnan(got[row:]).all()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("width", [16, 300])
+def test_decode_values_that_are_not_finite(hip, dtype, width):
+    """A seen infinity comes through with its sign, whatever its weight's bits (equal keys: weights of exactly 1 too); a NaN as
+    one; other values and other sequences as without them."""
+    for equal in (False, True):
+        b = Batch(dtype, 8, 2, 64, 16, [1] * 3, [200, 90, 70], seed=25, width=width)
+        if equal:
+            for i, n in enumerate(b.lens_list):
+                b.k[i] = torch.ones_like(b.k[i])
+                b.put(i, b.k[i], b.v[i])
+        want = kv.decode(b.q, b.cache, b.tables, b.lens, dtype=F32)
+        for where, value in ((0, math.inf), (63, -math.inf), (199, math.nan)):
+            v = b.v[0].clone()
+            v[where, :, 5] = value
+            b.put(0, b.k[0], v)
+            got = kv.decode(b.q, b.cache, b.tables, b.lens, dtype=F32)
+            seen = got[0, :, 5]
+            assert torch.isnan(seen).all() if math.isnan(value) else (seen == value).all(), (where, value, equal)
+            keep = torch.arange(64, device="cuda") != 5
+            assert torch.equal(got[0][:, keep], want[0][:, keep]) and torch.equal(got[1:], want[1:])
+
+
 @pytest.mark.parametrize("width", [16, 300])
 def test_decode_unseen_places(hip, width):
     """Positions past the length hold NaN in every test here; beside it, infinities in the pages of others."""
