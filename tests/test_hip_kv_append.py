@@ -143,6 +143,14 @@ def test_stride(hip):
     check(F16, BF16, 8, 2, 96, 16, [11, 30], [20, 30], stride=7, offset=3)
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,new,lens,cu", [
+    (17, 17, 32, [4003], [4010], True), (1, 1, 32, [70001], [70001], True), (16, 16, 64, [3, 3000, 0, 1200], [3, 3005, 0, 1300], True),
+    (15, 15, 32, [1] * 288, list(range(1, 289)), False), (57, 19, 96, [3600], [3600], True)])
+def test_two_heads_a_group(hip, heads, kv_heads, hd, new, lens, cu):
+    """Batches that fill the card, where a group takes two key heads: an odd number of them, and a single one."""
+    check(BF16, F32, heads, kv_heads, hd, 64, new, lens, seed=heads, cu=cu)
+
+
 def test_far_positions(hip):
     """A page late in a long context: the angles of position 2^20 are the definition's."""
     hd, heads, n = 64, 4, 20

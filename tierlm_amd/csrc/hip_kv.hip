@@ -9,9 +9,9 @@ bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
 
 /* ---- append ------------------------------------------------------------------
- * A group per block of 16 positions and key head: its up to 16 new rows of that head's G queries, key and value.  16
- * lanes hold a vector: lane s the pairs j = M s .. M s + M - 1 and their partners at hd / 2 + j (M = hd / 32), so the norm is
- * one 16-lane sum and the rotation stays in the lane.  Vectors go in the order of memory, 16 heads of a row at a time (a
+ * A group per block of 16 positions and hpg key heads, one or two: its up to 16 new rows of those heads' queries, keys and
+ * values.  16 lanes hold a vector: lane s the pairs j = M s .. M s + M - 1 and their partners at hd / 2 + j (M = hd / 32),
+ * so the norm is one 16-lane sum and the rotation stays in the lane.  Vectors go in the order of memory, 16 heads of a row at a time (a
  * row a lane group: 87 us for what takes 75), and values are turned over in registers (8 rows of one value to 16 bytes),
  * so the cache's block is written as whole pieces.
  * 8192 rows of 64 + 8 heads of 128, bf16: 75 us, 4.0 TB/s (63 us from an idle device); 61 rows of a decode step 5.5 us, a chain
@@ -24,7 +24,7 @@ struct AppendArgs {
     const float *qw, *kw;
     const double *freq;
     float eps, rope_scale;
-    int G;
+    int G, hpg;      /* queries a key head, key heads a group */
 };
 
 template <class X> __device__ __forceinline__ float to_f32(X v) { return (float)v; }
@@ -66,7 +66,8 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
             return (int)kv_append_items(r.n, kv_len(c, b));
         });
     if (it.b < 0) return;
-    const int kvh = blockIdx.y, G = a.G, H = G * c.heads;
+    const int kv0 = blockIdx.y * a.hpg, nh = c.heads - kv0 < a.hpg ? c.heads - kv0 : a.hpg;     /* the group's key heads */
+    const int H = a.G * c.heads, G = a.G * nh;                                                  /* its queries */
     const KvRows r = kv_rows(c, it.b);
     const int64_t p0 = kv_len(c, it.b) - r.n;                   /* position of the first new row */
     const int64_t blk = kv_floor16(p0) + it.i;
@@ -77,7 +78,8 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
     T *q = (T *)a.q + (r.first + lo - p0) * (int64_t)H * HD;
     int64_t at = -1;
     if (blk >= 0 && (blk >> c.sh) < c.table_pages)
-        at = kv_block(c, c.tables[it.b * c.table_stride + (blk >> c.sh)], blk, kvh);
+        at = kv_block(c, c.tables[it.b * c.table_stride + (blk >> c.sh)], blk, kv0);
+    const int64_t head = (int64_t)(KV_BLOCK * HD) << c.sh;      /* from a key head's block to the next one's */
 
     /* sine and cosine of the block's rows, once.  The angle is a double, less whole turns (2 pi as a sum of two
      * doubles): a far position's fraction of a turn keeps its bits, and the functions take a float in [-pi, pi]. */
@@ -147,8 +149,8 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
             }
             return p;
         };
-        const X *src = x + (int64_t)kvh * G * HD + M * sub;
-        T *dst = q + (int64_t)kvh * G * HD + M * sub;
+        const X *src = x + (int64_t)kv0 * a.G * HD + M * sub;
+        T *dst = q + (int64_t)kv0 * a.G * HD + M * sub;
         auto load = [&](float (&u)[M], float (&w)[M], At p) {
             if (p.t >= n) return;
             const X *v = src + p.t * a.xstride + p.j * HD;
@@ -173,46 +175,50 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
             p1 = next(p);
         }
     }
-    /* keys, a lane group a row */
-    if (at >= 0 && grp < n) {
-        float nw[2 * M], u[M], w[M];
+    if (at < 0) return;
+    /* keys, a lane group a row and head */
+    {
+        float nw[2 * M];
         weights(nw, a.kw);
-        const X *src = x + grp * a.xstride + (int64_t)(H + kvh) * HD + M * sub;
-        load_m<M>(u, src);
-        load_m<M>(w, src + HD / 2);
-        turn(u, w, nw, a.kw != nullptr, grp);
-        T *o = (T *)a.k + at;
-        const int pos = (int)(lo + grp - blk * KV_BLOCK);
-        if constexpr (16 % M == 0) {    /* M values of one piece */
-            store_m<M>(o + kv_key_at(pos, M * sub), u);
-            store_m<M>(o + kv_key_at(pos, HD / 2 + M * sub), w);
-        } else {
+        for (int i = grp; i < n * nh; i += 16) {
+            const int t = i / nh, j = i - t * nh;
+            float u[M], w[M];
+            const X *src = x + t * a.xstride + (int64_t)(H + kv0 + j) * HD + M * sub;
+            load_m<M>(u, src);
+            load_m<M>(w, src + HD / 2);
+            turn(u, w, nw, a.kw != nullptr, t);
+            T *o = (T *)a.k + at + j * head;
+            const int pos = (int)(lo + t - blk * KV_BLOCK);
+            if constexpr (16 % M == 0) {    /* M values of one piece */
+                store_m<M>(o + kv_key_at(pos, M * sub), u);
+                store_m<M>(o + kv_key_at(pos, HD / 2 + M * sub), w);
+            } else {
 #pragma unroll
-            for (int m = 0; m < M; m++) {
-                o[kv_key_at(pos, M * sub + m)] = (T)u[m];
-                o[kv_key_at(pos, HD / 2 + M * sub + m)] = (T)w[m];
+                for (int m = 0; m < M; m++) {
+                    o[kv_key_at(pos, M * sub + m)] = (T)u[m];
+                    o[kv_key_at(pos, HD / 2 + M * sub + m)] = (T)w[m];
+                }
             }
         }
     }
-    if (at < 0) return;
     /* values: a thread per value and half block.  (Read ahead of the angles they take the registers of a wave a SIMD and
      * the queries' loads wait behind them: 8192 rows 75 -> 82 us.) */
-    const X *src = x + (int64_t)(H + c.heads + kvh) * HD;
+    const X *src = x + (int64_t)(H + c.heads + kv0) * HD;
     const int first = (int)(lo - blk * KV_BLOCK), last = first + n;
-    T *o = (T *)a.v + at;
-    for (int i = tid; i < 2 * HD; i += 256) {
-        const int d = i % HD, half = i / HD * 8;
+    for (int i = tid; i < 2 * HD * nh; i += 256) {
+        const int j = i / (2 * HD), d = i % HD, half = i / HD % 2 * 8;
         if (half >= last || half + 8 <= first) continue;
+        T *o = (T *)a.v + at + j * head;
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            v[j] = half + j >= first && half + j < last ? to_f32(src[(half + j - first) * a.xstride + d]) : 0.0f;
+        for (int p = 0; p < 8; p++)
+            v[p] = half + p >= first && half + p < last ? to_f32(src[(half + p - first) * a.xstride + j * HD + d]) : 0.0f;
         if (half >= first && half + 8 <= last) {
             store_m<8>(o + kv_value_at(half, d), v);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (half + j >= first && half + j < last) o[kv_value_at(half + j, d)] = (T)v[j];
+            for (int p = 0; p < 8; p++)
+                if (half + p >= first && half + p < last) o[kv_value_at(half + p, d)] = (T)v[p];
         }
     }
 }
@@ -709,7 +715,11 @@ int tlm_hip_kv_append(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int 
     a.eps = eps;
     a.rope_scale = rope_scale;
     a.G = heads / c->kv_heads;
-    const dim3 grid((unsigned)items, (unsigned)c->kv_heads);
+    /* Two key heads a group share the rows' angles, worth it once the card is full without the second group: 8192 rows of
+     * 16 heads of 64 on 16 39.4 -> 30.6 us (four: 28.5), 32 of 128 on 32 101 -> 90 (four: 97), 1024 sequences of one row,
+     * 32 on 8, 22.6 -> 17.7 (four: 16.0); 64 of 64 on 8 45.3 -> 42.4 (four, 1024 groups: 50.9). */
+    a.hpg = items * c->kv_heads >= 2 * 2048 ? 2 : 1;
+    const dim3 grid((unsigned)items, (unsigned)((c->kv_heads + a.hpg - 1) / a.hpg));
     if (c->dt == DT_F16) append_x<_Float16>(dt, a, grid, (hipStream_t)stream);
     else append_x<__bf16>(dt, a, grid, (hipStream_t)stream);
     return tlmh_check(hipGetLastError(), "kv_append launch");
