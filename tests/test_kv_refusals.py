@@ -167,6 +167,31 @@ def test_python_refuses():
             fp8.add_rmsnorm(*a)
 
 
+def test_python_refuses_results_among_the_inputs():
+    """A result that overlaps the rows read, by a value at either end; one right behind or before passes this check (and
+    ends at the device's)."""
+    c = kv.Cache(4, 2, 64, page=16, dtype=torch.float16, device="cpu")
+    lens, tables, cu = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    m, n = 3 * 8 * 64, 3 * 12 * 64
+    flat = torch.zeros(2 * n + 64, dtype=torch.float16)
+    for at, match in ((0, "overlap"), (m - 1, "overlap"), (m, "device"), (m + 9, "device")):
+        for q, out in ((flat[:m], flat[at:at + m]), (flat[at:at + m], flat[:m])):
+            for call, more in ((kv.decode, ()), (kv.prompt, (cu,))):
+                with pytest.raises(ValueError, match=match):
+                    call(q.view(3, 8, 64), c, tables, lens, *more, out=out.view(3, 8, 64))
+    # rows further apart: their span counts, up to the last row's end
+    q = flat.as_strided((3, 8, 64), (600, 64, 1))
+    with pytest.raises(ValueError, match="overlap"):
+        kv.decode(q, c, tables, lens, out=flat[2 * 600 + 504:][:m].view(3, 8, 64))
+    with pytest.raises(ValueError, match="device"):
+        kv.decode(q, c, tables, lens, out=flat[2 * 600 + 512:][:m].view(3, 8, 64))
+    skip = -(flat.data_ptr() // 2) % 8                                   # append's result is 16-byte aligned
+    for at, match in ((0, "overlap"), (n - 8, "overlap"), (n, "device")):
+        with pytest.raises(ValueError, match=match):
+            kv.append(c, flat[skip:skip + n].view(3, 12 * 64), 8, tables, lens,
+                      out=flat[skip + at:skip + at + m].view(3, 8, 64))
+
+
 def test_places(tmp_path):
     exe = str(tmp_path / "places")
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover=all",

@@ -10,7 +10,7 @@ Sequence b's position p lies in page tables[b, p // page] (int32 [B, pages]); le
 the call's own rows, which are rows cu[b] .. cu[b + 1] - 1 (int32 [B + 1]; without cu, row b).  A length of 0 is a
 padded slot: nothing is written, attention gives zeros.  Page numbers outside the cache name no page, and what
 lies there is neither written nor seen.  Lengths, bounds and tables are read on the device: a captured
-graph follows them.
+graph follows them.  A result given as `out` lies apart from the rows that the call reads.
 
 Device memory is torch tensors on the current HIP device; work goes on torch's current stream.  Arguments that
 do not fit raise ValueError, sizes past a call's limits HipError, before anything is launched.
@@ -122,6 +122,13 @@ def _vector(t, n, dtype, what, dev):
     return t.data_ptr()
 
 
+def _apart(out, x, rows, stride, width):
+    """Refuses a result that begins or ends among the rows read: other groups may not have read theirs yet."""
+    a, b = x.data_ptr(), out.data_ptr()
+    if rows and a < b + out.numel() * out.element_size() and b < a + ((rows - 1) * stride + width) * x.element_size():
+        raise ValueError("out must not overlap the rows that the call reads")
+
+
 def append(cache, qkv, heads, tables, lens, cu=None, *, q_norm=None, k_norm=None, eps=1e-6, inv_freq=None,
            rope_scale=1.0, out=None):
     """Rows of q | k | v (float32, float16 or bfloat16 [T, (heads + 2 kv_heads) head_dim], any row stride): norms of
@@ -143,6 +150,8 @@ def append(cache, qkv, heads, tables, lens, cu=None, *, q_norm=None, k_norm=None
     elif out.shape != (T, heads, hd) or out.dtype is not cache.dtype or not out.is_contiguous() or \
             out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous {cache.dtype} [{T}, {heads}, {hd}], 16-byte aligned")
+    else:
+        _apart(out, qkv, T, qkv.stride(0), width)
     b = _batch(cache, T, tables, lens, cu, (qkv, out))
     rc = _append(cache._ref, C.byref(b), dt, qkv.data_ptr(), max(qkv.stride(0), width), heads, pq, pk, eps, pf,
                  rope_scale, out.data_ptr(), _raw_stream(dev))
@@ -178,6 +187,8 @@ def _queries(q, cache, scale, out, dtype):
             raise ValueError("dtype must be float32, float16 or bfloat16")
     elif out.shape != shape or out.dtype not in _TYPES or not out.is_contiguous():
         raise ValueError(f"out must be contiguous float32, float16 or bfloat16 {tuple(shape)}")
+    else:
+        _apart(out, q, T, stride, heads * hd)
     return T, stride, heads, scale, out
 
 
