@@ -224,7 +224,7 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
 }
 
 /* ---- decode --------------------------------------------------------------------
- * out = sum_j p_j v_j / sum_j p_j, p_j = 2^(scale log2(e) q . k_j - m), one pass over the cache with the running maximum m.
+ * out = sum_j p_j v_j / sum_j p_j, p_j = 2^(scale log2(e) (q . k_j - m)), one pass over the cache with the running maximum m.
  * A group takes a part of a sequence's positions for one key head and up to 16 NC of its queries; its NW waves take tiles
  * of 32 positions in turn, straight from memory into the matrix cores' operands (no LDS on the way), the next tile's
  * loads in flight, and merge their sums through LDS at the end.  The bytes of the cache bound it: 64 sequences of up to 8192,
@@ -399,29 +399,30 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
                 float top = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    z[j] = s[j >> 2][j & 3] * a.scale2;
+                    z[j] = s[j >> 2][j & 3];
                     if (!whole && j >= left) z[j] = -INFINITY;
                     top = fmaxf(top, z[j]);
                 }
-                if (__any(top > m[n] + KV_SLACK)) {
+                if (__any(kv_rises(top, m[n], a.scale2))) {
                     top = fmaxf(top, __shfl_xor(top, 16, 64));
                     top = fmaxf(top, __shfl_xor(top, 32, 64));
                     /* each column by its own scores: another's do not show in its bits */
-                    const float to = top > m[n] + KV_SLACK ? top : m[n], f = to == m[n] ? 1.0f : __builtin_amdgcn_exp2f(m[n] - to);
+                    const float to = kv_rises(top, m[n], a.scale2) ? top : m[n];
+                    const float f = to == m[n] ? 1.0f : kv_factor(m[n], to, a.scale2);
                     m[n] = to;
                     l[n] *= f;
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) o[n][dt] *= f;
                 }
                 /* before any score is above -infinity the maximum is taken as 0 */
-                const float base = (m[n] == -INFINITY ? 0.0f : m[n]) - KvType<T>::SHIFT;
+                const float base = m[n] == -INFINITY ? 0.0f : m[n];
                 /* Weights of 8 (bf16) or 11 bits, as the values that they are multiplied with have: a result is off by a third more
                  * than by its own rounding (bf16 2.2e-3 for 1.7e-3).  Two numbers a weight bring that back for 1 to 6% more
                  * time. */
                 x8 p;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float e = __builtin_amdgcn_exp2f(z[j] - base);
+                    const float e = __builtin_amdgcn_exp2f(fmaf(z[j] - base, a.scale2, KvType<T>::SHIFT));
                     l[n] += e;
                     p[j] = (T)e;
                 }
@@ -470,8 +471,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
 #pragma unroll
                 for (int n = 0; n < NC; n++) {
                     const float om = s_ml[wave][(n * 16 + col) * 2], ol = s_ml[wave][(n * 16 + col) * 2 + 1];
-                    const float to = fmaxf(m[n], om), base = to == -INFINITY ? 0.0f : to;
-                    const float fm = __builtin_amdgcn_exp2f(m[n] - base), fo = __builtin_amdgcn_exp2f(om - base);
+                    const float to = fmaxf(m[n], om);
+                    const float fm = kv_factor(m[n], to, a.scale2), fo = kv_factor(om, to, a.scale2);
                     m[n] = to;
                     l[n] = l[n] * fm + ol * fo;
 #pragma unroll
@@ -544,8 +545,7 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a)
             const int64_t w = (int64_t)kv_slot(w0 + i, i == 0) * H + head;
             const float mi = a.ml[2 * w], li = a.ml[2 * w + 1];
             const f32x4 oi = *(const f32x4 *)(a.part + w * HD + e);
-            const float to = fmaxf(m, mi), base = to == -INFINITY ? 0.0f : to;
-            const float f = __builtin_amdgcn_exp2f(m - base), fi = __builtin_amdgcn_exp2f(mi - base);
+            const float to = fmaxf(m, mi), f = kv_factor(m, to, a.scale2), fi = kv_factor(mi, to, a.scale2);
             o = o * f + oi * fi;
             l = l * f + li * fi;
             m = to;
@@ -562,11 +562,11 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a)
     if (r > 0 || hd >= a.hb || head >= H) return;
     float top = m;
     for (int i = 1; i < R; i++) top = fmaxf(top, s_ml[row + i][0]);
-    const float base = top == -INFINITY ? 0.0f : top, f = __builtin_amdgcn_exp2f(m - base);
+    const float f = kv_factor(m, top, a.scale2);
     o *= f;
     l *= f;
     for (int i = 1; i < R; i++) {
-        const float fi = __builtin_amdgcn_exp2f(s_ml[row + i][0] - base);
+        const float fi = kv_factor(s_ml[row + i][0], top, a.scale2);
         o += *(const f32x4 *)&s_o[row + i][e] * fi;
         l += s_ml[row + i][1] * fi;
     }

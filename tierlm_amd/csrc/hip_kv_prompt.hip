@@ -25,6 +25,9 @@ __device__ __forceinline__ void store_out(void *out, int dt, int64_t i, const fl
     else *(b4 *)((__bf16 *)out + i) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
 }
 
+/* Powers of two of weight from which a maximum is far */
+constexpr float KV_FAR = 4096.0f;
+
 /* What a page number outside the cache stands for: its positions are masked, and a finite value times weight 0 is 0 */
 __device__ const u32x4 kv_nothing[KV_BLOCK * 256 * 2 / 16] = {};
 
@@ -259,23 +262,33 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
         for (int t = 0; t < TP; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[t][r]);
-        top *= a.scale2;
-        if (__any(top > m + KV_SLACK)) {
+        if (__any(kv_rises(top, m, a.scale2))) {
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             /* each row by its own scores: another's do not show in its bits */
-            const float to = top > m + KV_SLACK ? top : m, f = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+            const float to = kv_rises(top, m, a.scale2) ? top : m, f = to == m ? 1.0f : kv_factor(m, to, a.scale2);
             m = to;
             l *= f;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) o[dt] *= f;
         }
-        const float sub = (m == -INFINITY ? 0.0f : m) - KvType<T>::SHIFT;
+        /* scale2 (s - m) + SHIFT.  Near 0 as one operation, scale2 s - (scale2 m - SHIFT), off by 2^-24 of the score; a row
+         * whose maximum is far takes the difference first (by itself: the others' bits stay). */
+        const float from = m == -INFINITY ? 0.0f : m, zfrom = from * a.scale2;
+        const bool far = fabsf(zfrom) > KV_FAR;
+        const float add = far ? KvType<T>::SHIFT : KvType<T>::SHIFT - zfrom;
+        if (__any(far)) {
+            const float first = far ? from : 0.0f;
+#pragma unroll
+            for (int t = 0; t < TP; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[t][r] -= first;
+        }
         x8 p[BLOCKS];
 #pragma unroll
         for (int t = 0; t < TP; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale2, -sub));
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale2, add));
                 l += e;
                 p[2 * t + (r >> 3)][r & 7] = (T)e;    /* as many bits as the values it is multiplied with */
             }
@@ -309,8 +322,8 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
         }
         __syncthreads();
         if (sg < half) {
-            const float om = ml[0][col], ol = ml[1][col], to = fmaxf(m, om), base = to == -INFINITY ? 0.0f : to;
-            const float fm = __builtin_amdgcn_exp2f(m - base), fo = __builtin_amdgcn_exp2f(om - base);
+            const float om = ml[0][col], ol = ml[1][col], to = fmaxf(m, om);
+            const float fm = kv_factor(m, to, a.scale2), fo = kv_factor(om, to, a.scale2);
             m = to;
             l = l * fm + ol * fo;
 #pragma unroll
@@ -394,8 +407,7 @@ template <int HD, int SG, int TP> __global__ __launch_bounds__(256) void k_kv_pr
             const int64_t at = at0 + (int64_t)i * ROWS + r;
             const float mi = a.ml[2 * at], li = a.ml[2 * at + 1];
             const f32x4 oi = *(const f32x4 *)(a.part + at * HD + e);
-            const float to = fmaxf(m, mi), base = to == -INFINITY ? 0.0f : to;
-            const float f = __builtin_amdgcn_exp2f(m - base), fi = __builtin_amdgcn_exp2f(mi - base);
+            const float to = fmaxf(m, mi), f = kv_factor(m, to, a.scale2), fi = kv_factor(mi, to, a.scale2);
             o = o * f + oi * fi;
             l = l * f + li * fi;
             m = to;

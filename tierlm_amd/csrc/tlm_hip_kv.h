@@ -134,6 +134,17 @@ template <> struct KvType<_Float16> {
  * scaled anew: the probabilities stay finite in either type and in the float sums, and most tiles scale nothing */
 constexpr float KV_SLACK = 6.0f;
 
+/* Running maxima are kept as scores are, before their scale: a difference of two scores is exact where it counts (within a
+ * factor of two of each other), so weights are 2^(scale2 (s - m) + SHIFT) whatever the scores' size.  (The scaled maximum
+ * rounded and then taken from an unrounded product leaves half a step of it: past 2^25 that is more than an exponent.)
+ *
+ * Does `top` rise over the maximum m by more than the slack (from -infinity: any score does)? */
+__device__ __forceinline__ bool kv_rises(float top, float m, float scale2) { return (top - m) * scale2 > KV_SLACK; }
+/* What scales sums kept by the maximum m where the maximum is `to` */
+__device__ __forceinline__ float kv_factor(float m, float to, float scale2) {
+    return __builtin_amdgcn_exp2f((m - (to == -INFINITY ? 0.0f : to)) * scale2);
+}
+
 template <class V> __device__ __forceinline__ V kv_bits(u32x4 v) { return __builtin_bit_cast(V, v); }
 
 /* 8 consecutive elements at any alignment of the type */
