@@ -368,6 +368,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
 
         f32x4 o[NC][DT];
         float m[NC], l[NC];
+        int seen = 0;        /* not 0: the wave's tiles hold a position */
 #pragma unroll
         for (int n = 0; n < NC; n++) {
             m[n] = -INFINITY;
@@ -378,6 +379,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
         auto compute = [&](Tile &t, int i) {
             const int p0 = begin + 32 * (wave + NW * i) + 8 * g;     /* the lane's first position */
             const bool whole = p0 - 8 * g + 32 <= stop && t.ok == 3;
+            seen |= t.ok;
             const int left = ((t.ok >> (g >> 1)) & 1) ? stop - p0 : 0;
             if (!whole) {    /* what a masked place holds may be anything, and 0 times it not 0 */
 #pragma unroll
@@ -450,6 +452,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
         for (int n = 0; n < NC; n++) {
             l[n] += __shfl_xor(l[n], 16, 64);
             l[n] += __shfl_xor(l[n], 32, 64);
+            if (seen) m[n] = fmaxf(m[n], KV_LOWEST);
         }
         /* merge the waves, half of them at a time, always in the same order */
 #pragma unroll
@@ -491,7 +494,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
                 if (h >= ncol) continue;
                 const int64_t head = kvh * a.G + col0 + h, H = (int64_t)a.G * c.heads;
                 if (take == units) {
-                    const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];     /* no position at all: zeros */
+                    const float inv = kv_inverse(l[n], m[n]);
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) {
                         const float v[4] = {o[n][dt][0] * inv, o[n][dt][1] * inv, o[n][dt][2] * inv, o[n][dt][3] * inv};
@@ -570,7 +573,7 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a)
         o += *(const f32x4 *)&s_o[row + i][e] * fi;
         l += s_ml[row + i][1] * fi;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = kv_inverse(l, top);
     const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     store_out(a.out, a.out_dt, ((int64_t)b * H + head) * HD + e, v);
 }

@@ -361,6 +361,21 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
             }
         }
     }
+    /* No weight at all, though the row reaches into the group's positions: is one of them a page's?  (rare) */
+    const int64_t from = (int64_t)t0 * POS;
+    if (__any(l == 0.0f && lim >= from)) {
+        const int last = BLOCKS * t1 - 1 < lastb ? BLOCKS * t1 - 1 : lastb;
+        int named = last + 1;          /* the first block that is */
+        for (int b0 = BLOCKS * t0; b0 <= last; b0 += 64) {
+            const int page = b0 + lane <= last ? table[(b0 + lane) >> c.sh] : -1;
+            const uint64_t in = __ballot((uint32_t)page < (uint32_t)c.n_pages);
+            if (in) {
+                named = b0 + __builtin_ctzll(in);
+                break;
+            }
+        }
+        if (l == 0.0f && named <= last && named * KV_BLOCK <= lim) m = KV_LOWEST;
+    }
     if (!real) return;
     if (PARTS && tiles > per) {
         const int64_t at = (((int64_t)w * c.heads + kvh) * a.parts + mypart) * ROWS + 32 * rg + col;
@@ -376,7 +391,7 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
         }
         return;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;    /* a row that sees nothing: zeros */
+    const float inv = kv_inverse(l, m);
     const int64_t at = ((rows.first + token) * H + kvh * G + (row - token * G)) * HD;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
@@ -413,7 +428,7 @@ template <int HD, int SG, int TP> __global__ __launch_bounds__(256) void k_kv_pr
             m = to;
         }
         const int row = pt.row0 + r, token = row / G;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = kv_inverse(l, m);
         const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
         store_out(a.out, a.out_dt, ((pt.rows.first + token) * H + kvh * G + (row - token * G)) * HD + e, v);
     }

@@ -144,6 +144,12 @@ __device__ __forceinline__ bool kv_rises(float top, float m, float scale2) { ret
 __device__ __forceinline__ float kv_factor(float m, float to, float scale2) {
     return __builtin_amdgcn_exp2f((m - (to == -INFINITY ? 0.0f : to)) * scale2);
 }
+/* A row that sees positions, all with a score of -infinity, has this maximum at the end of its pass: its weights are 0 / 0 and
+ * its result NaN.  One that sees none keeps -infinity, and gets zeros. */
+constexpr float KV_LOWEST = -3.4028234663852886e38f;
+__device__ __forceinline__ float kv_inverse(float l, float m) {
+    return l != 0.0f ? 1.0f / l : m == -INFINITY ? 0.0f : __builtin_nanf("");
+}
 
 template <class V> __device__ __forceinline__ V kv_bits(u32x4 v) { return __builtin_bit_cast(V, v); }
 
