@@ -695,7 +695,7 @@ int    tlm_hip_kv_append(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, i
  * j < lens[b], head h with key head h / (heads / kv_heads).  q in the cache's type (row b at q + b q_stride, heads
  * side by side), out [B][heads][head_dim] of out_dt (F32, F16 or BF16), overlapping no input; scale positive.  Sums, maxima and the softmax are
  * f32, its weights enter the second product rounded to the cache's type.  Positions that all have a score of -infinity give
- * NaN (0 / 0).  Sequences are split over their length as the batch's total asks, in the same way in every call with equal
+ * NaN (0 / 0); an infinite value gives that infinity whatever its weight's size (both infinities: NaN).  Sequences are split over their length as the batch's total asks, in the same way in every call with equal
  * lengths: a call repeats its bits.  workspace: tlm_hip_kv_decode_workspace_bytes bytes (0: none, by the sizes alone), 256-byte
  * aligned, nothing in it kept or zeroed; calls that may overlap need different ones. */
 size_t tlm_hip_kv_decode_workspace_bytes(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads);

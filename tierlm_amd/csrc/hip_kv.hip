@@ -454,6 +454,45 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
             l[n] += __shfl_xor(l[n], 32, 64);
             if (seen) m[n] = fmaxf(m[n], KV_LOWEST);
         }
+        /* sums that are not finite (and no score's doing): the wave's values that are not, each lane those that it holds in the
+         * operands, then to the lanes of their sums (rare) */
+        bool odd = false;
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            f32x4 z = {0, 0, 0, 0};
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) z[r] = fmaf(o[n][dt][r], 0.0f, z[r]);
+            const float none = z[0] + z[1] + (z[2] + z[3]);
+            odd |= none != none && l[n] == l[n];
+        }
+        if (__any(odd)) {
+            uint32_t found[DT] = {};
+#pragma unroll 1
+            for (int i = 0; i < mine; i++) {
+                if ((i & 31) == 0) names(i);
+                Tile t;
+                load(t, i);
+                const int left = ((t.ok >> (g >> 1)) & 1) ? stop - (begin + 32 * (wave + NW * i) + 8 * g) : 0;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int p = 0; p < 8; p++)
+                        found[dt] |= p < left ? kv_odd<T>(t.v[dt][p >> 1] >> 16 * (p & 1) & 0xFFFFu) : 0u;
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                found[dt] |= __shfl_xor(found[dt], 16, 64);
+                found[dt] |= __shfl_xor(found[dt], 32, 64);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t is = __shfl(found[dt], 4 * g + r, 64);
+#pragma unroll
+                    for (int n = 0; n < NC; n++) o[n][dt][r] = kv_put_odd(o[n][dt][r], is);
+                }
+            }
+        }
         /* merge the waves, half of them at a time, always in the same order */
 #pragma unroll
         for (int half = NW / 2; half >= 1; half >>= 1) {
@@ -478,10 +517,11 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
                     const float fm = kv_factor(m[n], to, a.scale2), fo = kv_factor(om, to, a.scale2);
                     m[n] = to;
                     l[n] = l[n] * fm + ol * fo;
+                    const float wm = kv_not_zero(fm), wo = kv_not_zero(fo);
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) {
                         const f32x4 w = *(const f32x4 *)&s_o[wave][(n * 16 + col) * LD + 16 * dt + 4 * g];
-                        o[n][dt] = o[n][dt] * fm + w * fo;
+                        o[n][dt] = o[n][dt] * wm + w * wo;
                     }
                 }
             }
@@ -549,7 +589,7 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a)
             const float mi = a.ml[2 * w], li = a.ml[2 * w + 1];
             const f32x4 oi = *(const f32x4 *)(a.part + w * HD + e);
             const float to = fmaxf(m, mi), f = kv_factor(m, to, a.scale2), fi = kv_factor(mi, to, a.scale2);
-            o = o * f + oi * fi;
+            o = o * kv_not_zero(f) + oi * kv_not_zero(fi);
             l = l * f + li * fi;
             m = to;
         }
@@ -566,11 +606,11 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a)
     float top = m;
     for (int i = 1; i < R; i++) top = fmaxf(top, s_ml[row + i][0]);
     const float f = kv_factor(m, top, a.scale2);
-    o *= f;
+    o *= kv_not_zero(f);
     l *= f;
     for (int i = 1; i < R; i++) {
         const float fi = kv_factor(s_ml[row + i][0], top, a.scale2);
-        o += *(const f32x4 *)&s_o[row + i][e] * fi;
+        o += *(const f32x4 *)&s_o[row + i][e] * kv_not_zero(fi);
         l += s_ml[row + i][1] * fi;
     }
     const float inv = kv_inverse(l, top);

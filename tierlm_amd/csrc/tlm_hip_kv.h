@@ -150,6 +150,25 @@ constexpr float KV_LOWEST = -3.4028234663852886e38f;
 __device__ __forceinline__ float kv_inverse(float l, float m) {
     return l != 0.0f ? 1.0f / l : m == -INFINITY ? 0.0f : __builtin_nanf("");
 }
+/* Values that are not finite come through whatever their weight, also where it or the factor that scales its sum rounds to 0
+ * (0 times infinity is NaN): sums that are not finite at the end have the values that made them so looked up and put in their
+ * place, and from then on keep them. */
+template <class T> __device__ __forceinline__ uint32_t kv_odd(uint32_t e) {   /* of a value's bits: 0 it is finite, 1 +inf, 2 -inf, 3 NaN */
+    constexpr uint32_t E = KvType<T>::EXP;
+    return (e & E) != E ? 0u : (e & 0x7FFFu) > E ? 3u : e >> 15 ? 2u : 1u;
+}
+__device__ __forceinline__ float kv_put_odd(float x, uint32_t odd) {         /* odd: of several values or-ed, both infinities are NaN */
+    return odd == 0 ? x : odd == 1 ? INFINITY : odd == 2 ? -INFINITY : __builtin_nanf("");
+}
+template <class T> __device__ __forceinline__ bool kv_any_odd(u32x4 v) {    /* of 8 values */
+    constexpr uint32_t E = KvType<T>::EXP;
+    bool odd = false;
+#pragma unroll
+    for (int w = 0; w < 4; w++) odd |= (v[w] & E) == E || (v[w] & (E << 16)) == E << 16;
+    return odd;
+}
+/* the factor for sums that may be infinite: at least 2^-149, which leaves an infinity and is nothing to a finite sum */
+__device__ __forceinline__ float kv_not_zero(float f) { return fmaxf(f, 0x1p-149f); }
 
 template <class V> __device__ __forceinline__ V kv_bits(u32x4 v) { return __builtin_bit_cast(V, v); }
 
