@@ -58,6 +58,23 @@ def _rows_ok(t):
     return (s1 == 1 or n == 1) and (s0 >= n or rows <= 1)
 
 
+def _rows_meet(a, b):
+    """Do two sets of rows (address, stride, width, count; bytes) share one?  No two rows of one set do."""
+    (pa, sa, wa, na), (pb, sb, wb, nb) = a, b
+    if not na or not nb or pa >= pb + (nb - 1) * sb + wb or pb >= pa + (na - 1) * sa + wa:
+        return False
+    if sa == sb and na == nb > 1:
+        d = (pb - pa) % sa              # the sets' spans overlap: so do two rows, or they lie side by side all along
+        return d < wa or d + wb > sa
+    if na > nb:
+        (pa, sa, wa, na), (pb, sb, wb, nb) = b, a
+    for p in range(pa, pa + na * sa, sa):
+        j = min((p + wa - 1 - pb) // sb, nb - 1)      # the last row of b that begins before this row's end
+        if j >= 0 and pb + j * sb + wb > p:
+            return True
+    return False
+
+
 def _out(t, shape, dtype, like, what):
     if t is None:
         return like.new_empty(shape, dtype=dtype)
@@ -123,11 +140,23 @@ def quantize(x, codes=None, scale=None):
     return codes, scale
 
 
+def _refuse_overlaps(place, read, given):
+    """place: the rows of the sum (None: not stored); read: those of weight, h and x; given: codes and scale."""
+    for i, r in enumerate(read if place else ()):
+        # h and x may be the place itself: a value is read by the thread that then writes it.  A weight is read later.
+        if _rows_meet(place, r) and (i == 0 or place != r):
+            raise ValueError("the sum's place must be h or x itself or not overlap what is read")
+    for g in given:
+        if any(_rows_meet(g, r) for r in read) or (place and _rows_meet(g, place)) or \
+                any(g is not o and _rows_meet(g, o) for o in given):
+            raise ValueError("codes and scale must not overlap what is read, the sum or each other")
+
+
 def add_rmsnorm(h, x, weight, eps=1e-6, out=None, codes=None, scale=None):
     """s = h + x (x None: h), rounded to h's dtype and stored in `out` (without it in h itself, the residual updated
     in place); returns the codes and scales of rmsnorm(s) weight as quantize() gives them.  h and x [T, n],
-    float32, float16 or bfloat16 each by itself, rows of any stride; weight float32 [n].  `out` is h or overlaps
-    neither."""
+    float32, float16 or bfloat16 each by itself, rows of any stride; weight float32 [n].  The sum's place may be h or x
+    itself; but for that nothing that is written (the sum, codes, scale) overlaps what is read."""
     shape = h.shape
     hdt = _TYPES.get(h.dtype)
     if hdt is None or len(shape) != 2 or not _rows_ok(h):
@@ -137,34 +166,54 @@ def add_rmsnorm(h, x, weight, eps=1e-6, out=None, codes=None, scale=None):
         raise ValueError("h must have at least one value a row")
     dev, po, px, xdt, xstride = h.get_device(), None, None, 0, 0
     here = dev >= 0 and dev == weight.get_device() == _current_device()
-    stride = ostride = max(h.stride(0), n)
+    stride = ostride = max(h.stride(0), n) if T > 1 else n
+    ph, pw, size = h.data_ptr(), weight.data_ptr(), h.element_size()
     if x is not None:
         xdt = _TYPES.get(x.dtype)
         if xdt is None or x.shape != shape or not _rows_ok(x):
             raise ValueError(f"x must be float32, float16 or bfloat16 [{T}, {n}] with contiguous rows")
-        px, xstride, po = x.data_ptr(), max(x.stride(0), n), h.data_ptr()
+        px, xstride, po = x.data_ptr(), max(x.stride(0), n) if T > 1 else n, ph
         here = here and x.get_device() == dev
     if weight.shape != (n,) or weight.dtype is not _F32 or not weight.is_contiguous():
         raise ValueError(f"weight must be contiguous float32 [{n}]")
     if out is not None:
         if out.shape != shape or out.dtype is not h.dtype or not _rows_ok(out):
             raise ValueError(f"out must be {h.dtype} [{T}, {n}] with contiguous rows")
-        po, ostride, here = out.data_ptr(), max(out.stride(0), n), here and out.get_device() == dev
-        if ostride != stride and T > 1 and po == h.data_ptr():
-            raise ValueError("out must be h itself or not overlap it")
+        po, ostride, here = out.data_ptr(), max(out.stride(0), n) if T > 1 else n, here and out.get_device() == dev
+    # spans that meet, but for the sum's over h's, are looked at row by row
     nb = -(-n // BLOCK)
+    hend, xend, wend, apart = ph + T * stride * size, 0 if px is None else px + 4 * T * xstride, pw + 4 * n, True
+    if po is not None:
+        end = po + T * ostride * size
+        apart = (po == ph and ostride == stride or ph >= end or po >= hend) and (px is None or px >= end or po >= xend) and \
+            (pw >= end or po >= wend)
     if codes is None:
         codes = h.new_empty((T, nb * BLOCK), dtype=E4M3)
     else:
         here = _out(codes, (T, nb * BLOCK), E4M3, h, "codes").get_device() == dev and here
+        a = codes.data_ptr()
+        b = a + T * nb * BLOCK
+        apart = apart and (b <= ph or a >= hend) and (px is None or b <= px or a >= xend) and (b <= pw or a >= wend) and \
+            (po is None or b <= po or a >= end)
     if scale is None:
         scale = weight.new_empty((T, nb))
     else:
         here = _out(scale, (T, nb), _F32, h, "scale").get_device() == dev and here
+        a = scale.data_ptr()
+        b, c = a + 4 * T * nb, codes.data_ptr()
+        apart = apart and (b <= ph or a >= hend) and (px is None or b <= px or a >= xend) and (b <= pw or a >= wend) and \
+            (po is None or b <= po or a >= end) and (b <= c or a >= c + T * nb * BLOCK)
+    if not apart:
+        read = [(pw, 4 * n, 4 * n, 1), (ph, stride * size, n * size, T)]
+        if px is not None:
+            read.append((px, xstride * x.element_size(), n * x.element_size(), T))
+        _refuse_overlaps((po, ostride * size, n * size, T) if po is not None else None, read,
+                         [(t.data_ptr(), t.numel() * t.element_size(), t.numel() * t.element_size(), min(T, 1))
+                          for t in (codes, scale)])
     if not here:
         _here(*(t for t in (h, x, weight, out, codes, scale) if t is not None))
-    rc = _add_rmsnorm(hdt, h.data_ptr(), stride, xdt, px, xstride, weight.data_ptr(), eps, n, T, po, ostride,
-                      codes.data_ptr(), scale.data_ptr(), _raw_stream(dev))
+    rc = _add_rmsnorm(hdt, ph, stride, xdt, px, xstride, pw, eps, n, T, po, ostride, codes.data_ptr(),
+                      scale.data_ptr(), _raw_stream(dev))
     if rc:
         check(rc)
     return codes, scale
