@@ -521,9 +521,6 @@ const Kernel &choose(int64_t rows, int nb, int64_t T) {
     return KERNELS[pick];
 }
 
-bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
-
 }  // namespace
 
 /* Row and length limits keep every launch inside the grid limits; sizes in bytes

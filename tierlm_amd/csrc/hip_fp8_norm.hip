@@ -140,9 +140,6 @@ template <class X> void launch_h(int hdt, const NormArgs &a, int64_t T, hipStrea
     else launch<X, __bf16>(a, T, s);
 }
 
-bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
-
 } // namespace
 
 extern "C" int tlm_hip_fp8_add_rmsnorm(int hdt, const void *h, int64_t hstride, int xdt, const void *x,

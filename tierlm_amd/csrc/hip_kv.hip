@@ -5,9 +5,6 @@
 
 namespace {
 
-bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
-
 /* ---- append ------------------------------------------------------------------
  * A group per block of 16 positions and hpg key heads, one or two: its up to 16 new rows of those heads' queries, keys and
  * values.  16 lanes hold a vector: lane s the pairs j = M s .. M s + M - 1 and their partners at hd / 2 + j (M = hd / 32),
@@ -246,15 +243,6 @@ struct DecodeArgs {
     int G, W, out_dt;
     int hb;                  /* heads of a group of the join */
 };
-
-__device__ __forceinline__ void store_out(void *out, int dt, int64_t i, const float (&v)[4]) {
-    typedef _Float16 h4 __attribute__((ext_vector_type(4), aligned(2)));
-    typedef __bf16 b4 __attribute__((ext_vector_type(4), aligned(2)));
-    typedef f32x4 f4 __attribute__((aligned(4)));
-    if (dt == DT_F32) *(f4 *)((float *)out + i) = f4{v[0], v[1], v[2], v[3]};
-    else if (dt == DT_F16) *(h4 *)((_Float16 *)out + i) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-    else *(b4 *)((__bf16 *)out + i) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-}
 
 __device__ __forceinline__ int decode_len(const KvView &c, int b) {
     const int64_t len = kv_len(c, b), cap = kv_cap(c);
@@ -538,7 +526,7 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) {
                         const float v[4] = {o[n][dt][0] * inv, o[n][dt][1] * inv, o[n][dt][2] * inv, o[n][dt][3] * inv};
-                        store_out(a.out, a.out_dt, (b * H + head) * HD + 16 * dt + 4 * g, v);
+                        kv_store(a.out, a.out_dt, (b * H + head) * HD + 16 * dt + 4 * g, v);
                     }
                 } else {
                     const int64_t w = kv_slot(worker, first == 0) * H + head;
@@ -615,7 +603,7 @@ template <int HD> __global__ __launch_bounds__(256) void k_kv_join(DecodeArgs a)
     }
     const float inv = kv_inverse(l, top);
     const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-    store_out(a.out, a.out_dt, ((int64_t)b * H + head) * HD + e, v);
+    kv_store(a.out, a.out_dt, ((int64_t)b * H + head) * HD + e, v);
 }
 
 /* ---- launches -------------------------------------------------------------- */
@@ -690,7 +678,6 @@ template <class T> void decode(const DecodeArgs &a, const DecodePlan &p, hipStre
 
 } // namespace
 
-/* What all three calls ask of a cache and a batch; *v is filled for the kernels */
 int kv_check(const char *who, const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads, KvView *v) {
     if (!c || !b) return tlmh_seterr(TLM_HIP_EINVAL, "%s: NULL argument", who);
     if (c->dt != DT_F16 && c->dt != DT_BF16)

@@ -2,8 +2,6 @@
  * step per prompt token, src/lib/tlm_model.c:1105-1113, attn_heads :683-749).  Layout and work items: tlm_hip_kv.h. */
 #include "tlm_hip_kv.h"
 
-int kv_check(const char *who, const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads, KvView *v);
-
 namespace {
 
 struct PromptArgs {
@@ -15,15 +13,6 @@ struct PromptArgs {
     float scale2;            /* scale log2(e) */
     int G, out_dt, parts;
 };
-
-__device__ __forceinline__ void store_out(void *out, int dt, int64_t i, const float (&v)[4]) {
-    typedef _Float16 h4 __attribute__((ext_vector_type(4), aligned(2)));
-    typedef __bf16 b4 __attribute__((ext_vector_type(4), aligned(2)));
-    typedef f32x4 f4 __attribute__((aligned(4)));
-    if (dt == DT_F32) *(f4 *)((float *)out + i) = f4{v[0], v[1], v[2], v[3]};
-    else if (dt == DT_F16) *(h4 *)((_Float16 *)out + i) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-    else *(b4 *)((__bf16 *)out + i) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-}
 
 /* Powers of two of weight from which a maximum is far */
 constexpr float KV_FAR = 4096.0f;
@@ -428,7 +417,7 @@ __global__ __launch_bounds__(256, (SG == 4 && HD > 64) || (SG == 2 && HD > 128) 
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const float v[4] = {o[dt][4 * r] * inv, o[dt][4 * r + 1] * inv, o[dt][4 * r + 2] * inv, o[dt][4 * r + 3] * inv};
-            store_out(a.out, a.out_dt, at + 32 * dt + 8 * r + 4 * h, v);
+            kv_store(a.out, a.out_dt, at + 32 * dt + 8 * r + 4 * h, v);
         }
 }
 
@@ -460,7 +449,7 @@ template <int HD, int SG, int TP> __global__ __launch_bounds__(256) void k_kv_pr
         const int row = pt.row0 + r, token = row / G;
         const float inv = kv_inverse(l, m);
         const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-        store_out(a.out, a.out_dt, ((pt.rows.first + token) * H + kvh * G + (row - token * G)) * HD + e, v);
+        kv_store(a.out, a.out_dt, ((pt.rows.first + token) * H + kvh * G + (row - token * G)) * HD + e, v);
     }
 }
 
@@ -515,9 +504,6 @@ template <class T> void prompt(const PromptArgs &a, const PromptPlan &p, hipStre
         launch<T, 160>, launch<T, 192>, launch<T, 224>, launch<T, 256>};
     by_width[a.c.hd / 32 - 1](a, p, s);
 }
-
-bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
 
 } // namespace
 

@@ -33,6 +33,9 @@ enum { FAILED_KV = 27, FAILED_FP8 = 28, FAILED_PRODUCTS = 29, FAILED_EXP = 30 };
 void tlmh_set_failed(int mask);
 /* TLM_HIP_OK, or the error of a call whose kernels failed the self-test */
 int tlmh_refuse_failed(int bit, const char *who);
+/* what the entries check of pointers and of the types that they take as float, binary16 or bfloat16 (0: none of them) */
+static inline bool aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+static inline int type_bytes(int dt) { return dt == DT_F32 ? 4 : dt == DT_F16 || dt == DT_BF16 ? 2 : 0; }
 #define HIPCHK(call) do { hipError_t _e = (call); if (_e != hipSuccess) return tlmh_check(_e, #call); } while (0)
 
 /* ---- format geometry (host + device) ------------------------------------ */

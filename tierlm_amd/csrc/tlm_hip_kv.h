@@ -99,6 +99,9 @@ TLM_HD int64_t kv_prompt_most(int64_t rows, int64_t B, int64_t group, int64_t ti
 }
 
 #ifdef __HIPCC__
+/* What all calls ask of a cache and a batch; *v is filled for the kernels (hip_kv.hip) */
+int kv_check(const char *who, const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads, KvView *v);
+
 /* constant memory: what no launch under way writes; uniform reads go through the scalar cache */
 #define CAS __attribute__((address_space(4)))
 
@@ -169,6 +172,16 @@ template <class T> __device__ __forceinline__ bool kv_any_odd(u32x4 v) {    /* o
 }
 /* the factor for sums that may be infinite: at least 2^-149, which leaves an infinity and is nothing to a finite sum */
 __device__ __forceinline__ float kv_not_zero(float f) { return fmaxf(f, 0x1p-149f); }
+
+/* four values of a result, rounded to its type */
+__device__ __forceinline__ void kv_store(void *out, int dt, int64_t i, const float (&v)[4]) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef __bf16 b4 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef f32x4 f4 __attribute__((aligned(4)));
+    if (dt == DT_F32) *(f4 *)((float *)out + i) = f4{v[0], v[1], v[2], v[3]};
+    else if (dt == DT_F16) *(h4 *)((_Float16 *)out + i) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    else *(b4 *)((__bf16 *)out + i) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+}
 
 template <class V> __device__ __forceinline__ V kv_bits(u32x4 v) { return __builtin_bit_cast(V, v); }
 
