@@ -9,7 +9,8 @@
  * Q6_K and Q8_K, the exponential against this host's libm expf, the
  * matrix cores' float products against v_mul_f32, and the 8-bit floating-point
  * quantiser (codes and scales) and product (within the roundings of a float sum),
- * at one size, of the row groups.
+ * at one size, of the row groups; the paged cache in both types at every head width, and a prompt's and a decode step's ways
+ * through their launches at one width or two each.
  * Returns the number of failing kernels; bit dt of *mask is set for every dtype
  * whose kernels failed, FAILED_EXP for the exponential, FAILED_PRODUCTS for the
  * products, FAILED_FP8 for 8-bit floating point, FAILED_KV for the paged cache. */
@@ -358,30 +359,46 @@ double from_half(int dt, uint16_t h) {
     return f;
 }
 
-/* The paged cache: two sequences (19 rows, and 3 behind 20 positions that a first call appended) of 4 heads on 2 of 32,
- * with norms and rotation; their attention as prompts, and of the last rows alone, whole and in shares (a wide table). */
-bool kv_ok(uint32_t *s) {
-    constexpr int H = 4, KV = 2, HD = 32, PAGE = 16, PAGES = 5, WIDE = 40, ROW = (H + 2 * KV) * HD, B = 2, FIRST = 20, T = 22;
-    const int n[B] = {19, 3}, len[B] = {19, 23}, table[B][3] = {{4, 1, -1}, {0, 3, -1}};
-    const size_t cache = (size_t)PAGES * KV * PAGE * HD * 2, ws = (size_t)2 * 256 * H * (HD + 4) * 4;
-    const size_t o_k = ((size_t)(FIRST + T) * ROW * 4 + 255) & ~(size_t)255, o_v = o_k + cache, o_q = o_v + cache,
-                 o_y = o_q + 16384, o_i = o_y + 16384, o_w = o_i + 4096;
-    std::vector<float> x((FIRST + T) * ROW), norm(2 * HD), gy(T * H * HD), gd(B * H * HD);
-    std::vector<double> freq(HD / 2);
+/* The paged cache: two sequences (19 rows, and 3 behind `past` positions that a first call appended) with norms and rotation;
+ * their attention as prompts, and of the last rows alone, each with tables of their length and with far-reaching ones. */
+struct KvShape {
+    int H, KV, HD, past, each;      /* every each-th head is compared */
+};
+bool kv_shape_ok(uint32_t *s, const KvShape &shape) {
+    constexpr int PAGE = 16, WIDE = 128, B = 2;
+    const int H = shape.H, KV = shape.KV, HD = shape.HD, FIRST = shape.past, G = H / KV, ROW = (H + 2 * KV) * HD;
+    const int n[B] = {19, 3}, len[B] = {19, FIRST + 3}, T = n[0] + n[1], need = (len[1] + PAGE - 1) / PAGE, PAGES = 2 + need + 1;
+    const float scale = 1.0f / sqrtf((float)HD);
+    std::vector<float> x((size_t)(FIRST + T) * ROW), norm(2 * HD), gy(T * H * HD), gd(B * H * HD);
+    std::vector<double> freq(HD / 2), turn((size_t)len[1] * HD);
     std::vector<int32_t> ints(8 + B * WIDE, -1);
     std::vector<uint16_t> gq(T * H * HD);
     for (auto &e : x) e = (float)(st_rng(s) & 0xFFFF) / 16384.0f - 2.0f;
     for (auto &e : norm) e = 0.5f + (float)(st_rng(s) & 0xFF) / 256.0f;
     for (int j = 0; j < HD / 2; j++) freq[j] = pow(1e4, -2.0 * j / HD);
+    for (int p = 0; p < len[1]; p++)
+        for (int j = 0; j < HD / 2; j++) {
+            turn[p * HD + j] = cos(p * freq[j]);
+            turn[p * HD + HD / 2 + j] = sin(p * freq[j]);
+        }
     const int32_t head[8] = {0, n[0], T, len[0], len[1], 0, FIRST, FIRST};   /* cu, lens; the first call's cu and length */
     for (int i = 0; i < 8; i++) ints[i] = head[i];
-    for (int b = 0; b < B; b++)
-        for (int i = 0; i < 3; i++) ints[8 + b * WIDE + i] = table[b][i];
+    for (int i = 0; i < 2 + need; i++) ints[8 + (i < 2 ? i : WIDE + i - 2)] = (7 * i + 3) % PAGES;       /* 13 or 5 pages */
+    const size_t ALIGN = 255, cache = ((size_t)PAGES * KV * PAGE * HD * 2 + ALIGN) & ~ALIGN;
+    const size_t rows = (size_t)(FIRST > T ? FIRST : T) * H * HD;
+    const int32_t *any = ints.data();        /* the sizes decide, not what is there */
+    const tlm_hip_kv_cache sizes = {DT_F16, KV, HD, PAGE, PAGES, (void *)256, (void *)256};
+    const tlm_hip_kv_batch wide_p = {B, T, any, any, any, WIDE, WIDE}, wide_d = {B, B, nullptr, any, any, WIDE, WIDE};
+    size_t ws = 256;
+    for (const size_t w : {tlm_hip_kv_prompt_workspace_bytes(&sizes, &wide_p, H), tlm_hip_kv_decode_workspace_bytes(&sizes, &wide_d, H)})
+        ws = w > ws ? w : ws;
+    const size_t o_k = (x.size() * 4 + ALIGN) & ~ALIGN, o_v = o_k + cache, o_q = o_v + cache, o_y = o_q + ((rows * 2 + ALIGN) & ~ALIGN),
+                 o_i = o_y + ((gy.size() * 4 + ALIGN) & ~ALIGN), o_w = o_i + 8192;
     uint8_t *dev = nullptr;
     if (hipMalloc((void **)&dev, o_w + ws) != hipSuccess) return false;
     const int32_t *di = (const int32_t *)(dev + o_i);
-    double *df = (double *)(dev + o_i + 1024);
-    float *dn = (float *)(dev + o_i + 2048), *dx = (float *)dev;
+    double *df = (double *)(dev + o_i + 4096);
+    float *dn = (float *)(dev + o_i + 4096 + 2048), *dx = (float *)dev;
     void *q = dev + o_q, *y = dev + o_y;
     bool ok = hipMemcpy(dx, x.data(), x.size() * 4, hipMemcpyHostToDevice) == hipSuccess &&
               hipMemcpy(dev + o_i, ints.data(), ints.size() * 4, hipMemcpyHostToDevice) == hipSuccess &&
@@ -391,90 +408,92 @@ bool kv_ok(uint32_t *s) {
     auto turned = [&](const float *src, const float *w, int pos, double *o) {
         double ss = 0.0;
         for (int i = 0; i < HD; i++) ss += (double)src[i] * src[i];
-        const double r = 1.0 / sqrt(ss / HD + 1e-6);
+        const double r = 1.0 / sqrt(ss / HD + 1e-6), *c = &turn[(size_t)pos * HD], *sn = c + HD / 2;
         for (int j = 0; j < HD / 2; j++) {
-            const double a = src[j] * r * w[j], d = src[HD / 2 + j] * r * w[HD / 2 + j], ang = pos * freq[j];
-            o[j] = a * cos(ang) - d * sin(ang);
-            o[HD / 2 + j] = d * cos(ang) + a * sin(ang);
+            const double a = src[j] * r * w[j], d = src[HD / 2 + j] * r * w[HD / 2 + j];
+            o[j] = a * c[j] - d * sn[j];
+            o[HD / 2 + j] = d * c[j] + a * sn[j];
         }
     };
     for (int dt : {DT_F16, DT_BF16}) {
         const double half = dt == DT_F16 ? 0x1p-11 : 0x1p-8;
         const tlm_hip_kv_cache c = {dt, KV, HD, PAGE, PAGES, dev + o_k, dev + o_v};
-        const tlm_hip_kv_batch first = {1, FIRST, di + 5, di + 7, di + 8 + WIDE, WIDE, 3}, b = {B, T, di, di + 3, di + 8, WIDE, 3};
+        const tlm_hip_kv_batch first = {1, FIRST, di + 5, di + 7, di + 8 + WIDE, WIDE, need}, b = {B, T, di, di + 3, di + 8, WIDE, need};
         ok = ok && tlm_hip_kv_append(&c, &first, DT_F32, dx, ROW, H, dn, dn + HD, 1e-6f, df, 1.0f, q, nullptr) == TLM_HIP_OK &&
-             tlm_hip_kv_append(&c, &b, DT_F32, dx + FIRST * ROW, ROW, H, dn, dn + HD, 1e-6f, df, 1.0f, q, nullptr) == TLM_HIP_OK &&
-             tlm_hip_kv_prompt(&c, &b, q, H * HD, H, 0.25f, DT_F32, y, nullptr, nullptr) == TLM_HIP_OK &&
-             hipMemcpy(gq.data(), q, gq.size() * 2, hipMemcpyDeviceToHost) == hipSuccess &&
-             hipMemcpy(gy.data(), y, gy.size() * 4, hipMemcpyDeviceToHost) == hipSuccess;
-        if (!ok) break;
-        std::vector<double> k[B], v[B];
-        for (int i = 0; i < B; i++) {
-            k[i].resize(len[i] * KV * HD);
-            v[i].resize(len[i] * KV * HD);
-            for (int p = 0; p < len[i]; p++) {
-                const float *row = x.data() + (i == 0 ? FIRST + p : p < FIRST ? p : FIRST + n[0] + p - FIRST) * ROW;
-                for (int h = 0; h < KV; h++) {
-                    double *o = &k[i][(p * KV + h) * HD];
-                    turned(row + (H + h) * HD, norm.data() + HD, p, o);
-                    for (int e = 0; e < HD; e++) {
-                        o[e] = to_half(dt, o[e]);
-                        v[i][(p * KV + h) * HD + e] = to_half(dt, row[(H + KV + h) * HD + e]);
-                    }
-                }
-            }
+             tlm_hip_kv_append(&c, &b, DT_F32, dx + (size_t)FIRST * ROW, ROW, H, dn, dn + HD, 1e-6f, df, 1.0f, q, nullptr) == TLM_HIP_OK &&
+             hipMemcpy(gq.data(), q, gq.size() * 2, hipMemcpyDeviceToHost) == hipSuccess;
+        /* Every row and each last row's results, of the heads compared.  A query is within a half step of its definition, f32
+         * roundings beside it.  A key next to the border of two steps may be the other one here: a step (two half ones) of each
+         * product of a score, so a weight is off by twice the largest score's steps; and each weight is rounded once. */
+        std::vector<double> k((size_t)len[1] * HD), v(k.size()), e(len[1]), qv(HD);
+        std::vector<float> got[4];       /* prompts, last rows; tables of the length and wide ones */
+        for (int i = 0; ok && i < 4; i++) {
+            const int pages = i & 1 ? WIDE : need;
+            const tlm_hip_kv_batch all = {B, T, di, di + 3, di + 8, WIDE, pages}, last = {B, B, nullptr, di + 3, di + 8, WIDE, pages};
+            got[i].resize((size_t)(i < 2 ? T : B) * H * HD);
+            ok = (i < 2 ? tlm_hip_kv_prompt(&c, &all, q, H * HD, H, scale, DT_F32, y, dev + o_w, nullptr)
+                        : tlm_hip_kv_decode(&c, &last, (const uint16_t *)q + (n[0] - 1) * H * HD, n[1] * H * HD, H, scale, DT_F32, y,
+                                            dev + o_w, nullptr)) == TLM_HIP_OK &&
+                 hipMemcpy(got[i].data(), y, got[i].size() * 4, hipMemcpyDeviceToHost) == hipSuccess;
         }
-        /* Row t of the call, at position p of sequence i.  A query is within a half step of its definition, f32 roundings beside it.
-         * A key next to the border of two steps may be the other one here: a step (two half ones) of each product of a score, so a
-         * weight is off by twice the largest score's steps; and each weight is rounded once. */
-        auto check = [&](const float *got, int i, int t, int p) {
-            for (int h = 0; h < H; h++) {
-                double qv[HD], e[32], top = -1e300, sum = 0.0, size = 0.0;
-                turned(x.data() + (FIRST + t) * ROW + h * HD, norm.data(), p, qv);
-                for (int d = 0; d < HD; d++) {
-                    const double g = from_half(dt, gq[(t * H + h) * HD + d]);
-                    ok = ok && fabs(g - qv[d]) <= half * fabs(qv[d]) + 1e-5;
-                    qv[d] = g;
-                }
-                for (int j = 0; j <= p; j++) {
-                    double mag = e[j] = 0.0;
+        for (int h = 0; ok && h < H; h += shape.each)
+            for (int i = 0, t0 = 0; i < B; t0 += n[i++]) {
+                for (int p = 0; p < len[i]; p++) {
+                    const float *row = x.data() + (size_t)(i == 0 ? FIRST + p : p < FIRST ? p : FIRST + n[0] + p - FIRST) * ROW;
+                    turned(row + (H + h / G) * HD, norm.data() + HD, p, &k[p * HD]);
                     for (int d = 0; d < HD; d++) {
-                        const double u = qv[d] * k[i][(j * KV + h / 2) * HD + d] * 0.25;
-                        e[j] += u;
-                        mag += fabs(u);
+                        k[p * HD + d] = to_half(dt, k[p * HD + d]);
+                        v[p * HD + d] = to_half(dt, row[(H + KV + h / G) * HD + d]);
                     }
-                    top = fmax(top, e[j]);
-                    size = fmax(size, mag);
                 }
-                for (int j = 0; j <= p; j++) sum += e[j] = exp(e[j] - top);
-                for (int d = 0; d < HD; d++) {
-                    double o = 0.0, mag = 0.0;
-                    for (int j = 0; j <= p; j++) {
-                        const double u = e[j] / sum * v[i][(j * KV + h / 2) * HD + d];
-                        o += u;
-                        mag += fabs(u);
+                for (int r = 0; r < n[i]; r++) {
+                    const int t = t0 + r, p = len[i] - n[i] + r;
+                    double top = -1e300, sum = 0.0, size = 0.0;
+                    turned(x.data() + (size_t)(FIRST + t) * ROW + h * HD, norm.data(), p, qv.data());
+                    for (int d = 0; d < HD; d++) {
+                        const double g = from_half(dt, gq[(t * H + h) * HD + d]);
+                        ok = ok && fabs(g - qv[d]) <= half * fabs(qv[d]) + 1e-5;
+                        qv[d] = g;
                     }
-                    ok = ok && fabs(got[h * HD + d] - o) <= mag * (half * (1.0 + 4.0 * size) + 1e-5) + 1e-6;
+                    for (int j = 0; j <= p; j++) {
+                        double mag = e[j] = 0.0;
+                        for (int d = 0; d < HD; d++) {
+                            const double u = qv[d] * k[j * HD + d] * scale;
+                            e[j] += u;
+                            mag += fabs(u);
+                        }
+                        top = fmax(top, e[j]);
+                        size = fmax(size, mag);
+                    }
+                    for (int j = 0; j <= p; j++) sum += e[j] = exp(e[j] - top);
+                    for (int d = 0; d < HD; d++) {
+                        double o = 0.0, mag = 0.0;
+                        for (int j = 0; j <= p; j++) {
+                            const double u = e[j] / sum * v[j * HD + d];
+                            o += u;
+                            mag += fabs(u);
+                        }
+                        const double tol = mag * (half * (1.0 + 4.0 * size) + 1e-5) + 1e-6;
+                        for (int a = 0; a < (r == n[i] - 1 ? 4 : 2); a++)
+                            ok = ok && fabs(got[a][((size_t)(a < 2 ? t : i) * H + h) * HD + d] - o) <= tol;
+                    }
                 }
             }
-        };
-        for (int i = 0, t = 0; i < B; i++)
-            for (int r = 0; r < n[i]; r++, t++) check(&gy[t * H * HD], i, t, len[i] - n[i] + r);
-        /* the last row of each sequence: rows n[0] - 1 and n[0] + n[1] - 1 */
-        for (int pages : {3, WIDE}) {
-            const tlm_hip_kv_batch last = {B, B, nullptr, di + 3, di + 8, WIDE, pages};
-            ok = ok && tlm_hip_kv_decode_workspace_bytes(&c, &last, H) <= ws &&
-                 tlm_hip_kv_decode(&c, &last, (const uint16_t *)q + (n[0] - 1) * H * HD, n[1] * H * HD, H, 0.25f, DT_F32, y,
-                                   dev + o_w, nullptr) == TLM_HIP_OK &&
-                 hipMemcpy(gd.data(), y, gd.size() * 4, hipMemcpyDeviceToHost) == hipSuccess;
-            if (!ok) break;
-            check(&gd[0], 0, n[0] - 1, len[0] - 1);
-            check(&gd[H * HD], 1, T - 1, len[1] - 1);
-        }
     }
     (void)hipDeviceSynchronize();
     (void)hipFree(dev);
     return ok;
+}
+/* Every head width, in shares and parts; then enough key heads that a prompt's group takes 64 rows (narrow and wide heads) and
+ * 128, and more than 16 queries a key head. */
+bool kv_ok(uint32_t *s) {
+    static const KvShape shapes[] = {
+        {4, 2, 32, 150, 1},  {4, 2, 64, 150, 1},   {6, 3, 96, 150, 1},    {8, 2, 128, 150, 1},   {2, 1, 160, 150, 1},  {2, 2, 192, 150, 1},
+        {3, 1, 224, 150, 1}, {4, 2, 256, 150, 1},  {34, 1, 64, 150, 11},  {80, 80, 64, 20, 27},  {40, 40, 128, 20, 13},
+        {260, 260, 32, 20, 87}, {130, 130, 160, 20, 43}};
+    for (const KvShape &shape : shapes)
+        if (!kv_shape_ok(s, shape)) return false;
+    return true;
 }
 
 }  // namespace
