@@ -97,14 +97,36 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
     const int sub = tid & 15, grp = tid >> 4;
     auto turn = [&](float (&u)[M], float (&w)[M], const float (&nw)[2 * M], bool norm, int t) {
         if (norm) {
-            float ss = 0.0f;
+            auto mean = [&](float eps) {
+                float ss = 0.0f;
 #pragma unroll
-            for (int m = 0; m < M; m++) ss = fmaf(u[m], u[m], fmaf(w[m], w[m], ss));
-            ss += dpp_f32<DPP_XOR1>(ss);
-            ss += dpp_f32<DPP_XOR2>(ss);
-            ss += dpp_f32<DPP_HALF_MIRROR>(ss);
-            ss += dpp_f32<DPP_MIRROR>(ss);
-            const float f = rsqrtf(fmaf(ss, 1.0f / HD, a.eps));
+                for (int m = 0; m < M; m++) ss = fmaf(u[m], u[m], fmaf(w[m], w[m], ss));
+                ss += dpp_f32<DPP_XOR1>(ss);
+                ss += dpp_f32<DPP_XOR2>(ss);
+                ss += dpp_f32<DPP_HALF_MIRROR>(ss);
+                ss += dpp_f32<DPP_MIRROR>(ss);
+                return fmaf(ss, 1.0f / HD, eps);
+            };
+            float s = mean(a.eps);
+            const bool odd = !(s > 0x1p-100f && s < 0x1p100f);
+            if (__any(odd)) {
+                /* squares past a float: that vector times a power of two that brings its largest value near 1 (or to 2^-49: no
+                 * further than eps's own square stays finite), which the result does not show (rare) */
+                uint32_t top = 0;
+#pragma unroll
+                for (int m = 0; m < M; m++) {
+                    const uint32_t x = __float_as_uint(u[m]) & 0x7FFFFFFFu, y = __float_as_uint(w[m]) & 0x7FFFFFFFu;
+                    top = max(top, max(x, y));
+                }
+                const int e = odd ? max((int)(group_max_u32<16>(top) >> 23) - 127, -100) : 0;
+#pragma unroll
+                for (int m = 0; m < M; m++) {
+                    u[m] = ldexpf(u[m], -e);
+                    w[m] = ldexpf(w[m], -e);
+                }
+                s = mean(ldexpf(a.eps, -2 * e));
+            }
+            const float f = rsqrtf(s);
 #pragma unroll
             for (int m = 0; m < M; m++) {
                 u[m] = u[m] * f * nw[m];
