@@ -481,15 +481,16 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
             uint32_t found[DT] = {};
 #pragma unroll 1
             for (int i = 0; i < mine; i++) {
-                if ((i & 31) == 0) names(i);
-                Tile t;
-                load(t, i);
-                const int left = ((t.ok >> (g >> 1)) & 1) ? stop - (begin + 32 * (wave + NW * i) + 8 * g) : 0;
+                const int p0 = begin + 32 * (wave + NW * i) + 8 * g, blk = p0 / KV_BLOCK;
+                const int64_t at = p0 < stop ? kv_block(c, table[blk >> c.sh], blk, kvh) : -1;
+                if (at < 0) continue;
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++)
+                for (int dt = 0; dt < DT; dt++) {
+                    const u32x4 v = *(const u32x4 *)((const T *)a.v + at + voff + 256 * dt);
 #pragma unroll
                     for (int p = 0; p < 8; p++)
-                        found[dt] |= p < left ? kv_odd<T>(t.v[dt][p >> 1] >> 16 * (p & 1) & 0xFFFFu) : 0u;
+                        found[dt] |= p < stop - p0 ? kv_odd<T>(v[p >> 1] >> 16 * (p & 1) & 0xFFFFu) : 0u;
+                }
             }
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
