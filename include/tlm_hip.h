@@ -694,17 +694,19 @@ int    tlm_hip_kv_append(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, i
 /* Attention of one row a sequence (b->cu NULL): out[b][h] = sum_j p_j v_j, p = softmax of scale q . k_j over the positions
  * j < lens[b], head h with key head h / (heads / kv_heads).  q in the cache's type (row b at q + b q_stride, heads
  * side by side), out [B][heads][head_dim] of out_dt (F32, F16 or BF16), overlapping no input; scale positive.  Scores before
- * their scale, maxima, the softmax and its sums are f32, weights enter the second product rounded to the cache's type; sums are
- * divided at the end, so those of BF16 values past 2^122 / lens[b] may overflow.  Positions that all have a score of -infinity give
- * NaN (0 / 0); an infinite value gives that infinity whatever its weight's size (both infinities: NaN).  Sequences are split over their length as the batch's total asks, in the same way in every call with equal
- * lengths: a call repeats its bits.  workspace: tlm_hip_kv_decode_workspace_bytes bytes (0: none, by the sizes alone), 256-byte
- * aligned, nothing in it kept or zeroed; calls that may overlap need different ones. */
+ * their scale, maxima, the softmax and its sums are f32; weights enter the second product as two numbers of the cache's type
+ * (16 bits of BF16, 22 of F16).  Sums are divided at the end, so those of BF16 values past 2^122 / lens[b] may overflow.
+ * Positions that all have a score of -infinity give NaN (0 / 0); an infinite value gives that infinity whatever its weight's
+ * size (both infinities: NaN).  Sequences are split over their length as the batch's total asks, in the same way in every call
+ * with equal lengths: a call repeats its bits.  workspace: tlm_hip_kv_decode_workspace_bytes bytes (0: none, by the sizes
+ * alone), 256-byte aligned, nothing in it kept or zeroed; calls that may overlap need different ones. */
 size_t tlm_hip_kv_decode_workspace_bytes(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads);
 int    tlm_hip_kv_decode(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, const void *q, int64_t q_stride, int heads,
                          float scale, int out_dt, void *out, void *workspace, void *stream);
 /* Attention of packed rows, causal: a row at position p sees the positions 0 .. p of its sequence (cached ones
- * included).  q and out as above, [rows] for [B].  workspace: tlm_hip_kv_prompt_workspace_bytes bytes (0: none, by the sizes
- * alone: few rows over far-reaching tables have their positions split), as tlm_hip_kv_decode's. */
+ * included).  q and out as above, [rows] for [B]; weights enter the second product rounded once to the cache's type.
+ * workspace: tlm_hip_kv_prompt_workspace_bytes bytes (0: none, by the sizes alone: few rows over far-reaching tables have their
+ * positions split), as tlm_hip_kv_decode's. */
 size_t tlm_hip_kv_prompt_workspace_bytes(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads);
 int    tlm_hip_kv_prompt(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, const void *q, int64_t q_stride, int heads,
                          float scale, int out_dt, void *out, void *workspace, void *stream);
