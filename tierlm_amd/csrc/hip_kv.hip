@@ -313,8 +313,14 @@ struct DecodeBatch {
     }
 };
 
+/* Waves a SIMD that the registers must leave room for: where a sequence is a group's, as many groups a unit as narrow heads
+ * allow (three of 32, two of 64 and 160 wide; 96 wide one, and the next when half of its waves are done); shares are a group
+ * a unit. */
+constexpr int decode_waves(int HD, int NW, bool WHOLE) {
+    return NW == 8 ? (HD == 32 ? 6 : HD == 64 ? 4 : HD == 96 ? 3 : 2) : WHOLE && HD == 160 ? 2 : 1;
+}
 template <class T, int HD, int NC, int NW, bool WHOLE>
-__global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeArgs a) {
+__global__ __launch_bounds__(NW * 64, decode_waves(HD, NW, WHOLE)) void k_kv_decode(DecodeArgs a) {
     typedef typename KvType<T>::x8 x8;
     constexpr int KS = HD / 32, DT = HD / 16;    /* steps of the first product, result tiles of the second */
     constexpr int LD = HD + 4;                   /* a merged column in LDS: 16 lanes' float4 on all banks */
@@ -378,7 +384,6 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
 
         f32x4 o[NC][DT];
         float m[NC], l[NC];
-        int seen = 0;        /* not 0: the wave's tiles hold a position */
 #pragma unroll
         for (int n = 0; n < NC; n++) {
             m[n] = -INFINITY;
@@ -389,14 +394,10 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
         auto compute = [&](Tile &t, int i) {
             const int p0 = begin + 32 * (wave + NW * i) + 8 * g;     /* the lane's first position */
             const bool whole = p0 - 8 * g + 32 <= stop && t.ok == 3;
-            seen |= t.ok;
             const int left = ((t.ok >> (g >> 1)) & 1) ? stop - p0 : 0;
             if (!whole) {    /* what a masked place holds may be anything, and 0 times it not 0 */
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                    for (int w = 0; w < 4; w++)
-                        t.v[dt][w] &= (2 * w < left ? 0xFFFFu : 0u) | (2 * w + 1 < left ? 0xFFFF0000u : 0u);
+                for (int dt = 0; dt < DT; dt++) t.v[dt] = kv_upto(t.v[dt], left);
             }
 #pragma unroll
             for (int n = 0; n < NC; n++) {
@@ -436,13 +437,15 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
                     const float e = __builtin_amdgcn_exp2f(fmaf(z[j] - base, a.scale2, KvType<T>::SHIFT));
                     l[n] += e;
                     p[j] = (T)e;
-                    rest[j] = (T)(e - (float)p[j]);
+                    z[j] = e;
                 }
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    o[n][dt] = KvType<T>::mma(kv_bits<x8>(t.v[dt]), p, o[n][dt]);
-                    o[n][dt] = KvType<T>::mma(kv_bits<x8>(t.v[dt]), rest, o[n][dt]);
-                }
+                for (int dt = 0; dt < DT; dt++) o[n][dt] = KvType<T>::mma(kv_bits<x8>(t.v[dt]), p, o[n][dt]);
+                __builtin_amdgcn_sched_barrier(0);      /* the second numbers behind: ahead they take narrow heads' registers */
+#pragma unroll
+                for (int j = 0; j < 8; j++) rest[j] = (T)(z[j] - (float)p[j]);
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[n][dt] = KvType<T>::mma(kv_bits<x8>(t.v[dt]), rest, o[n][dt]);
             }
         };
         const int mine = (tiles - wave + NW - 1) / NW;      /* this wave's tiles */
@@ -460,15 +463,8 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
                 if (i + 1 < mine) compute(tb, i + 1);
             }
         }
-        /* the lanes of a column hold different positions' weights */
-#pragma unroll
-        for (int n = 0; n < NC; n++) {
-            l[n] += __shfl_xor(l[n], 16, 64);
-            l[n] += __shfl_xor(l[n], 32, 64);
-            if (seen) m[n] = fmaxf(m[n], KV_LOWEST);
-        }
-        /* sums that are not finite (and no score's doing): the wave's values that are not, each lane those that it holds in the
-         * operands, then to the lanes of their sums (rare) */
+        /* No score above -infinity, or sums that are not finite: is there a position, and which of the wave's values are not
+         * finite, each lane those that it holds in the operands, then to the lanes of their sums (rare) */
         bool odd = false;
 #pragma unroll
         for (int n = 0; n < NC; n++) {
@@ -478,34 +474,48 @@ __global__ __launch_bounds__(NW * 64, NW == 8 ? 2 : 1) void k_kv_decode(DecodeAr
 #pragma unroll
                 for (int r = 0; r < 4; r++) z[r] = fmaf(o[n][dt][r], 0.0f, z[r]);
             const float none = z[0] + z[1] + (z[2] + z[3]);
-            odd |= none != none && l[n] == l[n];
+            odd |= none != none || m[n] == -INFINITY;
         }
-        if (__any(odd)) {
-            uint32_t found[DT] = {};
+        if (__builtin_expect(mine > 0 && __any(odd), 0)) {
+            float found[DT] = {};
+            bool seen = false;
 #pragma unroll 1
             for (int i = 0; i < mine; i++) {
                 const int p0 = begin + 32 * (wave + NW * i) + 8 * g, blk = p0 / KV_BLOCK;
                 const int64_t at = p0 < stop ? kv_block(c, table[blk >> c.sh], blk, kvh) : -1;
                 if (at < 0) continue;
+                seen = true;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
-                    const u32x4 v = *(const u32x4 *)((const T *)a.v + at + voff + 256 * dt);
+                    x8 v = kv_bits<x8>(kv_upto(*(const u32x4 *)((const T *)a.v + at + voff + 256 * dt), stop - p0));
 #pragma unroll
-                    for (int p = 0; p < 8; p++)
-                        found[dt] |= p < stop - p0 ? kv_odd<T>(v[p >> 1] >> 16 * (p & 1) & 0xFFFFu) : 0u;
+                    for (int p = 0; p < 8; p++) {     /* 0 for what is finite */
+                        const float x = (float)v[p];
+                        found[dt] += x - __builtin_amdgcn_fmed3f(x, -3.4028234663852886e38f, 3.4028234663852886e38f);
+                    }
                 }
             }
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
-                found[dt] |= __shfl_xor(found[dt], 16, 64);
-                found[dt] |= __shfl_xor(found[dt], 32, 64);
+                found[dt] += __shfl_xor(found[dt], 16, 64);
+                found[dt] += __shfl_xor(found[dt], 32, 64);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const uint32_t is = __shfl(found[dt], 4 * g + r, 64);
+                    const float is = __shfl(found[dt], 4 * g + r, 64);
 #pragma unroll
-                    for (int n = 0; n < NC; n++) o[n][dt][r] = kv_put_odd(o[n][dt][r], is);
+                    for (int n = 0; n < NC; n++) o[n][dt][r] = is == 0.0f ? o[n][dt][r] : is;
                 }
             }
+            if (__any(seen)) {
+#pragma unroll
+                for (int n = 0; n < NC; n++) m[n] = fmaxf(m[n], KV_LOWEST);
+            }
+        }
+        /* the lanes of a column hold different positions' weights */
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            l[n] += __shfl_xor(l[n], 16, 64);
+            l[n] += __shfl_xor(l[n], 32, 64);
         }
         /* merge the waves, half of them at a time, always in the same order */
 #pragma unroll

@@ -151,7 +151,7 @@ __device__ __forceinline__ float kv_factor(float m, float to, float scale2) {
  * its result NaN.  One that sees none keeps -infinity, and gets zeros. */
 constexpr float KV_LOWEST = -3.4028234663852886e38f;
 __device__ __forceinline__ float kv_inverse(float l, float m) {
-    return l != 0.0f ? 1.0f / l : m == -INFINITY ? 0.0f : __builtin_nanf("");
+    return l != 0.0f ? __builtin_amdgcn_rcpf(l) : m == -INFINITY ? 0.0f : __builtin_nanf("");   /* to one unit of 2^-23 */
 }
 /* Values that are not finite come through whatever their weight, also where it or the factor that scales its sum rounds to 0
  * (0 times infinity is NaN): sums that are not finite at the end have the values that made them so looked up and put in their
@@ -184,6 +184,12 @@ __device__ __forceinline__ void kv_store(void *out, int dt, int64_t i, const flo
 }
 
 template <class V> __device__ __forceinline__ V kv_bits(u32x4 v) { return __builtin_bit_cast(V, v); }
+/* 8 values, zeros from the left-th on */
+__device__ __forceinline__ u32x4 kv_upto(u32x4 v, int left) {
+#pragma unroll
+    for (int w = 0; w < 4; w++) v[w] &= (2 * w < left ? 0xFFFFu : 0u) | (2 * w + 1 < left ? 0xFFFF0000u : 0u);
+    return v;
+}
 
 /* 8 consecutive elements at any alignment of the type */
 template <class T> __device__ __forceinline__ u32x4 kv_load8(const T *p) {
