@@ -11,8 +11,8 @@ namespace {
  * so the norm is one 16-lane sum and the rotation stays in the lane.  Vectors go in the order of memory, 16 heads of a row at a time (a
  * row a lane group: 87 us for what takes 75), and values are turned over in registers (8 rows of one value to 16 bytes),
  * so the cache's block is written as whole pieces.
- * 8192 rows of 64 + 8 heads of 128, bf16: 75 us, 4.0 TB/s (63 us from an idle device); 61 rows of a decode step 5.5 us, a chain
- * of four reads and a launch. */
+ * 8192 rows of 64 + 8 heads of 128, bf16: 75 us, 4.0 TB/s (64 us from an idle device); 61 rows of a decode step 5 to 6 us, a
+ * chain of four reads and a launch. */
 struct AppendArgs {
     KvView c;
     const void *x;
@@ -247,14 +247,14 @@ template <class X, class T, int M> __global__ __launch_bounds__(256) void k_kv_a
  * A group takes a part of a sequence's positions for one key head and up to 16 NC of its queries; its NW waves take tiles
  * of 32 positions in turn, straight from memory into the matrix cores' operands (no LDS on the way), the next tile's
  * loads in flight, and merge their sums through LDS at the end.  The bytes of the cache bound it: 64 sequences of up to 8192,
- * 64 heads on 4 of 128, in 102 us (5.4 TB/s, some of it from the memory-side cache; a copy 5.14), one of 131071, 32 on 4, in 48.
+ * 64 heads on 4 of 128, in 102 us (5.4 TB/s, some of it from the memory-side cache; a copy 5.14), one of 131071, 32 on 4, in 50.
  *
  * Shares: the lengths are the device's, so every group works its share out for itself.  All sequences' positions lie end
  * to end in units of 128, and W workers a key head take equal parts of that line, across the sequences' ends: however
  * uneven the lengths are, the groups that fill the chip once end together.  A sequence inside one share is written at
  * once; the parts of the others go to the workspace, and k_kv_join adds a sequence's in order.  Where the tables are short
  * (DECODE_WHOLE) each sequence is a group's and one launch does.  With a fixed number of splits a sequence the 64 ragged ones
- * took 129 us instead of 113 with their join. */
+ * took 14% longer (129 us for 113, with their join; 106 now). */
 struct DecodeArgs {
     KvView c;
     const void *q, *k, *v;
@@ -659,8 +659,8 @@ template <class T> void append_x(int xdt, const AppendArgs &a, dim3 grid, hipStr
 }
 
 /* A sequence a group of eight waves and one launch, where the tables are as short as this; twice as long where there are groups
- * for every compute unit.  us whole / in shares, 32 heads on 4 of 128: one sequence of 500 8.1 / 8.8, of 1000 10.3 / 8.8; 64 of
- * 500 16.1 / 18.0, of 1000 24.8 / 27.1, of up to 1000 18.9 / 21.6; 256 of 1000 104 / 103; 300 of 8 on 2 of 64 5.3 / 8.1. */
+ * for every compute unit.  us whole / in shares, 32 heads on 4 of 128: one sequence of 500 8.5 / 9.1, of 1000 10.9 / 9.1; 64 of
+ * 500 16.1 / 17.9, of 1000 24.4 / 26.3, of up to 1000 18.9 / 21.2; 256 of 1000 106 / 103; 300 of 8 on 2 of 64 7.7 / 13.7. */
 constexpr int64_t DECODE_WHOLE = 512;
 
 struct DecodePlan {
@@ -668,9 +668,10 @@ struct DecodePlan {
 };
 DecodePlan decode_plan(const tlm_hip_kv_cache *c, const tlm_hip_kv_batch *b, int heads) {
     /* Columns of 16 queries a group.  A key head with more queries has a group for every 16, which read the cache again from
-     * the caches nearer by; narrow heads, whose tiles are little to read, take 32.  us with 16 / 32 / 64 a group: 48 sequences of up
-     * to 8192 with 64 heads on 1 of 128 36.6 / 36.5 / 44.9, 40 on 2 of 128 55 / 55, 128 on 4 of 64 55 / 46; one of 30000
-     * with 64 on 1 of 128 14.6 / 17.8 / 24.8, 64 on 2 of 256 22.5 / 28.4. */
+     * the caches nearer by; narrow heads, whose tiles are little to read, take 32.  us with 16 / 32 / 64 a group, one number a
+     * weight: 48 sequences of up to 8192 with 64 heads on 1 of 128 36.6 / 36.5 / 44.9 (two numbers: 38.7 with 16), 40 on 2 of
+     * 128 55 / 55, 128 on 4 of 64 55 / 46; one of 30000 with 64 on 1 of 128 14.6 / 17.8 / 24.8 (15.0), 64 on 2 of 256 22.5 / 28.4
+     * (23.2). */
     const int G = heads / c->kv_heads, nc = G > 16 && c->head_dim <= 64 ? 2 : 1, z = (G + nc * 16 - 1) / (nc * 16);
     const int64_t cap = (int64_t)b->table_pages * c->page;
     if (cap <= DECODE_WHOLE || (cap <= 2 * DECODE_WHOLE && b->B * c->kv_heads * z >= 256)) return {1, (int)b->B, nc, z, 0};

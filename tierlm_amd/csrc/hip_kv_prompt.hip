@@ -59,8 +59,8 @@ __device__ __forceinline__ int prompt_part(int tiles, int parts, int sg) {
  * Row i of a key operand is position 8 h + 4 u + e of its block for i = 8 u + 4 h + e: a lane's scores are then 8
  * consecutive positions a block, its operand of the second product.
  *
- * 16384 tokens, 32 heads on 4 of 128: 2.07 to 2.17 ms, 1013 to 1064 TFLOP/s (the library's large product 1337).  Matrix
- * instructions run in 49% of a SIMD's cycles, vector ones issue in 37%, and with two waves a SIMD they hardly overlap; three
+ * 16384 tokens, 32 heads on 4 of 128: 2.09 to 2.19 ms, 1004 to 1052 TFLOP/s (the library's large product 1337).  Matrix
+ * instructions run in 50% of a SIMD's cycles, vector ones issue in 38%, and with two waves a SIMD they hardly overlap; three
  * waves (stages of 32 positions), other orders of the loops and raised priorities for either part changed nothing.
  *
  * A masked place's value may be infinite or NaN, and its weight 0 does not silence it: in stages with a border the values
