@@ -350,9 +350,11 @@ __global__ __launch_bounds__(NW * 64, decode_waves(HD, NW, WHOLE)) void k_kv_dec
 
         /* A tile's two blocks: row i of key tile t is position 8 (i / 4) + 4 t + i % 4 (block i / 8), so that a lane's scores are
          * the positions 8 g .. 8 g + 7 (block g / 2), which are its operand of the second product. */
-        const int krow = 8 * (col >> 2) + (col & 3);
-        const int koff = kv_key_at(krow & 15, 0) + (g >> 1) * 256 + (g & 1) * 8;   /* + 64 t (four positions) + 512 ks */
-        const int voff = kv_value_at(0, col) + (g & 1) * 8;                        /* + 256 dt */
+        auto key_piece = [](int lane) {          /* + 64 t (four positions) + 512 ks */
+            const int col = lane & 15, g = lane >> 4, krow = 8 * (col >> 2) + (col & 3);
+            return kv_key_at(krow & 15, 0) + (g >> 1) * 256 + (g & 1) * 8;
+        };
+        auto value_piece = [](int lane) { return kv_value_at(0, lane & 15) + (lane >> 4 & 1) * 8; };     /* + 256 dt */
         struct Tile {
             u32x4 k[2][KS], v[DT];
             int ok;          /* bit i: block i is a page's */
@@ -371,8 +373,11 @@ __global__ __launch_bounds__(NW * 64, decode_waves(HD, NW, WHOLE)) void k_kv_dec
             t.ok = (o0 >= 0 ? 1 : 0) | (o1 >= 0 ? 2 : 0);
             o0 = o0 < 0 ? 0 : o0;    /* block 0 is inside the cache; what it holds is masked */
             o1 = o1 < 0 ? 0 : o1;
-            const GAS T *k = (const GAS T *)a.k + ((col & 8) ? o1 : o0) + koff;
-            const GAS T *v = (const GAS T *)a.v + (g >= 2 ? o1 : o0) + voff;
+            /* a sequence a group: the lane's places anew for each tile, kept they are the registers that narrow heads lack */
+            int own = lane;
+            if (WHOLE) asm volatile("" : "+v"(own));
+            const GAS T *k = (const GAS T *)a.k + ((own & 8) ? o1 : o0) + key_piece(own);
+            const GAS T *v = (const GAS T *)a.v + (own >= 32 ? o1 : o0) + value_piece(own);
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 t.k[0][ks] = *(const GAS u32x4 *)(k + 512 * ks);
@@ -437,13 +442,11 @@ __global__ __launch_bounds__(NW * 64, decode_waves(HD, NW, WHOLE)) void k_kv_dec
                     const float e = __builtin_amdgcn_exp2f(fmaf(z[j] - base, a.scale2, KvType<T>::SHIFT));
                     l[n] += e;
                     p[j] = (T)e;
-                    z[j] = e;
+                    rest[j] = (T)(e - (float)p[j]);
                 }
+                if (WHOLE) __builtin_amdgcn_sched_barrier(0);      /* products among them keep all eight weights' floats in registers */
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) o[n][dt] = KvType<T>::mma(kv_bits<x8>(t.v[dt]), p, o[n][dt]);
-                __builtin_amdgcn_sched_barrier(0);      /* the second numbers behind: ahead they take narrow heads' registers */
-#pragma unroll
-                for (int j = 0; j < 8; j++) rest[j] = (T)(z[j] - (float)p[j]);
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) o[n][dt] = KvType<T>::mma(kv_bits<x8>(t.v[dt]), rest, o[n][dt]);
             }
@@ -487,7 +490,7 @@ __global__ __launch_bounds__(NW * 64, decode_waves(HD, NW, WHOLE)) void k_kv_dec
                 seen = true;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
-                    x8 v = kv_bits<x8>(kv_upto(*(const u32x4 *)((const T *)a.v + at + voff + 256 * dt), stop - p0));
+                    x8 v = kv_bits<x8>(kv_upto(*(const u32x4 *)((const T *)a.v + at + value_piece(lane) + 256 * dt), stop - p0));
 #pragma unroll
                     for (int p = 0; p < 8; p++) {     /* 0 for what is finite */
                         const float x = (float)v[p];
