@@ -103,3 +103,20 @@ def test_neighbours_keep_their_bits(hip, dtype):
         got = kv.prompt(q, b.cache, b.tables, b.lens, b.cu, dtype=F32)
         keep = torch.arange(new[0], device="cuda") != 5
         assert torch.equal(got[keep], want[keep]) and not torch.equal(got[5], want[5])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("scale", [1e-30, 1e-38, 2e-44])
+def test_tiny_scales(hip, dtype, scale):
+    """Scales down to floats without a leading one: every weight is the same."""
+    from tests.kv_ref import close, reference
+    for lens, width in (([1, 33, 300], None), ([2900, 40], 200)):
+        b = Batch(dtype, 8, 2, 64, 16, [1] * len(lens), lens, seed=36, width=width)
+        got = kv.decode(b.q, b.cache, b.tables, b.lens, scale=scale, dtype=F32)
+        for i, n in enumerate(lens):
+            want, tol = reference(b.q[i:i + 1], b.k[i], b.v[i], scale, n - 1)
+            close(got[i:i + 1], want, tol)
+        p = Batch(dtype, 8, 2, 64, 16, [40], [lens[0] + 40], seed=37, width=width)
+        got = kv.prompt(p.q, p.cache, p.tables, p.lens, p.cu, scale=scale, dtype=F32)
+        want, tol = reference(p.q, p.k[0], p.v[0], scale, lens[0])
+        close(got, want, tol)
